@@ -8,7 +8,9 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libflashMoe.so")
 
-F32, BF16 = 0, 1
+F32, BF16, MXFP4 = 0, 1, 2
+ACT_SILU, ACT_GELU_TANH = 0, 1
+FFN_ROW_MAJOR, FFN_MXFP4 = 0, 1
 SCHED_AUTO, SCHED_STREAM, SCHED_TILED = 0, 1, 2
 FLAG_PACK_WEIGHTS = 1
 FLAG_WEIGHTS_PREPACKED = 2
@@ -39,6 +41,13 @@ class LayerDesc(ctypes.Structure):
         ("norm_weight", ctypes.c_void_p),
         ("norm_eps", ctypes.c_double),
     ]
+
+
+class FfnDesc(ctypes.Structure):
+    """Mirror of FlashMoeFfnDesc."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("hidden", "intermediate", "dtype", "activation", "weights")] + \
+               [(n, ctypes.c_void_p) for n in ("w13", "w2", "w13_scales", "w2_scales")]
 
 
 # name -> (restype, argtypes); every symbol include/flash_moe.h declares
@@ -74,6 +83,20 @@ C_ABI = {
                                             ctypes.c_void_p]),
     "flashMoeNoAllocStatus": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint), ctypes.c_void_p]),
     "flashMoeAbi": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_size_t)]),
+    "flashMoeFfnBytes": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_int] + [ctypes.POINTER(ctypes.c_size_t)] * 3),
+    "flashMoeFfnForward": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                          ctypes.c_longlong, ctypes.c_int] + [ctypes.c_void_p] * 3),
+    "flashMoeFfnBackward": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                           ctypes.c_longlong, ctypes.c_int] + [ctypes.c_void_p] * 3 +
+                            [ctypes.c_longlong] + [ctypes.c_void_p] * 3),
+    "flashMoeMxfp4Quantize": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_int] +
+                              [ctypes.c_void_p] * 3),
+    "flashMoeMxfp4Dequantize": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                               ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
+    "flashMoeMxfp4LinearBytes": (ctypes.c_int, [ctypes.c_int] * 4 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "flashMoeMxfp4Linear": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                           ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]),
     "flashMoeSetDenseSmallBatch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
 }
 ABI_VERSION = 3

@@ -60,7 +60,7 @@ def build(verbose=True):
     return LIB_PATH
 
 
-PY_SRC = os.path.join(CSRC, "py", "flashMoeLauncherModule.cpp")
+PY_SRCS = [os.path.join(CSRC, "py", name) for name in ("flashMoeLauncherModule.cpp", "flashFfnBindings.cpp")]
 ROOT = os.path.dirname(HERE)
 
 
@@ -71,8 +71,8 @@ def py_extension_path():
 
 
 def build_py_extension(verbose=True):
-    """The `flashMoeLauncher` Python extension (pybind11 over the C++ interface), next to the
-    package so that `import flashMoeLauncher` finds it with the repository root on sys.path.
+    """The `flashMoeLauncher` Python extension (pybind11 over the C++ interface and the C ABI), next to
+    the package so that `import flashMoeLauncher` finds it with the repository root on sys.path.
     Host code only: compiled with g++ against torch's headers."""
     import sysconfig
 
@@ -81,12 +81,22 @@ def build_py_extension(verbose=True):
 
     out = py_extension_path()
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-I" + sysconfig.get_paths()["include"]]
-    cmd += ["-I" + p for p in cpp_extension.include_paths()] + ["-I/opt/rocm/include"]
-    cmd += [PY_SRC, "-o", out, "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_hip",
+    compile_ = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+                "-I" + sysconfig.get_paths()["include"]]
+    compile_ += ["-I" + p for p in cpp_extension.include_paths()] + ["-I/opt/rocm/include"]
+    objs, procs = [], []
+    for src in PY_SRCS:
+        objs.append(os.path.join(LIB_DIR, os.path.basename(src) + ".o"))
+        cmd = compile_ + ["-c", src, "-o", objs[-1]]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append((cmd, subprocess.Popen(cmd)))
+    for cmd, p in procs:
+        if p.wait() != 0:
+            raise RuntimeError("g++ failed: " + " ".join(cmd))
+    cmd = ["g++", "-shared"] + objs + ["-o", out, "-L" + tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_hip",
             "-lc10_hip", "-ltorch_python", "-L" + LIB_DIR, "-lflashMoe", "-L/opt/rocm/lib",
             "-lamdhip64", "-Wl,-rpath,$ORIGIN/flash_distributed_moe_amd/lib", "-Wl,-rpath," + tlib]
     if verbose:

@@ -1,0 +1,234 @@
+// The tiled matrix product of the dense feed-forward kernels, C[m, n] = sum_k A(m, k) B(n, k).
+//
+// A workgroup of WM x WN waves takes a tile of WM*FM*16 by WN*FN*16 results; a wave FM by FN blocks
+// of 16 x 16. The matrix instructions get the rows of B as their first operand, so that a lane ends
+// up with 4 FN neighbouring columns of one row of C and stores them 16 bytes at a time.
+#pragma once
+#include "ffn_device.h"
+
+namespace fmoe {
+
+template <int KIND_, bool OUTER_A_, bool OUTER_B_, int EPI_, int WM_, int WN_, int FM_, int FN_>
+struct GemmShape {
+  static constexpr int KIND = KIND_;
+  static constexpr bool OUTER_A = OUTER_A_, OUTER_B = OUTER_B_;
+  static constexpr int EPI = EPI_, WM = WM_, WN = WN_, FM = FM_, FN = FN_;
+  static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
+  static constexpr int BM = WM * FM * 16, BN = WN * FN * 16;     // rows of the two tiles
+  static constexpr int CN = EPI == EPI_GATED ? BN / 2 : BN;      // columns of C a workgroup writes
+  static constexpr int STEP = step_k(KIND);
+  static constexpr int ESIZE = KIND == KIND_F32 ? 4 : 2;         // bytes a value (MXFP4: see bytes_of)
+  static constexpr int STAGE_BYTES = (BM + BN) * 128;
+};
+
+template <int KIND>
+__device__ __forceinline__ long long bytes_of(long long values) {
+  return KIND == KIND_MXFP4 ? values / 2 : KIND == KIND_F32 ? values * 4 : values * 2;
+}
+
+// One operand's loads: which bytes of memory this lane asks for in each of its pieces of a stage.
+// GATED: the tile's rows are gate rows of `matrix rows / 2` and the up rows of the same columns.
+template <int KIND, bool OUTER, int ROWS, int THREADS, int F, bool GATED>
+struct TileLoader {
+  static constexpr int PIECES = ROWS * 8 / THREADS;
+  static constexpr int PK = piece_k(KIND);
+  static constexpr int LINE = OUTER ? ROWS / PK : 8;  // pieces of a k, or of a row
+  static_assert(PIECES * THREADS == ROWS * 8, "whole pieces a thread");
+  static_assert(!GATED || !OUTER, "gated weights have their k inside the rows");
+  unsigned offset[PIECES];
+  const char* base;
+  long long step_bytes, up_bytes;
+
+  // k of this lane's piece i inside a stage (the first of its values)
+  __device__ __forceinline__ static int k_of(int i) {
+    const int at = i * THREADS + threadIdx.x;
+    return OUTER ? at / LINE : ((at & 7) ^ ((at >> 3) & 7)) * PK;
+  }
+
+  // row0: the tile's first row (gated: its first column of C) of `rows`
+  __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows) {
+    const int tid = threadIdx.x;
+    up_bytes = GATED ? bytes_of<KIND>(rows * ld) : 0;
+    if constexpr (!OUTER) {
+      base = static_cast<const char*>(p) + bytes_of<KIND>(row0 * ld);
+      step_bytes = 128;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int row = (i * THREADS + tid) >> 3, piece = (tid & 7) ^ (row & 7);
+        const int in_wave = row % (16 * F), f = in_wave >> 4, r = in_wave & 15;
+        const int src = GATED ? row / (16 * F) * (8 * F) + gated_row<F>(f, r) : row / (16 * F) * (16 * F) + dealt_row<F>(f, r);
+        offset[i] = row0 + src < rows ? static_cast<unsigned>(bytes_of<KIND>(src * ld)) + piece * 16 : kOutside;
+      }
+    } else {
+      base = static_cast<const char*>(p) + bytes_of<KIND>(row0);
+      step_bytes = bytes_of<KIND>(ld * step_k(KIND));
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int at = i * THREADS + tid, k = at / LINE;
+        int piece = at % LINE;
+        if constexpr (KIND == KIND_BF16) piece ^= k_row_swap<F>(k) & (LINE - 1);
+        offset[i] = row0 + piece * PK < rows ? static_cast<unsigned>(bytes_of<KIND>(k * ld)) + piece * 16 : kOutside;
+      }
+    }
+  }
+
+  // Stage s into `lds`; left: how many k there are from its first one on
+  __device__ __forceinline__ void load(char* lds, int s, int left) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const char* from = base + s * step_bytes;
+    char* to = lds + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int f = ((i * THREADS + wave * 64) >> 3) % (16 * F) / 16;  // gated: the same for all of a wave's lanes
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(from + (GATED && f >= F / 2 ? up_bytes : 0), 0x7FFFFFFFu);
+      const bool in = left >= step_k(KIND) || k_of(i) < left;
+      load_to_lds16(r, to + i * THREADS * 16, in ? offset[i] : kOutside);
+    }
+  }
+};
+
+// A wave's F blocks of an operand for one of the stage's two halves (KIND_BF16, KIND_F32, MXFP4: 32, 16, 128 k).
+// Lane l holds row l % 16 of each block and the (l / 16)-th quarter of the k, 16 bytes.
+template <int KIND, bool OUTER, int ROWS, int F>
+struct Fragments {
+  static constexpr int LINE_BYTES = ROWS * (KIND == KIND_F32 ? 4 : 2);  // of a k, where a row is one k
+  i32x4 v[F];
+
+  __device__ __forceinline__ void read(const char* tile, int wave_row, int half) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    if constexpr (!OUTER) {
+      const char* at = tile + (wave_row + r) * 128 + (((half * 4 + g) ^ (r & 7)) << 4);
+#pragma unroll
+      for (int f = 0; f < F; ++f) v[f] = *(const FFN_LDS i32x4*)(at + f * 2048);
+    } else if constexpr (KIND == KIND_BF16) {
+      const int k = half * 32 + g * 8 + (r >> 2), swap = k_row_swap<F>(r >> 2) & (ROWS / 8 - 1);
+      const char* line = tile + k * LINE_BYTES;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const int col = wave_row + 4 * F * (r & 3) + 4 * f;
+        const char* at = line + (((col >> 3) ^ swap) << 4) + (f & 1) * 8;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FFN_LDS s16x4*)(at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FFN_LDS s16x4*)(at + 4 * LINE_BYTES));
+        v[f] = __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const char* at = tile + (half * 16 + g * 4) * LINE_BYTES + (wave_row + dealt_row<F>(f, r)) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[f][j] = *(const FFN_LDS int*)(at + j * LINE_BYTES);
+      }
+    }
+  }
+};
+
+// The workgroup's tile. Neighbouring workgroup numbers lie on different XCDs, each with an L2 of its
+// own, so an XCD gets a run of the order; the order walks GROUP tile rows column by column, so
+// that the tiles in flight on an XCD share rows of both operands.
+__device__ __forceinline__ void tile_of(const GemmArgs& p, int& tile_m, int& tile_n) {
+  constexpr int XCDS = 8, GROUP = 8;
+  const int count = p.grid_m * p.grid_n, id = blockIdx.x;
+  const int xcd = id % XCDS, each = count / XCDS, extra = count % XCDS;
+  const int at = xcd * each + (xcd < extra ? xcd : extra) + id / XCDS;
+  const int first = at / (GROUP * p.grid_n) * GROUP;
+  const int rows = p.grid_m - first < GROUP ? p.grid_m - first : GROUP;
+  const int inside = at - first * p.grid_n;
+  tile_m = first + inside % rows;
+  tile_n = inside / rows;
+}
+
+template <class S>
+struct Accumulators {
+  f32x4 v[S::FM][S::FN];
+};
+
+// Eight (or, float32, four) neighbouring results
+__device__ __forceinline__ void store8(unsigned short* to, const float* f) {
+  *reinterpret_cast<u32x4*>(to) = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+}
+__device__ __forceinline__ void store4(float* to, const float* f) {
+  *reinterpret_cast<f32x4*>(to) = f32x4{f[0], f[1], f[2], f[3]};
+}
+// `n` (a multiple of 8) results of a row from column col on, as far as the matrix goes; rows of a
+// matrix whose width is no multiple of 8 are written value by value, they do not begin on 16 bytes
+template <int KIND, int COUNT>
+__device__ __forceinline__ void store_row(void* row, int col, int columns, const float* f) {
+  if constexpr (KIND == KIND_F32) {
+#pragma unroll
+    for (int c = 0; c < COUNT; c += 4)
+      if (col + c < columns) store4(static_cast<float*>(row) + col + c, f + c);
+  } else {
+    unsigned short* to = static_cast<unsigned short*>(row) + col;
+    if ((columns & 7) == 0) {
+#pragma unroll
+      for (int c = 0; c < COUNT; c += 8)
+        if (col + c < columns) store8(to + c, f + c);
+    } else {
+#pragma unroll
+      for (int c = 0; c < COUNT; ++c)
+        if (col + c < columns) to[c] = static_cast<unsigned short>(pack_bf16(f[c], 0.0f) & 0xFFFF);
+    }
+  }
+}
+
+// What becomes of the sums. A lane has, of its rows m of C, 4 FN neighbouring columns; of a gated
+// product the first half of the blocks are gate columns and the others the same up columns.
+template <class S>
+__device__ __forceinline__ void write_results(const GemmArgs& p, int m0, int n0, Accumulators<S>& acc) {
+  constexpr int FN = S::FN, FM = S::FM;
+  constexpr bool EXACT = S::KIND == KIND_F32;
+  constexpr int OUT = EXACT ? KIND_F32 : KIND_BF16, OSIZE = EXACT ? 4 : 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+  for (int fm = 0; fm < FM; ++fm) {
+    const int m = m0 + wm * FM * 16 + dealt_row<FM>(fm, r);
+    if (m >= p.M) continue;
+    if constexpr (S::EPI == EPI_STORE) {
+      float f[4 * FN];
+#pragma unroll
+      for (int fn = 0; fn < FN; ++fn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * fn + i] = acc.v[fm][fn][i];
+      store_row<OUT, 4 * FN>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, n0 + wn * FN * 16 + 4 * FN * g, p.N, f);
+    } else if constexpr (S::EPI == EPI_GATED) {
+      const int col = n0 + wn * FN * 8 + 2 * FN * g;
+      float h[2 * FN], gate[2 * FN], up[2 * FN];
+#pragma unroll
+      for (int i = 0; i < 2 * FN; ++i) {
+        gate[i] = acc.v[fm][i / 4][i % 4];
+        up[i] = acc.v[fm][FN / 2 + i / 4][i % 4];
+        h[i] = act_of<EXACT>(p.act, gate[i]) * up[i];
+      }
+      store_row<OUT, 2 * FN>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, col, p.N, h);
+      if (p.gu != nullptr) {
+        float* row = p.gu + m * (2LL * p.N);
+        store_row<KIND_F32, 2 * FN>(row, col, p.N, gate);
+        store_row<KIND_F32, 2 * FN>(row + p.N, col, p.N, up);
+      }
+    } else {
+      const int col = n0 + wn * FN * 16 + 4 * FN * g;
+      const float* row = p.gu + m * (2LL * p.N);
+      float dg[4 * FN], du[4 * FN];
+#pragma unroll
+      for (int c = 0; c < 4 * FN; c += 4) {
+        if (col + c >= p.N) continue;
+        const f32x4 gate = *reinterpret_cast<const f32x4*>(row + col + c);
+        const f32x4 up = *reinterpret_cast<const f32x4*>(row + p.N + col + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float dh = acc.v[fm][c / 4][i];
+          float a, slope;
+          act_and_slope<EXACT>(p.act, gate[i], a, slope);
+          dg[c + i] = dh * up[i] * slope;
+          du[c + i] = dh * a;
+        }
+      }
+      char* out = static_cast<char*>(p.c) + m * (2LL * p.N) * OSIZE;
+      store_row<OUT, 4 * FN>(out, col, p.N, dg);
+      store_row<OUT, 4 * FN>(out + static_cast<long long>(p.N) * OSIZE, col, p.N, du);
+    }
+  }
+}
+
+}  // namespace fmoe

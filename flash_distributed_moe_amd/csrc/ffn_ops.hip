@@ -1,0 +1,256 @@
+// C ABI of the dense gated feed-forward block and of MXFP4 (include/flash_moe.h): checks of the
+// arguments, workspace layouts, and which kernels a call takes.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "../../include/flash_moe.h"
+#include "ffn_params.h"
+
+#define FMOE_FILENAME (strrchr(__FILE__, '/') ? strrchr(__FILE__, '/') + 1 : __FILE__)
+
+// As the launcher's: print to stdout, return the first failing code.
+#define FMOE_HIP_CHECK(expr)                                               \
+  do {                                                                     \
+    const hipError_t fmoe_err_ = (expr);                                   \
+    if (fmoe_err_ != hipSuccess) {                                         \
+      printf("[MOE HIP ERROR: %s:%i]: %s\n", FMOE_FILENAME, __LINE__,      \
+             hipGetErrorString(fmoe_err_));                                \
+      fflush(stdout);                                                      \
+      return fmoe_err_;                                                    \
+    }                                                                      \
+  } while (0)
+
+#define FMOE_FAIL(code, fmt, ...)                                                      \
+  do {                                                                                 \
+    printf("[MOE ERROR: %s:%i]: " fmt "\n", FMOE_FILENAME, __LINE__, ##__VA_ARGS__);   \
+    fflush(stdout);                                                                    \
+    return (code);                                                                     \
+  } while (0)
+
+namespace {
+
+using fmoe::GemmArgs;
+
+// A tile's rows are addressed with 32 bits from its first one: 256 rows of up to this many values.
+constexpr long long kMaxStride = 1ll << 20;
+
+size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+size_t size_of(int dtype) { return dtype == FLASH_MOE_F32 ? 4 : 2; }
+
+// Rows of `width` values in memory: where they begin and how far apart they lie.
+hipError_t check_rows(const char* name, const void* p, long long ld, long long width, int dtype) {
+  if (p == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null %s pointer", name);
+  if (!aligned16(p)) FMOE_FAIL(hipErrorInvalidValue, "%s does not begin on 16 bytes", name);
+  if (ld < width || ld > kMaxStride || ld * static_cast<long long>(size_of(dtype)) % 16 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "%s: %lld values from row to row (at least %lld, at most %lld, whole 16 bytes)", name,
+              ld, width, kMaxStride);
+  return hipSuccess;
+}
+
+hipError_t validate(const FlashMoeFfnDesc* d, int tokens) {
+  if (d == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null description");
+  if (d->dtype != FLASH_MOE_F32 && d->dtype != FLASH_MOE_BF16)
+    FMOE_FAIL(hipErrorInvalidValue, "dtype %i is neither float32 (0) nor bfloat16 (1)", d->dtype);
+  if (d->activation != FLASH_MOE_ACT_SILU && d->activation != FLASH_MOE_ACT_GELU_TANH)
+    FMOE_FAIL(hipErrorInvalidValue, "activation %i is neither SiLU (0) nor GELU's tanh form (1)", d->activation);
+  if (d->weights != FLASH_MOE_FFN_ROW_MAJOR && d->weights != FLASH_MOE_FFN_MXFP4)
+    FMOE_FAIL(hipErrorInvalidValue, "weights %i are neither row-major (0) nor MXFP4 (1)", d->weights);
+  const bool mx = d->weights == FLASH_MOE_FFN_MXFP4;
+  const int of = mx ? 32 : 8;
+  if (d->hidden < of || d->hidden % of != 0 || d->intermediate < of || d->intermediate % of != 0 ||
+      d->hidden > kMaxStride || d->intermediate > kMaxStride / 2)
+    FMOE_FAIL(hipErrorInvalidValue, "H=%i, I=%i: multiples of %i up to %lld and half of that are admitted", d->hidden,
+              d->intermediate, of, kMaxStride);
+  if (mx && d->dtype != FLASH_MOE_BF16) FMOE_FAIL(hipErrorInvalidValue, "MXFP4 weights take bfloat16 tokens");
+  if (tokens < 0) FMOE_FAIL(hipErrorInvalidValue, "%i tokens", tokens);
+  return hipSuccess;
+}
+
+hipError_t validate_weights(const FlashMoeFfnDesc* d) {
+  if (d->w13 == nullptr || d->w2 == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null weight pointer");
+  if (!aligned16(d->w13) || !aligned16(d->w2)) FMOE_FAIL(hipErrorInvalidValue, "weights do not begin on 16 bytes");
+  if (d->weights == FLASH_MOE_FFN_MXFP4 && (d->w13_scales == nullptr || d->w2_scales == nullptr))
+    FMOE_FAIL(hipErrorInvalidValue, "MXFP4 weights without scales");
+  return hipSuccess;
+}
+
+// What a forward pass leaves for the backward pass: the two projections before the activation in
+// float32 and h in the layer's dtype; the gradients of the projections, the backward pass's own.
+size_t gu_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * 2 * d.intermediate * 4); }
+size_t h_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * d.intermediate * size_of(d.dtype)); }
+size_t dgu_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * 2 * d.intermediate * size_of(d.dtype)); }
+
+}  // namespace
+
+extern "C" {
+
+int flashMoeFfnBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* saved, size_t* forward, size_t* backward) {
+  const hipError_t v = validate(desc, tokens);
+  if (v != hipSuccess) return v;
+  if (saved != nullptr) *saved = gu_bytes(*desc, tokens) + h_bytes(*desc, tokens);
+  if (forward != nullptr) *forward = h_bytes(*desc, tokens);
+  if (backward != nullptr) *backward = dgu_bytes(*desc, tokens);
+  return hipSuccess;
+}
+
+int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx, void* y, long long ldy, int tokens,
+                       void* saved, void* workspace, void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  hipError_t v = validate(desc, tokens);
+  if (v != hipSuccess) return v;
+  if (tokens == 0) return hipSuccess;
+  const FlashMoeFfnDesc& d = *desc;
+  const int H = d.hidden, I = d.intermediate;
+  if ((v = validate_weights(desc)) != hipSuccess) return v;
+  if ((v = check_rows("x", x, ldx, H, d.dtype)) != hipSuccess) return v;
+  if ((v = check_rows("y", y, ldy, H, d.dtype)) != hipSuccess) return v;
+  const bool mx = d.weights == FLASH_MOE_FFN_MXFP4;
+  if (mx && saved != nullptr) FMOE_FAIL(hipErrorInvalidValue, "a block of MXFP4 weights has no backward pass");
+  if (workspace == nullptr && saved == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null workspace");
+  if (!aligned16(workspace) || !aligned16(saved)) FMOE_FAIL(hipErrorInvalidValue, "workspace does not begin on 16 bytes");
+  char* keep = static_cast<char*>(saved);
+  void* h = keep != nullptr ? keep + gu_bytes(d, tokens) : workspace;
+
+  GemmArgs up{};
+  up.a = x, up.b = d.w13, up.b_scales = static_cast<const unsigned char*>(d.w13_scales);
+  up.c = h, up.gu = reinterpret_cast<float*>(keep);
+  up.lda = ldx, up.ldb = H, up.ldc = I;
+  up.M = tokens, up.N = I, up.K = H, up.act = d.activation;
+  GemmArgs down{};
+  down.a = h, down.b = d.w2, down.b_scales = static_cast<const unsigned char*>(d.w2_scales);
+  down.c = y;
+  down.lda = I, down.ldb = I, down.ldc = ldy;
+  down.M = tokens, down.N = H, down.K = I;
+  if (mx) {
+    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_GATED, up, stream));
+    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_STORE, down, stream));
+  } else {
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, false, fmoe::EPI_GATED, up, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, false, fmoe::EPI_STORE, down, stream));
+  }
+  return hipSuccess;
+}
+
+int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ldx, const void* dy, long long lddy,
+                        int tokens, const void* saved, void* workspace, void* dx, long long lddx, void* dw13, void* dw2,
+                        void* stream_) {
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  hipError_t v = validate(desc, tokens);
+  if (v != hipSuccess) return v;
+  const FlashMoeFfnDesc& d = *desc;
+  const int H = d.hidden, I = d.intermediate;
+  if (d.weights != FLASH_MOE_FFN_ROW_MAJOR) FMOE_FAIL(hipErrorInvalidValue, "a block of MXFP4 weights has no backward pass");
+  if (!aligned16(dw13) || !aligned16(dw2)) FMOE_FAIL(hipErrorInvalidValue, "gradients do not begin on 16 bytes");
+  if (tokens > 0) {
+    if ((v = validate_weights(desc)) != hipSuccess) return v;
+    if ((v = check_rows("x", x, ldx, H, d.dtype)) != hipSuccess) return v;
+    if ((v = check_rows("dy", dy, lddy, H, d.dtype)) != hipSuccess) return v;
+    if (dx != nullptr && (v = check_rows("dx", dx, lddx, H, d.dtype)) != hipSuccess) return v;
+    if (saved == nullptr || !aligned16(saved)) FMOE_FAIL(hipErrorInvalidValue, "null or unaligned saved results");
+    if ((dx != nullptr || dw13 != nullptr) && (workspace == nullptr || !aligned16(workspace)))
+      FMOE_FAIL(hipErrorInvalidValue, "null or unaligned workspace");
+  }
+  const char* keep = static_cast<const char*>(saved);
+  if (tokens > 0 && (dx != nullptr || dw13 != nullptr)) {
+    // dh = dy W2, and with it the gradients of both projections
+    GemmArgs p{};
+    p.a = dy, p.b = d.w2, p.c = workspace, p.gu = reinterpret_cast<float*>(const_cast<char*>(keep));
+    p.lda = lddy, p.ldb = I, p.ldc = 2LL * I;
+    p.M = tokens, p.N = I, p.K = H, p.act = d.activation;
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_SLOPE, p, stream));
+  }
+  if (tokens > 0 && dx != nullptr) {
+    GemmArgs p{};
+    p.a = workspace, p.b = d.w13, p.c = dx;
+    p.lda = 2LL * I, p.ldb = H, p.ldc = lddx;
+    p.M = tokens, p.N = H, p.K = 2 * I;
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_STORE, p, stream));
+  }
+  // the weights' gradients sum over the tokens; of no tokens they are zeros
+  if (dw13 != nullptr) {
+    GemmArgs p{};
+    p.a = workspace, p.b = x, p.c = dw13;
+    p.lda = 2LL * I, p.ldb = ldx, p.ldc = H;
+    p.M = 2 * I, p.N = H, p.K = tokens;
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, true, fmoe::EPI_STORE, p, stream));
+  }
+  if (dw2 != nullptr) {
+    GemmArgs p{};
+    p.a = dy, p.b = keep + (tokens > 0 ? gu_bytes(d, tokens) : 0), p.c = dw2;
+    p.lda = lddy, p.ldb = I, p.ldc = I;
+    p.M = H, p.N = I, p.K = tokens;
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, true, fmoe::EPI_STORE, p, stream));
+  }
+  return hipSuccess;
+}
+
+int flashMoeMxfp4Quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales, void* stream) {
+  if (dtype != FLASH_MOE_F32 && dtype != FLASH_MOE_BF16)
+    FMOE_FAIL(hipErrorInvalidValue, "dtype %i is neither float32 (0) nor bfloat16 (1)", dtype);
+  if (rows < 0 || k < 32 || k % 32 != 0) FMOE_FAIL(hipErrorInvalidValue, "%i rows of %i values (a multiple of 32)", rows, k);
+  if (rows == 0) return hipSuccess;
+  if (codes == nullptr || scales == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null codes or scales pointer");
+  if (!aligned16(codes)) FMOE_FAIL(hipErrorInvalidValue, "codes do not begin on 16 bytes");
+  if (x == nullptr || !aligned16(x) || ldx < k || ldx * static_cast<long long>(size_of(dtype)) % 16 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "x: null, not on 16 bytes, or rows %lld values apart", ldx);
+  FMOE_HIP_CHECK(fmoe::launch_mxfp4_quantize(dtype, x, ldx, rows, k, codes, scales, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+int flashMoeMxfp4Dequantize(int dtype, const void* codes, const void* scales, int rows, int k, void* out, long long ldo,
+                            void* stream) {
+  if (dtype != FLASH_MOE_F32 && dtype != FLASH_MOE_BF16)
+    FMOE_FAIL(hipErrorInvalidValue, "dtype %i is neither float32 (0) nor bfloat16 (1)", dtype);
+  if (rows < 0 || k < 32 || k % 32 != 0) FMOE_FAIL(hipErrorInvalidValue, "%i rows of %i values (a multiple of 32)", rows, k);
+  if (rows == 0) return hipSuccess;
+  if (codes == nullptr || scales == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null codes or scales pointer");
+  if (!aligned16(codes)) FMOE_FAIL(hipErrorInvalidValue, "codes do not begin on 16 bytes");
+  if (out == nullptr || !aligned16(out) || ldo < k || ldo * static_cast<long long>(size_of(dtype)) % 16 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "out: null, not on 16 bytes, or rows %lld values apart", ldo);
+  FMOE_HIP_CHECK(fmoe::launch_mxfp4_dequantize(dtype, codes, scales, rows, k, out, ldo, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes) {
+  if (x_format != FLASH_MOE_BF16 && x_format != FLASH_MOE_MXFP4)
+    FMOE_FAIL(hipErrorInvalidValue, "x_format %i is neither bfloat16 (1) nor MXFP4 (2)", x_format);
+  if (rows < 0 || n < 0 || k < 32 || k % 32 != 0 || k > kMaxStride)
+    FMOE_FAIL(hipErrorInvalidValue, "%i x %i x %i (the last a multiple of 32 up to %lld)", rows, n, k, kMaxStride);
+  if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result pointer");
+  *bytes = 0;
+  return hipSuccess;
+}
+
+int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long long ldx, int rows, const void* codes,
+                        const void* scales, int n, int k, void* y, long long ldy, void* workspace, void* stream) {
+  size_t bytes = 0;
+  hipError_t v = static_cast<hipError_t>(flashMoeMxfp4LinearBytes(x_format, rows, n, k, &bytes));
+  if (v != hipSuccess) return v;
+  if (rows == 0 || n == 0) return hipSuccess;
+  if (bytes > 0 && (workspace == nullptr || !aligned16(workspace)))
+    FMOE_FAIL(hipErrorInvalidValue, "null or unaligned workspace");
+  const bool mx = x_format == FLASH_MOE_MXFP4;
+  if (mx) {
+    if (x == nullptr || x_scales == nullptr || !aligned16(x)) FMOE_FAIL(hipErrorInvalidValue, "x: null or unaligned pointer");
+    if (ldx != k) FMOE_FAIL(hipErrorInvalidValue, "MXFP4 rows lie one behind the other");
+  } else if ((v = check_rows("x", x, ldx, k, FLASH_MOE_BF16)) != hipSuccess) {
+    return v;
+  }
+  if (codes == nullptr || scales == nullptr || !aligned16(codes))
+    FMOE_FAIL(hipErrorInvalidValue, "null codes or scales pointer, or codes that do not begin on 16 bytes");
+  if (y == nullptr || ldy < n) FMOE_FAIL(hipErrorInvalidValue, "y: null, or rows %lld values apart", ldy);
+  if (n % 8 == 0 && (!aligned16(y) || ldy % 8 != 0))
+    FMOE_FAIL(hipErrorInvalidValue, "y: rows of a multiple of 8 values begin on 16 bytes");
+  GemmArgs p{};
+  p.a = x, p.a_scales = static_cast<const unsigned char*>(x_scales), p.lda = ldx;
+  p.b = codes, p.b_scales = static_cast<const unsigned char*>(scales), p.ldb = k;
+  p.c = y, p.ldc = ldy;
+  p.M = rows, p.N = n, p.K = k;
+  FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(mx, fmoe::EPI_STORE, p, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+}  // extern "C"

@@ -1,0 +1,35 @@
+// What the dense gated feed-forward block's and MXFP4's host code and kernels share.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace fmoe {
+
+// One matrix product C[m, n] = sum_k A(m, k) B(n, k) of a launch. An operand lies with its k
+// inside a row (A[m * lda + k]) or with a row a k (A[k * lda + m]); which, its type and what
+// becomes of the sums are template parameters of the kernel.
+struct GemmArgs {
+  const void* a;
+  const void* b;
+  const unsigned char* a_scales;  // MXFP4 operands: a byte for 32 k, rows of K / 32
+  const unsigned char* b_scales;
+  void* c;          // sums; h [M, N] of the gated kernels; the gradients of both projections [M, 2N] of the slope kernels
+  float* gu;        // gated: the projections [M, 2N] are written there, or NULL; slope: read
+  long long lda, ldb, ldc;  // elements between rows
+  int M, N, K;
+  int act;
+  int grid_m, grid_n;
+};
+
+enum { ACT_SILU = 0, ACT_GELU_TANH = 1 };
+enum { EPI_STORE = 0, EPI_GATED = 1, EPI_SLOPE = 2 };
+
+// A matrix product in bfloat16 or float32 (k_outer_*: the operand's rows are k); epi as above.
+hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
+// MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
+hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
+hipError_t launch_mxfp4_quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales,
+                                 hipStream_t stream);
+hipError_t launch_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int rows, int k, void* out,
+                                   long long ldo, hipStream_t stream);
+
+}  // namespace fmoe

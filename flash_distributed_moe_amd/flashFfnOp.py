@@ -1,0 +1,129 @@
+"""The dense gated feed-forward block and MXFP4 weights, beside the sparse layer.
+
+The models whose mixture-of-experts layer `flashMoeOp.FlashMoeBlockWrapper` runs also have dense
+blocks and shared experts of the same form, y = (act(x Wg^T) * (x Wu^T)) Wd^T, on the weight
+layouts of one expert (w13 [2I, H]: gate rows, then up rows; w2 [H, I]). `gated_ffn` is that block,
+differentiable; `FlashGatedFfn` a module of it over the weights of a block it is given.
+
+MXFP4 keeps 32 consecutive values of a row in 16 bytes and a scale byte (the Open Compute
+microscaling format): `quantize_mxfp4`, `dequantize_mxfp4`, `mxfp4_linear` for a product with such
+weights, and `gated_ffn` takes them in place of both weights (no gradients).
+
+There is no fallback: everything runs on the compiled `flashMoeLauncher` extension, on the current
+stream of the tensors' device, and can be captured into a HIP graph. Wrong arguments raise
+RuntimeError. (The reference has none of these operators; its wrapper,
+test/singleGPU/python/flashMoeOp.py:7-38, covers the sparse block only.)
+"""
+import os
+import sys
+from typing import NamedTuple
+
+import torch
+
+_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if _ROOT not in sys.path:
+    sys.path.insert(0, _ROOT)
+try:
+    import flashMoeLauncher
+except ImportError as e:  # no fallback: say how to build it
+    raise ImportError("the flashMoeLauncher extension is not built; run "
+                      "`python -m flash_distributed_moe_amd.build` (%s)" % e)
+
+ACTIVATIONS = {"silu": flashMoeLauncher.ACT_SILU, "gelu_tanh": flashMoeLauncher.ACT_GELU_TANH}
+
+
+class Mxfp4(NamedTuple):
+    """A tensor [..., K] in MXFP4: codes uint8 [..., K/2] (the even value in the low half of its
+    byte) and scales uint8 [..., K/32] (b stands for 2^(b-127), 255 for NaN)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_mxfp4(x):
+    """x [..., K] (float32 or bfloat16, K a multiple of 32) as Mxfp4. Not differentiable."""
+    return Mxfp4(*flashMoeLauncher.mxfp4_quantize(x.detach()))
+
+
+def dequantize_mxfp4(q, dtype=torch.bfloat16):
+    """The values of q, which both dtypes hold exactly."""
+    return flashMoeLauncher.mxfp4_dequantize(q.codes, q.scales, dtype)
+
+
+def mxfp4_linear(x, weight):
+    """x [..., K] (bfloat16, or Mxfp4) times the transpose of weight (Mxfp4 [N, K]): bfloat16 [..., N],
+    summed in float32. Not differentiable."""
+    if isinstance(x, Mxfp4):
+        return flashMoeLauncher.mxfp4_linear(x.codes, x.scales, weight.codes, weight.scales)
+    _refuse_grad(x)
+    return flashMoeLauncher.mxfp4_linear(x, None, weight.codes, weight.scales)
+
+
+def _refuse_grad(x):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("products with MXFP4 weights have no backward pass: detach x or use torch.no_grad()")
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2, activation):
+        y, saved = flashMoeLauncher.ffn_forward(x, w13, w2, None, None, activation, True)
+        ctx.save_for_backward(x, w13, w2, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        # Under create_graph the gradients would be taken for constants by whoever differentiates them again.
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_ffn has no second derivatives (create_graph=True)")
+        x, w13, w2, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*flashMoeLauncher.ffn_backward(x, w13, w2, ctx.activation, dy, saved, need[0], need[1], need[2]), None)
+
+
+def gated_ffn(x, w13, w2, activation="silu"):
+    """(act(x Wg^T) * (x Wu^T)) Wd^T for x [..., H], w13 [2I, H] (gate rows, then up rows) and w2 [H, I].
+
+    float32 or bfloat16 throughout, H and I multiples of 8; or x bfloat16 and both weights Mxfp4,
+    H and I multiples of 32. activation: "silu" or "gelu_tanh". Weights are contiguous; rows of x
+    may lie apart. Gradients (once) for x and row-major weights; a pass that needs them keeps the two
+    projections in float32 and h until its backward pass."""
+    if activation not in ACTIVATIONS:
+        raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
+    act = ACTIVATIONS[activation]
+    if isinstance(w13, Mxfp4) or isinstance(w2, Mxfp4):
+        if not (isinstance(w13, Mxfp4) and isinstance(w2, Mxfp4)):
+            raise RuntimeError("both weights must be MXFP4, or neither")
+        _refuse_grad(x)
+        return flashMoeLauncher.ffn_forward(x, w13.codes, w2.codes, w13.scales, w2.scales, act, False)[0]
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad):
+        return _GatedFfn.apply(x, w13, w2, act)
+    return flashMoeLauncher.ffn_forward(x, w13, w2, None, None, act, False)[0]
+
+
+class FlashGatedFfn(torch.nn.Module):
+    """`gated_ffn` over the weights of a dense block or shared expert: a module with
+    `gate_up_proj.weight` [2I, H] and `down_proj.weight` [H, I]. The parameters stay the block's own.
+    quantize="mxfp4" converts them once, into buffers of this module (the block is not kept)."""
+
+    def __init__(self, block, activation="silu", quantize=None):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
+        if quantize not in (None, "mxfp4"):
+            raise RuntimeError('quantize must be None or "mxfp4"')
+        self.activation, self.quantize = activation, quantize
+        w13, w2 = block.gate_up_proj.weight, block.down_proj.weight
+        if quantize is None:
+            self.w13, self.w2 = w13, w2
+        else:
+            for name, w in (("w13", w13), ("w2", w2)):
+                q = quantize_mxfp4(w)
+                self.register_buffer(name + "_codes", q.codes)
+                self.register_buffer(name + "_scales", q.scales)
+
+    def forward(self, x):
+        if self.quantize is None:
+            return gated_ffn(x, self.w13, self.w2, self.activation)
+        return gated_ffn(x, Mxfp4(self.w13_codes, self.w13_scales), Mxfp4(self.w2_codes, self.w2_scales), self.activation)

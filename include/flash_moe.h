@@ -271,6 +271,66 @@ int flashMoeAbi(int* version, size_t* desc_bytes);
  * returns hipSuccess. */
 int flashMoeSetDenseSmallBatch(FlashMoeLauncher* l, int enable);
 
+/* ---- The dense gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wd^T: the dense layers and
+ * shared experts of the models whose sparse layer is above, on the weight layouts of one of its
+ * experts. No counterpart in the reference, which has the sparse layer only
+ * (test/singleGPU/cpp/moe/reference/refFullMoe.h:9-70). These calls keep no state: everything
+ * they use is in their arguments, so calls on different streams or devices may overlap if they share
+ * no workspace, and a call can be captured into a HIP graph. They enqueue kernels and wait for
+ * nothing. (Entry points from here on: symbol version LIBFLASHMOE_MI355X_0.5, same interface revision.) */
+enum { FLASH_MOE_ACT_SILU = 0, FLASH_MOE_ACT_GELU_TANH = 1 };
+enum { FLASH_MOE_FFN_ROW_MAJOR = 0, FLASH_MOE_FFN_MXFP4 = 1 };
+
+typedef struct FlashMoeFfnDesc {
+  int hidden;       /* H, a multiple of 8 (MXFP4 weights: of 32), at most 2^20 */
+  int intermediate; /* I, likewise, at most 2^19 */
+  int dtype;        /* FLASH_MOE_F32 or FLASH_MOE_BF16: tokens, outputs, gradients, row-major weights */
+  int activation;   /* FLASH_MOE_ACT_*: g / (1 + exp(-g)), or GELU in its tanh form */
+  int weights;      /* FLASH_MOE_FFN_*; MXFP4 (below) takes bfloat16 tokens and has no backward pass */
+  const void* w13;  /* device, [2I,H]: rows 0..I-1 gate proj, I..2I-1 up proj; MXFP4: codes [2I,H/2] */
+  const void* w2;   /* device, [H,I]; MXFP4: codes [H,I/2] */
+  const void* w13_scales; /* MXFP4: device, [2I,H/32] bytes; else unused */
+  const void* w2_scales;  /* MXFP4: device, [H,I/32] bytes; else unused */
+} FlashMoeFfnDesc;
+
+/* Device bytes a batch of `tokens` needs (any result may be NULL): what a forward pass keeps for
+ * the backward pass, and the workspaces of both. Only the description's sizes are read. */
+int flashMoeFfnBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* saved, size_t* forward, size_t* backward);
+
+/* x [tokens, H] rows ldx values apart, y likewise with ldy (whole 16 bytes; at most 2^20 values); y may
+ * be x if its rows lie the same way. Every pointer begins on 16 bytes. saved: NULL, or device memory
+ * that flashMoeFfnBackward is given afterwards. workspace may be NULL when saved is not. 0 tokens: nothing
+ * is enqueued. hipErrorInvalidValue for whatever is wrong with the arguments; nothing is enqueued then. */
+int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx, void* y, long long ldy, int tokens,
+                       void* saved, void* workspace, void* stream);
+
+/* Gradients of the forward pass that filled `saved`, from dy [tokens, H]: dx [tokens, H] rows lddx apart,
+ * dw13 [2I,H], dw2 [H,I]; any of the three may be NULL. They are written, not added to; of 0 tokens the
+ * weights' gradients are zeros. `saved` is left as it is. dx may be dy or x only if dw13 and dw2 are NULL. */
+int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ldx, const void* dy, long long lddy,
+                        int tokens, const void* saved, void* workspace, void* dx, long long lddx, void* dw13, void* dw2,
+                        void* stream);
+
+/* ---- MXFP4, the 4-bit format of the Open Compute microscaling specification: 32 consecutive values of a
+ * row share a scale, a byte b that stands for 2^(b-127) (255: NaN), and a value is 4 bits: a sign and
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. codes [rows, k/2], the even value in the low half of its byte; scales
+ * [rows, k/32]; both without gaps, codes beginning on 16 bytes.
+ * Quantisation takes b - 127 = floor(log2(largest magnitude of the block)) - 2, at least -127, rounds to the
+ * nearest value, ties to the even code, and stops at 6. A block with an infinity or NaN becomes all NaN.
+ * k is a multiple of 32. x and out lie ldx / ldo values apart, whole 16 bytes. */
+enum { FLASH_MOE_MXFP4 = 2 };
+int flashMoeMxfp4Quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales, void* stream);
+int flashMoeMxfp4Dequantize(int dtype, const void* codes, const void* scales, int rows, int k, void* out, long long ldo,
+                            void* stream);
+
+/* y[rows, n] = x W^T in bfloat16, summed in float32, of MXFP4 weights W [n, k]. x: FLASH_MOE_BF16 rows ldx values
+ * apart (x_scales unused), or FLASH_MOE_MXFP4 codes with x_scales (ldx = k). y's rows lie ldy values apart;
+ * where n is a multiple of 8 they begin on 16 bytes. workspace: flashMoeMxfp4LinearBytes of device memory
+ * (0: may be NULL). */
+int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes);
+int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long long ldx, int rows, const void* codes,
+                        const void* scales, int n, int k, void* y, long long ldy, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
