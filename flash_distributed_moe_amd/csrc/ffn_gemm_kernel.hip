@@ -85,6 +85,7 @@ static hipError_t dispatch(bool oa, bool ob, int epi, const GemmArgs& p, hipStre
 }
 
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
+  if (!k_outer_a && !k_outer_b && ffn_skinny_takes(dtype, p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
   return dtype == 1 ? dispatch<KIND_BF16>(k_outer_a, k_outer_b, epi, p, stream)
                     : dispatch<KIND_F32>(k_outer_a, k_outer_b, epi, p, stream);
 }

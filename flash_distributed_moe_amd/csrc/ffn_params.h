@@ -27,6 +27,11 @@ enum { EPI_STORE = 0, EPI_GATED = 1, EPI_SLOPE = 2 };
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
 // MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
+// The same for few rows, where these take the call (A and B with their k inside the rows).
+bool ffn_skinny_takes(int dtype, const GemmArgs& p);
+bool mxfp4_skinny_takes(bool x_mxfp4, const GemmArgs& p);
+hipError_t launch_ffn_skinny(int dtype, bool gated, const GemmArgs& p, hipStream_t stream);
+hipError_t launch_mxfp4_skinny(bool x_mxfp4, bool gated, const GemmArgs& p, hipStream_t stream);
 hipError_t launch_mxfp4_quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales,
                                  hipStream_t stream);
 hipError_t launch_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int rows, int k, void* out,

@@ -205,8 +205,9 @@ static hipError_t launch(Kernel kernel, GemmArgs p, hipStream_t stream) {
 }
 
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream) {
+  if (x_mxfp4 && epi != EPI_STORE) return hipErrorInvalidValue;
+  if (mxfp4_skinny_takes(x_mxfp4, p)) return launch_mxfp4_skinny(x_mxfp4, epi == EPI_GATED, p, stream);
   if (x_mxfp4) {
-    if (epi != EPI_STORE) return hipErrorInvalidValue;
     typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4> S;
     return launch<S>(mxfp4_both_kernel<S>, p, stream);
   }
