@@ -32,26 +32,34 @@ __host__ __device__ constexpr int piece_k(int kind) { return step_k(kind) / 8; }
 
 constexpr unsigned kOutside = 0x80000000u;  // past the end of every descriptor
 
-// The F blocks of 16 rows a wave takes are dealt so that a lane's results are 4F neighbours: row r of
-// block f is row 4F * (r / 4) + 4f + r % 4 of the wave's 16F.
+// The F blocks of 16 rows a wave takes are dealt eight rows at a time: row r of block f is row
+// 8F * (r / 8) + 8f + r % 8 of the wave's 16F. So a lane and the one 16 on have, of one block, eight
+// neighbouring results between them, and of the next block the eight that follow.
 template <int F>
 __device__ __forceinline__ int dealt_row(int f, int r) {
-  return 4 * F * (r >> 2) + 4 * f + (r & 3);
+  return 8 * F * (r >> 3) + 8 * f + (r & 7);
 }
 
 // Rows of the gated kernels' weight tile: a wave's blocks are half gate and half up rows of the same columns.
 template <int F>
 __device__ __forceinline__ int gated_row(int f, int r) {
-  return 4 * (F / 2) * (r >> 2) + 4 * (f % (F / 2)) + (r & 3);
+  return 8 * (F / 2) * (r >> 3) + 8 * (f % (F / 2)) + (r & 7);
 }
 
-// Where a row is one k, a matrix instruction's operand is read transposed (ds_read_b64_tr_b16): 16
-// lanes read four rows' worth of 8-byte pieces, 8 * F bytes apart inside a row. The 16-byte pieces of
-// row k are swapped about by its last two bits so that those sixteen lie in different banks.
+// Where a row is one k, a matrix instruction's operand is read transposed (ds_read_b64_tr_b16): 16 lanes read four
+// rows of two 16-byte pieces F pieces apart, and the next 16 lanes the rows eight further on at the same
+// time. The pieces of row k are swapped about by bits 0, 1 and 3 of k so that these sixteen lie in
+// different banks. (With rows dealt four at a time half of the reads' time were conflicts.)
 template <int F>
 __device__ __forceinline__ int k_row_swap(int k) {
-  const int q = k & 3;
-  return F >= 8 ? q : F == 4 ? (q & 1) | ((q & 2) << 2) : q << 2;
+  const int q = k & 3, g = (k >> 3) & 1;
+  return F >= 8 ? q | g << 2 : F == 4 ? q | g << 3 : (q & 1) | (q & 2) << 1 | g << 3;
+}
+// float32: 4 bytes a lane of every k row, sixteen lanes two runs of 32 bytes, and four rows eight apart at once
+template <int F>
+__device__ __forceinline__ int f32_k_row_swap(int k) {
+  const int g = (k >> 3) & 3;
+  return F >= 4 ? g << 1 : (g & 1) << 1 | (g & 2) << 2;
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, unsigned bytes) {

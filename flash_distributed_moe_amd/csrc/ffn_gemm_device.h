@@ -67,6 +67,7 @@ struct TileLoader {
         const int at = i * THREADS + tid, k = at / LINE;
         int piece = at % LINE;
         if constexpr (KIND == KIND_BF16) piece ^= k_row_swap<F>(k) & (LINE - 1);
+        else piece ^= f32_k_row_swap<F>(k) & (LINE - 1);
         offset[i] = row0 + piece * PK < rows ? static_cast<unsigned>(bytes_of<KIND>(k * ld)) + piece * 16 : kOutside;
       }
     }
@@ -87,11 +88,11 @@ struct TileLoader {
   }
 };
 
-// A wave's F blocks of an operand for one of the stage's two halves (KIND_BF16, KIND_F32, MXFP4: 32, 16, 128 k).
+// A wave's F blocks of an operand for one of the stage's two halves (bfloat16 32 k, MXFP4 128).
 // Lane l holds row l % 16 of each block and the (l / 16)-th quarter of the k, 16 bytes.
 template <int KIND, bool OUTER, int ROWS, int F>
 struct Fragments {
-  static constexpr int LINE_BYTES = ROWS * (KIND == KIND_F32 ? 4 : 2);  // of a k, where a row is one k
+  static constexpr int LINE_BYTES = ROWS * 2;  // of a k, where a row is one k
   i32x4 v[F];
 
   __device__ __forceinline__ void read(const char* tile, int wave_row, int half) {
@@ -100,23 +101,17 @@ struct Fragments {
       const char* at = tile + (wave_row + r) * 128 + (((half * 4 + g) ^ (r & 7)) << 4);
 #pragma unroll
       for (int f = 0; f < F; ++f) v[f] = *(const FFN_LDS i32x4*)(at + f * 2048);
-    } else if constexpr (KIND == KIND_BF16) {
-      const int k = half * 32 + g * 8 + (r >> 2), swap = k_row_swap<F>(r >> 2) & (ROWS / 8 - 1);
+    } else {
+      static_assert(KIND == KIND_BF16, "read transposed");
+      const int k = half * 32 + g * 8 + (r >> 2), swap = k_row_swap<F>(g * 8 + (r >> 2)) & (ROWS / 8 - 1);
       const char* line = tile + k * LINE_BYTES;
 #pragma unroll
       for (int f = 0; f < F; ++f) {
-        const int col = wave_row + 4 * F * (r & 3) + 4 * f;
-        const char* at = line + (((col >> 3) ^ swap) << 4) + (f & 1) * 8;
+        const int col = wave_row + dealt_row<F>(f, (r & 3) * 4);
+        const char* at = line + (((col >> 3) ^ swap) << 4) + (r & 1) * 8;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FFN_LDS s16x4*)(at));
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FFN_LDS s16x4*)(at + 4 * LINE_BYTES));
         v[f] = __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-    } else {
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const char* at = tile + (half * 16 + g * 4) * LINE_BYTES + (wave_row + dealt_row<F>(f, r)) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[f][j] = *(const FFN_LDS int*)(at + j * LINE_BYTES);
       }
     }
   }
@@ -142,37 +137,58 @@ struct Accumulators {
   f32x4 v[S::FM][S::FN];
 };
 
-// Eight (or, float32, four) neighbouring results
-__device__ __forceinline__ void store8(unsigned short* to, const float* f) {
-  *reinterpret_cast<u32x4*>(to) = u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+__device__ __forceinline__ void store8(unsigned short* to, const f32x4& a, const f32x4& b) {
+  *reinterpret_cast<u32x4*>(to) = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
 }
-__device__ __forceinline__ void store4(float* to, const float* f) {
-  *reinterpret_cast<f32x4*>(to) = f32x4{f[0], f[1], f[2], f[3]};
+__device__ __forceinline__ void store4(unsigned short* to, const f32x4& a) {
+  *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
 }
-// `n` (a multiple of 8) results of a row from column col on, as far as the matrix goes; rows of a
-// matrix whose width is no multiple of 8 are written value by value, they do not begin on 16 bytes
+
+// Two blocks' results of a lane, four neighbours each, against those of the lane 16 on or back: afterwards the
+// lane has eight neighbours, of the first block if l / 16 is even and else of the second.
+__device__ __forceinline__ void trade(f32x4& a, f32x4& b) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[i]), __float_as_uint(b[i]), false, false);
+    a[i] = __uint_as_float(v[0]);
+    b[i] = __uint_as_float(v[1]);
+  }
+}
+
+// A lane's results v[COUNT] of one row of C: block f's are columns col + 8 f + 0..3 (col: with the lane's own 4 * (g % 2)).
+// bfloat16 rows of a matrix whose width is no multiple of 8 begin anywhere and are written value by value.
+// Every lane of a wave takes part, `in` says whether its row exists.
 template <int KIND, int COUNT>
-__device__ __forceinline__ void store_row(void* row, int col, int columns, const float* f) {
+__device__ __forceinline__ void store_row(void* row, int col, int columns, bool in, f32x4 (&v)[COUNT]) {
   if constexpr (KIND == KIND_F32) {
 #pragma unroll
-    for (int c = 0; c < COUNT; c += 4)
-      if (col + c < columns) store4(static_cast<float*>(row) + col + c, f + c);
+    for (int f = 0; f < COUNT; ++f)
+      if (in && col + 8 * f < columns) *reinterpret_cast<f32x4*>(static_cast<float*>(row) + col + 8 * f) = v[f];
   } else {
     unsigned short* to = static_cast<unsigned short*>(row) + col;
-    if ((columns & 7) == 0) {
+    if (columns & 7) {
 #pragma unroll
-      for (int c = 0; c < COUNT; c += 8)
-        if (col + c < columns) store8(to + c, f + c);
+      for (int f = 0; f < COUNT; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (in && col + 8 * f + i < columns) to[8 * f + i] = static_cast<unsigned short>(pack_bf16(v[f][i], 0.0f) & 0xFFFF);
+    } else if constexpr (COUNT == 1) {
+      if (in && col < columns) store4(to, v[0]);
     } else {
+      static_assert(COUNT % 2 == 0, "pairs of blocks");
+      const int odd = (threadIdx.x >> 4) & 1;
 #pragma unroll
-      for (int c = 0; c < COUNT; ++c)
-        if (col + c < columns) to[c] = static_cast<unsigned short>(pack_bf16(f[c], 0.0f) & 0xFFFF);
+      for (int f = 0; f < COUNT; f += 2) {
+        trade(v[f], v[f + 1]);
+        const int at = 8 * f + odd * 4;  // the second block's eight begin 4 before this lane's own column of it
+        if (in && col + at < columns) store8(to + at, v[f], v[f + 1]);
+      }
     }
   }
 }
 
-// What becomes of the sums. A lane has, of its rows m of C, 4 FN neighbouring columns; of a gated
-// product the first half of the blocks are gate columns and the others the same up columns.
+// What becomes of the sums. Of a gated product the first half of the blocks are gate columns and the others
+// the same up columns.
 template <class S>
 __device__ __forceinline__ void write_results(const GemmArgs& p, int m0, int n0, Accumulators<S>& acc) {
   constexpr int FN = S::FN, FM = S::FM;
@@ -183,50 +199,47 @@ __device__ __forceinline__ void write_results(const GemmArgs& p, int m0, int n0,
 #pragma unroll
   for (int fm = 0; fm < FM; ++fm) {
     const int m = m0 + wm * FM * 16 + dealt_row<FM>(fm, r);
-    if (m >= p.M) continue;
+    const bool in = m < p.M;
     if constexpr (S::EPI == EPI_STORE) {
-      float f[4 * FN];
-#pragma unroll
-      for (int fn = 0; fn < FN; ++fn)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[4 * fn + i] = acc.v[fm][fn][i];
-      store_row<OUT, 4 * FN>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, n0 + wn * FN * 16 + 4 * FN * g, p.N, f);
+      store_row<OUT, FN>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, n0 + wn * FN * 16 + dealt_row<FN>(0, 4 * g), p.N, in, acc.v[fm]);
     } else if constexpr (S::EPI == EPI_GATED) {
-      const int col = n0 + wn * FN * 8 + 2 * FN * g;
-      float h[2 * FN], gate[2 * FN], up[2 * FN];
+      const int col = n0 + wn * FN * 8 + gated_row<FN>(0, 4 * g);
+      f32x4 h[FN / 2], gate[FN / 2], up[FN / 2];
 #pragma unroll
-      for (int i = 0; i < 2 * FN; ++i) {
-        gate[i] = acc.v[fm][i / 4][i % 4];
-        up[i] = acc.v[fm][FN / 2 + i / 4][i % 4];
-        h[i] = act_of<EXACT>(p.act, gate[i]) * up[i];
+      for (int f = 0; f < FN / 2; ++f) {
+        gate[f] = acc.v[fm][f];
+        up[f] = acc.v[fm][FN / 2 + f];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[f][i] = act_of<EXACT>(p.act, gate[f][i]) * up[f][i];
       }
-      store_row<OUT, 2 * FN>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, col, p.N, h);
+      store_row<OUT, FN / 2>(static_cast<char*>(p.c) + m * p.ldc * OSIZE, col, p.N, in, h);
       if (p.gu != nullptr) {
         float* row = p.gu + m * (2LL * p.N);
-        store_row<KIND_F32, 2 * FN>(row, col, p.N, gate);
-        store_row<KIND_F32, 2 * FN>(row + p.N, col, p.N, up);
+        store_row<KIND_F32, FN / 2>(row, col, p.N, in, gate);
+        store_row<KIND_F32, FN / 2>(row + p.N, col, p.N, in, up);
       }
     } else {
-      const int col = n0 + wn * FN * 16 + 4 * FN * g;
+      const int col = n0 + wn * FN * 16 + dealt_row<FN>(0, 4 * g);
       const float* row = p.gu + m * (2LL * p.N);
-      float dg[4 * FN], du[4 * FN];
+      f32x4 dg[FN], du[FN];
 #pragma unroll
-      for (int c = 0; c < 4 * FN; c += 4) {
-        if (col + c >= p.N) continue;
-        const f32x4 gate = *reinterpret_cast<const f32x4*>(row + col + c);
-        const f32x4 up = *reinterpret_cast<const f32x4*>(row + p.N + col + c);
+      for (int f = 0; f < FN; ++f) {
+        dg[f] = du[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!in || col + 8 * f >= p.N) continue;
+        const f32x4 gate = *reinterpret_cast<const f32x4*>(row + col + 8 * f);
+        const f32x4 up = *reinterpret_cast<const f32x4*>(row + p.N + col + 8 * f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float dh = acc.v[fm][c / 4][i];
+          const float dh = acc.v[fm][f][i];
           float a, slope;
           act_and_slope<EXACT>(p.act, gate[i], a, slope);
-          dg[c + i] = dh * up[i] * slope;
-          du[c + i] = dh * a;
+          dg[f][i] = dh * up[i] * slope;
+          du[f][i] = dh * a;
         }
       }
       char* out = static_cast<char*>(p.c) + m * (2LL * p.N) * OSIZE;
-      store_row<OUT, 4 * FN>(out, col, p.N, dg);
-      store_row<OUT, 4 * FN>(out + static_cast<long long>(p.N) * OSIZE, col, p.N, du);
+      store_row<OUT, FN>(out, col, p.N, in, dg);
+      store_row<OUT, FN>(out + static_cast<long long>(p.N) * OSIZE, col, p.N, in, du);
     }
   }
 }

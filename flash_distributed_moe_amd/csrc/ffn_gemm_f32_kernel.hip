@@ -1,0 +1,188 @@
+// The dense block's matrix products in float32, on the bfloat16 matrix instructions.
+//
+// A float32 is split into three bfloat16 parts by cutting off its mantissa: x = hi + mid + lo exactly (8 bits
+// each). Of the nine products of parts the six largest are summed in float32; the three left out are
+// below 2^-23 of a product. Six instructions at 16 times the rate of the float32 ones: 2.7 times as fast.
+// The parts live in registers only; a tile in LDS is float32, and a wave splits what it reads.
+//
+// Where that does not give the float32 sum, the sum is taken again, one fused multiply-add after another:
+// where it is no finite number (an infinity has no parts), and where it is so small that parts of what it sums
+// were below what bfloat16 has (a value under 2^-103 loses its low part).
+#include "ffn_gemm_device.h"
+
+namespace fmoe {
+
+// Eight values a lane: the (l / 16)-th quarter of a stage's 32 k, of rows l % 16
+template <bool OUTER, int ROWS, int F>
+__device__ __forceinline__ void read_f32(float (&v)[8], const char* tile, int wave_row, int f) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  if constexpr (!OUTER) {
+    const char* row = tile + (wave_row + f * 16 + r) * 128;
+    const f32x4 lo = *(const FFN_LDS f32x4*)(row + (((2 * g) ^ (r & 7)) << 4));
+    const f32x4 hi = *(const FFN_LDS f32x4*)(row + (((2 * g + 1) ^ (r & 7)) << 4));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+  } else {
+    const int col = wave_row + dealt_row<F>(f, r);
+    const char* at = tile + g * 8 * ROWS * 4 + (((col >> 2) ^ f32_k_row_swap<F>(g * 8)) << 4) + (col & 3) * 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *(const FFN_LDS float*)(at + i * ROWS * 4);
+  }
+}
+
+struct Parts {
+  i32x4 hi, mid, lo;  // eight bfloat16 each
+};
+__device__ __forceinline__ Parts split(const float (&v)[8]) {
+  Parts p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i], b = v[2 * i + 1];
+    const float ar = a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u), br = b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+    const float al = ar - __uint_as_float(__float_as_uint(ar) & 0xFFFF0000u), bl = br - __uint_as_float(__float_as_uint(br) & 0xFFFF0000u);
+    // the upper halves of two words
+    p.hi[i] = static_cast<int>(__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u));
+    p.mid[i] = static_cast<int>(__builtin_amdgcn_perm(__float_as_uint(br), __float_as_uint(ar), 0x07060302u));
+    p.lo[i] = static_cast<int>(__builtin_amdgcn_perm(__float_as_uint(bl), __float_as_uint(al), 0x07060302u));
+  }
+  return p;
+}
+
+constexpr float kSmallSum = 2.6469779601696886e-23f;  // 2^-75: weights up to 2^20 times values under 2^-103 sum to less
+
+// C[m, n] by itself
+template <bool OUTER_A, bool OUTER_B>
+__device__ __noinline__ float plain_sum(const float* a, long long lda, const float* b, long long ldb, long long m, long long n, int K) {
+  const float* pa = OUTER_A ? a + m : a + m * lda;
+  const float* pb = OUTER_B ? b + n : b + n * ldb;
+  const long long sa = OUTER_A ? lda : 1, sb = OUTER_B ? ldb : 1;
+  float sum = 0.0f;
+  for (int k = 0; k < K; ++k) sum = fmaf(pa[k * sa], pb[k * sb], sum);
+  return sum;
+}
+
+template <class S>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_gemm_f32_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+  int tile_m, tile_n;
+  tile_of(p, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+
+  TileLoader<KIND_F32, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
+  TileLoader<KIND_F32, S::OUTER_B, S::BN, S::THREADS, S::FN, S::EPI == EPI_GATED> load_b;
+  load_a.init(p.a, p.lda, m0, p.M);
+  load_b.init(p.b, p.ldb, n0, p.N);
+
+  Accumulators<S> acc;
+#pragma unroll
+  for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int steps = (p.K + S::STEP - 1) / S::STEP;
+  auto load = [&](int s) {
+    char* to = lds + (s & 1) * S::STAGE_BYTES;
+    load_a.load(to, s, p.K - s * S::STEP);
+    load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
+  };
+  if (steps > 0) load(0);
+  for (int s = 0; s < steps; ++s) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of stage s have landed ...
+    __syncthreads();                // ... and everybody's; all are done with the other buffer
+    if (s + 1 < steps) load(s + 1);
+    const char* now = lds + (s & 1) * S::STAGE_BYTES;
+    Parts b[S::FN];
+#pragma unroll
+    for (int fn = 0; fn < S::FN; ++fn) {
+      float v[8];
+      read_f32<S::OUTER_B, S::BN, S::FN>(v, now + S::BM * 128, wn * S::FN * 16, fn);
+      b[fn] = split(v);
+    }
+#pragma unroll
+    for (int fm = 0; fm < S::FM; ++fm) {
+      float v[8];
+      read_f32<S::OUTER_A, S::BM, S::FM>(v, now, wm * S::FM * 16, fm);
+      const Parts a = split(v);
+      // the small products first
+      auto add = [&](const i32x4 Parts::*pb, const i32x4 Parts::*pa) {
+#pragma unroll
+        for (int fn = 0; fn < S::FN; ++fn)
+          acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[fn].*pb),
+                                                                  __builtin_bit_cast(bf16x8, a.*pa), acc.v[fm][fn], 0, 0, 0);
+      };
+      add(&Parts::lo, &Parts::hi);
+      add(&Parts::mid, &Parts::mid);
+      add(&Parts::hi, &Parts::lo);
+      add(&Parts::mid, &Parts::hi);
+      add(&Parts::hi, &Parts::mid);
+      add(&Parts::hi, &Parts::hi);
+    }
+  }
+
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+    for (int fn = 0; fn < S::FN; ++fn) {
+      bool again = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = fabsf(acc.v[fm][fn][i]);
+        again |= !(v < __builtin_inff()) || (v < kSmallSum && v != 0.0f);
+      }
+      if (!again) continue;
+      const long long m = m0 + wm * S::FM * 16 + dealt_row<S::FM>(fm, r);
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // (row of B of this result: gated, an up row if the block is one)
+        long long n;
+        bool in;
+        if constexpr (S::EPI == EPI_GATED) {
+          const int col = n0 + wn * S::FN * 8 + gated_row<S::FN>(fn, 4 * g + i);
+          in = col < p.N;
+          n = col + (fn >= S::FN / 2 ? p.N : 0);
+        } else {
+          n = n0 + wn * S::FN * 16 + dealt_row<S::FN>(fn, 4 * g + i);
+          in = n < p.N;
+        }
+        if (in) acc.v[fm][fn][i] = plain_sum<S::OUTER_A, S::OUTER_B>(static_cast<const float*>(p.a), p.lda, static_cast<const float*>(p.b),
+                                                                     p.ldb, m, n, p.K);
+      }
+    }
+  write_results<S>(p, m0, n0, acc);
+}
+
+template <class S>
+static hipError_t launch_f32(GemmArgs p, hipStream_t stream) {
+  p.grid_m = (p.M + S::BM - 1) / S::BM;
+  p.grid_n = (p.N + S::CN - 1) / S::CN;
+  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n;
+  if (blocks == 0) return hipSuccess;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(ffn_gemm_f32_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS), 0, stream, p);
+  return hipGetLastError();
+}
+
+// Large tiles split each value for more products, small ones fill more CUs. Measured on M=1001, N=768 gated, K=2048,
+// 128 x 128 / 128 x 64 / 64 x 64 rows of A and B: 105.9 / 69.6 / 62.5 us; M=N=K=4096 641 / 739 / 830.
+template <bool OA, bool OB, int EPI>
+static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
+  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
+  static const TileCost ways[] = {{128, 128 / PER, 1.65, 1.25}, {128, 64 / PER, 1.06, 0.72}, {64, 64 / PER, 0.65, 0.45}};
+  switch (pick_tile(ways, 3, p.M, p.N)) {
+    case 0: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4>>(p, stream);
+    case 1: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2>>(p, stream);
+    default: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+  }
+}
+
+hipError_t launch_ffn_gemm_f32(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
+  if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick_f32<false, false, EPI_GATED>(p, stream);
+  if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick_f32<false, true, EPI_SLOPE>(p, stream);
+  if (oa) return !ob ? hipErrorInvalidValue : pick_f32<true, true, EPI_STORE>(p, stream);
+  return ob ? pick_f32<false, true, EPI_STORE>(p, stream) : pick_f32<false, false, EPI_STORE>(p, stream);
+}
+
+}  // namespace fmoe

@@ -1,4 +1,4 @@
-// The matrix products of the dense gated feed-forward block, bfloat16 and float32.
+// The matrix products of the dense gated feed-forward block in bfloat16.
 #include "ffn_gemm_device.h"
 
 namespace fmoe {
@@ -23,38 +23,29 @@ __global__ __launch_bounds__(S::THREADS) void ffn_gemm_kernel(GemmArgs p) {
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int steps = (p.K + S::STEP - 1) / S::STEP;
-  if (steps > 0) {
-    load_a.load(lds, 0, p.K);
-    load_b.load(lds + S::BM * 128, 0, p.K);
-  }
+  auto load = [&](int s) {
+    char* to = lds + (s & 1) * S::STAGE_BYTES;
+    load_a.load(to, s, p.K - s * S::STEP);
+    load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
+  };
+  if (steps > 0) load(0);
   for (int s = 0; s < steps; ++s) {
     __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of stage s have landed ...
     __syncthreads();                // ... and everybody's; all are done with the other buffer
-    char* next = lds + ((s + 1) & 1) * S::STAGE_BYTES;
-    if (s + 1 < steps) {
-      load_a.load(next, s + 1, p.K - (s + 1) * S::STEP);
-      load_b.load(next + S::BM * 128, s + 1, p.K - (s + 1) * S::STEP);
-    }
+    if (s + 1 < steps) load(s + 1);
     const char* now = lds + (s & 1) * S::STAGE_BYTES;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      Fragments<S::KIND, S::OUTER_B, S::BN, S::FN> b;
-      Fragments<S::KIND, S::OUTER_A, S::BM, S::FM> a;
+      Fragments<KIND_BF16, S::OUTER_B, S::BN, S::FN> b;
+      Fragments<KIND_BF16, S::OUTER_A, S::BM, S::FM> a;
       b.read(now + S::BM * 128, wn * S::FN * 16, half);
       a.read(now, wm * S::FM * 16, half);
 #pragma unroll
       for (int fm = 0; fm < S::FM; ++fm)
 #pragma unroll
-        for (int fn = 0; fn < S::FN; ++fn) {
-          if constexpr (S::KIND == KIND_BF16) {
-            acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[fn]),
-                                                                    __builtin_bit_cast(bf16x8, a.v[fm]), acc.v[fm][fn], 0, 0, 0);
-          } else {
-            const f32x4 bf = __builtin_bit_cast(f32x4, b.v[fn]), af = __builtin_bit_cast(f32x4, a.v[fm]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[j], af[j], acc.v[fm][fn], 0, 0, 0);
-          }
-        }
+        for (int fn = 0; fn < S::FN; ++fn)
+          acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[fn]),
+                                                                  __builtin_bit_cast(bf16x8, a.v[fm]), acc.v[fm][fn], 0, 0, 0);
     }
   }
   write_results<S>(p, m0, n0, acc);
@@ -71,23 +62,33 @@ static hipError_t launch(GemmArgs p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int KIND, bool OA, bool OB, int EPI>
-static hipError_t pick(GemmArgs p, hipStream_t stream) {
-  return launch<GemmShape<KIND, OA, OB, EPI, 2, 2, 4, 4>>(p, stream);
+// Measured, 256 x 256 (sixteen waves) / 128 x 128 (eight) / 64 x 64 (four) rows of A and B, us: M=8192, N=4096, K=12288
+// 575 / 754 / 1570; M=4096, N=2048, K=6144 124 / 88 / 140; M=333, N=1344, K=736 19.5 / 8.8 / 5.6. (256 x 128 and 128 x 256
+// lie between their neighbours everywhere. 256 x 256 with eight waves takes 627: four waves a SIMD fill each
+// other's waits for LDS and for the barrier; a third stage, which would not fit, or operands read ahead into
+// registers gain nothing beside that. The library's product of that size takes 529.)
+template <bool OA, bool OB, int EPI>
+static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
+  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
+  static const TileCost ways[] = {{256, 256 / PER, 1.45, 1.45}, {128, 128 / PER, 0.53, 0.47}, {64, 64 / PER, 0.27, 0.2}};
+  switch (pick_tile(ways, 3, p.M, p.N)) {
+    case 0: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 4, 4, 4>>(p, stream);
+    case 1: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 2, 2, 4>>(p, stream);
+    default: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+  }
 }
 
-template <int KIND>
-static hipError_t dispatch(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
-  if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick<KIND, false, false, EPI_GATED>(p, stream);
-  if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick<KIND, false, true, EPI_SLOPE>(p, stream);
-  if (oa) return !ob ? hipErrorInvalidValue : pick<KIND, true, true, EPI_STORE>(p, stream);
-  return ob ? pick<KIND, false, true, EPI_STORE>(p, stream) : pick<KIND, false, false, EPI_STORE>(p, stream);
+static hipError_t launch_ffn_gemm_bf16(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
+  if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick<false, false, EPI_GATED>(p, stream);
+  if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick<false, true, EPI_SLOPE>(p, stream);
+  if (oa) return !ob ? hipErrorInvalidValue : pick<true, true, EPI_STORE>(p, stream);
+  return ob ? pick<false, true, EPI_STORE>(p, stream) : pick<false, false, EPI_STORE>(p, stream);
 }
 
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
   if (!k_outer_a && !k_outer_b && ffn_skinny_takes(dtype, p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
-  return dtype == 1 ? dispatch<KIND_BF16>(k_outer_a, k_outer_b, epi, p, stream)
-                    : dispatch<KIND_F32>(k_outer_a, k_outer_b, epi, p, stream);
+  return dtype == 1 ? launch_ffn_gemm_bf16(k_outer_a, k_outer_b, epi, p, stream)
+                    : launch_ffn_gemm_f32(k_outer_a, k_outer_b, epi, p, stream);
 }
 
 }  // namespace fmoe

@@ -20,6 +20,25 @@ struct GemmArgs {
   int grid_m, grid_n;
 };
 
+// A way to tile a product: rows and columns of C a workgroup takes, and what a step of its k loop costs a CU
+// while it has one such workgroup, and for each while it has several (microseconds, measured).
+struct TileCost {
+  int rows, columns;
+  double alone, shared;
+};
+// Which of `count` ways is done first on 256 CUs.
+inline int pick_tile(const TileCost* ways, int count, int M, int N) {
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < count; ++i) {
+    const long long tiles = ((M + ways[i].rows - 1LL) / ways[i].rows) * ((N + ways[i].columns - 1LL) / ways[i].columns);
+    const long long each = (tiles + 255) / 256;  // tiles of the fullest CU
+    const double cost = each == 1 ? ways[i].alone : each * ways[i].shared;
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  return best;
+}
+
 enum { ACT_SILU = 0, ACT_GELU_TANH = 1 };
 enum { EPI_STORE = 0, EPI_GATED = 1, EPI_SLOPE = 2 };
 
@@ -27,6 +46,7 @@ enum { EPI_STORE = 0, EPI_GATED = 1, EPI_SLOPE = 2 };
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
 // MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
+hipError_t launch_ffn_gemm_f32(bool k_outer_a, bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
 // The same for few rows, where these take the call (A and B with their k inside the rows).
 bool ffn_skinny_takes(int dtype, const GemmArgs& p);
 bool mxfp4_skinny_takes(bool x_mxfp4, const GemmArgs& p);

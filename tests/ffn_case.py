@@ -3,6 +3,8 @@
 A bound is a sum over what is rounded on the way to a value, element by element:
   * a float32 sum of K products is off by at most 2 K 2^-24 times the sum of the products' magnitudes;
   * a value stored in bfloat16 is off by at most 2^-8 of itself, one in float32 by 2^-24 (`half`);
+  * below 2^-126 float32 has no more relative precision: its numbers lie 2^-149 apart there, and each product and
+    each stored value may be off by half of that too (`TINY`, taken whole);
   * sigmoid(w) is off by (4 + 4 |w|) 2^-24 of itself with the library's exponential and division
     (float32 layers: one step each for w, exp, 1 + e and the division, and |w| of w's own), and by
     (8 + 8 |w|) 2^-23 with the hardware's (bfloat16 layers).
@@ -10,6 +12,7 @@ A bound is a sum over what is rounded on the way to a value, element by element:
 import torch
 
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+TINY = 2.0 ** -149
 C = (2.0 / torch.pi) ** 0.5
 
 
@@ -35,16 +38,16 @@ def block(x, w13, w2, act, dy=None):
     H, I = W2.shape
     Wg, Wu = W13[:I], W13[I:]
     g, u = X @ Wg.t(), X @ Wu.t()
-    eg, eu = _sum_error(H) * (X.abs() @ Wg.abs().t()), _sum_error(H) * (X.abs() @ Wu.abs().t())
+    eg, eu = (_sum_error(H) * (X.abs() @ w.abs().t()) + H * TINY for w in (Wg, Wu))
     a, slope, w, dw, s = parts(g, act)
     rel = (4 + 4 * w.abs()) * unit
     # a's own error, and g's through the largest slope (1.13 for both activations)
     ea = rel * a.abs() + 1.13 * eg
     h = a * u
     eh = ea * (u.abs() + eu) + a.abs() * eu
-    eh = eh + half * (h.abs() + eh) + 2.0 ** -24 * h.abs()
+    eh = eh + half * (h.abs() + eh) + 2.0 ** -24 * h.abs() + 3 * TINY
     y = h @ W2.t()
-    ey = eh @ W2.abs().t() + _sum_error(I) * ((h.abs() + eh) @ W2.abs().t())
+    ey = eh @ W2.abs().t() + _sum_error(I) * ((h.abs() + eh) @ W2.abs().t()) + I * TINY
     out = {"y": (y, ey + half * (y.abs() + ey))}
     if dy is None:
         return out

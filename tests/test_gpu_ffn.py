@@ -14,7 +14,7 @@ DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 # tokens, hidden, intermediate: one of everything, odd numbers of tokens, sizes on and around the
 # tiles' 64, 128 and 256, k that ends inside a step
 SHAPES = [(1, 8, 8), (3, 64, 32), (16, 256, 128), (17, 72, 40), (33, 520, 264), (64, 128, 512), (65, 1344, 736),
-          (129, 264, 136), (130, 256, 128), (257, 136, 328), (300, 512, 1024)]
+          (129, 264, 136), (130, 256, 128), (257, 136, 328), (300, 512, 1024), (5, 4096, 72), (12, 72, 4104), (27, 2048, 6144)]
 
 
 @pytest.fixture(scope="module")
@@ -53,6 +53,17 @@ def test_forward_and_backward(ops, T, H, I, act, dtype):
     # without gradients the same values come out, and nothing is kept
     y = ops.gated_ffn(x, w13, w2, activation=act)
     assert not y.requires_grad and torch.equal(y, got["y"])
+
+
+# many tiles of the largest size in one product each: gated and slope / both weights' gradients / output and x's gradient
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("T,H,I", [(3841, 72, 3600), (77, 3600, 3904), (3841, 3600, 40)])
+def test_large_tiles(ops, T, H, I, dtype):
+    x, w13, w2, dy = make(T, H, I, DTYPES[dtype], seed=6)
+    want = ffn_case.block(x, w13, w2, "silu", dy)
+    got = run(ops, x, w13, w2, dy, "silu")
+    for name, t in got.items():
+        ffn_case.check(t, *want[name], "%s of T=%d H=%d I=%d" % (name, T, H, I))
 
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
@@ -157,6 +168,22 @@ def test_rows_with_infinities_and_nan_keep_to_themselves(ops, value, dtype):
     rest = [t for t in range(T) if t != 5]
     assert torch.equal(got[rest], clean[rest])
     assert not torch.isfinite(got[5]).any()
+
+
+def test_float32_beyond_what_bfloat16_parts_hold(ops):
+    """Inputs so small that their parts are below bfloat16's range, and infinities of one sign: the sums are
+    float32's all the same."""
+    T, H, I = 130, 64, 64
+    x, w13, w2, dy = make(T, H, I, torch.float32, seed=8)
+    tiny = 2.0 ** -115
+    for scaled in ((x * tiny, w13, w2), (x, w13 * tiny, w2), (x, w13, w2 * tiny)):
+        want = ffn_case.block(*scaled, "silu")["y"]
+        ffn_case.check(ops.gated_ffn(*scaled), *want, "a tiny operand")
+    # positive everything: an infinite token gives infinite outputs, not NaN
+    x, w13, w2 = x.abs(), w13.abs(), w2.abs()
+    x[3, 5] = float("inf")
+    y = ops.gated_ffn(x, w13, w2)
+    assert torch.isposinf(y[3]).all() and torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()
 
 
 def test_large_projections_saturate(ops):
