@@ -6,6 +6,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <hip/hip_runtime.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <limits>
@@ -160,6 +162,55 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> ffn_backward(const at::Tensor& x,
   return {dx, dw13, dw2};
 }
 
+// A gradient of a leaf is accumulated on the stream on which its accumulator was made, by the first graph of it
+// that is still alive. Captured into a HIP graph, a backward pass that finds an accumulator of another
+// stream would make that stream wait inside the capture, and the process ends. So the forward pass that
+// would lead there is refused.
+void check_capture(const at::Tensor& leaf, const char* name) {
+  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!accumulator) return;
+  const auto stream = accumulator->stream();
+  TORCH_CHECK(!stream.has_value() || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().unwrap(), name,
+              " is part of an autograd graph made on another stream that is still alive: drop it before a step is captured");
+}
+
+struct GatedFfn : torch::autograd::Function<GatedFfn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w13,
+                            const at::Tensor& w2, int64_t activation) {
+    auto [y, saved] = ffn_forward(x, w13, w2, c10::nullopt, c10::nullopt, static_cast<int>(activation), true);
+    ctx->save_for_backward({x, w13, w2, saved});
+    ctx->saved_data["activation"] = activation;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    // Under create_graph the gradients would be taken for constants by whoever differentiates them again.
+    TORCH_CHECK(!at::GradMode::is_enabled(), "gated_ffn has no second derivatives (create_graph=True)");
+    const auto kept = ctx->get_saved_variables();
+    auto [dx, dw13, dw2] =
+        ffn_backward(kept[0], kept[1], kept[2], static_cast<int>(ctx->saved_data["activation"].toInt()), grads[0], kept[3],
+                     ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+    return {dx, dw13, dw2, at::Tensor()};
+  }
+};
+
+at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, int activation) {
+  TORCH_CHECK(x.defined() && w13.defined() && w2.defined(), "x or a weight tensor is undefined");
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w13.requires_grad() || w2.requires_grad()))
+    return std::get<0>(ffn_forward(x, w13, w2, c10::nullopt, c10::nullopt, activation, false));
+  if (x.is_cuda()) {
+    const DeviceGuard guard(x.device());
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    check_hip(hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &capturing), "hipStreamIsCapturing");
+    if (capturing != hipStreamCaptureStatusNone) {
+      check_capture(x, "x");
+      check_capture(w13, "w13");
+      check_capture(w2, "w2");
+    }
+  }
+  return GatedFfn::apply(x, w13, w2, static_cast<int64_t>(activation));
+}
+
 std::tuple<at::Tensor, at::Tensor> mxfp4_quantize(const at::Tensor& x) {
   TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 32 == 0, "x must be [..., K], K a multiple of 32");
@@ -244,6 +295,8 @@ void bind_ffn(py::module_& m) {
         py::arg("activation"), py::arg("save"));
   m.def("ffn_backward", &ffn_backward, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("activation"), py::arg("dy"),
         py::arg("saved"), py::arg("want_dx"), py::arg("want_dw13"), py::arg("want_dw2"));
+  m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("activation"),
+        py::call_guard<py::gil_scoped_release>());
   m.def("mxfp4_quantize", &mxfp4_quantize, py::arg("x"));
   m.def("mxfp4_dequantize",
         [](const at::Tensor& codes, const at::Tensor& scales, const py::object& dtype) {

@@ -64,31 +64,14 @@ def _refuse_grad(x):
         raise RuntimeError("products with MXFP4 weights have no backward pass: detach x or use torch.no_grad()")
 
 
-class _GatedFfn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w13, w2, activation):
-        y, saved = flashMoeLauncher.ffn_forward(x, w13, w2, None, None, activation, True)
-        ctx.save_for_backward(x, w13, w2, saved)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        # Under create_graph the gradients would be taken for constants by whoever differentiates them again.
-        if torch.is_grad_enabled():
-            raise RuntimeError("gated_ffn has no second derivatives (create_graph=True)")
-        x, w13, w2, saved = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*flashMoeLauncher.ffn_backward(x, w13, w2, ctx.activation, dy, saved, need[0], need[1], need[2]), None)
-
-
 def gated_ffn(x, w13, w2, activation="silu"):
     """(act(x Wg^T) * (x Wu^T)) Wd^T for x [..., H], w13 [2I, H] (gate rows, then up rows) and w2 [H, I].
 
     float32 or bfloat16 throughout, H and I multiples of 8; or x bfloat16 and both weights Mxfp4,
     H and I multiples of 32. activation: "silu" or "gelu_tanh". Weights are contiguous; rows of x
     may lie apart. Gradients (once) for x and row-major weights; a pass that needs them keeps the two
-    projections in float32 and h until its backward pass."""
+    projections in float32 and h until its backward pass. A step that is captured into a HIP graph wants no
+    eager graph of the same parameters alive: the call raises then."""
     if activation not in ACTIVATIONS:
         raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
     act = ACTIVATIONS[activation]
@@ -97,9 +80,7 @@ def gated_ffn(x, w13, w2, activation="silu"):
             raise RuntimeError("both weights must be MXFP4, or neither")
         _refuse_grad(x)
         return flashMoeLauncher.ffn_forward(x, w13.codes, w2.codes, w13.scales, w2.scales, act, False)[0]
-    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad):
-        return _GatedFfn.apply(x, w13, w2, act)
-    return flashMoeLauncher.ffn_forward(x, w13, w2, None, None, act, False)[0]
+    return flashMoeLauncher.gated_ffn(x, w13, w2, act)
 
 
 class FlashGatedFfn(torch.nn.Module):

@@ -253,6 +253,26 @@ def test_captured_step(ops, T):
                 assert torch.equal(a, want[k]), "replay %d: %s" % (rep, k)
 
 
+def test_capture_beside_a_living_eager_graph_is_refused(ops):
+    """Its leaves' accumulators belong to the eager graph's stream, which a captured backward pass would make wait."""
+    x, w13, w2, dy = make(20, 64, 32, torch.bfloat16)
+    leaves = [t.detach().requires_grad_() for t in (x, w13, w2)]
+    alive = ops.gated_ffn(*leaves)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            ops.gated_ffn(*leaves)
+    # without gradients there is nothing to refuse, and the eager graph still works
+    plain = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(plain), torch.no_grad():
+        y = ops.gated_ffn(*leaves)
+    plain.replay()
+    alive.backward(dy)
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive)
+    ffn_case.check(leaves[1].grad, *ffn_case.block(x, w13, w2, "silu", dy)["dw13"], "dw13")
+
+
 def test_same_bits_every_time(ops):
     x, w13, w2, dy = make(700, 512, 264, torch.bfloat16, seed=9)
     first = run(ops, x, w13, w2, dy, "silu")
