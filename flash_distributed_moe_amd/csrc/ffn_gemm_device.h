@@ -120,9 +120,9 @@ struct Fragments {
 // The workgroup's tile. Neighbouring workgroup numbers lie on different XCDs, each with an L2 of its
 // own, so an XCD gets a run of the order; the order walks GROUP tile rows column by column, so
 // that the tiles in flight on an XCD share rows of both operands.
-__device__ __forceinline__ void tile_of(const GemmArgs& p, int& tile_m, int& tile_n) {
+__device__ __forceinline__ void tile_of(const GemmArgs& p, int id, int& tile_m, int& tile_n) {
   constexpr int XCDS = 8, GROUP = 8;
-  const int count = p.grid_m * p.grid_n, id = blockIdx.x;
+  const int count = p.grid_m * p.grid_n;
   const int xcd = id % XCDS, each = count / XCDS, extra = count % XCDS;
   const int at = xcd * each + (xcd < extra ? xcd : extra) + id / XCDS;
   const int first = at / (GROUP * p.grid_n) * GROUP;

@@ -61,11 +61,11 @@ __device__ __noinline__ float plain_sum(const float* a, long long lda, const flo
   return sum;
 }
 
+// Tile `id` of a product, by a workgroup with 2 * S::STAGE_BYTES of LDS
 template <class S>
-__global__ __launch_bounds__(S::THREADS, 2) void ffn_gemm_f32_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+__device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int id) {
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
 
@@ -155,6 +155,29 @@ __global__ __launch_bounds__(S::THREADS, 2) void ffn_gemm_f32_kernel(GemmArgs p)
 }
 
 template <class S>
+__global__ __launch_bounds__(S::THREADS, 2) void ffn_gemm_f32_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+  gemm_tile_f32<S>(p, lds, blockIdx.x);
+}
+
+// As ffn_grads_kernel
+template <int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ffn_grads_f32_kernel(FfnGrads p) {
+  typedef GemmShape<KIND_F32, false, true, EPI_STORE, WM, WN, FM, FN> X;
+  typedef GemmShape<KIND_F32, true, true, EPI_STORE, WM, WN, FM, FN> W;
+  __shared__ __attribute__((aligned(128))) char lds[2 * X::STAGE_BYTES];
+  const int id = blockIdx.x;
+  if (id < p.begin[1]) {
+    if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile_f32<X>(p.dx, lds, id);
+  } else {
+    const bool second = id >= p.begin[2];
+    const GemmArgs& dw = second ? p.dw2 : p.dw13;
+    const int at = id - p.begin[second ? 2 : 1];
+    if (at < dw.grid_m * dw.grid_n) gemm_tile_f32<W>(dw, lds, at);
+  }
+}
+
+template <class S>
 static hipError_t launch_f32(GemmArgs p, hipStream_t stream) {
   p.grid_m = (p.M + S::BM - 1) / S::BM;
   p.grid_n = (p.N + S::CN - 1) / S::CN;
@@ -181,8 +204,20 @@ static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
 hipError_t launch_ffn_gemm_f32(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
   if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick_f32<false, false, EPI_GATED>(p, stream);
   if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick_f32<false, true, EPI_SLOPE>(p, stream);
-  if (oa) return !ob ? hipErrorInvalidValue : pick_f32<true, true, EPI_STORE>(p, stream);
-  return ob ? pick_f32<false, true, EPI_STORE>(p, stream) : pick_f32<false, false, EPI_STORE>(p, stream);
+  return oa || ob ? hipErrorInvalidValue : pick_f32<false, false, EPI_STORE>(p, stream);
+}
+
+hipError_t launch_ffn_grads_f32(FfnGrads p, hipStream_t stream) {
+  static const TileCost ways[] = {{128, 128, 1.65, 1.25}, {128, 64, 1.06, 0.72}, {64, 64, 0.65, 0.45}};
+  const int way = pick_grads_tile(ways, 3, 32, p);
+  const long long blocks = lay_out_grads(p, ways[way].rows, ways[way].columns);
+  if (blocks == 0) return hipSuccess;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (way == 0) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 4>), grid, dim3(256), 0, stream, p);
+  else if (way == 1) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 2>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 2, 2>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
 }
 
 }  // namespace fmoe

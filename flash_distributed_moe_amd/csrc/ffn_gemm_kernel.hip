@@ -3,11 +3,11 @@
 
 namespace fmoe {
 
+// Tile `id` of a product, by a workgroup with 2 * S::STAGE_BYTES of LDS
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void ffn_gemm_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+__device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) {
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
 
@@ -52,6 +52,31 @@ __global__ __launch_bounds__(S::THREADS) void ffn_gemm_kernel(GemmArgs p) {
 }
 
 template <class S>
+__global__ __launch_bounds__(S::THREADS) void ffn_gemm_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+  gemm_tile<S>(p, lds, blockIdx.x);
+}
+
+// The gradients of x (a product with its weights' rows as k) and of both weights (sums over the tokens) in one
+// launch: none waits for another, and the CUs that the last tiles of one leave empty take the next one's.
+// The longest sums first.
+template <int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM * WN * 64) void ffn_grads_kernel(FfnGrads p) {
+  typedef GemmShape<KIND_BF16, false, true, EPI_STORE, WM, WN, FM, FN> X;
+  typedef GemmShape<KIND_BF16, true, true, EPI_STORE, WM, WN, FM, FN> W;
+  __shared__ __attribute__((aligned(128))) char lds[2 * X::STAGE_BYTES];
+  const int id = blockIdx.x;
+  if (id < p.begin[1]) {
+    if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile<X>(p.dx, lds, id);
+  } else {
+    const bool second = id >= p.begin[2];
+    const GemmArgs& dw = second ? p.dw2 : p.dw13;
+    const int at = id - p.begin[second ? 2 : 1];
+    if (at < dw.grid_m * dw.grid_n) gemm_tile<W>(dw, lds, at);
+  }
+}
+
+template <class S>
 static hipError_t launch(GemmArgs p, hipStream_t stream) {
   p.grid_m = (p.M + S::BM - 1) / S::BM;
   p.grid_n = (p.N + S::CN - 1) / S::CN;
@@ -78,17 +103,33 @@ static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
   }
 }
 
+hipError_t launch_ffn_grads_bf16(FfnGrads p, hipStream_t stream) {
+  static const TileCost ways[] = {{256, 256, 1.55, 1.55}, {128, 128, 0.6, 0.49}, {64, 64, 0.3, 0.22}};
+  const int way = pick_grads_tile(ways, 3, 64, p), side = ways[way].rows;
+  const long long blocks = lay_out_grads(p, side, side);
+  if (blocks == 0) return hipSuccess;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (way == 0) hipLaunchKernelGGL((ffn_grads_kernel<4, 4, 4, 4>), grid, dim3(1024), 0, stream, p);
+  else if (way == 1) hipLaunchKernelGGL((ffn_grads_kernel<4, 2, 2, 4>), grid, dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((ffn_grads_kernel<2, 2, 2, 2>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
 static hipError_t launch_ffn_gemm_bf16(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
   if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick<false, false, EPI_GATED>(p, stream);
   if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick<false, true, EPI_SLOPE>(p, stream);
-  if (oa) return !ob ? hipErrorInvalidValue : pick<true, true, EPI_STORE>(p, stream);
-  return ob ? pick<false, true, EPI_STORE>(p, stream) : pick<false, false, EPI_STORE>(p, stream);
+  return oa || ob ? hipErrorInvalidValue : pick<false, false, EPI_STORE>(p, stream);
 }
 
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
   if (!k_outer_a && !k_outer_b && ffn_skinny_takes(dtype, p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
   return dtype == 1 ? launch_ffn_gemm_bf16(k_outer_a, k_outer_b, epi, p, stream)
                     : launch_ffn_gemm_f32(k_outer_a, k_outer_b, epi, p, stream);
+}
+
+hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, hipStream_t stream) {
+  return dtype == 1 ? launch_ffn_grads_bf16(p, stream) : launch_ffn_grads_f32(p, stream);
 }
 
 }  // namespace fmoe

@@ -162,28 +162,27 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
     p.M = tokens, p.N = I, p.K = H, p.act = d.activation;
     FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_SLOPE, p, stream));
   }
+  // the weights' gradients sum over the tokens; of no tokens they are zeros
+  fmoe::FfnGrads grads{};
   if (tokens > 0 && dx != nullptr) {
-    GemmArgs p{};
+    GemmArgs& p = grads.dx;
     p.a = workspace, p.b = d.w13, p.c = dx;
     p.lda = 2LL * I, p.ldb = H, p.ldc = lddx;
     p.M = tokens, p.N = H, p.K = 2 * I;
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_STORE, p, stream));
   }
-  // the weights' gradients sum over the tokens; of no tokens they are zeros
   if (dw13 != nullptr) {
-    GemmArgs p{};
+    GemmArgs& p = grads.dw13;
     p.a = workspace, p.b = x, p.c = dw13;
     p.lda = 2LL * I, p.ldb = ldx, p.ldc = H;
     p.M = 2 * I, p.N = H, p.K = tokens;
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, true, fmoe::EPI_STORE, p, stream));
   }
   if (dw2 != nullptr) {
-    GemmArgs p{};
+    GemmArgs& p = grads.dw2;
     p.a = dy, p.b = keep + (tokens > 0 ? gu_bytes(d, tokens) : 0), p.c = dw2;
     p.lda = lddy, p.ldb = I, p.ldc = I;
     p.M = H, p.N = I, p.K = tokens;
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, true, fmoe::EPI_STORE, p, stream));
   }
+  FMOE_HIP_CHECK(fmoe::launch_ffn_grads(d.dtype, grads, stream));
   return hipSuccess;
 }
 

@@ -42,10 +42,54 @@ inline int pick_tile(const TileCost* ways, int count, int M, int N) {
 enum { ACT_SILU = 0, ACT_GELU_TANH = 1 };
 enum { EPI_STORE = 0, EPI_GATED = 1, EPI_SLOPE = 2 };
 
+// The three products of a backward pass that depend on no other of them; one that is not wanted has no rows
+// (M = 0). begin: the first workgroup of each.
+struct FfnGrads {
+  GemmArgs dx, dw13, dw2;
+  int begin[3];
+};
+
+// Workgroup ranges for tiles of rows x columns, each begun on a multiple of 8 (see tile_of); their number.
+inline long long lay_out_grads(FfnGrads& p, int rows, int columns) {
+  GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
+  long long at = 0;
+  for (int i = 0; i < 3; ++i) {
+    of[i]->grid_m = (of[i]->M + rows - 1) / rows;
+    of[i]->grid_n = (of[i]->N + columns - 1) / columns;
+    p.begin[i] = static_cast<int>(at < 0x7FFFFFFF ? at : 0x7FFFFFFF);
+    at = (at + static_cast<long long>(of[i]->grid_m) * of[i]->grid_n + 7) / 8 * 8;
+  }
+  return at;
+}
+
+// Which of `count` ways is done with all three first on 256 CUs, which take tiles as they come: the work
+// spread over all of them and, as the ends never meet, half of the shortest tile; or the longest tile alone.
+inline int pick_grads_tile(const TileCost* ways, int count, int step, const FfnGrads& p) {
+  const GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < count; ++i) {
+    double work = 0, longest = 0, shortest = 0;
+    for (const GemmArgs* g : of) {
+      const double tiles = static_cast<double>((g->M + ways[i].rows - 1LL) / ways[i].rows) * ((g->N + ways[i].columns - 1LL) / ways[i].columns);
+      if (tiles == 0) continue;
+      const double steps = (g->K + step - 1) / step;
+      work += tiles * steps * ways[i].shared / 256;
+      longest = longest > steps * ways[i].alone ? longest : steps * ways[i].alone;
+      shortest = shortest == 0 || steps * ways[i].shared < shortest ? steps * ways[i].shared : shortest;
+    }
+    const double cost = work + shortest / 2 > longest ? work + shortest / 2 : longest;
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  return best;
+}
+
 // A matrix product in bfloat16 or float32 (k_outer_*: the operand's rows are k); epi as above.
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
 // MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
+hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, hipStream_t stream);
+hipError_t launch_ffn_grads_f32(FfnGrads p, hipStream_t stream);
 hipError_t launch_ffn_gemm_f32(bool k_outer_a, bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
 // The same for few rows, where these take the call (A and B with their k inside the rows).
 bool ffn_skinny_takes(int dtype, const GemmArgs& p);

@@ -16,7 +16,7 @@ template <class S>
 __global__ __launch_bounds__(S::THREADS) void mxfp4_both_kernel(GemmArgs p) {
   __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(S::THREADS) void mxfp4_weights_kernel(GemmArgs p) {
   __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
   static_assert(S::FN % 4 == 0, "pairs of blocks on one side");
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(S::THREADS) void mxfp4_both_tiled_kernel(GemmArgs p
   constexpr int TILES = S::STAGE_BYTES, STAGE = TILES + ScaleA::BYTES + ScaleB::BYTES;
   __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(S::THREADS) void mxfp4_weights_tiled_kernel(GemmArg
   static_assert(S::FN % 4 == 0, "pairs of blocks on one side");
   __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
   int tile_m, tile_n;
-  tile_of(p, tile_m, tile_n);
+  tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
