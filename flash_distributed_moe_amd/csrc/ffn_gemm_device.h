@@ -8,17 +8,19 @@
 
 namespace fmoe {
 
-template <int KIND_, bool OUTER_A_, bool OUTER_B_, int EPI_, int WM_, int WN_, int FM_, int FN_>
+// GROUPS such sets of waves share a tile's steps of k, each with LDS of its own, and add up their sums in the end.
+template <int KIND_, bool OUTER_A_, bool OUTER_B_, int EPI_, int WM_, int WN_, int FM_, int FN_, int GROUPS_ = 1>
 struct GemmShape {
   static constexpr int KIND = KIND_;
   static constexpr bool OUTER_A = OUTER_A_, OUTER_B = OUTER_B_;
-  static constexpr int EPI = EPI_, WM = WM_, WN = WN_, FM = FM_, FN = FN_;
+  static constexpr int EPI = EPI_, WM = WM_, WN = WN_, FM = FM_, FN = FN_, GROUPS = GROUPS_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int BM = WM * FM * 16, BN = WN * FN * 16;     // rows of the two tiles
   static constexpr int CN = EPI == EPI_GATED ? BN / 2 : BN;      // columns of C a workgroup writes
   static constexpr int STEP = step_k(KIND);
   static constexpr int ESIZE = KIND == KIND_F32 ? 4 : 2;         // bytes a value (MXFP4: see bytes_of)
   static constexpr int STAGE_BYTES = (BM + BN) * 128;
+  static constexpr int LDS_BYTES = 2 * GROUPS * STAGE_BYTES;
 };
 
 template <int KIND>
@@ -38,16 +40,17 @@ struct TileLoader {
   unsigned offset[PIECES];
   const char* base;
   long long step_bytes, up_bytes;
+  int tid;  // of the THREADS that load
 
   // k of this lane's piece i inside a stage (the first of its values)
-  __device__ __forceinline__ static int k_of(int i) {
-    const int at = i * THREADS + threadIdx.x;
+  __device__ __forceinline__ int k_of(int i) const {
+    const int at = i * THREADS + tid;
     return OUTER ? at / LINE : ((at & 7) ^ ((at >> 3) & 7)) * PK;
   }
 
   // row0: the tile's first row (gated: its first column of C) of `rows`
-  __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows) {
-    const int tid = threadIdx.x;
+  __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows, int tid_) {
+    tid = tid_;
     up_bytes = GATED ? bytes_of<KIND>(rows * ld) : 0;
     if constexpr (!OUTER) {
       base = static_cast<const char*>(p) + bytes_of<KIND>(row0 * ld);
@@ -75,7 +78,7 @@ struct TileLoader {
 
   // Stage s into `lds`; left: how many k there are from its first one on
   __device__ __forceinline__ void load(char* lds, int s, int left) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const char* from = base + s * step_bytes;
     char* to = lds + wave * 1024;
 #pragma unroll
@@ -142,6 +145,32 @@ __device__ __forceinline__ void store8(unsigned short* to, const f32x4& a, const
 }
 __device__ __forceinline__ void store4(unsigned short* to, const f32x4& a) {
   *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
+}
+
+// The groups' sums of a tile, into the first group's, in the groups' order. Of the others nobody is left to write results.
+template <class S, int ROOM = S::LDS_BYTES>
+__device__ __forceinline__ void add_groups(char* lds, int group, Accumulators<S>& acc) {
+  if constexpr (S::GROUPS > 1) {
+    f32x4* part = reinterpret_cast<f32x4*>(lds);
+    const int tid = threadIdx.x % S::THREADS;
+    static_assert((S::GROUPS - 1) * S::BM * S::BN * 4 <= ROOM, "room for the others' sums");
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+        for (int fn = 0; fn < S::FN; ++fn) part[(((group - 1) * S::FM + fm) * S::FN + fn) * S::THREADS + tid] = acc.v[fm][fn];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int other = 1; other < S::GROUPS; ++other)
+#pragma unroll
+        for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+          for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] += part[(((other - 1) * S::FM + fm) * S::FN + fn) * S::THREADS + tid];
+    }
+  }
 }
 
 // Two blocks' results of a lane, four neighbours each, against those of the lane 16 on or back: afterwards the

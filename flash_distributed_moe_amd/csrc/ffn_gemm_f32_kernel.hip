@@ -61,18 +61,20 @@ __device__ __noinline__ float plain_sum(const float* a, long long lda, const flo
   return sum;
 }
 
-// Tile `id` of a product, by a workgroup with 2 * S::STAGE_BYTES of LDS
+// Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
 template <class S>
 __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int id) {
   int tile_m, tile_n;
   tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  char* mine = lds + group * 2 * S::STAGE_BYTES;
 
   TileLoader<KIND_F32, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
   TileLoader<KIND_F32, S::OUTER_B, S::BN, S::THREADS, S::FN, S::EPI == EPI_GATED> load_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
+  load_a.init(p.a, p.lda, m0, p.M, tid);
+  load_b.init(p.b, p.ldb, n0, p.N, tid);
 
   Accumulators<S> acc;
 #pragma unroll
@@ -81,17 +83,22 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int steps = (p.K + S::STEP - 1) / S::STEP;
-  auto load = [&](int s) {
-    char* to = lds + (s & 1) * S::STAGE_BYTES;
+  // a group's turns: stages group, group + GROUPS, ...
+  const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  auto load = [&](int turn) {
+    const int s = turn * S::GROUPS + group;
+    if (S::GROUPS > 1 && s >= steps) return;
+    char* to = mine + (turn & 1) * S::STAGE_BYTES;
     load_a.load(to, s, p.K - s * S::STEP);
     load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
   };
-  if (steps > 0) load(0);
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of stage s have landed ...
+  if (turns > 0) load(0);
+  for (int turn = 0; turn < turns; ++turn) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of the stage have landed ...
     __syncthreads();                // ... and everybody's; all are done with the other buffer
-    if (s + 1 < steps) load(s + 1);
-    const char* now = lds + (s & 1) * S::STAGE_BYTES;
+    if (turn + 1 < turns) load(turn + 1);
+    if (S::GROUPS > 1 && turn * S::GROUPS + group >= steps) continue;
+    const char* now = mine + (turn & 1) * S::STAGE_BYTES;
     Parts b[S::FN];
 #pragma unroll
     for (int fn = 0; fn < S::FN; ++fn) {
@@ -120,6 +127,8 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
     }
   }
 
+  add_groups<S>(lds, group, acc);
+  if (group != 0) return;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int fm = 0; fm < S::FM; ++fm)
@@ -155,8 +164,8 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
 }
 
 template <class S>
-__global__ __launch_bounds__(S::THREADS, 2) void ffn_gemm_f32_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+__global__ __launch_bounds__(S::THREADS * S::GROUPS, 2) void ffn_gemm_f32_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(128))) char lds[S::LDS_BYTES];
   gemm_tile_f32<S>(p, lds, blockIdx.x);
 }
 
@@ -165,7 +174,7 @@ template <int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ffn_grads_f32_kernel(FfnGrads p) {
   typedef GemmShape<KIND_F32, false, true, EPI_STORE, WM, WN, FM, FN> X;
   typedef GemmShape<KIND_F32, true, true, EPI_STORE, WM, WN, FM, FN> W;
-  __shared__ __attribute__((aligned(128))) char lds[2 * X::STAGE_BYTES];
+  __shared__ __attribute__((aligned(128))) char lds[X::LDS_BYTES];
   const int id = blockIdx.x;
   if (id < p.begin[1]) {
     if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile_f32<X>(p.dx, lds, id);
@@ -184,20 +193,29 @@ static hipError_t launch_f32(GemmArgs p, hipStream_t stream) {
   const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n;
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(ffn_gemm_f32_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS), 0, stream, p);
+  hipLaunchKernelGGL(ffn_gemm_f32_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
   return hipGetLastError();
 }
 
-// Large tiles split each value for more products, small ones fill more CUs. Measured on M=1001, N=768 gated, K=2048,
-// 128 x 128 / 128 x 64 / 64 x 64 rows of A and B: 105.9 / 69.6 / 62.5 us; M=N=K=4096 641 / 739 / 830.
+// Large tiles split each value for more products, small ones fill more CUs, and groups of waves that share a tile's k fill
+// their waits. Measured on M=1001, N=768 gated, K=2048, 128 x 128 / 128 x 64 / 64 x 64 rows of A and B, us:
+// 114 / 76 / 65 in one group, 87 / 57 / 57 in two, 64 x 64 in four 64; M=1001, N=768, K=2048 with B's rows as k
+// 120 / 84 / 55, 97 / 60 / 38, 34; M=N=K=4096 641 / 739 / 830 in one.
 template <bool OA, bool OB, int EPI>
 static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
   constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  static const TileCost ways[] = {{128, 128 / PER, 1.65, 1.25}, {128, 64 / PER, 1.06, 0.72}, {64, 64 / PER, 0.65, 0.45}};
-  switch (pick_tile(ways, 3, p.M, p.N)) {
+  static const TileCost ways[] = {{128, 128 / PER, 0, 1.7, 2.5, 1.25}, {128, 128 / PER, 1, 1.32, 2.7, 1.35},
+                                  {128, 64 / PER, 0, 1.1, 1.6, 0.72},  {128, 64 / PER, 0.8, 0.86, 1.8, 0.9},
+                                  {64, 64 / PER, 0, 0.78, 0.98, 0.42}, {64, 64 / PER, 0.8, 0.54, 0.85, 0.45},
+                                  {64, 64 / PER, 1.8, 0.48, 0.95, 0.48}};
+  switch (pick_tile(ways, 7, 32, p)) {
     case 0: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4>>(p, stream);
-    case 1: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2>>(p, stream);
-    default: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+    case 1: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4, 2>>(p, stream);
+    case 2: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2>>(p, stream);
+    case 3: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2, 2>>(p, stream);
+    case 4: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+    case 5: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
+    default: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 4>>(p, stream);
   }
 }
 
@@ -208,7 +226,7 @@ hipError_t launch_ffn_gemm_f32(bool oa, bool ob, int epi, const GemmArgs& p, hip
 }
 
 hipError_t launch_ffn_grads_f32(FfnGrads p, hipStream_t stream) {
-  static const TileCost ways[] = {{128, 128, 1.65, 1.25}, {128, 64, 1.06, 0.72}, {64, 64, 0.65, 0.45}};
+  static const TileCost ways[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 64, 0, 1.1, 1.6, 0.72}, {64, 64, 0, 0.78, 0.98, 0.45}};
   const int way = pick_grads_tile(ways, 3, 32, p);
   const long long blocks = lay_out_grads(p, ways[way].rows, ways[way].columns);
   if (blocks == 0) return hipSuccess;

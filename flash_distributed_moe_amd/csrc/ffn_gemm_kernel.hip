@@ -3,18 +3,20 @@
 
 namespace fmoe {
 
-// Tile `id` of a product, by a workgroup with 2 * S::STAGE_BYTES of LDS
+// Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
 template <class S>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) {
   int tile_m, tile_n;
   tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  char* mine = lds + group * 2 * S::STAGE_BYTES;
 
   TileLoader<S::KIND, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
   TileLoader<S::KIND, S::OUTER_B, S::BN, S::THREADS, S::FN, S::EPI == EPI_GATED> load_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
+  load_a.init(p.a, p.lda, m0, p.M, tid);
+  load_b.init(p.b, p.ldb, n0, p.N, tid);
 
   Accumulators<S> acc;
 #pragma unroll
@@ -23,17 +25,22 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) 
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int steps = (p.K + S::STEP - 1) / S::STEP;
-  auto load = [&](int s) {
-    char* to = lds + (s & 1) * S::STAGE_BYTES;
+  // a group's turns: stages group, group + GROUPS, ...
+  const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  auto load = [&](int turn) {
+    const int s = turn * S::GROUPS + group;
+    if (S::GROUPS > 1 && s >= steps) return;
+    char* to = mine + (turn & 1) * S::STAGE_BYTES;
     load_a.load(to, s, p.K - s * S::STEP);
     load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
   };
-  if (steps > 0) load(0);
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of stage s have landed ...
+  if (turns > 0) load(0);
+  for (int turn = 0; turn < turns; ++turn) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of the stage have landed ...
     __syncthreads();                // ... and everybody's; all are done with the other buffer
-    if (s + 1 < steps) load(s + 1);
-    const char* now = lds + (s & 1) * S::STAGE_BYTES;
+    if (turn + 1 < turns) load(turn + 1);
+    if (S::GROUPS > 1 && turn * S::GROUPS + group >= steps) continue;
+    const char* now = mine + (turn & 1) * S::STAGE_BYTES;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       Fragments<KIND_BF16, S::OUTER_B, S::BN, S::FN> b;
@@ -48,12 +55,13 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) 
                                                                   __builtin_bit_cast(bf16x8, a.v[fm]), acc.v[fm][fn], 0, 0, 0);
     }
   }
-  write_results<S>(p, m0, n0, acc);
+  add_groups<S>(lds, group, acc);
+  if (group == 0) write_results<S>(p, m0, n0, acc);
 }
 
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void ffn_gemm_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
+__global__ __launch_bounds__(S::THREADS * S::GROUPS) void ffn_gemm_kernel(GemmArgs p) {
+  __shared__ __attribute__((aligned(128))) char lds[S::LDS_BYTES];
   gemm_tile<S>(p, lds, blockIdx.x);
 }
 
@@ -64,7 +72,7 @@ template <int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM * WN * 64) void ffn_grads_kernel(FfnGrads p) {
   typedef GemmShape<KIND_BF16, false, true, EPI_STORE, WM, WN, FM, FN> X;
   typedef GemmShape<KIND_BF16, true, true, EPI_STORE, WM, WN, FM, FN> W;
-  __shared__ __attribute__((aligned(128))) char lds[2 * X::STAGE_BYTES];
+  __shared__ __attribute__((aligned(128))) char lds[X::LDS_BYTES];
   const int id = blockIdx.x;
   if (id < p.begin[1]) {
     if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile<X>(p.dx, lds, id);
@@ -83,7 +91,7 @@ static hipError_t launch(GemmArgs p, hipStream_t stream) {
   const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n;
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(ffn_gemm_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS), 0, stream, p);
+  hipLaunchKernelGGL(ffn_gemm_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -92,19 +100,26 @@ static hipError_t launch(GemmArgs p, hipStream_t stream) {
 // lie between their neighbours everywhere. 256 x 256 with eight waves takes 627: four waves a SIMD fill each
 // other's waits for LDS and for the barrier; a third stage, which would not fit, or operands read ahead into
 // registers gain nothing beside that. The library's product of that size takes 529.)
+// Where CUs have one small tile or two, groups of waves share its k, 1 / 2 / 4 groups: M=64, N=2048, K=6144 28.2 / 20.9 / 17.9;
+// M=1024 50.1 / 38.2 / 53.1; M=333, N=1344, K=736 6.0 / 5.5 / 5.8; 128 x 128 in 1 / 2: M=1024, N=2048, K=6144 65.1 / 52.2.
 template <bool OA, bool OB, int EPI>
 static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
   constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  static const TileCost ways[] = {{256, 256 / PER, 1.45, 1.45}, {128, 128 / PER, 0.53, 0.47}, {64, 64 / PER, 0.27, 0.2}};
-  switch (pick_tile(ways, 3, p.M, p.N)) {
+  static const TileCost ways[] = {{256, 256 / PER, 0, 1.45, 2.9, 1.45}, {128, 128 / PER, 0, 0.55, 0.96, 0.48},
+                                  {128, 128 / PER, 0.8, 0.45, 1.0, 0.55}, {64, 64 / PER, 0, 0.33, 0.5, 0.21},
+                                  {64, 64 / PER, 0.8, 0.25, 0.37, 0.245}, {64, 64 / PER, 1.8, 0.2, 0.53, 0.27}};
+  switch (pick_tile(ways, 6, 64, p)) {
     case 0: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 4, 4, 4>>(p, stream);
     case 1: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 2, 2, 4>>(p, stream);
-    default: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+    case 2: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 2, 2, 4, 2>>(p, stream);
+    case 3: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+    case 4: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
+    default: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2, 4>>(p, stream);
   }
 }
 
 hipError_t launch_ffn_grads_bf16(FfnGrads p, hipStream_t stream) {
-  static const TileCost ways[] = {{256, 256, 1.55, 1.55}, {128, 128, 0.6, 0.49}, {64, 64, 0.3, 0.22}};
+  static const TileCost ways[] = {{256, 256, 0, 1.55, 3.1, 1.55}, {128, 128, 0, 0.6, 0.98, 0.49}, {64, 64, 0, 0.33, 0.5, 0.22}};
   const int way = pick_grads_tile(ways, 3, 64, p), side = ways[way].rows;
   const long long blocks = lay_out_grads(p, side, side);
   if (blocks == 0) return hipSuccess;

@@ -20,20 +20,23 @@ struct GemmArgs {
   int grid_m, grid_n;
 };
 
-// A way to tile a product: rows and columns of C a workgroup takes, and what a step of its k loop costs a CU
-// while it has one such workgroup, and for each while it has several (microseconds, measured).
+// A way to tile a product: rows and columns of C a workgroup takes, and what it costs a CU in microseconds, measured:
+// once, and for a step of the k loop while the CU has one such workgroup, two, and for each while it has more.
 struct TileCost {
   int rows, columns;
-  double alone, shared;
+  double once, one, two, more;
 };
-// Which of `count` ways is done first on 256 CUs.
-inline int pick_tile(const TileCost* ways, int count, int M, int N) {
+inline double tile_count(const TileCost& way, const GemmArgs& p) {
+  return static_cast<double>((p.M + way.rows - 1LL) / way.rows) * ((p.N + way.columns - 1LL) / way.columns);
+}
+// Which of `count` ways is done first on 256 CUs; step: k of a step.
+inline int pick_tile(const TileCost* ways, int count, int step, const GemmArgs& p) {
   int best = 0;
   double least = 0;
   for (int i = 0; i < count; ++i) {
-    const long long tiles = ((M + ways[i].rows - 1LL) / ways[i].rows) * ((N + ways[i].columns - 1LL) / ways[i].columns);
-    const long long each = (tiles + 255) / 256;  // tiles of the fullest CU
-    const double cost = each == 1 ? ways[i].alone : each * ways[i].shared;
+    const TileCost& way = ways[i];
+    const long long each = static_cast<long long>((tile_count(way, p) + 255) / 256);  // tiles of the fullest CU
+    const double cost = way.once + (p.K + step - 1) / step * (each <= 1 ? way.one : each == 2 ? way.two : each * way.more);
     if (i == 0 || cost < least) best = i, least = cost;
   }
   return best;
@@ -71,12 +74,12 @@ inline int pick_grads_tile(const TileCost* ways, int count, int step, const FfnG
   for (int i = 0; i < count; ++i) {
     double work = 0, longest = 0, shortest = 0;
     for (const GemmArgs* g : of) {
-      const double tiles = static_cast<double>((g->M + ways[i].rows - 1LL) / ways[i].rows) * ((g->N + ways[i].columns - 1LL) / ways[i].columns);
+      const double tiles = tile_count(ways[i], *g);
       if (tiles == 0) continue;
       const double steps = (g->K + step - 1) / step;
-      work += tiles * steps * ways[i].shared / 256;
-      longest = longest > steps * ways[i].alone ? longest : steps * ways[i].alone;
-      shortest = shortest == 0 || steps * ways[i].shared < shortest ? steps * ways[i].shared : shortest;
+      work += tiles * steps * ways[i].more / 256;
+      longest = longest > steps * ways[i].one ? longest : steps * ways[i].one;
+      shortest = shortest == 0 || steps * ways[i].more < shortest ? steps * ways[i].more : shortest;
     }
     const double cost = work + shortest / 2 > longest ? work + shortest / 2 : longest;
     if (i == 0 || cost < least) best = i, least = cost;

@@ -1,92 +1,31 @@
-// Matrix products with MXFP4 weights: 32 consecutive values of a row share a scale 2^(byte - 127), a
+// Matrix products of many rows with MXFP4 weights: 32 consecutive values of a row share a scale 2^(byte - 127), a
 // value is 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the even one in its low half.
+//
+// MXFP4 rows go through the scaled matrix instructions, 16 x 16 x 128: a lane's operand is one block of 32 values
+// (16 bytes) and that block's scale, and a step of 256 k has the bfloat16 kernels' 128 bytes a row.
+// With bfloat16 rows the weights stay in 4 bits up to the wave that multiplies them and become bfloat16
+// there, which holds every one of their values. A step is 64 k, of which lane l takes the (l / 16)-th
+// quarter: 16 weights (8 bytes) under one scale, and 16-byte pieces 2 (l / 16) and 2 (l / 16) + 1 of its rows of A.
+//
+// Scales go through LDS, byte by byte through registers, a stage ahead. (Read from memory by the lane that needs one,
+// when it needs it, they had taken more time than everything else: M=2048, N=8192, K=4096 250 us instead of 112.) Of
+// two operands in 4 bits there are as many scales as make that felt, and where rows of scales begin on 4 bytes (K a
+// multiple of 128) they are loaded 4 at a time straight to LDS: M=4096, N=8192, K=4096 99 us by bytes, 86 by fours.
 #include "ffn_gemm_device.h"
 
 namespace fmoe {
 
-// The scale byte of a lane's 32 k (block `kb` of `blocks`) of one of its rows. Behind the last block
-// the values are zeros, and so must the scale be a number.
-__device__ __forceinline__ unsigned scale_byte(const unsigned char* row, int kb, int blocks) {
-  return kb < blocks ? row[kb] : 127u;
+__device__ __forceinline__ unsigned lds_byte(const char* p) { return *(const FFN_LDS unsigned char*)p; }
+
+__device__ __forceinline__ bf16x8 eight_values(unsigned codes, float scale) {
+  const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
+  const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+  const bf16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
+  const bf16x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+  return bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 }
 
-// MXFP4 rows times MXFP4 weights on the scaled matrix instructions: 16 x 16 x 128, a lane's operand is
-// one block of 32 values (16 bytes) and that block's scale.
-template <class S>
-__global__ __launch_bounds__(S::THREADS) void mxfp4_both_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(128))) char lds[2 * S::STAGE_BYTES];
-  int tile_m, tile_n;
-  tile_of(p, blockIdx.x, tile_m, tile_n);
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
-
-  TileLoader<S::KIND, false, S::BM, S::THREADS, S::FM, false> load_a;
-  TileLoader<S::KIND, false, S::BN, S::THREADS, S::FN, false> load_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
-  const int blocks = p.K / 32;
-  const unsigned char* scale_a[S::FM];
-  const unsigned char* scale_b[S::FN];
-#pragma unroll
-  for (int f = 0; f < S::FM; ++f) {
-    const int m = m0 + wm * S::FM * 16 + dealt_row<S::FM>(f, r);
-    scale_a[f] = p.a_scales + static_cast<long long>(m < p.M ? m : 0) * blocks;
-  }
-#pragma unroll
-  for (int f = 0; f < S::FN; ++f) {
-    const int n = n0 + wn * S::FN * 16 + dealt_row<S::FN>(f, r);
-    scale_b[f] = p.b_scales + static_cast<long long>(n < p.N ? n : 0) * blocks;
-  }
-
-  Accumulators<S> acc;
-#pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
-#pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  const int steps = (p.K + S::STEP - 1) / S::STEP;
-  if (steps > 0) {
-    load_a.load(lds, 0, p.K);
-    load_b.load(lds + S::BM * 128, 0, p.K);
-  }
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    char* next = lds + ((s + 1) & 1) * S::STAGE_BYTES;
-    if (s + 1 < steps) {
-      load_a.load(next, s + 1, p.K - (s + 1) * S::STEP);
-      load_b.load(next + S::BM * 128, s + 1, p.K - (s + 1) * S::STEP);
-    }
-    const char* now = lds + (s & 1) * S::STAGE_BYTES;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      Fragments<S::KIND, false, S::BN, S::FN> b;
-      Fragments<S::KIND, false, S::BM, S::FM> a;
-      b.read(now + S::BM * 128, wn * S::FN * 16, half);
-      a.read(now, wm * S::FM * 16, half);
-      unsigned sa[S::FM], sb[S::FN];
-#pragma unroll
-      for (int f = 0; f < S::FM; ++f) sa[f] = scale_byte(scale_a[f], s * 8 + half * 4 + g, blocks);
-#pragma unroll
-      for (int f = 0; f < S::FN; ++f) sb[f] = scale_byte(scale_b[f], s * 8 + half * 4 + g, blocks);
-#pragma unroll
-      for (int fm = 0; fm < S::FM; ++fm)
-#pragma unroll
-        for (int fn = 0; fn < S::FN; ++fn) {
-          const i32x8 bv = {b.v[fn][0], b.v[fn][1], b.v[fn][2], b.v[fn][3], 0, 0, 0, 0};
-          const i32x8 av = {a.v[fm][0], a.v[fm][1], a.v[fm][2], a.v[fm][3], 0, 0, 0, 0};
-          acc.v[fm][fn] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bv, av, acc.v[fm][fn], 4, 4, 0, sb[fn], 0, sa[fm]);
-        }
-    }
-  }
-  write_results<S>(p, m0, n0, acc);
-}
-
-// bfloat16 rows times MXFP4 weights: the weights stay in 4 bits up to the wave that multiplies them and
-// become bfloat16 there, which holds every one of their values. A step is 64 k, of which lane l takes
-// the (l / 16)-th quarter: 16 weights (8 bytes) under one scale, and 16-byte pieces 2 (l / 16) and
-// 2 (l / 16) + 1 of its rows of A.
+// The weights' codes of bfloat16 rows' products: of each block of 16 rows a step's first 16 bytes, then the other 16.
 template <int ROWS, int THREADS, int F, bool GATED>
 struct CodeLoader {
   static constexpr int PIECES = (ROWS * 2 + THREADS - 1) / THREADS;
@@ -94,20 +33,22 @@ struct CodeLoader {
   unsigned offset[PIECES];
   const char* base;
   long long up_bytes;
+  int tid;
 
-  __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows) {
+  __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows, int tid_) {
+    tid = tid_;
     base = static_cast<const char*>(p) + row0 * ld / 2;
     up_bytes = GATED ? rows * ld / 2 : 0;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int at = i * THREADS + threadIdx.x, block = at >> 5, r = at & 15, half = (at >> 4) & 1, f = block % F;
+      const int at = i * THREADS + tid, block = at >> 5, r = at & 15, half = (at >> 4) & 1, f = block % F;
       const int src = GATED ? block / F * (8 * F) + gated_row<F>(f, r) : block / F * (16 * F) + dealt_row<F>(f, r);
       offset[i] = block * 16 < ROWS && row0 + src < rows ? static_cast<unsigned>(src * ld / 2) + half * 16 : kOutside;
     }
   }
   __device__ __forceinline__ void load(char* lds, int s, int left) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int half = (threadIdx.x >> 4) & 1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = (tid >> 4) & 1;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       // a wave loads two blocks of 16 rows, which the gated kernels' F >= 4 keep on one side
@@ -118,113 +59,41 @@ struct CodeLoader {
   }
 };
 
-__device__ __forceinline__ bf16x8 eight_values(unsigned codes, float scale) {
-  const bf16x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
-  const bf16x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
-  const bf16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
-  const bf16x2 v3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
-  return bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+// Which row of the matrix (gated: which column of C) lies at `row` of a tile, from its first one
+template <int F, bool GATED>
+__device__ __forceinline__ int row_of_tile(int row) {
+  const int f = row % (16 * F) >> 4, r = row & 15;
+  return GATED ? row / (16 * F) * (8 * F) + gated_row<F>(f, r) : row / (16 * F) * (16 * F) + dealt_row<F>(f, r);
 }
 
-template <class S>
-__global__ __launch_bounds__(S::THREADS) void mxfp4_weights_kernel(GemmArgs p) {
-  constexpr bool GATED = S::EPI == EPI_GATED;
-  constexpr int STAGE = S::BM * 128 + CodeLoader<S::BN, S::THREADS, S::FN, GATED>::BYTES;
-  __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
-  static_assert(S::FN % 4 == 0, "pairs of blocks on one side");
-  int tile_m, tile_n;
-  tile_of(p, blockIdx.x, tile_m, tile_n);
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+// A tile's scales, PER blocks of a row a step; block kb lies at byte kb % 8 of its row's 8. Behind the last block of a row
+// the values are zeros, and so must the scale be a number: zero is one.
+template <int ROWS, int THREADS, int F, bool GATED, int PER, bool FOURS>
+struct ScaleLoader;
 
-  TileLoader<KIND_BF16, false, S::BM, S::THREADS, S::FM, false> load_a;
-  CodeLoader<S::BN, S::THREADS, S::FN, GATED> load_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
-  const int blocks = p.K / 32;
-  const unsigned char* scale_b[S::FN];
-#pragma unroll
-  for (int f = 0; f < S::FN; ++f) {
-    const int n = GATED ? n0 + wn * S::FN * 8 + gated_row<S::FN>(f, r) : n0 + wn * S::FN * 16 + dealt_row<S::FN>(f, r);
-    const int row = n < p.N ? n + (GATED && f >= S::FN / 2 ? p.N : 0) : 0;
-    scale_b[f] = p.b_scales + static_cast<long long>(row) * blocks;
-  }
-
-  Accumulators<S> acc;
-#pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
-#pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  const int steps = (p.K + 63) / 64;
-  if (steps > 0) {
-    load_a.load(lds, 0, p.K);
-    load_b.load(lds + S::BM * 128, 0, p.K);
-  }
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    char* next = lds + ((s + 1) & 1) * STAGE;
-    if (s + 1 < steps) {
-      load_a.load(next, s + 1, p.K - (s + 1) * 64);
-      load_b.load(next + S::BM * 128, s + 1, p.K - (s + 1) * 64);
-    }
-    const char* now = lds + (s & 1) * STAGE;
-    u32x2 codes[S::FN];
-    float scale[S::FN];
-#pragma unroll
-    for (int f = 0; f < S::FN; ++f) {
-      codes[f] = *(const FFN_LDS u32x2*)(now + S::BM * 128 + (wn * S::FN + f) * 512 + (g >> 1) * 256 + r * 16 + (g & 1) * 8);
-      scale[f] = __uint_as_float(scale_byte(scale_b[f], s * 2 + (g >> 1), blocks) << 23);
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      bf16x8 b[S::FN];
-#pragma unroll
-      for (int f = 0; f < S::FN; ++f) b[f] = eight_values(codes[f][half], scale[f]);
-#pragma unroll
-      for (int fm = 0; fm < S::FM; ++fm) {
-        const bf16x8 a = *(const FFN_LDS bf16x8*)(now + ((wm * S::FM + fm) * 16 + r) * 128 + (((2 * g + half) ^ (r & 7)) << 4));
-#pragma unroll
-        for (int fn = 0; fn < S::FN; ++fn)
-          acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[fn], a, acc.v[fm][fn], 0, 0, 0);
-      }
-    }
-  }
-  write_results<S>(p, m0, n0, acc);
-}
-
-// ------------------------------------------------------------------ scales on 4-byte boundaries
-// The kernels below take their scales through LDS, 8 bytes of a row (256 k) a stage: 2 KiB for 256 rows, a load of
-// 4 bytes a lane. That wants rows of scales on 4 bytes: K a multiple of 128. (The ones above read single bytes
-// from memory whenever they need one, and wait for them: 258 us against 105 at M=2048, N=8192, K=4096.)
-template <int ROWS, int THREADS, int F, bool GATED>
-struct ScaleLoader {
+template <int ROWS, int THREADS, int F, bool GATED, int PER>
+struct ScaleLoader<ROWS, THREADS, F, GATED, PER, true> {
   static constexpr int PIECES = (ROWS * 2 + THREADS - 1) / THREADS;
   static constexpr int BYTES = PIECES * THREADS * 4;  // in LDS; behind the rows, zeros
   unsigned offset[PIECES];
   const unsigned char* base;
-  int blocks;
+  long long up;
+  int blocks, tid;
 
-  __device__ __forceinline__ void init(const unsigned char* p, int row0, int rows, int blocks_) {
-    blocks = blocks_;
+  __device__ __forceinline__ void init(const unsigned char* p, int row0, int rows, int blocks_, int tid_) {
+    blocks = blocks_, tid = tid_;
     base = p + static_cast<long long>(row0) * blocks;
-    const int tid = threadIdx.x;
+    up = GATED ? static_cast<long long>(rows) * blocks : 0;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int at = i * THREADS + tid, row = at >> 1, f = row % (16 * F) >> 4, r = row & 15;
-      const int src = GATED ? row / (16 * F) * (8 * F) + gated_row<F>(f, r) : row / (16 * F) * (16 * F) + dealt_row<F>(f, r);
+      const int at = i * THREADS + tid, row = at >> 1, src = row_of_tile<F, GATED>(row);
       offset[i] = row < ROWS && row0 + src < rows ? static_cast<unsigned>(src * blocks) + (at & 1) * 4 : kOutside;
     }
-    up = GATED ? static_cast<long long>(rows) * blocks : 0;
   }
-  long long up;
-
-  // the 8 blocks from `first` (a multiple of 8) on
-  __device__ __forceinline__ void load(char* lds, int first) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool in = first + (threadIdx.x & 1) * 4 < blocks;
+  // a step's blocks and, where they are fewer, the rest of the row's 8
+  __device__ __forceinline__ void load(char* lds, int s) {
+    const int first = s * PER & ~7, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool in = first + (tid & 1) * 4 < blocks;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int f = ((i * THREADS + wave * 64) >> 1) % (16 * F) >> 4;  // a wave loads two blocks of 16 rows, on one side
@@ -233,51 +102,96 @@ struct ScaleLoader {
                                                static_cast<int>(in ? offset[i] : kOutside), 0, 0, 0);
     }
   }
+  __device__ __forceinline__ void landed(char*, int) const {}
 };
 
-__device__ __forceinline__ unsigned lds_byte(const char* p) { return *(const FFN_LDS unsigned char*)p; }
+template <int ROWS, int THREADS, int F, bool GATED, int PER>
+struct ScaleLoader<ROWS, THREADS, F, GATED, PER, false> {
+  static constexpr int PIECES = (ROWS * PER + THREADS - 1) / THREADS, BYTES = ROWS * 8;
+  unsigned value[PIECES];
+  const unsigned char* base;
+  long long up;
+  int blocks, tid, left;  // left: rows from this tile's first one on
+
+  __device__ __forceinline__ void init(const unsigned char* p, int row0, int rows, int blocks_, int tid_) {
+    blocks = blocks_, tid = tid_, left = rows - row0;
+    base = p + static_cast<long long>(row0) * blocks;
+    up = GATED ? static_cast<long long>(rows) * blocks : 0;
+  }
+  __device__ __forceinline__ void load(char*, int s) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int at = i * THREADS + tid, row = at / PER, kb = s * PER + at % PER, src = row_of_tile<F, GATED>(row);
+      const bool in = row < ROWS && src < left && kb < blocks;
+      const long long from = static_cast<long long>(src) * blocks + kb + (GATED && row % (16 * F) / 16 >= F / 2 ? up : 0);
+      value[i] = in ? base[from] : 0u;
+    }
+  }
+  // what load asked for, to LDS: behind the wait for it, before the barrier
+  __device__ __forceinline__ void landed(char* lds, int s) const {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int at = i * THREADS + tid, row = at / PER, kb = s * PER + at % PER;
+      if (row < ROWS) *(FFN_LDS unsigned char*)(lds + row * 8 + (kb & 7)) = static_cast<unsigned char>(value[i]);
+    }
+  }
+};
 
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void mxfp4_both_tiled_kernel(GemmArgs p) {
-  typedef ScaleLoader<S::BM, S::THREADS, S::FM, false> ScaleA;
-  typedef ScaleLoader<S::BN, S::THREADS, S::FN, false> ScaleB;
+__device__ __forceinline__ void clear(Accumulators<S>& acc) {
+#pragma unroll
+  for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+template <class S, bool FOURS>
+__global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(GemmArgs p) {
+  typedef ScaleLoader<S::BM, S::THREADS, S::FM, false, 8, FOURS> ScaleA;
+  typedef ScaleLoader<S::BN, S::THREADS, S::FN, false, 8, FOURS> ScaleB;
   constexpr int TILES = S::STAGE_BYTES, STAGE = TILES + ScaleA::BYTES + ScaleB::BYTES;
-  __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(128))) char lds[2 * S::GROUPS * STAGE];
   int tile_m, tile_n;
   tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  char* mine = lds + group * 2 * STAGE;
 
   TileLoader<S::KIND, false, S::BM, S::THREADS, S::FM, false> load_a;
   TileLoader<S::KIND, false, S::BN, S::THREADS, S::FN, false> load_b;
   ScaleA scale_a;
   ScaleB scale_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
-  scale_a.init(p.a_scales, m0, p.M, p.K / 32);
-  scale_b.init(p.b_scales, n0, p.N, p.K / 32);
-
+  load_a.init(p.a, p.lda, m0, p.M, tid);
+  load_b.init(p.b, p.ldb, n0, p.N, tid);
+  scale_a.init(p.a_scales, m0, p.M, p.K / 32, tid);
+  scale_b.init(p.b_scales, n0, p.N, p.K / 32, tid);
   Accumulators<S> acc;
-#pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
-#pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  clear(acc);
 
-  const int steps = (p.K + S::STEP - 1) / S::STEP;
-  auto load = [&](int s) {
-    char* to = lds + (s & 1) * STAGE;
+  const int steps = (p.K + S::STEP - 1) / S::STEP, turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  auto load = [&](int turn) {
+    const int s = turn * S::GROUPS + group;
+    if (S::GROUPS > 1 && s >= steps) return;
+    char* to = mine + (turn & 1) * STAGE;
     load_a.load(to, s, p.K - s * S::STEP);
     load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
-    scale_a.load(to + TILES, s * 8);
-    scale_b.load(to + TILES + ScaleA::BYTES, s * 8);
+    scale_a.load(to + TILES, s);
+    scale_b.load(to + TILES + ScaleA::BYTES, s);
   };
-  if (steps > 0) load(0);
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (s + 1 < steps) load(s + 1);
-    const char* now = lds + (s & 1) * STAGE;
+  load(0);
+  for (int turn = 0; turn < turns; ++turn) {
+    const int s = turn * S::GROUPS + group;
+    char* now = mine + (turn & 1) * STAGE;
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of the stage have landed ...
+    if (S::GROUPS == 1 || s < steps) {
+      scale_a.landed(now + TILES, s);
+      scale_b.landed(now + TILES + ScaleA::BYTES, s);
+    }
+    __syncthreads();  // ... and everybody's; all are done with the other buffer
+    if (turn + 1 < turns) load(turn + 1);
+    if (S::GROUPS > 1 && s >= steps) continue;
     const char* sa_at = now + TILES + (wm * S::FM * 16 + r) * 8 + g;
     const char* sb_at = now + TILES + ScaleA::BYTES + (wn * S::FN * 16 + r) * 8 + g;
 #pragma unroll
@@ -301,117 +215,85 @@ __global__ __launch_bounds__(S::THREADS) void mxfp4_both_tiled_kernel(GemmArgs p
         }
     }
   }
-  write_results<S>(p, m0, n0, acc);
-}
-
-// The k loop of bfloat16 rows times MXFP4 weights. A stage is multiplied in four parts, two halves of its k for two
-// halves of the wave's rows of A, each part while the next one's operands come from LDS. Before the last part
-// all of the stage is in registers, and its buffer is loaded with the stage after next. (With eight waves,
-// which convert each weight twice; sixteen, in the plain loop of the other kernels, convert it four times:
-// M=2048, N=8192, K=4096 113 us and 125.) LOADS: load instructions of a wave for a stage.
-template <int LOADS, class A, class B, class Load, class ReadA, class ReadB, class Multiply>
-__device__ __forceinline__ void stage_loop(int steps, Load load, ReadA read_a, ReadB read_b, Multiply multiply) {
-  if (steps == 0) return;
-  A a0, a1;
-  B b0, b1;
-  load(0);
-  if (steps > 1) load(1);
-  // stage 0 has landed when no more than the other's loads are on their way
-  if (steps > 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-  __builtin_amdgcn_s_barrier();
-  read_b(b0, 0, 0);
-  read_a(a0, 0, 0, 0);
-  for (int s = 0; s < steps; ++s) {
-    read_a(a1, s, 0, 1);
-    multiply(a0, b0, 0);
-    read_b(b1, s, 1);
-    read_a(a0, s, 1, 0);
-    multiply(a1, b0, 1);
-    read_a(a1, s, 1, 1);
-    multiply(a0, b1, 0);
-    // stage s + 1 has landed, stage s is read
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-    __builtin_amdgcn_s_barrier();
-    if (s + 2 < steps) load(s + 2);
-    if (s + 1 < steps) {
-      read_b(b0, s + 1, 0);
-      read_a(a0, s + 1, 0, 0);
-    }
-    multiply(a1, b1, 1);
-  }
+  add_groups<S>(lds, group, acc);
+  if (group == 0) write_results<S>(p, m0, n0, acc);
 }
 
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void mxfp4_weights_tiled_kernel(GemmArgs p) {
+__global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(GemmArgs p) {
   constexpr bool GATED = S::EPI == EPI_GATED;
   typedef CodeLoader<S::BN, S::THREADS, S::FN, GATED> Codes;
-  typedef ScaleLoader<S::BN, S::THREADS, S::FN, GATED> ScaleB;
+  typedef ScaleLoader<S::BN, S::THREADS, S::FN, GATED, 2, false> ScaleB;
   constexpr int TILES = S::BM * 128 + Codes::BYTES, STAGE = TILES + ScaleB::BYTES;
+  constexpr int SUMS = (S::GROUPS - 1) * S::BM * S::BN * 4, ALL = 2 * S::GROUPS * STAGE;
   static_assert(S::FN % 4 == 0, "pairs of blocks on one side");
-  __shared__ __attribute__((aligned(128))) char lds[2 * STAGE];
+  __shared__ __attribute__((aligned(128))) char lds[SUMS > ALL ? SUMS : ALL];
   int tile_m, tile_n;
   tile_of(p, blockIdx.x, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  char* mine = lds + group * 2 * STAGE;
 
   TileLoader<KIND_BF16, false, S::BM, S::THREADS, S::FM, false> load_a;
   Codes load_b;
   ScaleB scale_b;
-  load_a.init(p.a, p.lda, m0, p.M);
-  load_b.init(p.b, p.ldb, n0, p.N);
-  scale_b.init(p.b_scales, n0, p.N, p.K / 32);
-
+  load_a.init(p.a, p.lda, m0, p.M, tid);
+  load_b.init(p.b, p.ldb, n0, p.N, tid);
+  scale_b.init(p.b_scales, n0, p.N, p.K / 32, tid);
   Accumulators<S> acc;
-#pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
-#pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  clear(acc);
 
-  constexpr int HM = S::FM / 2, LOADS = S::BM * 8 / S::THREADS + Codes::PIECES + ScaleB::PIECES;
-  struct A {
-    bf16x8 v[HM];
+  const int steps = (p.K + 63) / 64, turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  auto load = [&](int turn) {
+    const int s = turn * S::GROUPS + group;
+    if (S::GROUPS > 1 && s >= steps) return;
+    char* to = mine + (turn & 1) * STAGE;
+    load_a.load(to, s, p.K - s * 64);
+    load_b.load(to + S::BM * 128, s, p.K - s * 64);
+    scale_b.load(to + TILES, s);
   };
-  struct B {
-    unsigned codes[S::FN];
+  // rows of A and weights of a stage's half from LDS
+  auto a_at = [&](const char* now, int fm, int half) {
+    return *(const FFN_LDS bf16x8*)(now + ((wm * S::FM + fm) * 16 + r) * 128 + (((2 * g + half) ^ (r & 7)) << 4));
+  };
+  auto codes_at = [&](const char* now, int fn) { return now + S::BM * 128 + (wn * S::FN + fn) * 512 + (g >> 1) * 256 + r * 16 + (g & 1) * 8; };
+  auto scale_at = [&](const char* now, int fn, int s) {
+    return __uint_as_float(lds_byte(now + TILES + ((wn * S::FN + fn) * 16 + r) * 8 + (s * 2 & 7) + (g >> 1)) << 23);
+  };
+  load(0);
+  for (int turn = 0; turn < turns; ++turn) {
+    const int s = turn * S::GROUPS + group;
+    char* now = mine + (turn & 1) * STAGE;
+    __builtin_amdgcn_s_waitcnt(0);
+    if (S::GROUPS == 1 || s < steps) scale_b.landed(now + TILES, s);
+    __syncthreads();
+    if (turn + 1 < turns) load(turn + 1);
+    if (S::GROUPS > 1 && s >= steps) continue;
+    u32x2 codes[S::FN];
     float scale[S::FN];
-  };
-  stage_loop<LOADS, A, B>(
-      (p.K + 63) / 64,
-      [&](int s) {
-        char* to = lds + (s & 1) * STAGE;
-        load_a.load(to, s, p.K - s * 64);
-        load_b.load(to + S::BM * 128, s, p.K - s * 64);
-        scale_b.load(to + TILES, s * 2 & ~7);
-      },
-      [&](A& a, int s, int half, int group) {
 #pragma unroll
-        for (int f = 0; f < HM; ++f)
-          a.v[f] = *(const FFN_LDS bf16x8*)(lds + (s & 1) * STAGE + ((wm * S::FM + group * HM + f) * 16 + r) * 128 +
-                                            (((2 * g + half) ^ (r & 7)) << 4));
-      },
-      [&](B& b, int s, int half) {
-        const char* from = lds + (s & 1) * STAGE;
+    for (int f = 0; f < S::FN; ++f) {
+      codes[f] = *(const FFN_LDS u32x2*)codes_at(now, f);
+      scale[f] = scale_at(now, f, s);
+    }
 #pragma unroll
-        for (int f = 0; f < S::FN; ++f) {
-          const int block = wn * S::FN + f;
-          b.codes[f] = *(const FFN_LDS unsigned*)(from + S::BM * 128 + block * 512 + (g >> 1) * 256 + r * 16 + (g & 1) * 8 + half * 4);
-          b.scale[f] = __uint_as_float(lds_byte(from + TILES + (block * 16 + r) * 8 + (s * 2 & 7) + (g >> 1)) << 23);
-        }
-      },
-      [&](const A& a, const B& b, int group) {
+    for (int half = 0; half < 2; ++half) {
+      bf16x8 b[S::FN];
 #pragma unroll
-        for (int fn = 0; fn < S::FN; ++fn) {
-          const bf16x8 w = eight_values(b.codes[fn], b.scale[fn]);
+      for (int f = 0; f < S::FN; ++f) b[f] = eight_values(codes[f][half], scale[f]);
 #pragma unroll
-          for (int fm = 0; fm < HM; ++fm) {
-            f32x4& c = acc.v[group * HM + fm][fn];
-            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, a.v[fm], c, 0, 0, 0);
-          }
-        }
-      });
-  write_results<S>(p, m0, n0, acc);
+      for (int fm = 0; fm < S::FM; ++fm) {
+        const bf16x8 a = a_at(now, fm, half);
+#pragma unroll
+        for (int fn = 0; fn < S::FN; ++fn)
+          acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[fn], a, acc.v[fm][fn], 0, 0, 0);
+      }
+    }
+  }
+  add_groups<S, sizeof(lds)>(lds, group, acc);
+  if (group == 0) write_results<S>(p, m0, n0, acc);
 }
 
 template <class S, typename Kernel>
@@ -421,8 +303,62 @@ static hipError_t launch(Kernel kernel, GemmArgs p, hipStream_t stream) {
   const long long tiles = static_cast<long long>(p.grid_m) * p.grid_n;
   if (tiles == 0) return hipSuccess;
   if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(S::THREADS), 0, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
   return hipGetLastError();
+}
+
+// Measured at N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four) / 64 x 128 in four groups / 64 x 64 in four
+// groups of two waves, us: M=2048 112 / 140 / 226 / 304; M=1024 99 / 67 / 114 / 153; M=256 96 / 48 / 29 / 38; M=64
+// 88 / 44 / 24 / 17.
+template <int EPI>
+static hipError_t launch_weights(const GemmArgs& p, hipStream_t stream) {
+  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
+  static const TileCost ways[] = {{256, 256 / PER, 0, 1.7, 3.4, 1.7}, {128, 128 / PER, 0, 0.68, 1.02, 0.53},
+                                  {64, 128 / PER, 1, 0.4, 0.9, 0.45}, {64, 64 / PER, 1, 0.22, 0.55, 0.28}};
+  switch (pick_tile(ways, 4, 64, p)) {
+    case 0: {
+      typedef GemmShape<KIND_BF16, false, false, EPI, 4, 4, 4, 4> S;
+      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+    }
+    case 1: {
+      typedef GemmShape<KIND_BF16, false, false, EPI, 2, 2, 4, 4> S;
+      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+    }
+    case 2: {
+      typedef GemmShape<KIND_BF16, false, false, EPI, 2, 2, 2, 4, 4> S;
+      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+    }
+    default: {
+      typedef GemmShape<KIND_BF16, false, false, EPI, 2, 1, 2, 4, 4> S;
+      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+    }
+  }
+}
+
+// Measured at N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four) / the same in two groups / 64 x 64 in two
+// groups, us: M=4096 86 / 99 / 122 / 163; M=512 32 / 19 / 17 / 22; M=128 28 / 16 / 14 / 8.6.
+template <bool FOURS>
+static hipError_t launch_both(const GemmArgs& p, hipStream_t stream) {
+  static const TileCost ways[] = {{256, 256, 0, 2.5, 5.2, 2.6}, {128, 128, 0, 1.0, 1.7, 0.77}, {128, 128, 0.5, 0.87, 1.9, 0.95},
+                                  {64, 64, 0.5, 0.35, 0.65, 0.31}};
+  switch (pick_tile(ways, 4, 256, p)) {
+    case 0: {
+      typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 4, 4, 4, 4> S;
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+    }
+    case 1: {
+      typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4> S;
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+    }
+    case 2: {
+      typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4, 2> S;
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+    }
+    default: {
+      typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 2, 2, 2> S;
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+    }
+  }
 }
 
 // Whether both kinds of scales can be read 4 bytes at a time
@@ -431,32 +367,10 @@ static bool scales_on_fours(const GemmArgs& p) {
   return p.K % 128 == 0 && fours(p.b_scales) && fours(p.a_scales);
 }
 
-// Measured at M=2048, N=8192, K=4096, 256 x 256 (eight waves) / 128 x 128 (four): 113 / 134 us; M=256 94 / 46.
-template <int EPI>
-static hipError_t launch_weights(const GemmArgs& p, hipStream_t stream) {
-  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  typedef GemmShape<KIND_BF16, false, false, EPI, 2, 2, 4, 4> Small;
-  typedef GemmShape<KIND_BF16, false, false, EPI, 2, 4, 8, 4> Large;
-  if (!scales_on_fours(p)) return launch<Small>(mxfp4_weights_kernel<Small>, p, stream);
-  static const TileCost ways[] = {{256, 256 / PER, 1.75, 1.75}, {128, 128 / PER, 0.68, 0.52}};
-  if (pick_tile(ways, 2, p.M, p.N) == 0) return launch<Large>(mxfp4_weights_tiled_kernel<Large>, p, stream);
-  return launch<Small>(mxfp4_weights_tiled_kernel<Small>, p, stream);
-}
-
-// Measured at M=4096, N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four): 80.5 / 93.1 us; M=512 31.5 / 18.0.
-static hipError_t launch_both(const GemmArgs& p, hipStream_t stream) {
-  typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4> Small;
-  typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 4, 4, 4, 4> Large;
-  if (!scales_on_fours(p)) return launch<Small>(mxfp4_both_kernel<Small>, p, stream);
-  static const TileCost ways[] = {{256, 256, 2.4, 2.4}, {128, 128, 1.0, 0.73}};
-  if (pick_tile(ways, 2, p.M, p.N) == 0) return launch<Large>(mxfp4_both_tiled_kernel<Large>, p, stream);
-  return launch<Small>(mxfp4_both_tiled_kernel<Small>, p, stream);
-}
-
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream) {
   if (x_mxfp4 && epi != EPI_STORE) return hipErrorInvalidValue;
   if (mxfp4_skinny_takes(x_mxfp4, p)) return launch_mxfp4_skinny(x_mxfp4, epi == EPI_GATED, p, stream);
-  if (x_mxfp4) return launch_both(p, stream);
+  if (x_mxfp4) return scales_on_fours(p) ? launch_both<true>(p, stream) : launch_both<false>(p, stream);
   return epi == EPI_GATED ? launch_weights<EPI_GATED>(p, stream) : launch_weights<EPI_STORE>(p, stream);
 }
 
