@@ -205,16 +205,14 @@ template <bool OA, bool OB, int EPI>
 static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
   constexpr int PER = EPI == EPI_GATED ? 2 : 1;
   static const TileCost ways[] = {{128, 128 / PER, 0, 1.7, 2.5, 1.25}, {128, 128 / PER, 1, 1.32, 2.7, 1.35},
-                                  {128, 64 / PER, 0, 1.1, 1.6, 0.72},  {128, 64 / PER, 0.8, 0.86, 1.8, 0.9},
-                                  {64, 64 / PER, 0, 0.78, 0.98, 0.42}, {64, 64 / PER, 0.8, 0.54, 0.85, 0.45},
-                                  {64, 64 / PER, 1.8, 0.48, 0.95, 0.48}};
-  switch (pick_tile(ways, 7, 32, p)) {
+                                  {128, 64 / PER, 0, 1.1, 1.6, 0.72},  {64, 64 / PER, 0, 0.78, 0.98, 0.42},
+                                  {64, 64 / PER, 0.8, 0.54, 0.85, 0.45}, {64, 64 / PER, 1.8, 0.48, 0.95, 0.48}};
+  switch (pick_tile(ways, 6, 32, p)) {
     case 0: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4>>(p, stream);
     case 1: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4, 2>>(p, stream);
     case 2: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2>>(p, stream);
-    case 3: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2, 2>>(p, stream);
-    case 4: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
-    case 5: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
+    case 3: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
+    case 4: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
     default: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 4>>(p, stream);
   }
 }

@@ -308,7 +308,7 @@ static hipError_t go(const GemmArgs& p, hipStream_t stream) {
 static int pick_groups(const GemmArgs& p, int least, int most, bool gated, double w_bytes, double x_bytes) {
   int best = least;
   double least_cost = 0;
-  for (int hb = least; hb <= most; hb *= 2) {
+  for (int hb = least; hb <= most; hb = hb == 4 && most == 6 ? 6 : hb * 2) {
     const long long columns = (gated ? hb / 2 : hb) * 8, groups = (p.N + columns - 1) / columns;
     const double cost = static_cast<double>((groups + 255) / 256) * (hb * 8 * w_bytes + 0.5 * p.M * x_bytes);
     if (hb == least || cost < least_cost) best = hb, least_cost = cost;
@@ -336,8 +336,9 @@ static hipError_t go_plain(const GemmArgs& p, hipStream_t stream) {
 template <int KIND, int XB>
 static hipError_t go_gated(const GemmArgs& p, hipStream_t stream) {
   constexpr double W = KIND == SKINNY_F32 ? 4 : KIND == SKINNY_BF16 ? 2 : 0.53, X = KIND == SKINNY_F32 ? 4 : 2;
-  const int hb = pick_groups(p, 2, KIND == SKINNY_MXFP4_WEIGHTS ? 4 : 8, true, W, X);
+  const int hb = pick_groups(p, 2, KIND == SKINNY_MXFP4_WEIGHTS ? 6 : 8, true, W, X);
   if constexpr (KIND == SKINNY_MXFP4_WEIGHTS) {
+    if (hb == 6) return go<KIND, true, 6, XB, 4, 1>(p, stream);
     return hb == 2 ? go<KIND, true, 2, XB, 4, 1>(p, stream) : go<KIND, true, 4, XB, 4, 1>(p, stream);
   } else {
     if (hb == 2) return go<KIND, true, 2, XB, 8, 2>(p, stream);

@@ -57,7 +57,7 @@ def test_forward_and_backward(ops, T, H, I, act, dtype):
 
 # many tiles of the largest size in one product each: gated and slope / both weights' gradients / output and x's gradient
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
-@pytest.mark.parametrize("T,H,I", [(3841, 72, 3600), (77, 3600, 3904), (3841, 3600, 40)])
+@pytest.mark.parametrize("T,H,I", [(3841, 72, 3600), (77, 3600, 3904), (3841, 3600, 40), (2000, 640, 1000), (1100, 1304, 2600)])
 def test_large_tiles(ops, T, H, I, dtype):
     x, w13, w2, dy = make(T, H, I, DTYPES[dtype], seed=6)
     want = ffn_case.block(x, w13, w2, "silu", dy)
