@@ -266,7 +266,7 @@ __device__ __forceinline__ void write_results(const GemmArgs& p, int m0, int n0,
           du[f][i] = dh * a;
         }
       }
-      char* out = static_cast<char*>(p.c) + m * (2LL * p.N) * OSIZE;
+      char* out = static_cast<char*>(p.c) + m * p.ldc * OSIZE;
       store_row<OUT, FN>(out, col, p.N, in, dg);
       store_row<OUT, FN>(out + static_cast<long long>(p.N) * OSIZE, col, p.N, in, du);
     }

@@ -61,8 +61,8 @@ hipError_t validate(const FlashMoeFfnDesc* d, int tokens) {
   const bool mx = d->weights == FLASH_MOE_FFN_MXFP4;
   const int of = mx ? 32 : 8;
   if (d->hidden < of || d->hidden % of != 0 || d->intermediate < of || d->intermediate % of != 0 ||
-      d->hidden > kMaxStride || d->intermediate > kMaxStride / 2)
-    FMOE_FAIL(hipErrorInvalidValue, "H=%i, I=%i: multiples of %i up to %lld and half of that are admitted", d->hidden,
+      d->hidden > kMaxStride || d->intermediate >= kMaxStride / 2)
+    FMOE_FAIL(hipErrorInvalidValue, "H=%i, I=%i: multiples of %i, H up to %lld, I below half of that", d->hidden,
               d->intermediate, of, kMaxStride);
   if (mx && d->dtype != FLASH_MOE_BF16) FMOE_FAIL(hipErrorInvalidValue, "MXFP4 weights take bfloat16 tokens");
   if (tokens < 0) FMOE_FAIL(hipErrorInvalidValue, "%i tokens", tokens);
@@ -77,11 +77,19 @@ hipError_t validate_weights(const FlashMoeFfnDesc* d) {
   return hipSuccess;
 }
 
+// Rows of the library's own buffers do not lie a multiple of 4 KiB apart: a tile's rows would begin in the same few
+// channels of the L2 (8192 x 4096 x 4096, rows of A and B 8 KiB apart 208 to 228 us, 64 values more 194).
+long long apart(long long width, int dtype) { return width * static_cast<long long>(size_of(dtype)) % 4096 == 0 ? width + 64 : width; }
+
 // What a forward pass leaves for the backward pass: the two projections before the activation in
 // float32 and h in the layer's dtype; the gradients of the projections, the backward pass's own.
 size_t gu_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * 2 * d.intermediate * 4); }
-size_t h_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * d.intermediate * size_of(d.dtype)); }
-size_t dgu_bytes(const FlashMoeFfnDesc& d, int tokens) { return align_up(size_t(tokens) * 2 * d.intermediate * size_of(d.dtype)); }
+size_t h_bytes(const FlashMoeFfnDesc& d, int tokens) {
+  return align_up(size_t(tokens) * apart(d.intermediate, d.dtype) * size_of(d.dtype));
+}
+size_t dgu_bytes(const FlashMoeFfnDesc& d, int tokens) {
+  return align_up(size_t(tokens) * apart(2LL * d.intermediate, d.dtype) * size_of(d.dtype));
+}
 
 }  // namespace
 
@@ -117,12 +125,12 @@ int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx
   GemmArgs up{};
   up.a = x, up.b = d.w13, up.b_scales = static_cast<const unsigned char*>(d.w13_scales);
   up.c = h, up.gu = reinterpret_cast<float*>(keep);
-  up.lda = ldx, up.ldb = H, up.ldc = I;
+  up.lda = ldx, up.ldb = H, up.ldc = apart(I, d.dtype);
   up.M = tokens, up.N = I, up.K = H, up.act = d.activation;
   GemmArgs down{};
   down.a = h, down.b = d.w2, down.b_scales = static_cast<const unsigned char*>(d.w2_scales);
   down.c = y;
-  down.lda = I, down.ldb = I, down.ldc = ldy;
+  down.lda = up.ldc, down.ldb = I, down.ldc = ldy;
   down.M = tokens, down.N = H, down.K = I;
   if (mx) {
     FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_GATED, up, stream));
@@ -154,11 +162,12 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
       FMOE_FAIL(hipErrorInvalidValue, "null or unaligned workspace");
   }
   const char* keep = static_cast<const char*>(saved);
+  const long long ld_h = apart(I, d.dtype), ld_dgu = apart(2LL * I, d.dtype);
   if (tokens > 0 && (dx != nullptr || dw13 != nullptr)) {
     // dh = dy W2, and with it the gradients of both projections
     GemmArgs p{};
     p.a = dy, p.b = d.w2, p.c = workspace, p.gu = reinterpret_cast<float*>(const_cast<char*>(keep));
-    p.lda = lddy, p.ldb = I, p.ldc = 2LL * I;
+    p.lda = lddy, p.ldb = I, p.ldc = ld_dgu;
     p.M = tokens, p.N = I, p.K = H, p.act = d.activation;
     FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_SLOPE, p, stream));
   }
@@ -167,19 +176,19 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
   if (tokens > 0 && dx != nullptr) {
     GemmArgs& p = grads.dx;
     p.a = workspace, p.b = d.w13, p.c = dx;
-    p.lda = 2LL * I, p.ldb = H, p.ldc = lddx;
+    p.lda = ld_dgu, p.ldb = H, p.ldc = lddx;
     p.M = tokens, p.N = H, p.K = 2 * I;
   }
   if (dw13 != nullptr) {
     GemmArgs& p = grads.dw13;
     p.a = workspace, p.b = x, p.c = dw13;
-    p.lda = 2LL * I, p.ldb = ldx, p.ldc = H;
+    p.lda = ld_dgu, p.ldb = ldx, p.ldc = H;
     p.M = 2 * I, p.N = H, p.K = tokens;
   }
   if (dw2 != nullptr) {
     GemmArgs& p = grads.dw2;
     p.a = dy, p.b = keep + (tokens > 0 ? gu_bytes(d, tokens) : 0), p.c = dw2;
-    p.lda = lddy, p.ldb = I, p.ldc = I;
+    p.lda = lddy, p.ldb = ld_h, p.ldc = I;
     p.M = H, p.N = I, p.K = tokens;
   }
   FMOE_HIP_CHECK(fmoe::launch_ffn_grads(d.dtype, grads, stream));

@@ -283,7 +283,7 @@ enum { FLASH_MOE_FFN_ROW_MAJOR = 0, FLASH_MOE_FFN_MXFP4 = 1 };
 
 typedef struct FlashMoeFfnDesc {
   int hidden;       /* H, a multiple of 8 (MXFP4 weights: of 32), at most 2^20 */
-  int intermediate; /* I, likewise, at most 2^19 */
+  int intermediate; /* I, likewise, below 2^19 */
   int dtype;        /* FLASH_MOE_F32 or FLASH_MOE_BF16: tokens, outputs, gradients, row-major weights */
   int activation;   /* FLASH_MOE_ACT_*: g / (1 + exp(-g)), or GELU in its tanh form */
   int weights;      /* FLASH_MOE_FFN_*; MXFP4 (below) takes bfloat16 tokens and has no backward pass */
