@@ -84,6 +84,7 @@ C_ABI = {
     "flashMoeNoAllocStatus": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint), ctypes.c_void_p]),
     "flashMoeAbi": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_size_t)]),
     "flashMoeFfnBytes": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_int] + [ctypes.POINTER(ctypes.c_size_t)] * 3),
+    "flashMoeFfnSavingBytes": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "flashMoeFfnForward": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                           ctypes.c_longlong, ctypes.c_int] + [ctypes.c_void_p] * 3),
     "flashMoeFfnBackward": (ctypes.c_int, [ctypes.POINTER(FfnDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,

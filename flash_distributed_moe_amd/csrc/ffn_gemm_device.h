@@ -120,6 +120,18 @@ struct Fragments {
   }
 };
 
+// Workgroup `id`'s share of the tile's k: steps first .. first + count - 1. Splits of a tile lie a whole round of tiles
+// apart, so id becomes the tile's number.
+__device__ __forceinline__ void share_of(const GemmArgs& p, int steps, int& id, int& split, int& first, int& count) {
+  split = first = 0, count = steps;
+  if (p.splits > 1) {
+    const int tiles = p.grid_m * p.grid_n;
+    split = id / tiles, id -= split * tiles;
+    first = split * p.per;
+    count = steps - first < p.per ? steps - first : p.per;
+  }
+}
+
 // The workgroup's tile. Neighbouring workgroup numbers lie on different XCDs, each with an L2 of its
 // own, so an XCD gets a run of the order; the order walks GROUP tile rows column by column, so
 // that the tiles in flight on an XCD share rows of both operands.
@@ -211,6 +223,31 @@ __device__ __forceinline__ void store_row(void* row, int col, int columns, bool 
         trade(v[f], v[f + 1]);
         const int at = 8 * f + odd * 4;  // the second block's eight begin 4 before this lane's own column of it
         if (in && col + at < columns) store8(to + at, v[f], v[f + 1]);
+      }
+    }
+  }
+}
+
+// A split's sums as they are: of a gated product gate columns and, behind the N of them, up columns
+template <class S>
+__device__ __forceinline__ void write_partial(const GemmArgs& p, int split, int m0, int n0, Accumulators<S>& acc) {
+  constexpr int FN = S::FN, FM = S::FM;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  const long long ld = partial_ld(S::EPI == EPI_GATED ? 2 * p.N : p.N);
+  float* part = p.partial + split * (p.M * ld);
+#pragma unroll
+  for (int fm = 0; fm < FM; ++fm) {
+    const int m = m0 + wm * FM * 16 + dealt_row<FM>(fm, r);
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) {
+      if constexpr (S::EPI == EPI_GATED) {
+        const int col = n0 + wn * FN * 8 + gated_row<FN>(fn, 4 * g);
+        if (col < p.N) *reinterpret_cast<f32x4*>(part + m * ld + (fn >= FN / 2 ? p.N : 0) + col) = acc.v[fm][fn];
+      } else {
+        const int col = n0 + wn * FN * 16 + dealt_row<FN>(fn, 4 * g);
+        if (col < p.N) *reinterpret_cast<f32x4*>(part + m * ld + col) = acc.v[fm][fn];
       }
     }
   }

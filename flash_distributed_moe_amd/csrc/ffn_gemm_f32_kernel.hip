@@ -50,21 +50,22 @@ __device__ __forceinline__ Parts split(const float (&v)[8]) {
 
 constexpr float kSmallSum = 2.6469779601696886e-23f;  // 2^-75: weights up to 2^20 times values under 2^-103 sum to less
 
-// C[m, n] by itself
+// C[m, n] by itself, over k from `from` to `to`
 template <bool OUTER_A, bool OUTER_B>
-__device__ __noinline__ float plain_sum(const float* a, long long lda, const float* b, long long ldb, long long m, long long n, int K) {
+__device__ __noinline__ float plain_sum(const float* a, long long lda, const float* b, long long ldb, long long m, long long n, int from, int to) {
   const float* pa = OUTER_A ? a + m : a + m * lda;
   const float* pb = OUTER_B ? b + n : b + n * ldb;
   const long long sa = OUTER_A ? lda : 1, sb = OUTER_B ? ldb : 1;
   float sum = 0.0f;
-  for (int k = 0; k < K; ++k) sum = fmaf(pa[k * sa], pb[k * sb], sum);
+  for (int k = from; k < to; ++k) sum = fmaf(pa[k * sa], pb[k * sb], sum);
   return sum;
 }
 
 // Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
 template <class S>
 __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int id) {
-  int tile_m, tile_n;
+  int share, first, steps, tile_m, tile_n;
+  share_of(p, (p.K + S::STEP - 1) / S::STEP, id, share, first, steps);
   tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
@@ -82,15 +83,14 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
 #pragma unroll
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int steps = (p.K + S::STEP - 1) / S::STEP;
   // a group's turns: stages group, group + GROUPS, ...
   const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
     const int s = turn * S::GROUPS + group;
     if (S::GROUPS > 1 && s >= steps) return;
     char* to = mine + (turn & 1) * S::STAGE_BYTES;
-    load_a.load(to, s, p.K - s * S::STEP);
-    load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
+    load_a.load(to, first + s, p.K - (first + s) * S::STEP);
+    load_b.load(to + S::BM * 128, first + s, p.K - (first + s) * S::STEP);
   };
   if (turns > 0) load(0);
   for (int turn = 0; turn < turns; ++turn) {
@@ -130,6 +130,7 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
   add_groups<S>(lds, group, acc);
   if (group != 0) return;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int from = first * S::STEP, end = (first + steps) * S::STEP, to = end < p.K ? end : p.K;
 #pragma unroll
   for (int fm = 0; fm < S::FM; ++fm)
 #pragma unroll
@@ -157,10 +158,11 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
           in = n < p.N;
         }
         if (in) acc.v[fm][fn][i] = plain_sum<S::OUTER_A, S::OUTER_B>(static_cast<const float*>(p.a), p.lda, static_cast<const float*>(p.b),
-                                                                     p.ldb, m, n, p.K);
+                                                                     p.ldb, m, n, from, to);
       }
     }
-  write_results<S>(p, m0, n0, acc);
+  if (p.splits > 1) write_partial<S>(p, share, m0, n0, acc);
+  else write_results<S>(p, m0, n0, acc);
 }
 
 template <class S>
@@ -177,63 +179,79 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ffn_grads_f32_kernel(FfnGrads
   __shared__ __attribute__((aligned(128))) char lds[X::LDS_BYTES];
   const int id = blockIdx.x;
   if (id < p.begin[1]) {
-    if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile_f32<X>(p.dx, lds, id);
+    if (id < p.dx.grid_m * p.dx.grid_n * p.dx.splits) gemm_tile_f32<X>(p.dx, lds, id);
   } else {
     const bool second = id >= p.begin[2];
     const GemmArgs& dw = second ? p.dw2 : p.dw13;
     const int at = id - p.begin[second ? 2 : 1];
-    if (at < dw.grid_m * dw.grid_n) gemm_tile_f32<W>(dw, lds, at);
+    if (at < dw.grid_m * dw.grid_n * dw.splits) gemm_tile_f32<W>(dw, lds, at);
   }
 }
 
 template <class S>
-static hipError_t launch_f32(GemmArgs p, hipStream_t stream) {
+static hipError_t launch_f32(GemmArgs p, const TilePlan& plan, hipStream_t stream) {
   p.grid_m = (p.M + S::BM - 1) / S::BM;
   p.grid_n = (p.N + S::CN - 1) / S::CN;
-  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n;
+  p.splits = plan.splits, p.per = plan.per;
+  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n * p.splits;
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL(ffn_gemm_f32_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || p.splits == 1 ? e : launch_ffn_finish(0, S::EPI, p, stream);
 }
 
 // Large tiles split each value for more products, small ones fill more CUs, and groups of waves that share a tile's k fill
 // their waits. Measured on M=1001, N=768 gated, K=2048, 128 x 128 / 128 x 64 / 64 x 64 rows of A and B, us:
 // 114 / 76 / 65 in one group, 87 / 57 / 57 in two, 64 x 64 in four 64; M=1001, N=768, K=2048 with B's rows as k
 // 120 / 84 / 55, 97 / 60 / 38, 34; M=N=K=4096 641 / 739 / 830 in one.
-template <bool OA, bool OB, int EPI>
+static const TileCost kF32Ways[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 128, 1, 1.32, 2.7, 1.35}, {128, 64, 0, 1.1, 1.6, 0.72},
+                                    {64, 64, 0, 0.78, 0.98, 0.42}, {64, 64, 0.8, 0.54, 0.85, 0.45}, {64, 64, 1.8, 0.48, 0.95, 0.48}};
+static const TileCost kF32GatedWays[] = {{128, 64, 0, 1.7, 2.5, 1.25}, {128, 64, 1, 1.32, 2.7, 1.35}, {128, 32, 0, 1.1, 1.6, 0.72},
+                                         {64, 32, 0, 0.78, 0.98, 0.42}, {64, 32, 0.8, 0.54, 0.85, 0.45}, {64, 32, 1.8, 0.48, 0.95, 0.48}};
+
+static TilePlan plan_f32(int epi, const GemmArgs& p, bool split) {
+  return plan_tiles(epi == EPI_GATED ? kF32GatedWays : kF32Ways, 6, 32, p, epi == EPI_GATED ? 2 * p.N : p.N, split);
+}
+
+template <bool OB, int EPI>
 static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
-  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  static const TileCost ways[] = {{128, 128 / PER, 0, 1.7, 2.5, 1.25}, {128, 128 / PER, 1, 1.32, 2.7, 1.35},
-                                  {128, 64 / PER, 0, 1.1, 1.6, 0.72},  {64, 64 / PER, 0, 0.78, 0.98, 0.42},
-                                  {64, 64 / PER, 0.8, 0.54, 0.85, 0.45}, {64, 64 / PER, 1.8, 0.48, 0.95, 0.48}};
-  switch (pick_tile(ways, 6, 32, p)) {
-    case 0: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4>>(p, stream);
-    case 1: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 4, 2>>(p, stream);
-    case 2: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 4, 2>>(p, stream);
-    case 3: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
-    case 4: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
-    default: return launch_f32<GemmShape<KIND_F32, OA, OB, EPI, 2, 2, 2, 2, 4>>(p, stream);
+  const TilePlan chosen = plan_f32(EPI, p, p.partial != nullptr);
+  switch (chosen.way) {
+    case 0: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 4, 4>>(p, chosen, stream);
+    case 1: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 4, 4, 2>>(p, chosen, stream);
+    case 2: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 4, 2>>(p, chosen, stream);
+    case 3: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 2, 2>>(p, chosen, stream);
+    case 4: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 2, 2, 2>>(p, chosen, stream);
+    default: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 2, 2, 4>>(p, chosen, stream);
   }
 }
 
-hipError_t launch_ffn_gemm_f32(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
-  if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick_f32<false, false, EPI_GATED>(p, stream);
-  if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick_f32<false, true, EPI_SLOPE>(p, stream);
-  return oa || ob ? hipErrorInvalidValue : pick_f32<false, false, EPI_STORE>(p, stream);
+hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream) {
+  if (epi == EPI_SLOPE) return pick_f32<true, EPI_SLOPE>(p, stream);
+  return epi == EPI_GATED ? pick_f32<false, EPI_GATED>(p, stream) : pick_f32<false, EPI_STORE>(p, stream);
 }
 
-hipError_t launch_ffn_grads_f32(FfnGrads p, hipStream_t stream) {
-  static const TileCost ways[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 64, 0, 1.1, 1.6, 0.72}, {64, 64, 0, 0.78, 0.98, 0.45}};
-  const int way = pick_grads_tile(ways, 3, 32, p);
-  const long long blocks = lay_out_grads(p, ways[way].rows, ways[way].columns);
+size_t ffn_gemm_f32_bytes(bool, int epi, const GemmArgs& p) {
+  return partial_bytes(plan_f32(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
+}
+
+static const TileCost kF32GradsWays[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 64, 0, 1.1, 1.6, 0.72}, {64, 64, 0, 0.78, 0.98, 0.45}};
+
+hipError_t launch_ffn_grads_f32(FfnGrads p, float* partial, size_t room, hipStream_t stream) {
+  GradsPlan chosen = plan_grads(kF32GradsWays, 3, 32, p, partial != nullptr);
+  if (plan_bytes(chosen, p) > room) chosen = plan_grads(kF32GradsWays, 3, 32, p, false);
+  const long long blocks = lay_out_grads(chosen, kF32GradsWays[chosen.way], p, partial);
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (way == 0) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 4>), grid, dim3(256), 0, stream, p);
-  else if (way == 1) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 2>), grid, dim3(256), 0, stream, p);
+  if (chosen.way == 0) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 4>), grid, dim3(256), 0, stream, p);
+  else if (chosen.way == 1) hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 4, 2>), grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL((ffn_grads_f32_kernel<2, 2, 2, 2>), grid, dim3(256), 0, stream, p);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : launch_ffn_finish_grads(0, p, stream);
 }
+
+size_t ffn_grads_f32_bytes(const FfnGrads& p) { return plan_bytes(plan_grads(kF32GradsWays, 3, 32, p, true), p); }
 
 }  // namespace fmoe

@@ -6,7 +6,8 @@ namespace fmoe {
 // Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
 template <class S>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) {
-  int tile_m, tile_n;
+  int split, first, steps, tile_m, tile_n;
+  share_of(p, (p.K + S::STEP - 1) / S::STEP, id, split, first, steps);
   tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
@@ -24,15 +25,14 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) 
 #pragma unroll
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int steps = (p.K + S::STEP - 1) / S::STEP;
   // a group's turns: stages group, group + GROUPS, ...
   const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
     const int s = turn * S::GROUPS + group;
     if (S::GROUPS > 1 && s >= steps) return;
     char* to = mine + (turn & 1) * S::STAGE_BYTES;
-    load_a.load(to, s, p.K - s * S::STEP);
-    load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
+    load_a.load(to, first + s, p.K - (first + s) * S::STEP);
+    load_b.load(to + S::BM * 128, first + s, p.K - (first + s) * S::STEP);
   };
   if (turns > 0) load(0);
   for (int turn = 0; turn < turns; ++turn) {
@@ -56,7 +56,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) 
     }
   }
   add_groups<S>(lds, group, acc);
-  if (group == 0) write_results<S>(p, m0, n0, acc);
+  if (group != 0) return;
+  if (p.splits > 1) write_partial<S>(p, split, m0, n0, acc);
+  else write_results<S>(p, m0, n0, acc);
 }
 
 template <class S>
@@ -75,24 +77,26 @@ __global__ __launch_bounds__(WM * WN * 64) void ffn_grads_kernel(FfnGrads p) {
   __shared__ __attribute__((aligned(128))) char lds[X::LDS_BYTES];
   const int id = blockIdx.x;
   if (id < p.begin[1]) {
-    if (id < p.dx.grid_m * p.dx.grid_n) gemm_tile<X>(p.dx, lds, id);
+    if (id < p.dx.grid_m * p.dx.grid_n * p.dx.splits) gemm_tile<X>(p.dx, lds, id);
   } else {
     const bool second = id >= p.begin[2];
     const GemmArgs& dw = second ? p.dw2 : p.dw13;
     const int at = id - p.begin[second ? 2 : 1];
-    if (at < dw.grid_m * dw.grid_n) gemm_tile<W>(dw, lds, at);
+    if (at < dw.grid_m * dw.grid_n * dw.splits) gemm_tile<W>(dw, lds, at);
   }
 }
 
 template <class S>
-static hipError_t launch(GemmArgs p, hipStream_t stream) {
+static hipError_t launch(GemmArgs p, const TilePlan& plan, hipStream_t stream) {
   p.grid_m = (p.M + S::BM - 1) / S::BM;
   p.grid_n = (p.N + S::CN - 1) / S::CN;
-  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n;
+  p.splits = plan.splits, p.per = plan.per;
+  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n * p.splits;
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL(ffn_gemm_kernel<S>, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || p.splits == 1 ? e : launch_ffn_finish(1, S::EPI, p, stream);
 }
 
 // Measured, 256 x 256 (sixteen waves) / 128 x 128 (eight) / 64 x 64 (four) rows of A and B, us: M=8192, N=4096, K=12288
@@ -102,49 +106,63 @@ static hipError_t launch(GemmArgs p, hipStream_t stream) {
 // registers gain nothing beside that. The library's product of that size takes 529.)
 // Where CUs have one small tile or two, groups of waves share its k, 1 / 2 / 4 groups: M=64, N=2048, K=6144 28.2 / 20.9 / 17.9;
 // M=1024 50.1 / 38.2 / 53.1; M=333, N=1344, K=736 6.0 / 5.5 / 5.8; 128 x 128 in 1 / 2: M=1024, N=2048, K=6144 65.1 / 52.2.
-template <bool OA, bool OB, int EPI>
+static const TileCost kWays[] = {{256, 256, 0, 1.45, 2.9, 1.45}, {128, 128, 0, 0.55, 0.96, 0.48}, {128, 128, 0.8, 0.45, 1.0, 0.55},
+                                 {64, 64, 0, 0.33, 0.5, 0.21},   {64, 64, 0.8, 0.25, 0.37, 0.245}, {64, 64, 1.8, 0.2, 0.53, 0.27}};
+static const TileCost kGatedWays[] = {{256, 128, 0, 1.45, 2.9, 1.45}, {128, 64, 0, 0.55, 0.96, 0.48}, {128, 64, 0.8, 0.45, 1.0, 0.55},
+                                      {64, 32, 0, 0.33, 0.5, 0.21},   {64, 32, 0.8, 0.25, 0.37, 0.245}, {64, 32, 1.8, 0.2, 0.53, 0.27}};
+
+static TilePlan plan(int epi, const GemmArgs& p, bool split) {
+  return plan_tiles(epi == EPI_GATED ? kGatedWays : kWays, 6, 64, p, epi == EPI_GATED ? 2 * p.N : p.N, split);
+}
+
+template <bool OB, int EPI>
 static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
-  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  static const TileCost ways[] = {{256, 256 / PER, 0, 1.45, 2.9, 1.45}, {128, 128 / PER, 0, 0.55, 0.96, 0.48},
-                                  {128, 128 / PER, 0.8, 0.45, 1.0, 0.55}, {64, 64 / PER, 0, 0.33, 0.5, 0.21},
-                                  {64, 64 / PER, 0.8, 0.25, 0.37, 0.245}, {64, 64 / PER, 1.8, 0.2, 0.53, 0.27}};
-  switch (pick_tile(ways, 6, 64, p)) {
-    case 0: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 4, 4, 4>>(p, stream);
-    case 1: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 2, 2, 4>>(p, stream);
-    case 2: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 4, 2, 2, 4, 2>>(p, stream);
-    case 3: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2>>(p, stream);
-    case 4: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2, 2>>(p, stream);
-    default: return launch<GemmShape<KIND_BF16, OA, OB, EPI, 2, 2, 2, 2, 4>>(p, stream);
+  const TilePlan chosen = plan(EPI, p, p.partial != nullptr);
+  switch (chosen.way) {
+    case 0: return launch<GemmShape<KIND_BF16, false, OB, EPI, 4, 4, 4, 4>>(p, chosen, stream);
+    case 1: return launch<GemmShape<KIND_BF16, false, OB, EPI, 4, 2, 2, 4>>(p, chosen, stream);
+    case 2: return launch<GemmShape<KIND_BF16, false, OB, EPI, 4, 2, 2, 4, 2>>(p, chosen, stream);
+    case 3: return launch<GemmShape<KIND_BF16, false, OB, EPI, 2, 2, 2, 2>>(p, chosen, stream);
+    case 4: return launch<GemmShape<KIND_BF16, false, OB, EPI, 2, 2, 2, 2, 2>>(p, chosen, stream);
+    default: return launch<GemmShape<KIND_BF16, false, OB, EPI, 2, 2, 2, 2, 4>>(p, chosen, stream);
   }
 }
 
-hipError_t launch_ffn_grads_bf16(FfnGrads p, hipStream_t stream) {
-  static const TileCost ways[] = {{256, 256, 0, 1.55, 3.1, 1.55}, {128, 128, 0, 0.6, 0.98, 0.49}, {64, 64, 0, 0.33, 0.5, 0.22}};
-  const int way = pick_grads_tile(ways, 3, 64, p), side = ways[way].rows;
-  const long long blocks = lay_out_grads(p, side, side);
+static const TileCost kGradsWays[] = {{256, 256, 0, 1.55, 3.1, 1.55}, {128, 128, 0, 0.6, 0.98, 0.49}, {64, 64, 0, 0.33, 0.5, 0.22}};
+
+static hipError_t launch_ffn_grads_bf16(FfnGrads p, float* partial, size_t room, hipStream_t stream) {
+  GradsPlan chosen = plan_grads(kGradsWays, 3, 64, p, partial != nullptr);
+  if (plan_bytes(chosen, p) > room) chosen = plan_grads(kGradsWays, 3, 64, p, false);
+  const long long blocks = lay_out_grads(chosen, kGradsWays[chosen.way], p, partial);
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (way == 0) hipLaunchKernelGGL((ffn_grads_kernel<4, 4, 4, 4>), grid, dim3(1024), 0, stream, p);
-  else if (way == 1) hipLaunchKernelGGL((ffn_grads_kernel<4, 2, 2, 4>), grid, dim3(512), 0, stream, p);
+  if (chosen.way == 0) hipLaunchKernelGGL((ffn_grads_kernel<4, 4, 4, 4>), grid, dim3(1024), 0, stream, p);
+  else if (chosen.way == 1) hipLaunchKernelGGL((ffn_grads_kernel<4, 2, 2, 4>), grid, dim3(512), 0, stream, p);
   else hipLaunchKernelGGL((ffn_grads_kernel<2, 2, 2, 2>), grid, dim3(256), 0, stream, p);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : launch_ffn_finish_grads(1, p, stream);
 }
 
-static hipError_t launch_ffn_gemm_bf16(bool oa, bool ob, int epi, const GemmArgs& p, hipStream_t stream) {
-  if (epi == EPI_GATED) return oa || ob ? hipErrorInvalidValue : pick<false, false, EPI_GATED>(p, stream);
-  if (epi == EPI_SLOPE) return oa || !ob ? hipErrorInvalidValue : pick<false, true, EPI_SLOPE>(p, stream);
-  return oa || ob ? hipErrorInvalidValue : pick<false, false, EPI_STORE>(p, stream);
+hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
+  if (k_outer_b != (epi == EPI_SLOPE)) return hipErrorInvalidValue;
+  if (!k_outer_b && ffn_skinny_takes(p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
+  if (dtype != 1) return launch_ffn_gemm_f32(k_outer_b, epi, p, stream);
+  if (epi == EPI_SLOPE) return pick<true, EPI_SLOPE>(p, stream);
+  return epi == EPI_GATED ? pick<false, EPI_GATED>(p, stream) : pick<false, EPI_STORE>(p, stream);
 }
 
-hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
-  if (!k_outer_a && !k_outer_b && ffn_skinny_takes(dtype, p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
-  return dtype == 1 ? launch_ffn_gemm_bf16(k_outer_a, k_outer_b, epi, p, stream)
-                    : launch_ffn_gemm_f32(k_outer_a, k_outer_b, epi, p, stream);
+size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p) {
+  if (!k_outer_b && ffn_skinny_takes(p)) return 0;
+  return dtype != 1 ? ffn_gemm_f32_bytes(k_outer_b, epi, p) : partial_bytes(plan(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
-hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, hipStream_t stream) {
-  return dtype == 1 ? launch_ffn_grads_bf16(p, stream) : launch_ffn_grads_f32(p, stream);
+hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream) {
+  return dtype == 1 ? launch_ffn_grads_bf16(p, partial, room, stream) : launch_ffn_grads_f32(p, partial, room, stream);
+}
+
+size_t ffn_grads_bytes(int dtype, const FfnGrads& p) {
+  return dtype != 1 ? ffn_grads_f32_bytes(p) : plan_bytes(plan_grads(kGradsWays, 3, 64, p, true), p);
 }
 
 }  // namespace fmoe

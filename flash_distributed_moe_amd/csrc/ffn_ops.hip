@@ -91,6 +91,51 @@ size_t dgu_bytes(const FlashMoeFfnDesc& d, int tokens) {
   return align_up(size_t(tokens) * apart(2LL * d.intermediate, d.dtype) * size_of(d.dtype));
 }
 
+
+// The products of a call, without their matrices; a workspace holds the partial sums of one whose k is split
+// (one product at a time has some) behind what the passes lay there.
+GemmArgs up_sizes(const FlashMoeFfnDesc& d, int tokens) {
+  GemmArgs p{};
+  p.M = tokens, p.N = d.intermediate, p.K = d.hidden, p.act = d.activation;
+  return p;
+}
+GemmArgs down_sizes(const FlashMoeFfnDesc& d, int tokens) {
+  GemmArgs p{};
+  p.M = tokens, p.N = d.hidden, p.K = d.intermediate;
+  return p;
+}
+fmoe::FfnGrads grads_sizes(const FlashMoeFfnDesc& d, int tokens, bool dx, bool dw13, bool dw2) {
+  const int H = d.hidden, I = d.intermediate;
+  fmoe::FfnGrads g{};
+  if (tokens > 0 && dx) g.dx.M = tokens, g.dx.N = H, g.dx.K = 2 * I;
+  if (dw13) g.dw13.M = 2 * I, g.dw13.N = H, g.dw13.K = tokens;
+  if (dw2) g.dw2.M = H, g.dw2.N = I, g.dw2.K = tokens;
+  return g;
+}
+size_t product_bytes(const FlashMoeFfnDesc& d, int epi, const GemmArgs& p) {
+  return d.weights == FLASH_MOE_FFN_MXFP4 ? fmoe::mxfp4_gemm_bytes(false, epi, p)
+                                          : fmoe::ffn_gemm_bytes(d.dtype, epi == fmoe::EPI_SLOPE, epi, p);
+}
+size_t forward_partial_bytes(const FlashMoeFfnDesc& d, int tokens) {
+  const size_t up = product_bytes(d, fmoe::EPI_GATED, up_sizes(d, tokens));
+  const size_t down = product_bytes(d, fmoe::EPI_STORE, down_sizes(d, tokens));
+  return align_up(up > down ? up : down);
+}
+// Fewer gradients than three are split differently: x's alone and the weights' alone have their room, and what finds
+// none is not split.
+size_t backward_partial_bytes(const FlashMoeFfnDesc& d, int tokens) {
+  const size_t of[] = {product_bytes(d, fmoe::EPI_SLOPE, up_sizes(d, tokens)),
+                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, true, true, true)),
+                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, true, false, false)),
+                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, false, true, true))};
+  size_t most = 0;
+  for (const size_t bytes : of) most = bytes > most ? bytes : most;
+  return align_up(most);
+}
+float* as_partial(void* workspace, size_t behind, size_t bytes) {
+  return workspace == nullptr || bytes == 0 ? nullptr : reinterpret_cast<float*>(static_cast<char*>(workspace) + behind);
+}
+
 }  // namespace
 
 extern "C" {
@@ -99,8 +144,19 @@ int flashMoeFfnBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* saved, siz
   const hipError_t v = validate(desc, tokens);
   if (v != hipSuccess) return v;
   if (saved != nullptr) *saved = gu_bytes(*desc, tokens) + h_bytes(*desc, tokens);
-  if (forward != nullptr) *forward = h_bytes(*desc, tokens);
-  if (backward != nullptr) *backward = dgu_bytes(*desc, tokens);
+  if (forward != nullptr) *forward = h_bytes(*desc, tokens) + forward_partial_bytes(*desc, tokens);
+  if (backward != nullptr) {
+    const bool mx = desc->weights == FLASH_MOE_FFN_MXFP4;  // no backward pass
+    *backward = dgu_bytes(*desc, tokens) + (mx ? 0 : backward_partial_bytes(*desc, tokens));
+  }
+  return hipSuccess;
+}
+
+int flashMoeFfnSavingBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* forward) {
+  const hipError_t v = validate(desc, tokens);
+  if (v != hipSuccess) return v;
+  if (forward == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result pointer");
+  *forward = forward_partial_bytes(*desc, tokens);
   return hipSuccess;
 }
 
@@ -122,22 +178,20 @@ int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx
   char* keep = static_cast<char*>(saved);
   void* h = keep != nullptr ? keep + gu_bytes(d, tokens) : workspace;
 
-  GemmArgs up{};
+  GemmArgs up = up_sizes(d, tokens), down = down_sizes(d, tokens);
+  up.partial = down.partial = as_partial(workspace, keep != nullptr ? 0 : h_bytes(d, tokens), forward_partial_bytes(d, tokens));
   up.a = x, up.b = d.w13, up.b_scales = static_cast<const unsigned char*>(d.w13_scales);
   up.c = h, up.gu = reinterpret_cast<float*>(keep);
   up.lda = ldx, up.ldb = H, up.ldc = apart(I, d.dtype);
-  up.M = tokens, up.N = I, up.K = H, up.act = d.activation;
-  GemmArgs down{};
   down.a = h, down.b = d.w2, down.b_scales = static_cast<const unsigned char*>(d.w2_scales);
   down.c = y;
   down.lda = up.ldc, down.ldb = I, down.ldc = ldy;
-  down.M = tokens, down.N = H, down.K = I;
   if (mx) {
     FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_GATED, up, stream));
     FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_STORE, down, stream));
   } else {
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, false, fmoe::EPI_GATED, up, stream));
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, false, fmoe::EPI_STORE, down, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_GATED, up, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_STORE, down, stream));
   }
   return hipSuccess;
 }
@@ -163,35 +217,34 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
   }
   const char* keep = static_cast<const char*>(saved);
   const long long ld_h = apart(I, d.dtype), ld_dgu = apart(2LL * I, d.dtype);
+  const size_t room = backward_partial_bytes(d, tokens);
+  float* partial = as_partial(workspace, dgu_bytes(d, tokens), room);
   if (tokens > 0 && (dx != nullptr || dw13 != nullptr)) {
     // dh = dy W2, and with it the gradients of both projections
-    GemmArgs p{};
+    GemmArgs p = up_sizes(d, tokens);
+    p.partial = partial;
     p.a = dy, p.b = d.w2, p.c = workspace, p.gu = reinterpret_cast<float*>(const_cast<char*>(keep));
     p.lda = lddy, p.ldb = I, p.ldc = ld_dgu;
-    p.M = tokens, p.N = I, p.K = H, p.act = d.activation;
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, true, fmoe::EPI_SLOPE, p, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, fmoe::EPI_SLOPE, p, stream));
   }
   // the weights' gradients sum over the tokens; of no tokens they are zeros
-  fmoe::FfnGrads grads{};
+  fmoe::FfnGrads grads = grads_sizes(d, tokens, dx != nullptr, dw13 != nullptr, dw2 != nullptr);
   if (tokens > 0 && dx != nullptr) {
     GemmArgs& p = grads.dx;
     p.a = workspace, p.b = d.w13, p.c = dx;
     p.lda = ld_dgu, p.ldb = H, p.ldc = lddx;
-    p.M = tokens, p.N = H, p.K = 2 * I;
   }
   if (dw13 != nullptr) {
     GemmArgs& p = grads.dw13;
     p.a = workspace, p.b = x, p.c = dw13;
     p.lda = ld_dgu, p.ldb = ldx, p.ldc = H;
-    p.M = 2 * I, p.N = H, p.K = tokens;
   }
   if (dw2 != nullptr) {
     GemmArgs& p = grads.dw2;
     p.a = dy, p.b = keep + (tokens > 0 ? gu_bytes(d, tokens) : 0), p.c = dw2;
     p.lda = lddy, p.ldb = ld_h, p.ldc = I;
-    p.M = H, p.N = I, p.K = tokens;
   }
-  FMOE_HIP_CHECK(fmoe::launch_ffn_grads(d.dtype, grads, stream));
+  FMOE_HIP_CHECK(fmoe::launch_ffn_grads(d.dtype, grads, partial, room, stream));
   return hipSuccess;
 }
 
@@ -228,7 +281,9 @@ int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes
   if (rows < 0 || n < 0 || k < 32 || k % 32 != 0 || k > kMaxStride)
     FMOE_FAIL(hipErrorInvalidValue, "%i x %i x %i (the last a multiple of 32 up to %lld)", rows, n, k, kMaxStride);
   if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result pointer");
-  *bytes = 0;
+  GemmArgs p{};
+  p.M = rows, p.N = n, p.K = k;
+  *bytes = rows == 0 || n == 0 ? 0 : fmoe::mxfp4_gemm_bytes(x_format == FLASH_MOE_MXFP4, fmoe::EPI_STORE, p);
   return hipSuccess;
 }
 
@@ -257,6 +312,7 @@ int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long 
   p.b = codes, p.b_scales = static_cast<const unsigned char*>(scales), p.ldb = k;
   p.c = y, p.ldc = ldy;
   p.M = rows, p.N = n, p.K = k;
+  p.partial = as_partial(workspace, 0, bytes);
   FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(mx, fmoe::EPI_STORE, p, static_cast<hipStream_t>(stream)));
   return hipSuccess;
 }

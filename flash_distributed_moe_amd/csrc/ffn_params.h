@@ -1,6 +1,7 @@
 // What the dense gated feed-forward block's and MXFP4's host code and kernels share.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <stddef.h>
 
 namespace fmoe {
 
@@ -18,7 +19,12 @@ struct GemmArgs {
   int M, N, K;
   int act;
   int grid_m, grid_n;
+  // A product whose k is dealt to `splits` workgroups a tile, `per` steps each: their sums go to partial,
+  // [splits, M, partial_ld(columns of B's rows)] float32, and a kernel of its own finishes. One split: unused.
+  float* partial;
+  int splits, per;
 };
+__host__ __device__ inline long long partial_ld(int columns) { return (columns + 7LL) / 8 * 8; }
 
 // A way to tile a product: rows and columns of C a workgroup takes, and what it costs a CU in microseconds, measured:
 // once, and for a step of the k loop while the CU has one such workgroup, two, and for each while it has more.
@@ -29,17 +35,38 @@ struct TileCost {
 inline double tile_count(const TileCost& way, const GemmArgs& p) {
   return static_cast<double>((p.M + way.rows - 1LL) / way.rows) * ((p.N + way.columns - 1LL) / way.columns);
 }
-// Which of `count` ways is done first on 256 CUs; step: k of a step.
-inline int pick_tile(const TileCost* ways, int count, int step, const GemmArgs& p) {
-  int best = 0;
-  double least = 0;
+// Which way is done first on 256 CUs, and with how many workgroups sharing a tile's k.
+struct TilePlan {
+  int way, splits, per;
+};
+// What it takes to write and read `splits` partial sums of M x columns and to launch the kernel that does the latter:
+// an estimate, a short kernel's time and the rate of a copy
+inline double finish_cost(int splits, double sums) { return splits > 1 ? 3.0 + splits * sums * 8 / 4.5e6 : 0.0; }
+inline double tile_cost(const TileCost& way, double tiles, int steps) {
+  const long long each = static_cast<long long>((tiles + 255) / 256);  // tiles of the fullest CU
+  return way.once + steps * (each <= 1 ? way.one : each == 2 ? way.two : each * way.more);
+}
+// step: k of a step; columns: rows of B; split: whether there is memory for partial sums. Measured, a whole call
+// without and with splits, us: T=87, H=144, I=6520 bf16 39 and 18 (the second product has 6 tiles of 64 x 64);
+// MXFP4 weights, T=67, H=384, I=7680 40 and 22; a product with MXFP4 weights, M=703, N=591, K=7520 36 and 24; a training
+// step, T=2480, H=416, I=8520 bf16 547 and 406.
+inline TilePlan plan_tiles(const TileCost* ways, int count, int step, const GemmArgs& p, int columns, bool split) {
+  const int steps = (p.K + step - 1) / step;
+  TilePlan best = {0, 1, steps};
+  double least = -1;
   for (int i = 0; i < count; ++i) {
-    const TileCost& way = ways[i];
-    const long long each = static_cast<long long>((tile_count(way, p) + 255) / 256);  // tiles of the fullest CU
-    const double cost = way.once + (p.K + step - 1) / step * (each <= 1 ? way.one : each == 2 ? way.two : each * way.more);
-    if (i == 0 || cost < least) best = i, least = cost;
+    const double tiles = tile_count(ways[i], p);
+    for (int splits = 1; splits == 1 || (split && tiles * splits <= 1024 && splits <= 64 && splits * 4 <= steps);
+         splits += splits < 4 ? 1 : splits / 2) {
+      const int per = (steps + splits - 1) / splits, used = steps == 0 ? 1 : (steps + per - 1) / per;
+      const double cost = tile_cost(ways[i], tiles * used, per) + finish_cost(used, static_cast<double>(p.M) * columns);
+      if (least < 0 || cost < least) best = {i, used, per}, least = cost;
+    }
   }
   return best;
+}
+inline size_t partial_bytes(const TilePlan& plan, int M, int columns) {
+  return plan.splits > 1 ? static_cast<size_t>(plan.splits) * M * partial_ld(columns) * 4 : 0;
 }
 
 enum { ACT_SILU = 0, ACT_GELU_TANH = 1 };
@@ -52,50 +79,93 @@ struct FfnGrads {
   int begin[3];
 };
 
-// Workgroup ranges for tiles of rows x columns, each begun on a multiple of 8 (see tile_of); their number.
-inline long long lay_out_grads(FfnGrads& p, int rows, int columns) {
-  GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
-  long long at = 0;
-  for (int i = 0; i < 3; ++i) {
-    of[i]->grid_m = (of[i]->M + rows - 1) / rows;
-    of[i]->grid_n = (of[i]->N + columns - 1) / columns;
-    p.begin[i] = static_cast<int>(at < 0x7FFFFFFF ? at : 0x7FFFFFFF);
-    at = (at + static_cast<long long>(of[i]->grid_m) * of[i]->grid_n + 7) / 8 * 8;
-  }
-  return at;
-}
-
-// Which of `count` ways is done with all three first on 256 CUs, which take tiles as they come: the work
-// spread over all of them and, as the ends never meet, half of the shortest tile; or the longest tile alone.
-inline int pick_grads_tile(const TileCost* ways, int count, int step, const FfnGrads& p) {
+// Which of `count` ways is done with all three first on 256 CUs, which take tiles as they come: the work spread over
+// all of them and, as the ends never meet, half of the shortest tile; or the longest tile alone. Splits are
+// for what would be longest; x's gradient and the weights' have numbers of their own.
+struct GradsPlan {
+  int way;
+  TilePlan of[3];
+};
+inline GradsPlan plan_grads(const TileCost* ways, int count, int step, const FfnGrads& p, bool split) {
   const GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
-  int best = 0;
-  double least = 0;
+  GradsPlan best{};
+  double least = -1;
   for (int i = 0; i < count; ++i) {
-    double work = 0, longest = 0, shortest = 0;
-    for (const GemmArgs* g : of) {
-      const double tiles = tile_count(ways[i], *g);
-      if (tiles == 0) continue;
-      const double steps = (g->K + step - 1) / step;
-      work += tiles * steps * ways[i].more / 256;
-      longest = longest > steps * ways[i].one ? longest : steps * ways[i].one;
-      shortest = shortest == 0 || steps * ways[i].more < shortest ? steps * ways[i].more : shortest;
+    bool bound = false;  // by the work, which more splits do not lessen
+    for (int sx = 1; (sx == 1 || (split && sx <= 64 && p.dx.M > 0)) && !bound; sx *= 2) {
+      bound = false;
+      for (int sw = 1; sw <= (split ? 64 : 1) && !bound; sw *= 2) {
+        GradsPlan plan{i, {}};
+        double work = 0, longest = 0, shortest = 0, finish = 0, sums = 0;
+        bool fine = true;
+        for (int k = 0; k < 3; ++k) {
+          const GemmArgs& g = *of[k];
+          const int steps = (g.K + step - 1) / step, wanted = k == 0 ? sx : sw;
+          const int per = (steps + wanted - 1) / wanted, used = steps == 0 ? 1 : (steps + per - 1) / per;
+          plan.of[k] = {i, used, per};
+          if (g.M == 0) continue;
+          fine = fine && (wanted == 1 || wanted * 4 <= steps);
+          work += tile_count(ways[i], g) * steps * ways[i].more / 256;
+          longest = longest > per * ways[i].one ? longest : per * ways[i].one;
+          shortest = shortest == 0 || per * ways[i].more < shortest ? per * ways[i].more : shortest;
+          if (used > 1) finish = 3.0, sums += static_cast<double>(used) * g.M * g.N;
+        }
+        const double cost = (work + shortest / 2 > longest ? work + shortest / 2 : longest) + finish + sums * 8 / 4.5e6;
+        if (!fine) break;
+        if (least < 0 || cost < least) best = plan, least = cost;
+        bound = work + shortest / 2 >= longest;
+        if (bound && sw > 1) {
+          bound = false;
+          break;
+        }
+      }
     }
-    const double cost = work + shortest / 2 > longest ? work + shortest / 2 : longest;
-    if (i == 0 || cost < least) best = i, least = cost;
   }
   return best;
 }
 
-// A matrix product in bfloat16 or float32 (k_outer_*: the operand's rows are k); epi as above.
-hipError_t launch_ffn_gemm(int dtype, bool k_outer_a, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
+// Workgroup ranges and partial sums of a plan; the number of workgroups (each range begun on a multiple of 8, see
+// tile_of). partial: plan_bytes of memory, or NULL without splits.
+inline long long lay_out_grads(const GradsPlan& plan, const TileCost& way, FfnGrads& p, float* partial) {
+  GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
+  long long at = 0;
+  for (int i = 0; i < 3; ++i) {
+    GemmArgs& g = *of[i];
+    g.grid_m = (g.M + way.rows - 1) / way.rows;
+    g.grid_n = (g.N + way.columns - 1) / way.columns;
+    g.splits = plan.of[i].splits, g.per = plan.of[i].per, g.partial = partial;
+    if (g.M > 0) partial += partial_bytes(plan.of[i], g.M, g.N) / 4;
+    p.begin[i] = static_cast<int>(at < 0x7FFFFFFF ? at : 0x7FFFFFFF);
+    at = (at + static_cast<long long>(g.grid_m) * g.grid_n * g.splits + 7) / 8 * 8;
+  }
+  return at;
+}
+inline size_t plan_bytes(const GradsPlan& plan, const FfnGrads& p) {
+  const GemmArgs* of[] = {&p.dx, &p.dw13, &p.dw2};
+  size_t bytes = 0;
+  for (int i = 0; i < 3; ++i) bytes += of[i]->M > 0 ? partial_bytes(plan.of[i], of[i]->M, of[i]->N) : 0;
+  return bytes;
+}
+
+// A matrix product in bfloat16 or float32 (k_outer_b: a row of B is one k); epi as above. *_bytes: memory for
+// p.partial that a call with these sizes can use (0: none); without it k is not split.
+hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
+size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p);
+hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
+size_t ffn_gemm_f32_bytes(bool k_outer_b, int epi, const GemmArgs& p);
+// (partial of `room` bytes: gradients that need more, or find none, are not split)
+hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream);
+size_t ffn_grads_bytes(int dtype, const FfnGrads& p);
+hipError_t launch_ffn_grads_f32(FfnGrads p, float* partial, size_t room, hipStream_t stream);
+size_t ffn_grads_f32_bytes(const FfnGrads& p);
+// What a split product's partial sums become; of the three gradients those that were split.
+hipError_t launch_ffn_finish(int dtype, int epi, const GemmArgs& p, hipStream_t stream);
+hipError_t launch_ffn_finish_grads(int dtype, const FfnGrads& p, hipStream_t stream);
 // MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
 hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
-hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, hipStream_t stream);
-hipError_t launch_ffn_grads_f32(FfnGrads p, hipStream_t stream);
-hipError_t launch_ffn_gemm_f32(bool k_outer_a, bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
+size_t mxfp4_gemm_bytes(bool x_mxfp4, int epi, const GemmArgs& p);
 // The same for few rows, where these take the call (A and B with their k inside the rows).
-bool ffn_skinny_takes(int dtype, const GemmArgs& p);
+bool ffn_skinny_takes(const GemmArgs& p);
 bool mxfp4_skinny_takes(bool x_mxfp4, const GemmArgs& p);
 hipError_t launch_ffn_skinny(int dtype, bool gated, const GemmArgs& p, hipStream_t stream);
 hipError_t launch_mxfp4_skinny(bool x_mxfp4, bool gated, const GemmArgs& p, hipStream_t stream);

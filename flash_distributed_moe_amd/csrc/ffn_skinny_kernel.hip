@@ -354,7 +354,7 @@ static hipError_t pick(bool gated, const GemmArgs& p, hipStream_t stream) {
   return p.M <= 8 ? go_plain<KIND, 1>(p, stream) : p.M <= 16 ? go_plain<KIND, 2>(p, stream) : go_plain<KIND, 4>(p, stream);
 }
 
-bool ffn_skinny_takes(int dtype, const GemmArgs& p) { return p.M <= 32; }
+bool ffn_skinny_takes(const GemmArgs& p) { return p.M <= 32; }
 
 // (the scales of a workgroup's rows have to fit LDS beside the rest, and are read 4 bytes and more at a time)
 bool mxfp4_skinny_takes(bool x_mxfp4, const GemmArgs& p) {

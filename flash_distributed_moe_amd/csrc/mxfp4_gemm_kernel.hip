@@ -151,8 +151,9 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(Gemm
   typedef ScaleLoader<S::BN, S::THREADS, S::FN, false, 8, FOURS> ScaleB;
   constexpr int TILES = S::STAGE_BYTES, STAGE = TILES + ScaleA::BYTES + ScaleB::BYTES;
   __shared__ __attribute__((aligned(128))) char lds[2 * S::GROUPS * STAGE];
-  int tile_m, tile_n;
-  tile_of(p, blockIdx.x, tile_m, tile_n);
+  int id = blockIdx.x, split, first, steps, tile_m, tile_n;
+  share_of(p, (p.K + S::STEP - 1) / S::STEP, id, split, first, steps);
+  tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
@@ -170,15 +171,15 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(Gemm
   Accumulators<S> acc;
   clear(acc);
 
-  const int steps = (p.K + S::STEP - 1) / S::STEP, turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
     const int s = turn * S::GROUPS + group;
     if (S::GROUPS > 1 && s >= steps) return;
     char* to = mine + (turn & 1) * STAGE;
-    load_a.load(to, s, p.K - s * S::STEP);
-    load_b.load(to + S::BM * 128, s, p.K - s * S::STEP);
-    scale_a.load(to + TILES, s);
-    scale_b.load(to + TILES + ScaleA::BYTES, s);
+    load_a.load(to, first + s, p.K - (first + s) * S::STEP);
+    load_b.load(to + S::BM * 128, first + s, p.K - (first + s) * S::STEP);
+    scale_a.load(to + TILES, first + s);
+    scale_b.load(to + TILES + ScaleA::BYTES, first + s);
   };
   load(0);
   for (int turn = 0; turn < turns; ++turn) {
@@ -186,8 +187,8 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(Gemm
     char* now = mine + (turn & 1) * STAGE;
     __builtin_amdgcn_s_waitcnt(0);  // this wave's pieces of the stage have landed ...
     if (S::GROUPS == 1 || s < steps) {
-      scale_a.landed(now + TILES, s);
-      scale_b.landed(now + TILES + ScaleA::BYTES, s);
+      scale_a.landed(now + TILES, first + s);
+      scale_b.landed(now + TILES + ScaleA::BYTES, first + s);
     }
     __syncthreads();  // ... and everybody's; all are done with the other buffer
     if (turn + 1 < turns) load(turn + 1);
@@ -216,7 +217,9 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(Gemm
     }
   }
   add_groups<S>(lds, group, acc);
-  if (group == 0) write_results<S>(p, m0, n0, acc);
+  if (group != 0) return;
+  if (p.splits > 1) write_partial<S>(p, split, m0, n0, acc);
+  else write_results<S>(p, m0, n0, acc);
 }
 
 template <class S>
@@ -228,8 +231,9 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
   constexpr int SUMS = (S::GROUPS - 1) * S::BM * S::BN * 4, ALL = 2 * S::GROUPS * STAGE;
   static_assert(S::FN % 4 == 0, "pairs of blocks on one side");
   __shared__ __attribute__((aligned(128))) char lds[SUMS > ALL ? SUMS : ALL];
-  int tile_m, tile_n;
-  tile_of(p, blockIdx.x, tile_m, tile_n);
+  int id = blockIdx.x, split, first, steps, tile_m, tile_n;
+  share_of(p, (p.K + 64 - 1) / 64, id, split, first, steps);
+  tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
@@ -245,14 +249,14 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
   Accumulators<S> acc;
   clear(acc);
 
-  const int steps = (p.K + 63) / 64, turns = (steps + S::GROUPS - 1) / S::GROUPS;
+  const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
     const int s = turn * S::GROUPS + group;
     if (S::GROUPS > 1 && s >= steps) return;
     char* to = mine + (turn & 1) * STAGE;
-    load_a.load(to, s, p.K - s * 64);
-    load_b.load(to + S::BM * 128, s, p.K - s * 64);
-    scale_b.load(to + TILES, s);
+    load_a.load(to, first + s, p.K - (first + s) * 64);
+    load_b.load(to + S::BM * 128, first + s, p.K - (first + s) * 64);
+    scale_b.load(to + TILES, first + s);
   };
   // rows of A and weights of a stage's half from LDS
   auto a_at = [&](const char* now, int fm, int half) {
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
     const int s = turn * S::GROUPS + group;
     char* now = mine + (turn & 1) * STAGE;
     __builtin_amdgcn_s_waitcnt(0);
-    if (S::GROUPS == 1 || s < steps) scale_b.landed(now + TILES, s);
+    if (S::GROUPS == 1 || s < steps) scale_b.landed(now + TILES, first + s);
     __syncthreads();
     if (turn + 1 < turns) load(turn + 1);
     if (S::GROUPS > 1 && s >= steps) continue;
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
 #pragma unroll
     for (int f = 0; f < S::FN; ++f) {
       codes[f] = *(const FFN_LDS u32x2*)codes_at(now, f);
-      scale[f] = scale_at(now, f, s);
+      scale[f] = scale_at(now, f, first + s);
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -293,70 +297,83 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
     }
   }
   add_groups<S, sizeof(lds)>(lds, group, acc);
-  if (group == 0) write_results<S>(p, m0, n0, acc);
+  if (group != 0) return;
+  if (p.splits > 1) write_partial<S>(p, split, m0, n0, acc);
+  else write_results<S>(p, m0, n0, acc);
 }
 
 template <class S, typename Kernel>
-static hipError_t launch(Kernel kernel, GemmArgs p, hipStream_t stream) {
+static hipError_t launch(Kernel kernel, GemmArgs p, const TilePlan& plan, hipStream_t stream) {
   p.grid_m = (p.M + S::BM - 1) / S::BM;
   p.grid_n = (p.N + S::CN - 1) / S::CN;
-  const long long tiles = static_cast<long long>(p.grid_m) * p.grid_n;
-  if (tiles == 0) return hipSuccess;
-  if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
-  return hipGetLastError();
+  p.splits = plan.splits, p.per = plan.per;
+  const long long blocks = static_cast<long long>(p.grid_m) * p.grid_n * p.splits;
+  if (blocks == 0) return hipSuccess;
+  if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(S::THREADS * S::GROUPS), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || p.splits == 1 ? e : launch_ffn_finish(1, S::EPI, p, stream);
 }
 
 // Measured at N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four) / 64 x 128 in four groups / 64 x 64 in four
 // groups of two waves, us: M=2048 112 / 140 / 226 / 304; M=1024 99 / 67 / 114 / 153; M=256 96 / 48 / 29 / 38; M=64
 // 88 / 44 / 24 / 17.
+static const TileCost kWeightsWays[] = {{256, 256, 0, 1.7, 3.4, 1.7}, {128, 128, 0, 0.68, 1.02, 0.53}, {64, 128, 1, 0.4, 0.9, 0.45},
+                                        {64, 64, 1, 0.22, 0.55, 0.28}};
+static const TileCost kGatedWeightsWays[] = {{256, 128, 0, 1.7, 3.4, 1.7}, {128, 64, 0, 0.68, 1.02, 0.53}, {64, 64, 1, 0.4, 0.9, 0.45},
+                                             {64, 32, 1, 0.22, 0.55, 0.28}};
+// Measured at N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four) / the same in two groups / 64 x 64 in two
+// groups, us: M=4096 86 / 99 / 122 / 163; M=512 32 / 19 / 17 / 22; M=128 28 / 16 / 14 / 8.6.
+static const TileCost kBothWays[] = {{256, 256, 0, 2.5, 5.2, 2.6}, {128, 128, 0, 1.0, 1.7, 0.77}, {128, 128, 0.5, 0.87, 1.9, 0.95},
+                                     {64, 64, 0.5, 0.35, 0.65, 0.31}};
+
+static TilePlan plan(bool both, int epi, const GemmArgs& p, bool split) {
+  if (both) return plan_tiles(kBothWays, 4, 256, p, p.N, split);
+  return epi == EPI_GATED ? plan_tiles(kGatedWeightsWays, 4, 64, p, 2 * p.N, split) : plan_tiles(kWeightsWays, 4, 64, p, p.N, split);
+}
+
 template <int EPI>
 static hipError_t launch_weights(const GemmArgs& p, hipStream_t stream) {
-  constexpr int PER = EPI == EPI_GATED ? 2 : 1;
-  static const TileCost ways[] = {{256, 256 / PER, 0, 1.7, 3.4, 1.7}, {128, 128 / PER, 0, 0.68, 1.02, 0.53},
-                                  {64, 128 / PER, 1, 0.4, 0.9, 0.45}, {64, 64 / PER, 1, 0.22, 0.55, 0.28}};
-  switch (pick_tile(ways, 4, 64, p)) {
+  const TilePlan chosen = plan(false, EPI, p, p.partial != nullptr);
+  switch (chosen.way) {
     case 0: {
       typedef GemmShape<KIND_BF16, false, false, EPI, 4, 4, 4, 4> S;
-      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+      return launch<S>(mxfp4_weights_kernel<S>, p, chosen, stream);
     }
     case 1: {
       typedef GemmShape<KIND_BF16, false, false, EPI, 2, 2, 4, 4> S;
-      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+      return launch<S>(mxfp4_weights_kernel<S>, p, chosen, stream);
     }
     case 2: {
       typedef GemmShape<KIND_BF16, false, false, EPI, 2, 2, 2, 4, 4> S;
-      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+      return launch<S>(mxfp4_weights_kernel<S>, p, chosen, stream);
     }
     default: {
       typedef GemmShape<KIND_BF16, false, false, EPI, 2, 1, 2, 4, 4> S;
-      return launch<S>(mxfp4_weights_kernel<S>, p, stream);
+      return launch<S>(mxfp4_weights_kernel<S>, p, chosen, stream);
     }
   }
 }
 
-// Measured at N=8192, K=4096, 256 x 256 (sixteen waves) / 128 x 128 (four) / the same in two groups / 64 x 64 in two
-// groups, us: M=4096 86 / 99 / 122 / 163; M=512 32 / 19 / 17 / 22; M=128 28 / 16 / 14 / 8.6.
 template <bool FOURS>
 static hipError_t launch_both(const GemmArgs& p, hipStream_t stream) {
-  static const TileCost ways[] = {{256, 256, 0, 2.5, 5.2, 2.6}, {128, 128, 0, 1.0, 1.7, 0.77}, {128, 128, 0.5, 0.87, 1.9, 0.95},
-                                  {64, 64, 0.5, 0.35, 0.65, 0.31}};
-  switch (pick_tile(ways, 4, 256, p)) {
+  const TilePlan chosen = plan(true, EPI_STORE, p, p.partial != nullptr);
+  switch (chosen.way) {
     case 0: {
       typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 4, 4, 4, 4> S;
-      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, chosen, stream);
     }
     case 1: {
       typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4> S;
-      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, chosen, stream);
     }
     case 2: {
       typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 4, 4, 2> S;
-      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, chosen, stream);
     }
     default: {
       typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 2, 2, 2, 2, 2> S;
-      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, stream);
+      return launch<S>(mxfp4_both_kernel<S, FOURS>, p, chosen, stream);
     }
   }
 }
@@ -372,6 +389,11 @@ hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stre
   if (mxfp4_skinny_takes(x_mxfp4, p)) return launch_mxfp4_skinny(x_mxfp4, epi == EPI_GATED, p, stream);
   if (x_mxfp4) return scales_on_fours(p) ? launch_both<true>(p, stream) : launch_both<false>(p, stream);
   return epi == EPI_GATED ? launch_weights<EPI_GATED>(p, stream) : launch_weights<EPI_STORE>(p, stream);
+}
+
+size_t mxfp4_gemm_bytes(bool x_mxfp4, int epi, const GemmArgs& p) {
+  if (mxfp4_skinny_takes(x_mxfp4, p)) return 0;
+  return partial_bytes(plan(x_mxfp4, epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
 }  // namespace fmoe

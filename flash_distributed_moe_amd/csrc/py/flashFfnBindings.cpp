@@ -124,11 +124,13 @@ std::tuple<at::Tensor, at::Tensor> ffn_forward(const at::Tensor& x, const at::Te
   const DeviceGuard guard(x.device());
   const Rows rows = rows_of(x, "x");
   size_t saved_bytes = 0, work_bytes = 0;
-  check_hip(flashMoeFfnBytes(&d, rows.count, &saved_bytes, &work_bytes, nullptr), "flashMoeFfnBytes");
+  check_hip(flashMoeFfnBytes(&d, rows.count, save ? &saved_bytes : nullptr, save ? nullptr : &work_bytes, nullptr),
+            "flashMoeFfnBytes");
+  if (save) check_hip(flashMoeFfnSavingBytes(&d, rows.count, &work_bytes), "flashMoeFfnSavingBytes");
   at::Tensor y = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
   at::Tensor saved, work;
   if (save) saved = bytes_on(x, saved_bytes);
-  else work = bytes_on(x, work_bytes);
+  if (work_bytes > 0) work = bytes_on(x, work_bytes);
   check_hip(flashMoeFfnForward(&d, pointer(rows.t), rows.stride, pointer(y), d.hidden, rows.count, pointer(saved),
                                pointer(work), current_stream()),
             "flashMoeFfnForward");

@@ -296,10 +296,14 @@ typedef struct FlashMoeFfnDesc {
 /* Device bytes a batch of `tokens` needs (any result may be NULL): what a forward pass keeps for
  * the backward pass, and the workspaces of both. Only the description's sizes are read. */
 int flashMoeFfnBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* saved, size_t* forward, size_t* backward);
+/* The workspace of a forward pass that keeps `saved` (0: none); it may be NULL, and then long sums are not
+ * shared between workgroups, which takes longer where few of them have a part of the result. */
+int flashMoeFfnSavingBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* forward);
 
 /* x [tokens, H] rows ldx values apart, y likewise with ldy (whole 16 bytes; at most 2^20 values); y may
  * be x if its rows lie the same way. Every pointer begins on 16 bytes. saved: NULL, or device memory
- * that flashMoeFfnBackward is given afterwards. workspace may be NULL when saved is not. 0 tokens: nothing
+ * that flashMoeFfnBackward is given afterwards. workspace: of flashMoeFfnBytes, or with saved of
+ * flashMoeFfnSavingBytes or NULL. 0 tokens: nothing
  * is enqueued. hipErrorInvalidValue for whatever is wrong with the arguments; nothing is enqueued then. */
 int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx, void* y, long long ldy, int tokens,
                        void* saved, void* workspace, void* stream);

@@ -36,6 +36,24 @@ def test_sizes():
     assert rc == 0 and saved >= (1 << 20) * 12288 * 10
 
 
+def test_workspaces_of_shared_sums():
+    def saving(d, tokens):
+        n = ctypes.c_size_t(0)
+        assert _lib.load().flashMoeFfnSavingBytes(ctypes.byref(d), tokens, ctypes.byref(n)) == 0
+        return n.value
+
+    for weights in (0, 1):
+        few = desc(hidden=384, intermediate=7680, weights=weights)  # 67 x 384 results of 7680 products each
+        assert saving(few, 67) >= 2 * 67 * 384 * 4
+        assert sizes(few, 67)[1][1] >= 67 * 7680 * 2 + saving(few, 67)
+        assert saving(few, 0) == 0
+    assert saving(desc(hidden=4096, intermediate=12288), 8192) == 0
+    assert saving(desc(), 100) == 0
+    assert sizes(desc(hidden=4096, intermediate=12288), 8192)[1][2] < 8192 * (2 * 12288 + 64) * 2 + 1024
+    assert _lib.load().flashMoeFfnSavingBytes(ctypes.byref(desc()), 1, None) == BAD
+    assert _lib.load().flashMoeFfnSavingBytes(ctypes.byref(desc()), -1, ctypes.byref(ctypes.c_size_t(0))) == BAD
+
+
 @pytest.mark.parametrize("kw", [dict(dtype=2), dict(dtype=-1), dict(activation=2), dict(weights=2), dict(hidden=0), dict(hidden=60),
                                 dict(hidden=(1 << 20) + 8), dict(intermediate=4), dict(intermediate=(1 << 19) + 8),
                                 dict(weights=1, hidden=72), dict(weights=1, intermediate=40), dict(weights=1, dtype=0)])

@@ -66,6 +66,49 @@ def test_large_tiles(ops, T, H, I, dtype):
         ffn_case.check(t, *want[name], "%s of T=%d H=%d I=%d" % (name, T, H, I))
 
 
+# few tiles and long sums, shared between workgroups: gated (H long), output and x's gradient (I long), slope (H long),
+# the weights' gradients (T long)
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("T,H,I", [(67, 384, 7680), (9, 136, 4104), (50, 4360, 72), (8200, 72, 40), (2100, 200, 3000), (1, 136, 5000)])
+def test_long_sums(ops, T, H, I, dtype):
+    x, w13, w2, dy = make(T, H, I, DTYPES[dtype], seed=7)
+    want = ffn_case.block(x, w13, w2, "gelu_tanh", dy)
+    got = run(ops, x, w13, w2, dy, "gelu_tanh")
+    for name, t in got.items():
+        ffn_case.check(t, *want[name], "%s of T=%d H=%d I=%d" % (name, T, H, I))
+    for name, t in run(ops, x, w13, w2, dy, "gelu_tanh").items():
+        assert torch.equal(t, got[name]), name
+    for only in ("dx", "dw13", "dw2"):
+        leaves = [v.detach().requires_grad_(n == only) for n, v in (("dx", x), ("dw13", w13), ("dw2", w2))]
+        leaf = next(v for v in leaves if v.requires_grad)
+        one, = torch.autograd.grad(ops.gated_ffn(*leaves, activation="gelu_tanh"), [leaf], dy)
+        ffn_case.check(one, *want[only], "%s alone of T=%d H=%d I=%d" % (only, T, H, I))
+
+
+def test_saving_without_a_workspace():
+    """A C caller's forward pass that keeps its results needs no workspace, and then shares no sums; with one it
+    writes nothing behind it."""
+    lib = _lib.load()
+    T, H, I = 67, 384, 7680
+    x, w13, w2, _ = make(T, H, I, torch.bfloat16, seed=8)
+    want = ffn_case.block(x, w13, w2, "silu")["y"]
+    d = _lib.FfnDesc(H, I, _lib.BF16, _lib.ACT_SILU, _lib.FFN_ROW_MAJOR, w13.data_ptr(), w2.data_ptr(), None, None)
+    saved, work = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert lib.flashMoeFfnBytes(ctypes.byref(d), T, ctypes.byref(saved), None, None) == 0
+    assert lib.flashMoeFfnSavingBytes(ctypes.byref(d), T, ctypes.byref(work)) == 0
+    assert work.value > 0
+    keep = torch.full((saved.value + 256,), 0xA5, dtype=torch.uint8, device="cuda")
+    room = torch.full((work.value + 256,), 0xA5, dtype=torch.uint8, device="cuda")
+    for workspace in (None, room.data_ptr()):
+        y = torch.empty_like(x)
+        rc = lib.flashMoeFfnForward(ctypes.byref(d), x.data_ptr(), H, y.data_ptr(), H, T, keep.data_ptr(), workspace,
+                                    torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert rc == 0
+        ffn_case.check(y, *want, "y")
+    assert (keep[saved.value:] == 0xA5).all() and (room[work.value:] == 0xA5).all()
+
+
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_gradients_against_differences(ops, dtype):
     """Central differences of the float64 definition along random directions: the analytic gradients
