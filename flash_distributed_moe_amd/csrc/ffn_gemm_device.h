@@ -152,11 +152,23 @@ struct Accumulators {
   f32x4 v[S::FM][S::FN];
 };
 
+struct __attribute__((packed, aligned(2))) Anywhere16 {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(2))) Anywhere8 {
+  u32x2 v;
+};
 __device__ __forceinline__ void store8(unsigned short* to, const f32x4& a, const f32x4& b) {
-  *reinterpret_cast<u32x4*>(to) = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
+  reinterpret_cast<Anywhere16*>(to)->v = u32x4{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
 }
 __device__ __forceinline__ void store4(unsigned short* to, const f32x4& a) {
-  *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
+  reinterpret_cast<Anywhere8*>(to)->v = u32x2{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3])};
+}
+// the first `count` of eight
+__device__ __forceinline__ void store_some(unsigned short* to, int count, const f32x4& a, const f32x4& b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < count) to[j] = static_cast<unsigned short>(pack_bf16(j < 4 ? a[j & 3] : b[j & 3], 0.0f) & 0xFFFF);
 }
 
 // The groups' sums of a tile, into the first group's, in the groups' order. Of the others nobody is left to write results.
@@ -197,7 +209,8 @@ __device__ __forceinline__ void trade(f32x4& a, f32x4& b) {
 }
 
 // A lane's results v[COUNT] of one row of C: block f's are columns col + 8 f + 0..3 (col: with the lane's own 4 * (g % 2)).
-// bfloat16 rows of a matrix whose width is no multiple of 8 begin anywhere and are written value by value.
+// bfloat16 rows of a matrix whose width is no multiple of 8 begin anywhere: the same wide writes, which memory takes at
+// any address, but value by value across a row's end.
 // Every lane of a wave takes part, `in` says whether its row exists.
 template <int KIND, int COUNT>
 __device__ __forceinline__ void store_row(void* row, int col, int columns, bool in, f32x4 (&v)[COUNT]) {
@@ -207,14 +220,9 @@ __device__ __forceinline__ void store_row(void* row, int col, int columns, bool 
       if (in && col + 8 * f < columns) *reinterpret_cast<f32x4*>(static_cast<float*>(row) + col + 8 * f) = v[f];
   } else {
     unsigned short* to = static_cast<unsigned short*>(row) + col;
-    if (columns & 7) {
-#pragma unroll
-      for (int f = 0; f < COUNT; ++f)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (in && col + 8 * f + i < columns) to[8 * f + i] = static_cast<unsigned short>(pack_bf16(v[f][i], 0.0f) & 0xFFFF);
-    } else if constexpr (COUNT == 1) {
-      if (in && col < columns) store4(to, v[0]);
+    if constexpr (COUNT == 1) {
+      if (in && col + 4 <= columns) store4(to, v[0]);
+      else if (in && col < columns) store_some(to, columns - col, v[0], v[0]);
     } else {
       static_assert(COUNT % 2 == 0, "pairs of blocks");
       const int odd = (threadIdx.x >> 4) & 1;
@@ -222,7 +230,8 @@ __device__ __forceinline__ void store_row(void* row, int col, int columns, bool 
       for (int f = 0; f < COUNT; f += 2) {
         trade(v[f], v[f + 1]);
         const int at = 8 * f + odd * 4;  // the second block's eight begin 4 before this lane's own column of it
-        if (in && col + at < columns) store8(to + at, v[f], v[f + 1]);
+        if (in && col + at + 8 <= columns) store8(to + at, v[f], v[f + 1]);
+        else if (in && col + at < columns) store_some(to + at, columns - col - at, v[f], v[f + 1]);
       }
     }
   }
