@@ -179,7 +179,8 @@ int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx
   void* h = keep != nullptr ? keep + gu_bytes(d, tokens) : workspace;
 
   GemmArgs up = up_sizes(d, tokens), down = down_sizes(d, tokens);
-  up.partial = down.partial = as_partial(workspace, keep != nullptr ? 0 : h_bytes(d, tokens), forward_partial_bytes(d, tokens));
+  // (MXFP4 weights whose scales' address counts too may plan otherwise than flashMoeFfnBytes, which does not see it)
+  up.partial = down.partial = as_partial(workspace, keep != nullptr ? 0 : h_bytes(d, tokens), mx ? forward_partial_bytes(d, tokens) : 1);
   up.a = x, up.b = d.w13, up.b_scales = static_cast<const unsigned char*>(d.w13_scales);
   up.c = h, up.gu = reinterpret_cast<float*>(keep);
   up.lda = ldx, up.ldb = H, up.ldc = apart(I, d.dtype);
@@ -217,7 +218,9 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
   }
   const char* keep = static_cast<const char*>(saved);
   const long long ld_h = apart(I, d.dtype), ld_dgu = apart(2LL * I, d.dtype);
-  const size_t room = backward_partial_bytes(d, tokens);
+  // gradients that backward_partial_bytes counts find their room by themselves
+  const bool counted = (dw13 != nullptr) == (dw2 != nullptr);
+  const size_t room = counted ? ~size_t{0} : backward_partial_bytes(d, tokens);
   float* partial = as_partial(workspace, dgu_bytes(d, tokens), room);
   if (tokens > 0 && (dx != nullptr || dw13 != nullptr)) {
     // dh = dy W2, and with it the gradients of both projections
