@@ -5,12 +5,27 @@
 
 namespace fmoe {
 
+constexpr int EIGHT = 8;       // splits a thread asks for at a time
+constexpr int THREADS = 64;    // few results are on many CUs
+
 // four neighbours of a row, `at` values from its beginning
 __device__ __forceinline__ f32x4 sum_splits(const GemmArgs& p, long long ld, long long row, int at) {
   const float* from = p.partial + row * ld + at;
   const long long apart = p.M * ld;
-  f32x4 sum = *reinterpret_cast<const f32x4*>(from);
-  for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(from + s * apart);
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  int s = 0;
+  for (; s + EIGHT <= p.splits; s += EIGHT) {
+    f32x4 v[EIGHT];
+#pragma unroll
+    for (int i = 0; i < EIGHT; ++i) v[i] = *reinterpret_cast<const f32x4*>(from + (s + i) * apart);
+#pragma unroll
+    for (int i = 0; i < EIGHT; ++i) sum += v[i];
+  }
+  f32x4 v[EIGHT];
+#pragma unroll
+  for (int i = 0; i < EIGHT; ++i) v[i] = s + i < p.splits ? *reinterpret_cast<const f32x4*>(from + (s + i) * apart) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < EIGHT; ++i) sum += v[i];
   return sum;
 }
 
@@ -73,18 +88,18 @@ __device__ __forceinline__ void finish_four(const GemmArgs& p, long long at) {
 }
 
 template <bool F32, int EPI>
-__global__ __launch_bounds__(256) void ffn_finish_kernel(GemmArgs p) {
-  finish_four<F32, EPI>(p, blockIdx.x * 256LL + threadIdx.x);
+__global__ __launch_bounds__(THREADS) void ffn_finish_kernel(GemmArgs p) {
+  finish_four<F32, EPI>(p, blockIdx.x * static_cast<long long>(THREADS) + threadIdx.x);
 }
 
 // begin: the first workgroup of each gradient's
 template <bool F32>
-__global__ __launch_bounds__(256) void ffn_finish_grads_kernel(FfnGrads p) {
+__global__ __launch_bounds__(THREADS) void ffn_finish_grads_kernel(FfnGrads p) {
   const int id = blockIdx.x, which = id >= p.begin[2] ? 2 : id >= p.begin[1] ? 1 : 0;
-  finish_four<F32, EPI_STORE>(which == 0 ? p.dx : which == 1 ? p.dw13 : p.dw2, (id - p.begin[which]) * 256LL + threadIdx.x);
+  finish_four<F32, EPI_STORE>(which == 0 ? p.dx : which == 1 ? p.dw13 : p.dw2, (id - p.begin[which]) * static_cast<long long>(THREADS) + threadIdx.x);
 }
 
-static long long blocks_for(const GemmArgs& p) { return (static_cast<long long>(p.M) * ((p.N + 3) / 4) + 255) / 256; }
+static long long blocks_for(const GemmArgs& p) { return (static_cast<long long>(p.M) * ((p.N + 3) / 4) + THREADS - 1) / THREADS; }
 
 hipError_t launch_ffn_finish(int dtype, int epi, const GemmArgs& p, hipStream_t stream) {
   const long long blocks = blocks_for(p);
@@ -93,7 +108,7 @@ hipError_t launch_ffn_finish(int dtype, int epi, const GemmArgs& p, hipStream_t 
                                                                                                         : ffn_finish_kernel<false, EPI_SLOPE>)
                            : (epi == EPI_STORE ? ffn_finish_kernel<true, EPI_STORE> : epi == EPI_GATED ? ffn_finish_kernel<true, EPI_GATED>
                                                                                                        : ffn_finish_kernel<true, EPI_SLOPE>);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -108,7 +123,7 @@ hipError_t launch_ffn_finish_grads(int dtype, const FfnGrads& grads, hipStream_t
   if (at == 0) return hipSuccess;
   if (at > 0x7FFFFFFF) return hipErrorInvalidValue;
   auto kernel = dtype == 1 ? ffn_finish_grads_kernel<false> : ffn_finish_grads_kernel<true>;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(at)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(at)), dim3(THREADS), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -41,7 +41,7 @@ struct TilePlan {
 };
 // What it takes to write and read `splits` partial sums of M x columns and to launch the kernel that does the latter:
 // an estimate, a short kernel's time and the rate of a copy
-inline double finish_cost(int splits, double sums) { return splits > 1 ? 3.0 + splits * sums * 8 / 4.5e6 : 0.0; }
+inline double finish_cost(int splits, double sums) { return splits > 1 ? 4.0 + splits * sums * 8 / 4.5e6 : 0.0; }
 inline double tile_cost(const TileCost& way, double tiles, int steps) {
   const long long each = static_cast<long long>((tiles + 255) / 256);  // tiles of the fullest CU
   return way.once + steps * (each <= 1 ? way.one : each == 2 ? way.two : each * way.more);
@@ -108,7 +108,7 @@ inline GradsPlan plan_grads(const TileCost* ways, int count, int step, const Ffn
           work += tile_count(ways[i], g) * steps * ways[i].more / 256;
           longest = longest > per * ways[i].one ? longest : per * ways[i].one;
           shortest = shortest == 0 || per * ways[i].more < shortest ? per * ways[i].more : shortest;
-          if (used > 1) finish = 3.0, sums += static_cast<double>(used) * g.M * g.N;
+          if (used > 1) finish = 4.0, sums += static_cast<double>(used) * g.M * g.N;
         }
         const double cost = (work + shortest / 2 > longest ? work + shortest / 2 : longest) + finish + sums * 8 / 4.5e6;
         if (!fine) break;
