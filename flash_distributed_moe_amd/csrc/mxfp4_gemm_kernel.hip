@@ -219,7 +219,7 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_both_kernel(Gemm
   add_groups<S>(lds, group, acc);
   if (group != 0) return;
   if (p.splits > 1) write_partial<S>(p, split, m0, n0, acc);
-  else write_results<S>(p, m0, n0, acc);
+  else write_results<S, S::EPI == EPI_STORE>(p, m0, n0, acc);
 }
 
 template <class S>
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(S::THREADS * S::GROUPS) void mxfp4_weights_kernel(G
   add_groups<S, sizeof(lds)>(lds, group, acc);
   if (group != 0) return;
   if (p.splits > 1) write_partial<S>(p, split, m0, n0, acc);
-  else write_results<S>(p, m0, n0, acc);
+  else write_results<S, S::EPI == EPI_STORE>(p, m0, n0, acc);
 }
 
 template <class S, typename Kernel>
