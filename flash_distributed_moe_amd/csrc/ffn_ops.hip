@@ -307,7 +307,8 @@ int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long 
   }
   if (codes == nullptr || scales == nullptr || !aligned16(codes))
     FMOE_FAIL(hipErrorInvalidValue, "null codes or scales pointer, or codes that do not begin on 16 bytes");
-  if (y == nullptr || ldy < n) FMOE_FAIL(hipErrorInvalidValue, "y: null, or rows %lld values apart", ldy);
+  if (y == nullptr || ldy < n || (reinterpret_cast<uintptr_t>(y) & 1) != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "y: null, at an odd address, or rows %lld values apart", ldy);
   if (n % 8 == 0 && (!aligned16(y) || ldy % 8 != 0))
     FMOE_FAIL(hipErrorInvalidValue, "y: rows of a multiple of 8 values begin on 16 bytes");
   GemmArgs p{};

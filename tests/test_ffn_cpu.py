@@ -114,7 +114,7 @@ def test_conversions_refuse(kw, capfd):
 
 @pytest.mark.parametrize("kw", [dict(fmt=0), dict(fmt=3), dict(x=None), dict(x=0x1004), dict(ldx=60), dict(k=80), dict(n=-1), dict(rows=-1),
                                 dict(codes=None), dict(codes=0x2004), dict(scales=None), dict(y=None), dict(y=0x5002), dict(ldy=7),
-                                dict(ldy=12), dict(fmt=2, ldx=128), dict(fmt=2, x_scales=None)])
+                                dict(ldy=12), dict(n=7, ldy=7, y=0x5001), dict(fmt=2, ldx=128), dict(fmt=2, x_scales=None)])
 def test_product_refuses(kw, capfd):
     a = dict(fmt=_lib.BF16, x=0x1000, x_scales=0x4000, ldx=64, rows=3, codes=0x2000, scales=0x3000, n=8, k=64, y=0x5000, ldy=8)
     a.update(kw)

@@ -163,6 +163,47 @@ def test_strides_and_leading_dimensions(ops, dtype):
         ffn_case.check(leaf.grad, *want[name], name + " of a sum")
 
 
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_broadcast_rows_and_gradients(ops, dtype):
+    """A row of x that all tokens share, and an output's gradient that is one number or lies transposed."""
+    dt = DTYPES[dtype]
+    T, H, I = 19, 72, 40
+    x, w13, w2, dy = make(T, H, I, dt, seed=9)
+    one = x[:1]
+    want = ffn_case.block(one.expand(T, H), w13, w2, "silu", torch.ones_like(x))
+    leaves = [v.detach().requires_grad_() for v in (one, w13, w2)]
+    ops.gated_ffn(leaves[0].expand(T, H), *leaves[1:]).sum().backward()
+    dx, far = want["dx"]
+    # autograd adds the rows' gradients in float32 and rounds once
+    total = 2 * T * 2.0 ** -24 * (dx.abs() + far).sum(0) + far.sum(0)
+    ffn_case.check(leaves[0].grad, dx.sum(0)[None], (total + ffn_case.HALF[dt] * (dx.sum(0).abs() + total))[None], "shared row")
+    for name, leaf in (("dw13", leaves[1]), ("dw2", leaves[2])):
+        ffn_case.check(leaf.grad, *want[name], name)
+    plain = run(ops, x, w13, w2, dy, "silu")
+    for other in (dy.t().contiguous().t(), torch.cat((dy, dy), 1)[:, :H]):
+        for name, v in run(ops, x, w13, w2, other, "silu").items():
+            assert torch.equal(v, plain[name]), name
+
+
+def test_graph_kept_and_weights_used_twice(ops):
+    T, H, I = 23, 64, 48
+    x, w13, w2, dy = make(T, H, I, torch.float32, seed=10)
+    leaves = [v.detach().requires_grad_() for v in (x, w13, w2)]
+    y = ops.gated_ffn(*leaves)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaves, dy)
+    # the same block twice, one output the other's input: the weights' gradients add up
+    mid = ops.gated_ffn(*leaves)
+    got = torch.autograd.grad(ops.gated_ffn(mid, *leaves[1:]), leaves, dy)
+    second = run(ops, mid.detach(), w13, w2, dy, "silu")
+    below = run(ops, x, w13, w2, second["dx"], "silu")
+    assert torch.equal(got[0], below["dx"])
+    assert torch.equal(got[1], second["dw13"] + below["dw13"]) and torch.equal(got[2], second["dw2"] + below["dw2"])
+
+
 def test_no_tokens(ops):
     x, w13, w2, dy = make(4, 64, 32, torch.bfloat16)
     got = run(ops, x[:0], w13, w2, dy[:0], "silu")

@@ -107,7 +107,8 @@ def check_product(got, x, w):
 PRODUCTS = [(1, 8, 32), (1, 1, 32), (2, 129, 96), (5, 136, 4096), (16, 64, 64), (17, 300, 160), (31, 257, 2048), (64, 128, 512),
             (65, 384, 288), (130, 257, 320), (257, 520, 544), (300, 1000, 1056), (33, 1000, 384), (257, 136, 640), (3841, 3600, 384),
             (3841, 3600, 160), (1024, 8200, 256), (256, 8200, 512), (64, 8200, 1056), (520, 8192, 2080),
-            (40, 37, 5120), (93, 200, 7520), (703, 72, 4096)]
+            (40, 37, 5120), (93, 200, 7520), (703, 72, 4096),
+            (8, 300, 16384), (16, 300, 16384), (32, 300, 16384), (32, 300, 16416)]  # the longest rows whose scales fit LDS, and longer
 
 
 @pytest.mark.parametrize("M,N,K", PRODUCTS)
@@ -182,7 +183,8 @@ def mx_block_bound(x, w13, w2, act):
 
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("T,H,I", [(1, 32, 32), (1, 256, 160), (4, 1344, 736), (16, 256, 128), (17, 96, 288), (63, 512, 1024),
-                                   (65, 160, 96), (200, 544, 320), (300, 128, 256), (3841, 256, 1920), (16, 512, 12288), (3, 96, 12288), (70, 1024, 2080), (67, 384, 7680), (50, 4352, 96)])
+                                   (65, 160, 96), (200, 544, 320), (300, 128, 256), (3841, 256, 1920), (16, 512, 12288), (3, 96, 12288), (70, 1024, 2080), (67, 384, 7680),
+                                   (50, 4352, 96), (32, 16384, 6144)])
 def test_block_on_mxfp4_weights(ops, T, H, I, act):
     x = normal(T, H, seed=8)
     w13, w2 = weights(ops, 2 * I, H, seed=9, sigma=H ** -0.5), weights(ops, H, I, seed=10, sigma=I ** -0.5)
