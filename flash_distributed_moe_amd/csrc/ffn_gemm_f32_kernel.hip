@@ -236,11 +236,10 @@ size_t ffn_gemm_f32_bytes(bool, int epi, const GemmArgs& p) {
   return partial_bytes(plan_f32(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
-static const TileCost kF32GradsWays[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 64, 0, 1.1, 1.6, 0.72}, {64, 64, 0, 0.78, 0.98, 0.45}};
+static const TileCost kF32GradsWays[] = {{128, 128, 0, 1.7, 2.5, 1.25, 2}, {128, 64, 0, 1.1, 1.6, 0.72, 3}, {64, 64, 0, 0.78, 0.98, 0.45, 4}};
 
 hipError_t launch_ffn_grads_f32(FfnGrads p, float* partial, size_t room, hipStream_t stream) {
-  GradsPlan chosen = plan_grads(kF32GradsWays, 3, 32, p, partial != nullptr);
-  if (plan_bytes(chosen, p) > room) chosen = plan_grads(kF32GradsWays, 3, 32, p, false);
+  const GradsPlan chosen = plan_grads(kF32GradsWays, 3, 32, p, partial != nullptr ? room : 0);
   const long long blocks = lay_out_grads(chosen, kF32GradsWays[chosen.way], p, partial);
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -252,6 +251,6 @@ hipError_t launch_ffn_grads_f32(FfnGrads p, float* partial, size_t room, hipStre
   return e != hipSuccess ? e : launch_ffn_finish_grads(0, p, stream);
 }
 
-size_t ffn_grads_f32_bytes(const FfnGrads& p) { return plan_bytes(plan_grads(kF32GradsWays, 3, 32, p, true), p); }
+size_t ffn_grads_f32_bytes(const FfnGrads& p) { return plan_bytes(plan_grads(kF32GradsWays, 3, 32, p, ~size_t{0}), p); }
 
 }  // namespace fmoe

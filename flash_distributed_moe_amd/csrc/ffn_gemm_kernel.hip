@@ -128,11 +128,10 @@ static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
   }
 }
 
-static const TileCost kGradsWays[] = {{256, 256, 0, 1.55, 3.1, 1.55}, {128, 128, 0, 0.6, 0.98, 0.49}, {64, 64, 0, 0.33, 0.5, 0.22}};
+static const TileCost kGradsWays[] = {{256, 256, 0, 1.55, 3.1, 1.55, 1}, {128, 128, 0, 0.6, 0.98, 0.49, 2}, {64, 64, 0, 0.33, 0.5, 0.22, 4}};
 
 static hipError_t launch_ffn_grads_bf16(FfnGrads p, float* partial, size_t room, hipStream_t stream) {
-  GradsPlan chosen = plan_grads(kGradsWays, 3, 64, p, partial != nullptr);
-  if (plan_bytes(chosen, p) > room) chosen = plan_grads(kGradsWays, 3, 64, p, false);
+  const GradsPlan chosen = plan_grads(kGradsWays, 3, 64, p, partial != nullptr ? room : 0);
   const long long blocks = lay_out_grads(chosen, kGradsWays[chosen.way], p, partial);
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -162,7 +161,7 @@ hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t
 }
 
 size_t ffn_grads_bytes(int dtype, const FfnGrads& p) {
-  return dtype != 1 ? ffn_grads_f32_bytes(p) : plan_bytes(plan_grads(kGradsWays, 3, 64, p, true), p);
+  return dtype != 1 ? ffn_grads_f32_bytes(p) : plan_bytes(plan_grads(kGradsWays, 3, 64, p, ~size_t{0}), p);
 }
 
 }  // namespace fmoe

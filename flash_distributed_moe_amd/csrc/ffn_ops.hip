@@ -121,16 +121,11 @@ size_t forward_partial_bytes(const FlashMoeFfnDesc& d, int tokens) {
   const size_t down = product_bytes(d, fmoe::EPI_STORE, down_sizes(d, tokens));
   return align_up(up > down ? up : down);
 }
-// Fewer gradients than three are split differently: x's alone and the weights' alone have their room, and what finds
-// none is not split.
+// (fewer gradients than three are split into what room these leave)
 size_t backward_partial_bytes(const FlashMoeFfnDesc& d, int tokens) {
-  const size_t of[] = {product_bytes(d, fmoe::EPI_SLOPE, up_sizes(d, tokens)),
-                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, true, true, true)),
-                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, true, false, false)),
-                       fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, false, true, true))};
-  size_t most = 0;
-  for (const size_t bytes : of) most = bytes > most ? bytes : most;
-  return align_up(most);
+  const size_t dh = product_bytes(d, fmoe::EPI_SLOPE, up_sizes(d, tokens));
+  const size_t grads = fmoe::ffn_grads_bytes(d.dtype, grads_sizes(d, tokens, true, true, true));
+  return align_up(dh > grads ? dh : grads);
 }
 float* as_partial(void* workspace, size_t behind, size_t bytes) {
   return workspace == nullptr || bytes == 0 ? nullptr : reinterpret_cast<float*>(static_cast<char*>(workspace) + behind);
@@ -213,14 +208,13 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
     if ((v = check_rows("dy", dy, lddy, H, d.dtype)) != hipSuccess) return v;
     if (dx != nullptr && (v = check_rows("dx", dx, lddx, H, d.dtype)) != hipSuccess) return v;
     if (saved == nullptr || !aligned16(saved)) FMOE_FAIL(hipErrorInvalidValue, "null or unaligned saved results");
-    if ((dx != nullptr || dw13 != nullptr) && (workspace == nullptr || !aligned16(workspace)))
+    if (((dx != nullptr || dw13 != nullptr) && workspace == nullptr) || !aligned16(workspace))
       FMOE_FAIL(hipErrorInvalidValue, "null or unaligned workspace");
   }
   const char* keep = static_cast<const char*>(saved);
   const long long ld_h = apart(I, d.dtype), ld_dgu = apart(2LL * I, d.dtype);
-  // gradients that backward_partial_bytes counts find their room by themselves
-  const bool counted = (dw13 != nullptr) == (dw2 != nullptr);
-  const size_t room = counted ? ~size_t{0} : backward_partial_bytes(d, tokens);
+  const bool all = dx != nullptr && dw13 != nullptr && dw2 != nullptr;  // which is what the workspace was made for
+  const size_t room = all ? ~size_t{0} : backward_partial_bytes(d, tokens);
   float* partial = as_partial(workspace, dgu_bytes(d, tokens), room);
   if (tokens > 0 && (dx != nullptr || dw13 != nullptr)) {
     // dh = dy W2, and with it the gradients of both projections
