@@ -45,8 +45,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, char* lds, int id) 
     for (int half = 0; half < 2; ++half) {
       Fragments<KIND_BF16, S::OUTER_B, S::BN, S::FN> b;
       Fragments<KIND_BF16, S::OUTER_A, S::BM, S::FM> a;
+      if constexpr (!S::OUTER_A) a.read(now, wm * S::FM * 16, half);
       b.read(now + S::BM * 128, wn * S::FN * 16, half);
-      a.read(now, wm * S::FM * 16, half);
+      if constexpr (S::OUTER_A) a.read(now, wm * S::FM * 16, half);
 #pragma unroll
       for (int fm = 0; fm < S::FM; ++fm)
 #pragma unroll
