@@ -299,9 +299,9 @@ __device__ __forceinline__ void write_partial(const GemmArgs& p, int split, int 
 
 // What becomes of the sums. Of a gated product the first half of the blocks are gate columns and the others
 // the same up columns.
-// The slope kernel at M=4096, N=6144, K=2048 bfloat16 (185 us): 123 without what follows its sums, 136 without
-// reading the projections, 163 without writing: 200 MB and 100 MB at memory's rate. Asking for all of a row's
-// projections together, a row ahead, makes no difference.
+// The slope kernel at M=4096, N=6144, K=2048 bfloat16 (174 us): 107 without what follows its sums, 131 without
+// reading the projections, 151 without writing: 200 MB and 100 MB at memory's rate. Asking for all of a row's
+// projections together, a row ahead, made no difference.
 template <class S, bool ANY_WIDTH = false>
 __device__ __forceinline__ void write_results(const GemmArgs& p, int m0, int n0, Accumulators<S>& acc) {
   constexpr int FN = S::FN, FM = S::FM;
