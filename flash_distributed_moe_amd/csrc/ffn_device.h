@@ -53,7 +53,7 @@ __device__ __forceinline__ int gated_row(int f, int r) {
 template <int F>
 __device__ __forceinline__ int k_row_swap(int k) {
   const int q = k & 3, g = (k >> 3) & 1;
-  return F >= 8 ? q | g << 2 : F == 4 ? q | g << 3 : (q & 1) | (q & 2) << 1 | g << 3;
+  return F == 4 ? q | g << 3 : (q & 1) | (q & 2) << 1 | g << 3;
 }
 // float32: 4 bytes a lane of every k row, sixteen lanes two runs of 32 bytes, and four rows eight apart at once
 template <int F>

@@ -232,7 +232,7 @@ hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipSt
   return epi == EPI_GATED ? pick_f32<false, EPI_GATED>(p, stream) : pick_f32<false, EPI_STORE>(p, stream);
 }
 
-size_t ffn_gemm_f32_bytes(bool, int epi, const GemmArgs& p) {
+size_t ffn_gemm_f32_bytes(int epi, const GemmArgs& p) {
   return partial_bytes(plan_f32(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 

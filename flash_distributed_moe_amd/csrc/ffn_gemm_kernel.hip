@@ -154,7 +154,7 @@ hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipSt
 
 size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p) {
   if (!k_outer_b && ffn_skinny_takes(p)) return 0;
-  return dtype != 1 ? ffn_gemm_f32_bytes(k_outer_b, epi, p) : partial_bytes(plan(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
+  return dtype != 1 ? ffn_gemm_f32_bytes(epi, p) : partial_bytes(plan(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
 hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream) {

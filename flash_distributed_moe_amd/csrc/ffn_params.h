@@ -173,7 +173,7 @@ inline size_t plan_bytes(const GradsPlan& plan, const FfnGrads& p) {
 hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
 size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p);
 hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
-size_t ffn_gemm_f32_bytes(bool k_outer_b, int epi, const GemmArgs& p);
+size_t ffn_gemm_f32_bytes(int epi, const GemmArgs& p);
 // (partial: `room` bytes or NULL)
 hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream);
 size_t ffn_grads_bytes(int dtype, const FfnGrads& p);
