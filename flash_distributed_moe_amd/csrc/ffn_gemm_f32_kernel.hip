@@ -210,13 +210,13 @@ static const TileCost kF32Ways[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 128, 1,
 static const TileCost kF32GatedWays[] = {{128, 64, 0, 1.7, 2.5, 1.25}, {128, 64, 1, 1.32, 2.7, 1.35}, {128, 32, 0, 1.1, 1.6, 0.72},
                                          {64, 32, 0, 0.78, 0.98, 0.42}, {64, 32, 0.8, 0.54, 0.85, 0.45}, {64, 32, 1.8, 0.48, 0.95, 0.48}};
 
-static TilePlan plan_f32(int epi, const GemmArgs& p, bool split) {
-  return plan_tiles(epi == EPI_GATED ? kF32GatedWays : kF32Ways, 6, 32, p, epi == EPI_GATED ? 2 * p.N : p.N, split);
+static TilePlan plan_f32(int epi, const GemmArgs& p, size_t room) {
+  return plan_tiles(epi == EPI_GATED ? kF32GatedWays : kF32Ways, 6, 32, p, epi == EPI_GATED ? 2 * p.N : p.N, room);
 }
 
 template <bool OB, int EPI>
-static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
-  const TilePlan chosen = plan_f32(EPI, p, p.partial != nullptr);
+static hipError_t pick_f32(const GemmArgs& p, size_t room, hipStream_t stream) {
+  const TilePlan chosen = plan_f32(EPI, p, p.partial != nullptr ? room : 0);
   switch (chosen.way) {
     case 0: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 4, 4>>(p, chosen, stream);
     case 1: return launch_f32<GemmShape<KIND_F32, false, OB, EPI, 2, 2, 4, 4, 2>>(p, chosen, stream);
@@ -227,13 +227,13 @@ static hipError_t pick_f32(const GemmArgs& p, hipStream_t stream) {
   }
 }
 
-hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream) {
-  if (epi == EPI_SLOPE) return pick_f32<true, EPI_SLOPE>(p, stream);
-  return epi == EPI_GATED ? pick_f32<false, EPI_GATED>(p, stream) : pick_f32<false, EPI_STORE>(p, stream);
+hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, size_t room, hipStream_t stream) {
+  if (epi == EPI_SLOPE) return pick_f32<true, EPI_SLOPE>(p, room, stream);
+  return epi == EPI_GATED ? pick_f32<false, EPI_GATED>(p, room, stream) : pick_f32<false, EPI_STORE>(p, room, stream);
 }
 
 size_t ffn_gemm_f32_bytes(int epi, const GemmArgs& p) {
-  return partial_bytes(plan_f32(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
+  return partial_bytes(plan_f32(epi, p, ~size_t{0}), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
 static const TileCost kF32GradsWays[] = {{128, 128, 0, 1.7, 2.5, 1.25, 2}, {128, 64, 0, 1.1, 1.6, 0.72, 3}, {64, 64, 0, 0.78, 0.98, 0.45, 4}};

@@ -112,13 +112,13 @@ static const TileCost kWays[] = {{256, 256, 0, 1.45, 2.9, 1.45}, {128, 128, 0, 0
 static const TileCost kGatedWays[] = {{256, 128, 0, 1.45, 2.9, 1.45}, {128, 64, 0, 0.55, 0.96, 0.48}, {128, 64, 0.8, 0.45, 1.0, 0.55},
                                       {64, 32, 0, 0.33, 0.5, 0.21},   {64, 32, 0.8, 0.25, 0.37, 0.245}, {64, 32, 1.8, 0.2, 0.53, 0.27}};
 
-static TilePlan plan(int epi, const GemmArgs& p, bool split) {
-  return plan_tiles(epi == EPI_GATED ? kGatedWays : kWays, 6, 64, p, epi == EPI_GATED ? 2 * p.N : p.N, split);
+static TilePlan plan(int epi, const GemmArgs& p, size_t room) {
+  return plan_tiles(epi == EPI_GATED ? kGatedWays : kWays, 6, 64, p, epi == EPI_GATED ? 2 * p.N : p.N, room);
 }
 
 template <bool OB, int EPI>
-static hipError_t pick(const GemmArgs& p, hipStream_t stream) {
-  const TilePlan chosen = plan(EPI, p, p.partial != nullptr);
+static hipError_t pick(const GemmArgs& p, size_t room, hipStream_t stream) {
+  const TilePlan chosen = plan(EPI, p, p.partial != nullptr ? room : 0);
   switch (chosen.way) {
     case 0: return launch<GemmShape<KIND_BF16, false, OB, EPI, 4, 4, 4, 4>>(p, chosen, stream);
     case 1: return launch<GemmShape<KIND_BF16, false, OB, EPI, 4, 2, 2, 4>>(p, chosen, stream);
@@ -144,17 +144,17 @@ static hipError_t launch_ffn_grads_bf16(FfnGrads p, float* partial, size_t room,
   return e != hipSuccess ? e : launch_ffn_finish_grads(1, p, stream);
 }
 
-hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream) {
+hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, size_t room, hipStream_t stream) {
   if (k_outer_b != (epi == EPI_SLOPE)) return hipErrorInvalidValue;
   if (!k_outer_b && ffn_skinny_takes(p)) return launch_ffn_skinny(dtype, epi == EPI_GATED, p, stream);
-  if (dtype != 1) return launch_ffn_gemm_f32(k_outer_b, epi, p, stream);
-  if (epi == EPI_SLOPE) return pick<true, EPI_SLOPE>(p, stream);
-  return epi == EPI_GATED ? pick<false, EPI_GATED>(p, stream) : pick<false, EPI_STORE>(p, stream);
+  if (dtype != 1) return launch_ffn_gemm_f32(k_outer_b, epi, p, room, stream);
+  if (epi == EPI_SLOPE) return pick<true, EPI_SLOPE>(p, room, stream);
+  return epi == EPI_GATED ? pick<false, EPI_GATED>(p, room, stream) : pick<false, EPI_STORE>(p, room, stream);
 }
 
 size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p) {
   if (!k_outer_b && ffn_skinny_takes(p)) return 0;
-  return dtype != 1 ? ffn_gemm_f32_bytes(epi, p) : partial_bytes(plan(epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
+  return dtype != 1 ? ffn_gemm_f32_bytes(epi, p) : partial_bytes(plan(epi, p, ~size_t{0}), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
 hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream) {

@@ -174,8 +174,10 @@ int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx
   void* h = keep != nullptr ? keep + gu_bytes(d, tokens) : workspace;
 
   GemmArgs up = up_sizes(d, tokens), down = down_sizes(d, tokens);
-  // (MXFP4 weights whose scales' address counts too may plan otherwise than flashMoeFfnBytes, which does not see it)
-  up.partial = down.partial = as_partial(workspace, keep != nullptr ? 0 : h_bytes(d, tokens), mx ? forward_partial_bytes(d, tokens) : 1);
+  // Plans that flashMoeFfnBytes made too fit what it asked for. With MXFP4 weights the scales' addresses, which it does not
+  // see, count for which kernel runs: a product may then want more, and gets what there is.
+  const size_t room = mx ? forward_partial_bytes(d, tokens) : ~size_t{0};
+  up.partial = down.partial = as_partial(workspace, keep != nullptr ? 0 : h_bytes(d, tokens), room);
   up.a = x, up.b = d.w13, up.b_scales = static_cast<const unsigned char*>(d.w13_scales);
   up.c = h, up.gu = reinterpret_cast<float*>(keep);
   up.lda = ldx, up.ldb = H, up.ldc = apart(I, d.dtype);
@@ -183,11 +185,11 @@ int flashMoeFfnForward(const FlashMoeFfnDesc* desc, const void* x, long long ldx
   down.c = y;
   down.lda = up.ldc, down.ldb = I, down.ldc = ldy;
   if (mx) {
-    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_GATED, up, stream));
-    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_STORE, down, stream));
+    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_GATED, up, room, stream));
+    FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(false, fmoe::EPI_STORE, down, room, stream));
   } else {
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_GATED, up, stream));
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_STORE, down, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_GATED, up, room, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, false, fmoe::EPI_STORE, down, room, stream));
   }
   return hipSuccess;
 }
@@ -222,7 +224,7 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
     p.partial = partial;
     p.a = dy, p.b = d.w2, p.c = workspace, p.gu = reinterpret_cast<float*>(const_cast<char*>(keep));
     p.lda = lddy, p.ldb = I, p.ldc = ld_dgu;
-    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, fmoe::EPI_SLOPE, p, stream));
+    FMOE_HIP_CHECK(fmoe::launch_ffn_gemm(d.dtype, true, fmoe::EPI_SLOPE, p, room, stream));
   }
   // the weights' gradients sum over the tokens; of no tokens they are zeros
   fmoe::FfnGrads grads = grads_sizes(d, tokens, dx != nullptr, dw13 != nullptr, dw2 != nullptr);
@@ -311,7 +313,7 @@ int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long 
   p.c = y, p.ldc = ldy;
   p.M = rows, p.N = n, p.K = k;
   p.partial = as_partial(workspace, 0, bytes);
-  FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(mx, fmoe::EPI_STORE, p, static_cast<hipStream_t>(stream)));
+  FMOE_HIP_CHECK(fmoe::launch_mxfp4_gemm(mx, fmoe::EPI_STORE, p, bytes, static_cast<hipStream_t>(stream)));
   return hipSuccess;
 }
 

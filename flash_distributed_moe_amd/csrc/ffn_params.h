@@ -48,28 +48,30 @@ inline double tile_cost(const TileCost& way, double tiles, int steps) {
   const long long each = static_cast<long long>((tiles + 255) / 256);  // tiles of the fullest CU
   return way.once + steps * (each <= 1 ? way.one : each == 2 ? way.two : each * way.more);
 }
-// step: k of a step; columns: rows of B; split: whether there is memory for partial sums. Measured, a whole call
+// step: k of a step; columns: rows of B; room: bytes of memory for partial sums. Measured, a whole call
 // without and with splits, us: T=87, H=144, I=6520 bf16 39 and 18 (the second product has 6 tiles of 64 x 64);
 // MXFP4 weights, T=67, H=384, I=7680 40 and 22; a product with MXFP4 weights, M=703, N=591, K=7520 36 and 24; a training
 // step, T=2480, H=416, I=8520 bf16 547 and 406. Against the best of all ways and splits this loses 0.3 to 0.9 % (40 random
 // calls of each type).
-inline TilePlan plan_tiles(const TileCost* ways, int count, int step, const GemmArgs& p, int columns, bool split) {
+inline size_t partial_bytes(const TilePlan& plan, int M, int columns) {
+  return plan.splits > 1 ? static_cast<size_t>(plan.splits) * M * partial_ld(columns) * 4 : 0;
+}
+inline TilePlan plan_tiles(const TileCost* ways, int count, int step, const GemmArgs& p, int columns, size_t room) {
   const int steps = (p.K + step - 1) / step;
   TilePlan best = {0, 1, steps};
   double least = -1;
   for (int i = 0; i < count; ++i) {
     const double tiles = tile_count(ways[i], p);
-    for (int splits = 1; splits == 1 || (split && tiles * splits <= 1024 && splits <= 64 && splits * 4 <= steps);
+    for (int splits = 1; splits == 1 || (room > 0 && tiles * splits <= 1024 && splits <= 64 && splits * 4 <= steps);
          splits += splits < 4 ? 1 : splits / 2) {
       const int per = (steps + splits - 1) / splits, used = steps == 0 ? 1 : (steps + per - 1) / per;
+      const TilePlan plan = {i, used, per};
+      if (partial_bytes(plan, p.M, columns) > room) continue;
       const double cost = tile_cost(ways[i], tiles * used, per) + finish_cost(used, static_cast<double>(p.M) * columns);
-      if (least < 0 || cost < least) best = {i, used, per}, least = cost;
+      if (least < 0 || cost < least) best = plan, least = cost;
     }
   }
   return best;
-}
-inline size_t partial_bytes(const TilePlan& plan, int M, int columns) {
-  return plan.splits > 1 ? static_cast<size_t>(plan.splits) * M * partial_ld(columns) * 4 : 0;
 }
 
 enum { ACT_SILU = 0, ACT_GELU_TANH = 1 };
@@ -169,10 +171,11 @@ inline size_t plan_bytes(const GradsPlan& plan, const FfnGrads& p) {
 }
 
 // A matrix product in bfloat16 or float32 (k_outer_b: a row of B is one k); epi as above. *_bytes: memory for
-// p.partial that a call with these sizes can use (0: none); without it k is not split.
-hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, hipStream_t stream);
+// p.partial that a call with these sizes can use (0: none); room: how much of it there is (with p.partial NULL
+// none): a call whose plan wants more takes one that wants less.
+hipError_t launch_ffn_gemm(int dtype, bool k_outer_b, int epi, GemmArgs p, size_t room, hipStream_t stream);
 size_t ffn_gemm_bytes(int dtype, bool k_outer_b, int epi, const GemmArgs& p);
-hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, hipStream_t stream);
+hipError_t launch_ffn_gemm_f32(bool k_outer_b, int epi, const GemmArgs& p, size_t room, hipStream_t stream);
 size_t ffn_gemm_f32_bytes(int epi, const GemmArgs& p);
 // (partial: `room` bytes or NULL)
 hipError_t launch_ffn_grads(int dtype, const FfnGrads& p, float* partial, size_t room, hipStream_t stream);
@@ -183,7 +186,7 @@ size_t ffn_grads_f32_bytes(const FfnGrads& p);
 hipError_t launch_ffn_finish(int dtype, int epi, const GemmArgs& p, hipStream_t stream);
 hipError_t launch_ffn_finish_grads(int dtype, const FfnGrads& p, hipStream_t stream);
 // MXFP4 weights b times bfloat16 rows (x_mxfp4 false) or MXFP4 rows; EPI_STORE or EPI_GATED (bfloat16 rows only).
-hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream);
+hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, const GemmArgs& p, size_t room, hipStream_t stream);
 size_t mxfp4_gemm_bytes(bool x_mxfp4, int epi, const GemmArgs& p);
 // The same for few rows, where these take the call (A and B with their k inside the rows).
 bool ffn_skinny_takes(const GemmArgs& p);

@@ -327,14 +327,14 @@ static const TileCost kGatedWeightsWays[] = {{256, 128, 0, 1.7, 3.4, 1.7}, {128,
 static const TileCost kBothWays[] = {{256, 256, 0, 2.5, 5.2, 2.6}, {128, 128, 0, 1.0, 1.7, 0.77}, {128, 128, 0.5, 0.87, 1.9, 0.95},
                                      {64, 64, 0.5, 0.35, 0.65, 0.31}};
 
-static TilePlan plan(bool both, int epi, const GemmArgs& p, bool split) {
-  if (both) return plan_tiles(kBothWays, 4, 256, p, p.N, split);
-  return epi == EPI_GATED ? plan_tiles(kGatedWeightsWays, 4, 64, p, 2 * p.N, split) : plan_tiles(kWeightsWays, 4, 64, p, p.N, split);
+static TilePlan plan(bool both, int epi, const GemmArgs& p, size_t room) {
+  if (both) return plan_tiles(kBothWays, 4, 256, p, p.N, room);
+  return epi == EPI_GATED ? plan_tiles(kGatedWeightsWays, 4, 64, p, 2 * p.N, room) : plan_tiles(kWeightsWays, 4, 64, p, p.N, room);
 }
 
 template <int EPI>
-static hipError_t launch_weights(const GemmArgs& p, hipStream_t stream) {
-  const TilePlan chosen = plan(false, EPI, p, p.partial != nullptr);
+static hipError_t launch_weights(const GemmArgs& p, size_t room, hipStream_t stream) {
+  const TilePlan chosen = plan(false, EPI, p, p.partial != nullptr ? room : 0);
   switch (chosen.way) {
     case 0: {
       typedef GemmShape<KIND_BF16, false, false, EPI, 4, 4, 4, 4> S;
@@ -356,8 +356,8 @@ static hipError_t launch_weights(const GemmArgs& p, hipStream_t stream) {
 }
 
 template <bool FOURS>
-static hipError_t launch_both(const GemmArgs& p, hipStream_t stream) {
-  const TilePlan chosen = plan(true, EPI_STORE, p, p.partial != nullptr);
+static hipError_t launch_both(const GemmArgs& p, size_t room, hipStream_t stream) {
+  const TilePlan chosen = plan(true, EPI_STORE, p, p.partial != nullptr ? room : 0);
   switch (chosen.way) {
     case 0: {
       typedef GemmShape<KIND_MXFP4, false, false, EPI_STORE, 4, 4, 4, 4> S;
@@ -384,16 +384,16 @@ static bool scales_on_fours(const GemmArgs& p) {
   return p.K % 128 == 0 && fours(p.b_scales) && fours(p.a_scales);
 }
 
-hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, GemmArgs p, hipStream_t stream) {
+hipError_t launch_mxfp4_gemm(bool x_mxfp4, int epi, const GemmArgs& p, size_t room, hipStream_t stream) {
   if (x_mxfp4 && epi != EPI_STORE) return hipErrorInvalidValue;
   if (mxfp4_skinny_takes(x_mxfp4, p)) return launch_mxfp4_skinny(x_mxfp4, epi == EPI_GATED, p, stream);
-  if (x_mxfp4) return scales_on_fours(p) ? launch_both<true>(p, stream) : launch_both<false>(p, stream);
-  return epi == EPI_GATED ? launch_weights<EPI_GATED>(p, stream) : launch_weights<EPI_STORE>(p, stream);
+  if (x_mxfp4) return scales_on_fours(p) ? launch_both<true>(p, room, stream) : launch_both<false>(p, room, stream);
+  return epi == EPI_GATED ? launch_weights<EPI_GATED>(p, room, stream) : launch_weights<EPI_STORE>(p, room, stream);
 }
 
 size_t mxfp4_gemm_bytes(bool x_mxfp4, int epi, const GemmArgs& p) {
   if (mxfp4_skinny_takes(x_mxfp4, p)) return 0;
-  return partial_bytes(plan(x_mxfp4, epi, p, true), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
+  return partial_bytes(plan(x_mxfp4, epi, p, ~size_t{0}), p.M, epi == EPI_GATED ? 2 * p.N : p.N);
 }
 
 }  // namespace fmoe

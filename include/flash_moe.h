@@ -318,7 +318,7 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
 /* ---- MXFP4, the 4-bit format of the Open Compute microscaling specification: 32 consecutive values of a
  * row share a scale, a byte b that stands for 2^(b-127) (255: NaN), and a value is 4 bits: a sign and
  * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. codes [rows, k/2], the even value in the low half of its byte; scales
- * [rows, k/32]; both without gaps, codes beginning on 16 bytes.
+ * [rows, k/32]; both without gaps, codes beginning on 16 bytes, scales anywhere (on 4 bytes is faster).
  * Quantisation takes b - 127 = floor(log2(largest magnitude of the block)) - 2, at least -127, rounds to the
  * nearest value, ties to the even code, and stops at 6. A block with an infinity or NaN becomes all NaN.
  * k is a multiple of 32. x and out lie ldx / ldo values apart, whole 16 bytes. */
