@@ -207,7 +207,8 @@ __device__ __forceinline__ void store_some(unsigned short* to, int count, const 
 }
 
 // The groups' sums of a tile, into the first group's, in the groups' order. Of the others nobody is left to write results.
-template <class S, int ROOM = S::LDS_BYTES>
+// FRUGAL: a row of blocks at a time, for callers with few registers left.
+template <class S, int ROOM = S::LDS_BYTES, bool FRUGAL = false>
 __device__ __forceinline__ void add_groups(char* lds, int group, Accumulators<S>& acc) {
   if constexpr (S::GROUPS > 1) {
     f32x4* part = reinterpret_cast<f32x4*>(lds);
@@ -225,9 +226,11 @@ __device__ __forceinline__ void add_groups(char* lds, int group, Accumulators<S>
 #pragma unroll
       for (int other = 1; other < S::GROUPS; ++other)
 #pragma unroll
-        for (int fm = 0; fm < S::FM; ++fm)
+        for (int fm = 0; fm < S::FM; ++fm) {
 #pragma unroll
           for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] += part[(((other - 1) * S::FM + fm) * S::FN + fn) * S::THREADS + tid];
+          if constexpr (FRUGAL) asm volatile("" : : : "memory");
+        }
     }
   }
 }

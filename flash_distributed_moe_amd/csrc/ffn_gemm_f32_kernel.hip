@@ -3,12 +3,15 @@
 // A float32 is split into three bfloat16 parts, each the rest rounded to nearest: x = hi + mid + lo exactly (8 bits
 // and a sign each). Of the nine products of parts the six largest are summed in float32; the three left out are
 // below 2^-24 of a product, of either sign, about what a rounded multiplication may be off by (with parts cut off instead
-// it is 2^-21, always towards zero; that took 78 us for T=1001, H=2048, I=768, forward, this takes 82). Six instructions at 16 times the rate of the float32 ones: 2.7 times as fast.
+// it is 2^-21, always towards zero, and 3 % faster). Six instructions at 16 times the rate of the float32 ones: 2.7 times as
+// fast.
 // The parts live in registers only; a tile in LDS is float32, and a wave splits what it reads.
 //
-// Where that does not give the float32 sum, the sum is taken again, one fused multiply-add after another:
-// where it is no finite number (an infinity has no parts), and where it is so small that parts of what it sums
-// were below what bfloat16 has (a value under 2^-103 loses its low part).
+// Parts below bfloat16's smallest number, 2^-133, are lost (the instruction keeps what is below 2^-126): an operand is its
+// parts to 2^-134. So a sum is taken again, on the float32 matrix instructions, if it is so small that this may count, and not
+// zero, or if it is no finite number (an infinity has no parts): a workgroup with such a sum goes over its k once more, other
+// sums stay as they are. That second pass takes 2 to 3 times a tile's time: a step T=1001, H=2048, I=768 0.47 ms with a NaN
+// among its tokens, 0.22 without.
 #include "ffn_gemm_device.h"
 
 namespace fmoe {
@@ -53,41 +56,19 @@ __device__ __forceinline__ Parts split(const float (&v)[8]) {
   return p;
 }
 
-constexpr float kSmallSum = 2.6469779601696886e-23f;  // 2^-75: weights up to 2^20 times values under 2^-103 sum to less
+// Sums of K products from here on are right to 2^-24 of themselves if their operands are up to 2^32: K 2^-77
+__device__ __forceinline__ float small_sum(int K) { return static_cast<float>(K) * 6.6174449004242214e-24f; }
 
-// C[m, n] by itself, over k from `from` to `to`
-template <bool OUTER_A, bool OUTER_B>
-__device__ __noinline__ float plain_sum(const float* a, long long lda, const float* b, long long ldb, long long m, long long n, int from, int to) {
-  const float* pa = OUTER_A ? a + m : a + m * lda;
-  const float* pb = OUTER_B ? b + n : b + n * ldb;
-  const long long sa = OUTER_A ? lda : 1, sb = OUTER_B ? ldb : 1;
-  float sum = 0.0f;
-  for (int k = from; k < to; ++k) sum = fmaf(pa[k * sa], pb[k * sb], sum);
-  return sum;
-}
-
-// Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
-template <class S>
-__device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int id) {
-  int share, first, steps, tile_m, tile_n;
-  share_of(p, (p.K + S::STEP - 1) / S::STEP, id, share, first, steps);
-  tile_of(p, id, tile_m, tile_n);
-  const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
-  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
-  char* mine = lds + group * 2 * S::STAGE_BYTES;
-
-  TileLoader<KIND_F32, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
-  TileLoader<KIND_F32, S::OUTER_B, S::BN, S::THREADS, S::FN, S::EPI == EPI_GATED> load_b;
-  load_a.init(p.a, p.lda, m0, p.M, tid);
-  load_b.init(p.b, p.ldb, n0, p.N, tid);
-
-  Accumulators<S> acc;
+// A workgroup's sums over its share of the k, in its GROUPS groups. PLAIN: with the float32 instructions, else with the
+// products of parts.
+template <class S, bool PLAIN, class LoaderA, class LoaderB>
+__device__ __forceinline__ void sum_tile_f32(const GemmArgs& p, const LoaderA& load_a, const LoaderB& load_b, char* mine, int group, int first,
+                                             int steps, Accumulators<S>& acc) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x % S::THREADS >> 6), wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
   for (int fm = 0; fm < S::FM; ++fm)
 #pragma unroll
     for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
   // a group's turns: stages group, group + GROUPS, ...
   const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
@@ -104,68 +85,116 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
     if (turn + 1 < turns) load(turn + 1);
     if (S::GROUPS > 1 && turn * S::GROUPS + group >= steps) continue;
     const char* now = mine + (turn & 1) * S::STAGE_BYTES;
-    Parts b[S::FN];
+    if constexpr (PLAIN) {
+      float b[S::FN][8];
 #pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) {
-      float v[8];
-      read_f32<S::OUTER_B, S::BN, S::FN>(v, now + S::BM * 128, wn * S::FN * 16, fn);
-      b[fn] = split(v);
-    }
+      for (int fn = 0; fn < S::FN; ++fn) read_f32<S::OUTER_B, S::BN, S::FN>(b[fn], now + S::BM * 128, wn * S::FN * 16, fn);
 #pragma unroll
-    for (int fm = 0; fm < S::FM; ++fm) {
-      float v[8];
-      read_f32<S::OUTER_A, S::BM, S::FM>(v, now, wm * S::FM * 16, fm);
-      const Parts a = split(v);
-      // the small products first
-      auto add = [&](const i32x4 Parts::*pb, const i32x4 Parts::*pa) {
+      for (int fm = 0; fm < S::FM; ++fm) {
+        float a[8];
+        read_f32<S::OUTER_A, S::BM, S::FM>(a, now, wm * S::FM * 16, fm);
 #pragma unroll
-        for (int fn = 0; fn < S::FN; ++fn)
-          acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[fn].*pb),
-                                                                  __builtin_bit_cast(bf16x8, a.*pa), acc.v[fm][fn], 0, 0, 0);
-      };
-      add(&Parts::lo, &Parts::hi);
-      add(&Parts::mid, &Parts::mid);
-      add(&Parts::hi, &Parts::lo);
-      add(&Parts::mid, &Parts::hi);
-      add(&Parts::hi, &Parts::mid);
-      add(&Parts::hi, &Parts::hi);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[fn][i], a[i], acc.v[fm][fn], 0, 0, 0);
+      }
+    } else {
+      Parts b[S::FN];
+#pragma unroll
+      for (int fn = 0; fn < S::FN; ++fn) {
+        float v[8];
+        read_f32<S::OUTER_B, S::BN, S::FN>(v, now + S::BM * 128, wn * S::FN * 16, fn);
+        b[fn] = split(v);
+      }
+#pragma unroll
+      for (int fm = 0; fm < S::FM; ++fm) {
+        float v[8];
+        read_f32<S::OUTER_A, S::BM, S::FM>(v, now, wm * S::FM * 16, fm);
+        const Parts a = split(v);
+        // the small products first
+        auto add = [&](const i32x4 Parts::*pb, const i32x4 Parts::*pa) {
+#pragma unroll
+          for (int fn = 0; fn < S::FN; ++fn)
+            acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[fn].*pb),
+                                                                    __builtin_bit_cast(bf16x8, a.*pa), acc.v[fm][fn], 0, 0, 0);
+        };
+        add(&Parts::lo, &Parts::hi);
+        add(&Parts::mid, &Parts::mid);
+        add(&Parts::hi, &Parts::lo);
+        add(&Parts::mid, &Parts::hi);
+        add(&Parts::hi, &Parts::mid);
+        add(&Parts::hi, &Parts::hi);
+      }
     }
   }
+}
 
+// A sum's place in the order infinity, NaN, zero, small to large
+__device__ __forceinline__ unsigned sum_order(float v) { return (__float_as_uint(v) << 1) + 0x01000000u; }
+__device__ __forceinline__ bool doubtful(float v, float small) { return sum_order(v) < sum_order(small) && v != 0.0f; }
+
+// Tile `id` of a product, by a workgroup with S::LDS_BYTES of LDS
+template <class S>
+__device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int id) {
+  int share, first, steps, tile_m, tile_n;
+  share_of(p, (p.K + S::STEP - 1) / S::STEP, id, share, first, steps);
+  tile_of(p, id, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  char* mine = lds + group * 2 * S::STAGE_BYTES;
+
+  TileLoader<KIND_F32, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
+  TileLoader<KIND_F32, S::OUTER_B, S::BN, S::THREADS, S::FN, S::EPI == EPI_GATED> load_b;
+  load_a.init(p.a, p.lda, m0, p.M, tid);
+  load_b.init(p.b, p.ldb, n0, p.N, tid);
+
+  Accumulators<S> acc;
+  sum_tile_f32<S, false>(p, load_a, load_b, mine, group, first, steps, acc);
   add_groups<S>(lds, group, acc);
-  if (group != 0) return;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int from = first * S::STEP, end = (first + steps) * S::STEP, to = end < p.K ? end : p.K;
+
+  const float small = small_sum(p.K);
+  bool odd = false;
+  if (group == 0) {  // (the others' sums are in this one's)
+    unsigned least = 0xFFFFFFFFu;
 #pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
+    for (int fm = 0; fm < S::FM; ++fm)
 #pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) {
-      bool again = false;
+      for (int fn = 0; fn < S::FN; ++fn)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = fabsf(acc.v[fm][fn][i]);
-        again |= !(v < __builtin_inff()) || (v < kSmallSum && v != 0.0f);
-      }
-      if (!again) continue;
-      const long long m = m0 + wm * S::FM * 16 + dealt_row<S::FM>(fm, r);
-      if (m >= p.M) continue;
+        for (int i = 0; i < 4; ++i) least = min(least, sum_order(acc.v[fm][fn][i]));
+    if (__any(least < sum_order(small))) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // (row of B of this result: gated, an up row if the block is one)
-        long long n;
-        bool in;
-        if constexpr (S::EPI == EPI_GATED) {
-          const int col = n0 + wn * S::FN * 8 + gated_row<S::FN>(fn, 4 * g + i);
-          in = col < p.N;
-          n = col + (fn >= S::FN / 2 ? p.N : 0);
-        } else {
-          n = n0 + wn * S::FN * 16 + dealt_row<S::FN>(fn, 4 * g + i);
-          in = n < p.N;
-        }
-        if (in) acc.v[fm][fn][i] = plain_sum<S::OUTER_A, S::OUTER_B>(static_cast<const float*>(p.a), p.lda, static_cast<const float*>(p.b),
-                                                                     p.ldb, m, n, from, to);
-      }
+      for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+        for (int fn = 0; fn < S::FN; ++fn)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd |= doubtful(acc.v[fm][fn][i], small);
     }
+  }
+  // (words in the stages' memory: beside LDS of another name the compiler waits, in the loop over k, for the next stage's
+  // loads before it reads this one's, 5 to 15 % of a call)
+  unsigned* words = reinterpret_cast<unsigned*>(lds);
+  const bool any = __any(odd);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = any;
+  __syncthreads();
+  unsigned again = 0;
+#pragma unroll
+  for (int w = 0; w < S::WAVES * S::GROUPS; ++w) again |= words[w];
+  if (__builtin_amdgcn_readfirstlane(again) != 0) {
+    __syncthreads();
+    Accumulators<S> plain;
+    sum_tile_f32<S, true>(p, load_a, load_b, mine, group, first, steps, plain);
+    add_groups<S, S::LDS_BYTES, true>(lds, group, plain);
+#pragma unroll
+    for (int fm = 0; fm < S::FM; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < S::FN; ++fn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (doubtful(acc.v[fm][fn][i], small)) acc.v[fm][fn][i] = plain.v[fm][fn][i];
+  }
+  if (group != 0) return;
   if (p.splits > 1) write_partial<S>(p, share, m0, n0, acc);
   else write_results<S>(p, m0, n0, acc);
 }
