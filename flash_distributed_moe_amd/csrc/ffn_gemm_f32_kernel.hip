@@ -8,10 +8,14 @@
 // The parts live in registers only; a tile in LDS is float32, and a wave splits what it reads.
 //
 // Parts below bfloat16's smallest number, 2^-133, are lost (the instruction keeps what is below 2^-126): an operand is its
-// parts to 2^-134. So a sum is taken again, on the float32 matrix instructions, if it is so small that this may count, and not
-// zero, or if it is no finite number (an infinity has no parts): a workgroup with such a sum goes over its k once more, other
-// sums stay as they are. That second pass takes 2 to 3 times a tile's time: a step T=1001, H=2048, I=768 0.47 ms with a NaN
-// among its tokens, 0.22 without.
+// parts to 2^-134. With operands below kLarge a sum of K products is off by less than K 2^-133 kLarge from that, which is below
+// 2^-24 of a sum of small_sum(K) and more. So a sum is taken again, on the float32 matrix instructions, if it is smaller than
+// that and not zero, if its row or column holds a larger operand, or if it is no finite number (an infinity has no parts): a
+// workgroup with such a sum goes over its k once more, other sums stay as they are. Larger operands are noticed by the sums of
+// the squares of all rows' high parts, one more instruction a block (T=1001, H=2048, I=768, forward 79 -> 83 us; the largest
+// magnitude by vector instructions costs twice that). That second pass takes 2 to 3 times a tile's time: a step of this size
+// 0.47 ms with a NaN among its tokens, 0.22 without. (A sum that comes out as zero is left: ordinary
+// ones do now and then. Of operands below 2^-134 alone, times others below kLarge, it may be off by K 2^-101.)
 #include "ffn_gemm_device.h"
 
 namespace fmoe {
@@ -56,19 +60,23 @@ __device__ __forceinline__ Parts split(const float (&v)[8]) {
   return p;
 }
 
-// Sums of K products from here on are right to 2^-24 of themselves if their operands are up to 2^32: K 2^-77
-__device__ __forceinline__ float small_sum(int K) { return static_cast<float>(K) * 6.6174449004242214e-24f; }
+constexpr float kLarge = 4294967296.0f;  // 2^32
+__device__ __forceinline__ float small_sum(int K) { return static_cast<float>(K) * 6.6174449004242214e-24f; }  // K 2^-77
 
-// A workgroup's sums over its share of the k, in its GROUPS groups. PLAIN: with the float32 instructions, else with the
-// products of parts.
+// A workgroup's sums over its share of the k, in its GROUPS groups. PLAIN: with the float32 instructions, and the largest
+// magnitudes that this lane read of each block's rows; else with the products of parts, and `squares`: of the rows' high
+// parts, summed (some of its elements are, and none is larger).
 template <class S, bool PLAIN, class LoaderA, class LoaderB>
 __device__ __forceinline__ void sum_tile_f32(const GemmArgs& p, const LoaderA& load_a, const LoaderB& load_b, char* mine, int group, int first,
-                                             int steps, Accumulators<S>& acc) {
+                                             int steps, Accumulators<S>& acc, f32x4& squares, float (&most_a)[S::FM], float (&most_b)[S::FN]) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x % S::THREADS >> 6), wm = wave / S::WN, wn = wave % S::WN;
+  squares = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int fm = 0; fm < S::FM; ++fm)
+  for (int fm = 0; fm < S::FM; ++fm) {
+    most_a[fm] = 0.0f;
 #pragma unroll
-    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, most_b[fn] = 0.0f;
+  }
   // a group's turns: stages group, group + GROUPS, ...
   const int turns = (steps + S::GROUPS - 1) / S::GROUPS;
   auto load = [&](int turn) {
@@ -88,29 +96,40 @@ __device__ __forceinline__ void sum_tile_f32(const GemmArgs& p, const LoaderA& l
     if constexpr (PLAIN) {
       float b[S::FN][8];
 #pragma unroll
-      for (int fn = 0; fn < S::FN; ++fn) read_f32<S::OUTER_B, S::BN, S::FN>(b[fn], now + S::BM * 128, wn * S::FN * 16, fn);
+      for (int fn = 0; fn < S::FN; ++fn) {
+        read_f32<S::OUTER_B, S::BN, S::FN>(b[fn], now + S::BM * 128, wn * S::FN * 16, fn);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most_b[fn] = fmaxf(most_b[fn], fabsf(b[fn][i]));
+      }
 #pragma unroll
       for (int fm = 0; fm < S::FM; ++fm) {
         float a[8];
         read_f32<S::OUTER_A, S::BM, S::FM>(a, now, wm * S::FM * 16, fm);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i) {
+          most_a[fm] = fmaxf(most_a[fm], fabsf(a[i]));
 #pragma unroll
           for (int fn = 0; fn < S::FN; ++fn) acc.v[fm][fn] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[fn][i], a[i], acc.v[fm][fn], 0, 0, 0);
+        }
       }
     } else {
       Parts b[S::FN];
+      auto square = [&](const i32x4& hi) {
+        squares = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, hi), squares, 0, 0, 0);
+      };
 #pragma unroll
       for (int fn = 0; fn < S::FN; ++fn) {
         float v[8];
         read_f32<S::OUTER_B, S::BN, S::FN>(v, now + S::BM * 128, wn * S::FN * 16, fn);
         b[fn] = split(v);
+        square(b[fn].hi);
       }
 #pragma unroll
       for (int fm = 0; fm < S::FM; ++fm) {
         float v[8];
         read_f32<S::OUTER_A, S::BM, S::FM>(v, now, wm * S::FM * 16, fm);
         const Parts a = split(v);
+        square(a.hi);
         // the small products first
         auto add = [&](const i32x4 Parts::*pb, const i32x4 Parts::*pa) {
 #pragma unroll
@@ -141,6 +160,7 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
   tile_of(p, id, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::CN;
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / S::THREADS), tid = threadIdx.x % S::THREADS;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / S::WN, wn = wave % S::WN;
   char* mine = lds + group * 2 * S::STAGE_BYTES;
 
   TileLoader<KIND_F32, S::OUTER_A, S::BM, S::THREADS, S::FM, false> load_a;
@@ -149,11 +169,15 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
   load_b.init(p.b, p.ldb, n0, p.N, tid);
 
   Accumulators<S> acc;
-  sum_tile_f32<S, false>(p, load_a, load_b, mine, group, first, steps, acc);
+  f32x4 squares;
+  float most_a[S::FM], most_b[S::FN];
+  sum_tile_f32<S, false>(p, load_a, load_b, mine, group, first, steps, acc, squares, most_a, most_b);
   add_groups<S>(lds, group, acc);
 
   const float small = small_sum(p.K);
   bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= !(fabsf(squares[i]) < kLarge * kLarge);
   if (group == 0) {  // (the others' sums are in this one's)
     unsigned least = 0xFFFFFFFFu;
 #pragma unroll
@@ -184,7 +208,30 @@ __device__ __forceinline__ void gemm_tile_f32(const GemmArgs& p, char* lds, int 
   if (__builtin_amdgcn_readfirstlane(again) != 0) {
     __syncthreads();
     Accumulators<S> plain;
-    sum_tile_f32<S, true>(p, load_a, load_b, mine, group, first, steps, plain);
+    sum_tile_f32<S, true>(p, load_a, load_b, mine, group, first, steps, plain, squares, most_a, most_b);
+    // the rows' largest values, of all groups
+    const int lane = threadIdx.x & 63, r = lane & 15;
+    unsigned* most = words + wm * S::FM * 16;
+    unsigned* most_of_b = words + S::BM + wn * S::FN * 16;
+    __syncthreads();
+    for (int i = threadIdx.x; i < S::BM + S::BN; i += S::THREADS * S::GROUPS) words[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int fm = 0; fm < S::FM; ++fm) atomicMax(&most[fm * 16 + r], __float_as_uint(most_a[fm]));
+#pragma unroll
+    for (int fn = 0; fn < S::FN; ++fn) atomicMax(&most_of_b[fn * 16 + r], __float_as_uint(most_b[fn]));
+    __syncthreads();
+#pragma unroll
+    for (int fm = 0; fm < S::FM; ++fm) {
+      const float row = __uint_as_float(most[fm * 16 + r]);
+#pragma unroll
+      for (int fn = 0; fn < S::FN; ++fn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float column = __uint_as_float(most_of_b[fn * 16 + (lane >> 4) * 4 + i]);
+          if (fmaxf(row, column) >= kLarge) acc.v[fm][fn][i] = __builtin_nanf("");
+        }
+    }
     add_groups<S, S::LDS_BYTES, true>(lds, group, plain);
 #pragma unroll
     for (int fm = 0; fm < S::FM; ++fm)

@@ -1,11 +1,51 @@
-"""float32 products whose sums bfloat16 parts do not give: infinities, NaN, and sums of very small values, in every product of
-the dense block, forward and backward."""
+"""float32 operands that bfloat16 parts do not hold, in every product of the dense block: very small ones beside very
+large ones, infinities and NaN. The sums are float32's all the same: single products to their roundings, and infinities and
+NaN where the definition has them."""
 import pytest
 import torch
 
 from tests import ffn_case
+from tests.test_ffn_products import DELTA, single_products
 
 pytestmark = pytest.mark.gpu
+
+SHAPES = [(33, 40, 16), (65, 136, 72), (130, 264, 328), (700, 1400, 4096)]
+
+
+def close(got, want, times, what, other=0.0):
+    """A product that is taken again is rounded once; `times` products in a row stay within DELTA each, and beyond float32's
+    normal numbers within 2^-149 of each value. A sum is not taken again if it comes out as zero, which a single product
+    does if an operand is below 2^-134 and has no parts: it is then below 2^-134 times the other one, of up to `other`."""
+    got, want = got.detach().double(), want.to(got.device)
+    off = (got - want).abs() - times * (DELTA * want.abs() + 2.0 ** -149)
+    off = torch.where((got == 0) & (want.abs() < 2.0 ** -134 * other), -1.0, off)
+    assert torch.isfinite(got).all() and float(off.max()) <= 0, what
+
+
+# powers of two for the tokens' values, the up weights, the down weights and the output's gradient; products stay within
+# float32's range, and the tokens' constant column and the gates are 64 as ever
+@pytest.mark.parametrize("scales", [(-118, 60, 0, 0), (60, -118, 0, 0), (-126, 90, 0, 0), (-140, 100, 0, 0), (-100, 30, 0, 0),
+                                    (-60, -20, 0, 0), (0, 0, 60, -118), (0, 0, -118, 60), (-10, -5, 100, -110), (0, -8, -115, 100),
+                                    (45, 40, -40, -50)])
+@pytest.mark.parametrize("T,H,I", SHAPES)
+def test_products_of_operands_far_apart(T, H, I, scales):
+    from flash_distributed_moe_amd import flashFfnOp as ops
+
+    sx, sw, sv, sd = (2.0 ** s for s in scales)
+    x, w13, w2, dy = single_products(T, H, I)
+    x[:, 1:] = (x[:, 1:].double() * sx).float()
+    w13[I:] = (w13[I:].double() * sw).float()
+    w2, dy = (w2.double() * sv).float(), (dy.double() * sd).float()
+    leaves = [t.cuda().requires_grad_() for t in (x, w13, w2)]
+    y = ops.gated_ffn(*leaves)
+    dx, dw13, dw2 = torch.autograd.grad(y, leaves, dy.cuda())
+    x, w13, w2, dy = (t.double() for t in (x, w13, w2, dy))
+    u = x[:, 1:] @ w13[I:, 1:].t()
+    h, dh = 64 * u, dy @ w2
+    close(y, h @ w2.t(), 2, "y")
+    close(dw2, dy.t() @ h, 2, "dw2")
+    close(dx[:, 1:], (64 * dh) @ w13[I:, 1:], 2, "dx")
+    close(dw13[I:, 1:], (64 * dh).t() @ x[:, 1:], 2, "dw13, up", other=min(2.0 ** 32, float((64 * dh).abs().max())))
 
 
 def make(T, H, I, seed=0):
