@@ -4,6 +4,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <hip/hip_runtime.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -31,6 +32,12 @@ void check_device(const at::Tensor& t, const char* name, const at::Tensor& like)
   TORCH_CHECK(t.defined(), name, " tensor is undefined");
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (ROCm)");
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", not on ", t.device());
+}
+
+// A dual tensor's result would come back without a tangent, which stands for a zero one.
+void refuse_tangent(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
+              " carries a tangent: there are no forward-mode derivatives here");
 }
 
 int dtype_of(const at::Tensor& t, const char* name) {
@@ -120,6 +127,9 @@ FlashMoeFfnDesc describe(const at::Tensor& x, const at::Tensor& w13, const at::T
 // (y, saved): saved is undefined unless `save`
 std::tuple<at::Tensor, at::Tensor> ffn_forward(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2,
                                                const OptTensor& s13, const OptTensor& s2, int activation, bool save) {
+  refuse_tangent(x, "x");
+  refuse_tangent(w13, "w13");
+  refuse_tangent(w2, "w2");
   const FlashMoeFfnDesc d = describe(x, w13, w2, s13, s2, activation);
   const DeviceGuard guard(x.device());
   const Rows rows = rows_of(x, "x");
@@ -259,6 +269,7 @@ at::Tensor mxfp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, a
 }
 
 at::Tensor mxfp4_linear(const at::Tensor& x, const OptTensor& x_scales, const at::Tensor& codes, const at::Tensor& scales) {
+  refuse_tangent(x, "x");
   const int k = check_mxfp4(codes, scales, "weights");
   TORCH_CHECK(codes.dim() == 2, "weights must be MXFP4 [N, K]");
   check_device(x, "x", codes);

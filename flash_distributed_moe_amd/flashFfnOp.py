@@ -11,7 +11,7 @@ weights, and `gated_ffn` takes them in place of both weights (no gradients).
 
 There is no fallback: everything runs on the compiled `flashMoeLauncher` extension, on the current
 stream of the tensors' device, and can be captured into a HIP graph. Wrong arguments raise
-RuntimeError. (The reference has none of these operators; its wrapper,
+RuntimeError, and so do inputs that carry a forward-mode tangent. (The reference has none of these operators; its wrapper,
 test/singleGPU/python/flashMoeOp.py:7-38, covers the sparse block only.)
 """
 import os

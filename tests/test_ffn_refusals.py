@@ -1,0 +1,41 @@
+"""Calls of the dense block and of MXFP4 that would give an answer that is not the caller's: refused, before anything about
+the tensors' device is looked at, so without a GPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from flash_distributed_moe_amd import flashFfnOp as ops
+
+
+def operands():
+    return torch.zeros(2, 64), torch.zeros(64, 64), torch.zeros(64, 32)
+
+
+def packed():
+    return ops.Mxfp4(torch.zeros(64, 32, dtype=torch.uint8), torch.zeros(64, 2, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(which, leaf):
+    """A dual tensor has no requires_grad: its tangent would be dropped without a word."""
+    args = list(operands())
+    with fwd.dual_level():
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        if leaf:
+            args[(which + 1) % 3].requires_grad_()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_ffn(*args)
+
+
+def test_forward_mode_is_refused_with_mxfp4_weights():
+    q = packed()
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(2, 64), torch.ones(2, 64))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.mxfp4_linear(x, q)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_ffn(x, q, q)
+        # detached values, and dual tensors that are not differentiated, are ordinary ones: the next check speaks
+        with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA tensor"):
+            ops.gated_ffn(x, *operands()[1:])
