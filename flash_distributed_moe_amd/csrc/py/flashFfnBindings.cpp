@@ -304,12 +304,12 @@ at::Tensor mxfp4_linear(const at::Tensor& x, const OptTensor& x_scales, const at
 void bind_ffn(py::module_& m) {
   m.attr("ACT_SILU") = static_cast<int>(FLASH_MOE_ACT_SILU);
   m.attr("ACT_GELU_TANH") = static_cast<int>(FLASH_MOE_ACT_GELU_TANH);
-  m.def("ffn_forward", &ffn_forward, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("w13_scales"), py::arg("w2_scales"),
-        py::arg("activation"), py::arg("save"));
-  m.def("ffn_backward", &ffn_backward, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("activation"), py::arg("dy"),
-        py::arg("saved"), py::arg("want_dx"), py::arg("want_dw13"), py::arg("want_dw2"));
   m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("activation"),
         py::call_guard<py::gil_scoped_release>());
+  m.def("gated_ffn_mxfp4",
+        [](const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const at::Tensor& w13_scales, const at::Tensor& w2_scales,
+           int activation) { return std::get<0>(ffn_forward(x, w13, w2, w13_scales, w2_scales, activation, false)); },
+        py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("w13_scales"), py::arg("w2_scales"), py::arg("activation"));
   m.def("mxfp4_quantize", &mxfp4_quantize, py::arg("x"));
   m.def("mxfp4_dequantize",
         [](const at::Tensor& codes, const at::Tensor& scales, const py::object& dtype) {

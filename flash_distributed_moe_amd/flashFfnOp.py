@@ -79,7 +79,7 @@ def gated_ffn(x, w13, w2, activation="silu"):
         if not (isinstance(w13, Mxfp4) and isinstance(w2, Mxfp4)):
             raise RuntimeError("both weights must be MXFP4, or neither")
         _refuse_grad(x)
-        return flashMoeLauncher.ffn_forward(x, w13.codes, w2.codes, w13.scales, w2.scales, act, False)[0]
+        return flashMoeLauncher.gated_ffn_mxfp4(x, w13.codes, w2.codes, w13.scales, w2.scales, act)
     return flashMoeLauncher.gated_ffn(x, w13, w2, act)
 
 

@@ -39,3 +39,9 @@ def test_forward_mode_is_refused_with_mxfp4_weights():
         # detached values, and dual tensors that are not differentiated, are ordinary ones: the next check speaks
         with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="CUDA tensor"):
             ops.gated_ffn(x, *operands()[1:])
+
+
+def test_the_extension_takes_no_saved_results():
+    """What a forward pass keeps is the autograd node's: no call takes it from its caller or hands it out."""
+    bound = [name for name in dir(ops.flashMoeLauncher) if "ffn" in name or "mxfp4" in name]
+    assert sorted(bound) == ["gated_ffn", "gated_ffn_mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_quantize"]
