@@ -85,8 +85,9 @@ def gated_ffn(x, w13, w2, activation="silu"):
 
 class FlashGatedFfn(torch.nn.Module):
     """`gated_ffn` over the weights of a dense block or shared expert: a module with
-    `gate_up_proj.weight` [2I, H] and `down_proj.weight` [H, I]. The parameters stay the block's own.
-    quantize="mxfp4" converts them once, into buffers of this module (the block is not kept)."""
+    `gate_up_proj.weight` [2I, H] and `down_proj.weight` [H, I], without biases. The parameters stay the block's own.
+    quantize="mxfp4" converts the weights
+    once, into buffers of this module (the block is not kept)."""
 
     def __init__(self, block, activation="silu", quantize=None):
         super().__init__()
@@ -94,6 +95,9 @@ class FlashGatedFfn(torch.nn.Module):
             raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
         if quantize not in (None, "mxfp4"):
             raise RuntimeError('quantize must be None or "mxfp4"')
+        for name in ("gate_up_proj", "down_proj"):
+            if getattr(getattr(block, name), "bias", None) is not None:
+                raise RuntimeError("%s has a bias, which gated_ffn does not add" % name)
         self.activation, self.quantize = activation, quantize
         w13, w2 = block.gate_up_proj.weight, block.down_proj.weight
         if quantize is None:
