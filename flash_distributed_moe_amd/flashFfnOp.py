@@ -83,21 +83,40 @@ def gated_ffn(x, w13, w2, activation="silu"):
     return flashMoeLauncher.gated_ffn(x, w13, w2, act)
 
 
+def _activation_of(act_fn):
+    """Which of ACTIVATIONS a block's activation is, by its values; of gates alone, or of gates and up projections side by
+    side (a vector of gates and ones tells)."""
+    g = torch.linspace(-6.0, 6.0, 97, dtype=torch.float32, device="cpu")
+    try:
+        with torch.no_grad():
+            a = act_fn(torch.cat((g, torch.ones_like(g))))[..., :97]
+        known = {"silu": torch.nn.functional.silu(g), "gelu_tanh": torch.nn.functional.gelu(g, approximate="tanh")}
+        for name, values in known.items():
+            if torch.allclose(a.float().cpu(), values, rtol=0, atol=1e-4):  # exact GELU is 5e-4 off its tanh form
+                return name
+    except Exception:  # whatever a stranger's code raises for these arguments
+        pass
+    raise RuntimeError("the block's act_fn is neither SiLU nor GELU's tanh form: pass activation to say which to use")
+
+
 class FlashGatedFfn(torch.nn.Module):
     """`gated_ffn` over the weights of a dense block or shared expert: a module with
     `gate_up_proj.weight` [2I, H] and `down_proj.weight` [H, I], without biases. The parameters stay the block's own.
-    quantize="mxfp4" converts the weights
+    activation: by default what the block's `act_fn` is, SiLU if it has none. quantize="mxfp4" converts the weights
     once, into buffers of this module (the block is not kept)."""
 
-    def __init__(self, block, activation="silu", quantize=None):
+    def __init__(self, block, activation=None, quantize=None):
         super().__init__()
-        if activation not in ACTIVATIONS:
+        if activation is not None and activation not in ACTIVATIONS:
             raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
         if quantize not in (None, "mxfp4"):
             raise RuntimeError('quantize must be None or "mxfp4"')
         for name in ("gate_up_proj", "down_proj"):
             if getattr(getattr(block, name), "bias", None) is not None:
                 raise RuntimeError("%s has a bias, which gated_ffn does not add" % name)
+        if activation is None:
+            act_fn = getattr(block, "act_fn", None)
+            activation = "silu" if act_fn is None else _activation_of(act_fn)
         self.activation, self.quantize = activation, quantize
         w13, w2 = block.gate_up_proj.weight, block.down_proj.weight
         if quantize is None:

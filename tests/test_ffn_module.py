@@ -15,10 +15,32 @@ class Block(torch.nn.Module):
             self.act_fn = act_fn
 
 
+class SiluAndMul(torch.nn.Module):
+    def forward(self, x):
+        g, u = x.chunk(2, -1)
+        return torch.nn.functional.silu(g) * u
+
+
 @pytest.mark.parametrize("bias", [(True, False), (False, True)])
 def test_biases_are_refused(bias):
     with pytest.raises(RuntimeError, match="has a bias"):
         ops.FlashGatedFfn(Block(bias=bias))
+
+
+@pytest.mark.parametrize("act_fn,name", [(None, "silu"), (torch.nn.SiLU(), "silu"), (torch.nn.functional.silu, "silu"), (SiluAndMul(), "silu"),
+                                         (torch.nn.GELU(approximate="tanh"), "gelu_tanh")])
+def test_the_block_says_which_activation(act_fn, name):
+    assert ops.FlashGatedFfn(Block(act_fn=act_fn)).activation == name
+    assert ops.FlashGatedFfn(Block(act_fn=act_fn), activation="gelu_tanh").activation == "gelu_tanh"
+
+
+@pytest.mark.parametrize("act_fn", [torch.nn.GELU(), torch.nn.ReLU(), torch.sum, "silu", lambda x: 1 / 0])
+def test_another_activation_is_refused(act_fn):
+    block = Block()
+    block.act_fn = act_fn
+    with pytest.raises(RuntimeError, match="pass activation"):
+        ops.FlashGatedFfn(block)
+    assert ops.FlashGatedFfn(block, activation="silu").activation == "silu"
 
 
 def test_the_parameters_stay_the_block_s():
@@ -36,7 +58,7 @@ def test_training_through_the_module(dtype, act_fn, name):
     block's weights and the module's answers."""
     torch.manual_seed(5)
     block = Block(136, 72, act_fn=act_fn, dtype=dtype, device="cuda")
-    module = ops.FlashGatedFfn(block, activation=name)
+    module = ops.FlashGatedFfn(block)
     total = {}
     for T in (40, 7):
         x, dy = torch.randn(T, 136, device="cuda", dtype=dtype), torch.randn(T, 136, device="cuda", dtype=dtype)
