@@ -84,10 +84,11 @@ __device__ __forceinline__ float act_of(int act, float g) {
   const float w = act == ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
   return g * sigmoid<EXACT>(w);
 }
-// act(g) and act'(g) = sigmoid(w) + g sigmoid(w) (1 - sigmoid(w)) dw/dg
+// act(g) and act'(g) = sigmoid(w) + g sigmoid(w) (1 - sigmoid(w)) dw/dg. The sigmoid is 0 or 1 long before g^2 is 10^12,
+// and with more dw/dg would be infinite from 2 * 10^19 on, which the zero beside it does not make a number again.
 template <bool EXACT>
 __device__ __forceinline__ void act_and_slope(int act, float g, float& a, float& slope) {
-  const float g2 = g * g;
+  const float g2 = fminf(g * g, 1e12f);
   const float w = act == ACT_SILU ? g : 1.5957691216057308f * (g + 0.044715f * g2 * g);
   const float dw = act == ACT_SILU ? 1.0f : 1.5957691216057308f * (1.0f + 0.134145f * g2);
   const float s = sigmoid<EXACT>(w);
