@@ -40,23 +40,40 @@ class Mxfp4(NamedTuple):
     scales: torch.Tensor
 
 
+# what reading an attribute of a stranger or handing it to the extension raises
+_STRANGERS = (AttributeError, TypeError)
+
+
+def _stranger(wanted, *args):
+    return RuntimeError("%s: not %s" % (wanted, ", ".join(type(a).__name__ for a in args)))
+
+
 def quantize_mxfp4(x):
     """x [..., K] (float32 or bfloat16, K a multiple of 32) as Mxfp4. Not differentiable."""
-    return Mxfp4(*flashMoeLauncher.mxfp4_quantize(x.detach()))
+    try:
+        return Mxfp4(*flashMoeLauncher.mxfp4_quantize(x.detach()))
+    except _STRANGERS:
+        raise _stranger("x must be a tensor", x) from None
 
 
 def dequantize_mxfp4(q, dtype=torch.bfloat16):
     """The values of q, which both dtypes hold exactly."""
-    return flashMoeLauncher.mxfp4_dequantize(q.codes, q.scales, dtype)
+    try:
+        return flashMoeLauncher.mxfp4_dequantize(q.codes, q.scales, dtype)
+    except _STRANGERS:
+        raise _stranger("q must be Mxfp4 and dtype a torch.dtype", q, dtype) from None
 
 
 def mxfp4_linear(x, weight):
     """x [..., K] (bfloat16, or Mxfp4) times the transpose of weight (Mxfp4 [N, K]): bfloat16 [..., N],
     summed in float32. Not differentiable."""
-    if isinstance(x, Mxfp4):
-        return flashMoeLauncher.mxfp4_linear(x.codes, x.scales, weight.codes, weight.scales)
-    _refuse_grad(x)
-    return flashMoeLauncher.mxfp4_linear(x, None, weight.codes, weight.scales)
+    try:
+        if isinstance(x, Mxfp4):
+            return flashMoeLauncher.mxfp4_linear(x.codes, x.scales, weight.codes, weight.scales)
+        _refuse_grad(x)
+        return flashMoeLauncher.mxfp4_linear(x, None, weight.codes, weight.scales)
+    except _STRANGERS:
+        raise _stranger("x must be a tensor or Mxfp4, weight Mxfp4", x, weight) from None
 
 
 def _refuse_grad(x):
@@ -72,15 +89,18 @@ def gated_ffn(x, w13, w2, activation="silu"):
     may lie apart. Gradients (once) for x and row-major weights; a pass that needs them keeps the two
     projections in float32 and h until its backward pass. A step that is captured into a HIP graph wants no
     eager graph of the same parameters alive: the call raises then."""
-    if activation not in ACTIVATIONS:
+    if not isinstance(activation, str) or activation not in ACTIVATIONS:
         raise RuntimeError("activation must be one of %s" % ", ".join(sorted(ACTIVATIONS)))
     act = ACTIVATIONS[activation]
-    if isinstance(w13, Mxfp4) or isinstance(w2, Mxfp4):
-        if not (isinstance(w13, Mxfp4) and isinstance(w2, Mxfp4)):
-            raise RuntimeError("both weights must be MXFP4, or neither")
-        _refuse_grad(x)
-        return flashMoeLauncher.gated_ffn_mxfp4(x, w13.codes, w2.codes, w13.scales, w2.scales, act)
-    return flashMoeLauncher.gated_ffn(x, w13, w2, act)
+    try:
+        if isinstance(w13, Mxfp4) or isinstance(w2, Mxfp4):
+            if not (isinstance(w13, Mxfp4) and isinstance(w2, Mxfp4)):
+                raise RuntimeError("both weights must be MXFP4, or neither")
+            _refuse_grad(x)
+            return flashMoeLauncher.gated_ffn_mxfp4(x, w13.codes, w2.codes, w13.scales, w2.scales, act)
+        return flashMoeLauncher.gated_ffn(x, w13, w2, act)
+    except _STRANGERS:
+        raise _stranger("x must be a tensor, the weights tensors or Mxfp4", x, w13, w2) from None
 
 
 def _activation_of(act_fn):

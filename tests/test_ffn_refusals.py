@@ -45,3 +45,27 @@ def test_the_extension_takes_no_saved_results():
     """What a forward pass keeps is the autograd node's: no call takes it from its caller or hands it out."""
     bound = [name for name in dir(ops.flashMoeLauncher) if "ffn" in name or "mxfp4" in name]
     assert sorted(bound) == ["gated_ffn", "gated_ffn_mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_quantize"]
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, w13, w2, q: ops.mxfp4_linear(x, w13),
+    lambda x, w13, w2, q: ops.mxfp4_linear(None, q),
+    lambda x, w13, w2, q: ops.mxfp4_linear([1.0], q),
+    lambda x, w13, w2, q: ops.mxfp4_linear(x, None),
+    lambda x, w13, w2, q: ops.dequantize_mxfp4(x),
+    lambda x, w13, w2, q: ops.dequantize_mxfp4(q, "bfloat16"),
+    lambda x, w13, w2, q: ops.quantize_mxfp4(q),
+    lambda x, w13, w2, q: ops.quantize_mxfp4(None),
+    lambda x, w13, w2, q: ops.gated_ffn(None, w13, w2),
+    lambda x, w13, w2, q: ops.gated_ffn(x, None, w2),
+    lambda x, w13, w2, q: ops.gated_ffn(x, w13, 3.0),
+    lambda x, w13, w2, q: ops.gated_ffn(q, q, q),
+    lambda x, w13, w2, q: ops.gated_ffn(x, ops.Mxfp4(q.codes, None), q),
+    lambda x, w13, w2, q: ops.mxfp4_linear(ops.Mxfp4(None, None), q),
+    lambda x, w13, w2, q: ops.dequantize_mxfp4(ops.Mxfp4(1, 2)),
+    lambda x, w13, w2, q: ops.gated_ffn(x, w13, w2, activation=["silu"]),
+])
+def test_arguments_of_another_kind(call):
+    """Wrong arguments raise RuntimeError, as the documentation says, whatever they are instead."""
+    with pytest.raises(RuntimeError):
+        call(*operands(), packed())
