@@ -35,6 +35,8 @@ using fmoe::GemmArgs;
 
 // A tile's rows are addressed with 32 bits from its first one: 256 rows of up to this many values.
 constexpr long long kMaxStride = 1ll << 20;
+// Rows of a product, or columns: with tiles' worth more they still count in 32 bits, and no launch takes more.
+constexpr int kMaxRows = 1 << 30;
 
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -65,7 +67,7 @@ hipError_t validate(const FlashMoeFfnDesc* d, int tokens) {
     FMOE_FAIL(hipErrorInvalidValue, "H=%i, I=%i: multiples of %i, H up to %lld, I below half of that", d->hidden,
               d->intermediate, of, kMaxStride);
   if (mx && d->dtype != FLASH_MOE_BF16) FMOE_FAIL(hipErrorInvalidValue, "MXFP4 weights take bfloat16 tokens");
-  if (tokens < 0) FMOE_FAIL(hipErrorInvalidValue, "%i tokens", tokens);
+  if (tokens < 0 || tokens > kMaxRows) FMOE_FAIL(hipErrorInvalidValue, "%i tokens (at most %i)", tokens, kMaxRows);
   return hipSuccess;
 }
 
@@ -277,8 +279,8 @@ int flashMoeMxfp4Dequantize(int dtype, const void* codes, const void* scales, in
 int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes) {
   if (x_format != FLASH_MOE_BF16 && x_format != FLASH_MOE_MXFP4)
     FMOE_FAIL(hipErrorInvalidValue, "x_format %i is neither bfloat16 (1) nor MXFP4 (2)", x_format);
-  if (rows < 0 || n < 0 || k < 32 || k % 32 != 0 || k > kMaxStride)
-    FMOE_FAIL(hipErrorInvalidValue, "%i x %i x %i (the last a multiple of 32 up to %lld)", rows, n, k, kMaxStride);
+  if (rows < 0 || rows > kMaxRows || n < 0 || n > kMaxRows || k < 32 || k % 32 != 0 || k > kMaxStride)
+    FMOE_FAIL(hipErrorInvalidValue, "%i x %i x %i (up to %i twice, the last a multiple of 32 up to %lld)", rows, n, k, kMaxRows, kMaxStride);
   if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result pointer");
   GemmArgs p{};
   p.M = rows, p.N = n, p.K = k;

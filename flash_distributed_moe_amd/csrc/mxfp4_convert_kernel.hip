@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const unsigned* c
 static bool grid_for(long long rows, int k, unsigned& blocks) {
   const long long n = (rows * (k / 32) * 4 + 255) / 256;
   blocks = static_cast<unsigned>(n);
-  return n <= 0x7FFFFFFF;
+  return n * 256 <= 0xFFFFFFFFll;  // threads of a launch
 }
 
 hipError_t launch_mxfp4_quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales,

@@ -293,7 +293,7 @@ typedef struct FlashMoeFfnDesc {
   const void* w2_scales;  /* MXFP4: device, [H,I/32] bytes; else unused */
 } FlashMoeFfnDesc;
 
-/* Device bytes a batch of `tokens` needs (any result may be NULL): what a forward pass keeps for
+/* Device bytes a batch of `tokens` (at most 2^30) needs (any result may be NULL): what a forward pass keeps for
  * the backward pass, and the workspaces of both. Only the description's sizes are read. */
 int flashMoeFfnBytes(const FlashMoeFfnDesc* desc, int tokens, size_t* saved, size_t* forward, size_t* backward);
 /* The workspace of a forward pass that keeps `saved` (0: none); it may be NULL, and then long sums are not
@@ -321,7 +321,7 @@ int flashMoeFfnBackward(const FlashMoeFfnDesc* desc, const void* x, long long ld
  * [rows, k/32]; both without gaps, codes beginning on 16 bytes, scales anywhere (on 4 bytes is faster).
  * Quantisation takes b - 127 = floor(log2(largest magnitude of the block)) - 2, at least -127, rounds to the
  * nearest value, ties to the even code, and stops at 6. A block with an infinity or NaN becomes all NaN.
- * k is a multiple of 32. x and out lie ldx / ldo values apart, whole 16 bytes. */
+ * k is a multiple of 32, rows * k below 2^35. x and out lie ldx / ldo values apart, whole 16 bytes. */
 enum { FLASH_MOE_MXFP4 = 2 };
 int flashMoeMxfp4Quantize(int dtype, const void* x, long long ldx, int rows, int k, void* codes, void* scales, void* stream);
 int flashMoeMxfp4Dequantize(int dtype, const void* codes, const void* scales, int rows, int k, void* out, long long ldo,
@@ -330,7 +330,7 @@ int flashMoeMxfp4Dequantize(int dtype, const void* codes, const void* scales, in
 /* y[rows, n] = x W^T in bfloat16, summed in float32, of MXFP4 weights W [n, k]. x: FLASH_MOE_BF16 rows ldx values
  * apart (x_scales unused), or FLASH_MOE_MXFP4 codes with x_scales (ldx = k). y's rows lie ldy values apart;
  * where n is a multiple of 8 they begin on 16 bytes. workspace: flashMoeMxfp4LinearBytes of device memory
- * (0: may be NULL). */
+ * (0: may be NULL). rows and n are at most 2^30, k at most 2^20. */
 int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes);
 int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long long ldx, int rows, const void* codes,
                         const void* scales, int n, int k, void* y, long long ldy, void* workspace, void* stream);

@@ -1,10 +1,12 @@
 """Calls of the dense block and of MXFP4 that would give an answer that is not the caller's: refused, before anything about
 the tensors' device is looked at, so without a GPU."""
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from flash_distributed_moe_amd import flashFfnOp as ops
+from flash_distributed_moe_amd import _lib, flashFfnOp as ops
 
 
 def operands():
@@ -69,3 +71,25 @@ def test_arguments_of_another_kind(call):
     """Wrong arguments raise RuntimeError, as the documentation says, whatever they are instead."""
     with pytest.raises(RuntimeError):
         call(*operands(), packed())
+
+
+HUGE = [(1 << 30) + 1, (1 << 31) - 64, (1 << 31) - 1]
+
+
+@pytest.mark.parametrize("n", HUGE)
+def test_batches_beyond_what_a_launch_counts(n, capfd):
+    """Sizes whose tiles would be counted beyond 32 bits, among them a sum over tokens that would have come out as zeros."""
+    lib = _lib.load()
+    d = _lib.FfnDesc(8, 8, _lib.BF16, _lib.ACT_SILU, _lib.FFN_ROW_MAJOR, 0x1000, 0x2000, None, None)
+    size = ctypes.c_size_t(0)
+    bad = _lib.HIP_ERROR_INVALID_VALUE
+    assert lib.flashMoeFfnBytes(ctypes.byref(d), n, ctypes.byref(size), None, None) == bad
+    assert lib.flashMoeFfnForward(ctypes.byref(d), 0x10000, 8, 0x20000, 8, n, None, 0x30000, None) == bad
+    assert lib.flashMoeFfnBackward(ctypes.byref(d), 0x10000, 8, 0x20000, 8, n, 0x30000, None, None, 8, None, 0x40000, None) == bad
+    for fmt in (_lib.BF16, _lib.MXFP4):
+        for rows, columns in ((n, 8), (1, n)):
+            assert lib.flashMoeMxfp4LinearBytes(fmt, rows, columns, 32, ctypes.byref(size)) == bad
+            assert lib.flashMoeMxfp4Linear(fmt, 0x10000, 0x1000, 32, rows, 0x20000, 0x2000, columns, 32, 0x30000, columns, 0x40000, None) == bad
+    assert lib.flashMoeMxfp4Quantize(_lib.BF16, 0x10000, 64, n, 64, 0x20000, 0x30000, None) == bad
+    assert lib.flashMoeMxfp4Dequantize(_lib.BF16, 0x10000, 0x20000, n, 64, 0x30000, 64, None) == bad
+    assert "[MOE" in capfd.readouterr().out
