@@ -321,7 +321,10 @@ static hipError_t go_plain(const GemmArgs& p, hipStream_t stream) {
   constexpr double W = KIND == SKINNY_F32 ? 4 : KIND == SKINNY_BF16 ? 2 : 0.53, X = KIND == SKINNY_F32 ? 4 : KIND == SKINNY_MXFP4_BOTH ? 0.53 : 2;
   if constexpr (KIND == SKINNY_MXFP4_WEIGHTS) {
     // The waves' rows of x take LDS: with long rows eight waves a workgroup pay, with short ones there are few steps
-    // for each. N=4096, K=12288, T=5, 4 / 8 waves 9.3 / 8.0 us; N=12288 gated, K=4096, T=5, 11.7 / 14.2.
+    // for each. Measured over 8 K, 5 N and M = 1, 5, 12 (graphs of 24 calls), us, 4 / 8 waves: M=5, N=2048, K=1024 3.1 / 3.7,
+    // 4096 5.4 / 5.4, 8192 7.5 / 6.9, 16384 12.0 / 9.6; N=8192 4.4 / 5.1, 7.0 / 7.6, 13.0 / 12.2, 21.0 / 19.9; M=12, N=512
+    // 3.6 / 4.4, 5.7 / 5.5, 9.2 / 7.8, 15.4 / 11.4. Behind, of what this rule chooses, are M=12, N=16384, K=8192 with
+    // 22.0 / 26.3 to K=12288 with 32.7 / 35.8, and by up to 10 % M=1 and 5 there with K=16384.
     const int hb = pick_groups(p, 2, 4, false, W, X);
     if (p.K >= 8192 && XB <= 2)
       return hb == 2 ? go<KIND, false, 2, XB, XB <= 2 ? 8 : 4, 1>(p, stream) : go<KIND, false, 4, XB, XB <= 2 ? 8 : 4, 1>(p, stream);
