@@ -12,9 +12,9 @@
 // 2^-24 of a sum of small_sum(K) and more. So a sum is taken again, on the float32 matrix instructions, if it is smaller than
 // that and not zero, if its row or column holds a larger operand, or if it is no finite number (an infinity has no parts): a
 // workgroup with such a sum goes over its k once more, other sums stay as they are. Larger operands are noticed by the sums of
-// the squares of all rows' high parts, one more instruction a block (T=1001, H=2048, I=768, forward 79 -> 83 us; the largest
-// magnitude by vector instructions costs twice that). That second pass takes 2 to 3 times a tile's time: a step of this size
-// 0.47 ms with a NaN among its tokens, 0.22 without. (A sum that comes out as zero is left: ordinary
+// the squares of all rows' high parts, one more instruction a block: 4 to 5 % of a call (T=1001, H=2048, I=768, step 222 ->
+// 232 us, with parts cut off and none of this 217, all in one run; the largest magnitude by vector instructions costs more).
+// That second pass takes 2 to 3 times a tile's time: a step of this size 0.47 ms with a NaN among its tokens. (A sum that comes out as zero is left: ordinary
 // ones do now and then. Of operands below 2^-134 alone, times others below kLarge, it may be off by K 2^-101.)
 #include "ffn_gemm_device.h"
 
@@ -284,8 +284,10 @@ static hipError_t launch_f32(GemmArgs p, const TilePlan& plan, hipStream_t strea
 
 // Large tiles split each value for more products, small ones fill more CUs, and groups of waves that share a tile's k fill
 // their waits. Measured on M=1001, N=768 gated, K=2048, 128 x 128 / 128 x 64 / 64 x 64 rows of A and B, us:
-// 114 / 76 / 65 in one group, 87 / 57 / 57 in two, 64 x 64 in four 64; M=1001, N=768, K=2048 with B's rows as k
-// 120 / 84 / 55, 97 / 60 / 38, 34; M=N=K=4096 641 / 739 / 830 in one.
+// 113 / 75 / 75 in one group, 91 / 62 / 67 in two, 64 x 64 in four 72; M=1001, N=768, K=2048 with B's rows as k
+// 122 / 79 / 55, 101 / 64 / 42, 37; M=N=K=4096 683 / 819 / 969 in one.
+// The costs below are those of parts that were cut off, before large operands were looked for, 5 to 20 % less; by the present ones
+// 60 random calls take 0.3 % more, and their steps 0.5 %.
 static const TileCost kF32Ways[] = {{128, 128, 0, 1.7, 2.5, 1.25}, {128, 128, 1, 1.32, 2.7, 1.35}, {128, 64, 0, 1.1, 1.6, 0.72},
                                     {64, 64, 0, 0.78, 0.98, 0.42}, {64, 64, 0.8, 0.54, 0.85, 0.45}, {64, 64, 1.8, 0.48, 0.95, 0.48}};
 static const TileCost kF32GatedWays[] = {{128, 64, 0, 1.7, 2.5, 1.25}, {128, 64, 1, 1.32, 2.7, 1.35}, {128, 32, 0, 1.1, 1.6, 0.72},
