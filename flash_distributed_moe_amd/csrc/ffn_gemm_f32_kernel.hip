@@ -14,8 +14,9 @@
 // workgroup with such a sum goes over its k once more, other sums stay as they are. Larger operands are noticed by the sums of
 // the squares of all rows' high parts, one more instruction a block: 4 to 5 % of a call (T=1001, H=2048, I=768, step 222 ->
 // 232 us, with parts cut off and none of this 217, all in one run; the largest magnitude by vector instructions costs more).
-// That second pass takes 2 to 3 times a tile's time: a step of this size 0.47 ms with a NaN among its tokens. (A sum that comes out as zero is left: ordinary
-// ones do now and then. Of operands below 2^-134 alone, times others below kLarge, it may be off by K 2^-101.)
+// That second pass takes 2 to 3 times a tile's time: a step of this size 0.47 ms with a NaN among its tokens. (A sum that
+// comes out as zero is left: ordinary ones do now and then. Of operands below 2^-134 alone, times others below kLarge, it may
+// be off by K 2^-101.)
 #include "ffn_gemm_device.h"
 
 namespace fmoe {
