@@ -50,6 +50,12 @@ class FfnDesc(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("w13", "w2", "w13_scales", "w2_scales")]
 
 
+class RouteDesc(ctypes.Structure):
+    """Mirror of FlashMoeRouteDesc."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("experts", "top_k", "dtype", "renormalize")]
+
+
 # name -> (restype, argtypes); every symbol include/flash_moe.h declares
 C_ABI = {
     "flashMoeVersion": (ctypes.c_char_p, []),
@@ -98,6 +104,11 @@ C_ABI = {
     "flashMoeMxfp4Linear": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                            ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]),
+    "flashMoeRouteBytes": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "flashMoeRoute": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                     ctypes.c_int] + [ctypes.c_void_p] * 8),
+    "flashMoeRouteBackward": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                             ctypes.c_int] + [ctypes.c_void_p] * 7 + [ctypes.c_longlong, ctypes.c_void_p]),
     "flashMoeSetDenseSmallBatch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
 }
 ABI_VERSION = 3

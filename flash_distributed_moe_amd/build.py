@@ -60,7 +60,7 @@ def build(verbose=True):
     return LIB_PATH
 
 
-PY_SRCS = [os.path.join(CSRC, "py", name) for name in ("flashMoeLauncherModule.cpp", "flashFfnBindings.cpp")]
+PY_SRCS = [os.path.join(CSRC, "py", name) for name in ("flashMoeLauncherModule.cpp", "flashFfnBindings.cpp", "flashLayerBindings.cpp")]
 ROOT = os.path.dirname(HERE)
 
 

@@ -1,86 +1,9 @@
 // The dense gated feed-forward block and MXFP4 in the `flashMoeLauncher` extension: checks of the
 // tensors, outputs and workspaces from torch's allocator, and the C ABI's calls on the current stream.
 // `flash_distributed_moe_amd/flashFfnOp.py` is the Python surface above them.
-#include <ATen/hip/HIPContext.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/AutogradState.h>
-#include <hip/hip_runtime.h>
-#include <pybind11/pybind11.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/variable.h>
-#include <torch/extension.h>
-
-#include <limits>
-
-#include "../../../include/flash_moe.h"
-
-namespace py = pybind11;
+#include "tensorChecks.h"
 
 namespace {
-
-using DeviceGuard = c10::hip::HIPGuardMasqueradingAsCUDA;
-using OptTensor = c10::optional<at::Tensor>;
-
-void* current_stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
-
-void check_hip(int e, const char* what) {
-  TORCH_CHECK(e == hipSuccess, what, " failed: ", hipGetErrorString(static_cast<hipError_t>(e)), " (hipError_t ", e, ")");
-}
-
-void check_device(const at::Tensor& t, const char* name, const at::Tensor& like) {
-  TORCH_CHECK(t.defined(), name, " tensor is undefined");
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (ROCm)");
-  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", not on ", t.device());
-}
-
-// A dual tensor's result would come back without a tangent, which stands for a zero one.
-void refuse_tangent(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
-              " carries a tangent: there are no forward-mode derivatives here");
-}
-
-int dtype_of(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16");
-  return t.scalar_type() == at::kFloat ? FLASH_MOE_F32 : FLASH_MOE_BF16;
-}
-
-int int_size(int64_t v, const char* name) {
-  TORCH_CHECK(v >= 0 && v <= std::numeric_limits<int>::max(), name, " is too large: ", v);
-  return static_cast<int>(v);
-}
-
-bool begins_on_16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-
-// A weight or code tensor as the kernels read it: without gaps. (One that is a view into something
-// larger, at an odd place, is refused rather than copied at every call.)
-void check_packed(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-  TORCH_CHECK(begins_on_16(t), name, " must begin on 16 bytes");
-}
-
-// t [..., width] as rows whose distance the kernels can take; copied where it cannot.
-struct Rows {
-  at::Tensor t;
-  int64_t stride;
-  int count;
-};
-constexpr int64_t kMaxStride = 1 << 20;
-Rows rows_of(const at::Tensor& t, const char* name) {
-  const int64_t width = t.size(-1), rows = width > 0 ? t.numel() / width : 0;
-  at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, width});
-  int64_t stride = flat.stride(0);
-  const bool apart = rows <= 1 || (stride >= width && stride <= kMaxStride && stride * flat.element_size() % 16 == 0);
-  if (flat.numel() > 0 && (flat.stride(1) != 1 || !apart || !begins_on_16(flat)))
-    flat = flat.clone(at::MemoryFormat::Contiguous);
-  stride = rows <= 1 ? width : flat.stride(0);
-  return {flat, stride, int_size(rows, name)};
-}
-
-at::Tensor bytes_on(const at::Tensor& like, size_t bytes) {
-  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte).requires_grad(false));
-}
-void* pointer(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 
 // The description of a block, from its weights. x is used for its device and dtype.
 FlashMoeFfnDesc describe(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptTensor& s13,
@@ -174,19 +97,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> ffn_backward(const at::Tensor& x,
   return {dx, dw13, dw2};
 }
 
-// A gradient of a leaf is accumulated on the stream on which its accumulator was made, by the first graph of it
-// that is still alive. Captured into a HIP graph, a backward pass that finds an accumulator of another
-// stream would make that stream wait inside the capture, and the process ends. So the forward pass that
-// would lead there is refused.
-void check_capture(const at::Tensor& leaf, const char* name) {
-  if (!leaf.requires_grad() || !leaf.is_leaf()) return;
-  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  if (!accumulator) return;
-  const auto stream = accumulator->stream();
-  TORCH_CHECK(!stream.has_value() || *stream == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().unwrap(), name,
-              " is part of an autograd graph made on another stream that is still alive: drop it before a step is captured");
-}
-
 struct GatedFfn : torch::autograd::Function<GatedFfn> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w13,
                             const at::Tensor& w2, int64_t activation) {
@@ -212,9 +122,7 @@ at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tenso
     return std::get<0>(ffn_forward(x, w13, w2, c10::nullopt, c10::nullopt, activation, false));
   if (x.is_cuda()) {
     const DeviceGuard guard(x.device());
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    check_hip(hipStreamIsCapturing(static_cast<hipStream_t>(current_stream()), &capturing), "hipStreamIsCapturing");
-    if (capturing != hipStreamCaptureStatusNone) {
+    if (capturing()) {
       check_capture(x, "x");
       check_capture(w13, "w13");
       check_capture(w2, "w2");

@@ -176,7 +176,8 @@ void pack_weights_in_place(const at::Tensor& ffn1, const at::Tensor& ffn2) {
 
 }  // namespace
 
-void bind_ffn(py::module_& m);  // flashFfnBindings.cpp: the dense block and MXFP4
+void bind_ffn(py::module_& m);    // flashFfnBindings.cpp: the dense block and MXFP4
+void bind_layer(py::module_& m);  // flashLayerBindings.cpp: what stands around a layer's blocks
 
 PYBIND11_MODULE(flashMoeLauncher, m) {
   m.doc() = "MI355X fused MoE layer launcher (drop-in for the reference's flashMoeLauncher extension)";
@@ -190,6 +191,7 @@ PYBIND11_MODULE(flashMoeLauncher, m) {
   m.def("pack_weights_in_place", &pack_weights_in_place, py::arg("ffn1_expert_weights"),
         py::arg("ffn2_expert_weights"));
   bind_ffn(m);
+  bind_layer(m);
   py::class_<Launcher>(m, "MoeKernelLauncher")
       .def(py::init())
       .def_static("getDistributedUniqueId", &Launcher::unique_id, py::arg("empty") = false,

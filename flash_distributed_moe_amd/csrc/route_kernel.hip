@@ -1,0 +1,464 @@
+// The router's choice as an operator of its own: from logits [T, E] the k experts of every token and their weights, how
+// many tokens each expert got, the loss that balances them and the one that keeps logits small; and the gradient of the logits.
+//
+//   p = softmax of a token's candidates (logits above their type's lowest value; padding has none)
+//   w_j = p of the j-th largest logit (the lowest index of equals), over the sum of the k if they are renormalised
+//   balance = E sum_e (counts_e / slots) (sum_t p_te / n),  z = sum_t lse_t^2 / n,  n rows with a candidate, slots winners
+//   dlogit = D + p (g - sum p g) + (2 dz / n) lse p,  g_e = dbalance E counts_e / (slots n),
+//   D = w_j (dw_j - sum w dw) at the winners, or with plain probabilities dw_j joins g there
+//
+// Sixteen lanes have a token, four logits of every 64 each, so that a load is whole lines of four tokens and every cross-lane step is a data
+// parallel primitive that serves four tokens. The winners are taken in k rounds. A round costs a subtraction and half a
+// three-way maximum a value, because a logit and its place are one whole number, no two of them equal: the next winner is the
+// largest of (key - last winner) in unsigned arithmetic, where what was taken already comes out small, so nothing has to be struck out.
+// A float32 logit has nine bits too many for that; where two neighbours among the first k + 1 agree in what is kept, the
+// wave takes its four tokens again by whole logits (of random ones one in some thousands).
+// Both directions are meant to be bound by reading the logits; the rounds are what competes with it.
+#include <float.h>
+
+#include "ffn_device.h"
+#include "lane_device.h"
+#include "layer_params.h"
+
+namespace fmoe {
+namespace {
+
+// A row's logits as they are in memory: value i of a lane is column 64 (i / 4) + 4 lane + i % 4.
+template <bool BF, int V>
+struct Raw {
+  unsigned u[BF ? V / 2 : V];
+};
+__device__ __forceinline__ int column(int lane, int i) { return (i >> 2) * 64 + lane * 4 + (i & 3); }
+
+// WHOLE: E is a multiple of four and rows begin on four values. Columns outside are -inf.
+template <bool BF, int V, bool WHOLE>
+__device__ __forceinline__ Raw<BF, V> load_row(const void* logits, size_t at, int lane, int E) {
+  Raw<BF, V> r;
+#pragma unroll
+  for (int c = 0; c < V / 4; ++c) {
+    const int col = c * 64 + lane * 4;
+    if constexpr (BF) {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(logits) + at + col;
+      u32x2 q = {0xFF80FF80u, 0xFF80FF80u};
+      if constexpr (WHOLE) {
+        if (col < E) q = *reinterpret_cast<const u32x2*>(p);
+      } else {
+        unsigned v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = col + i < E ? p[i] : 0xFF80u;
+        q = {v[0] | v[1] << 16, v[2] | v[3] << 16};
+      }
+      r.u[2 * c] = q.x, r.u[2 * c + 1] = q.y;
+    } else {
+      const unsigned* p = reinterpret_cast<const unsigned*>(logits) + at + col;
+      u32x4 q = {0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u};
+      if constexpr (WHOLE) {
+        if (col < E) q = *reinterpret_cast<const u32x4*>(p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < E) q[i] = p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.u[4 * c + i] = q[i];
+    }
+  }
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ float value_of(const unsigned* u, int i) {
+  if constexpr (BF) return __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
+  return __uint_as_float(u[i]);
+}
+template <bool BF>
+__device__ __forceinline__ float value_at(const void* logits, size_t at) {
+  if constexpr (BF) return __uint_as_float(unsigned(reinterpret_cast<const unsigned short*>(logits)[at]) << 16);
+  return reinterpret_cast<const float*>(logits)[at];
+}
+// Nothing at or below it is a candidate, and NaN is none.
+template <bool BF>
+__device__ __forceinline__ float lowest() {
+  return BF ? __uint_as_float(0xFF7F0000u) : -FLT_MAX;
+}
+// Greater logit <=> greater unsigned; the two zeros are equal.
+__device__ __forceinline__ unsigned ordered(float v) {
+  const unsigned u = __float_as_uint(v + 0.0f);
+  return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
+}
+
+// e^x of x <= 0 to about 2^-23: what the product with log2(e) leaves out is put back to first order. (Results
+// below 2^-126 are zeros.) A fourth of the library's instructions.
+__device__ __forceinline__ float exp_down(float x) {
+  x = x < -150.0f ? -150.0f : x;
+  const float t = x * 1.44269504f;
+  const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, rest * 0.693147181f, e);
+}
+
+// Winner j of a token lies in lane j % 16, the second sixteen in `second`: 1 + its column, 0 for a slot that stays empty.
+struct Winners {
+  unsigned first, second;
+};
+
+template <bool BF, int V>
+__device__ __forceinline__ Winners pick(const unsigned* u, bool open, int lane, int E, int k) {
+  unsigned key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float v = value_of<BF>(u, i);
+    // 31 bits: the logit's 16 (bfloat16) or first 23, and its place backwards, so that equals go to the lowest one
+    const unsigned bits = BF ? ordered(v) >> 16 << 8 : ordered(v) >> 1 & 0x7FFFFF00u;
+    key[i] = open && v > lowest<BF>() ? bits | (255 - column(lane, i)) : 0u;
+  }
+  const int rounds = BF ? k : min(k + 1, E);
+  unsigned last = 0x80000000u, first = 0, second = 0;
+  for (int j = 0; j < rounds; ++j) {
+    unsigned best = key[0] - last;
+#pragma unroll
+    for (int i = 1; i + 1 < V; i += 2) best = umax(umax(best, key[i] - last), key[i + 1] - last);
+    best = umax(best, key[V - 1] - last);
+    const unsigned next = last != 0 ? row16_max(best) + last : 0u;
+    last = next;
+    if (j < k && lane == (j & 15)) {
+      if (j < 16) first = last;
+      else second = last;
+    }
+  }
+  Winners w = {first != 0 ? 256 - (first & 255) : 0u, second != 0 ? 256 - (second & 255) : 0u};
+  if constexpr (!BF) {
+    // `last` is winner k's if there was a round for it
+    const unsigned extra = rounds > k ? last : 0u;
+    unsigned after = static_cast<unsigned>(dpp<kNextLane>(static_cast<int>(first)));
+    unsigned after2 = static_cast<unsigned>(dpp<kNextLane>(static_cast<int>(second)));
+    const unsigned second0 = __shfl(second, 0, 16);
+    if (lane == 15) after = second0;
+    if (lane == k - 1) after = extra;
+    if (lane == k - 17) after2 = extra;
+    const bool near = (lane < k && first != 0 && (first ^ after) >> 8 == 0) ||
+                      (lane + 16 < k && second != 0 && (second ^ after2) >> 8 == 0);
+    if (__any(near)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float v = value_of<BF>(u, i);
+        key[i] = open && v > lowest<BF>() ? ordered(v) : 0u;
+      }
+      w = {0u, 0u};
+      for (int j = 0; j < k; ++j) {
+        unsigned best = 0, at = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (key[i] > best) best = key[i], at = column(lane, i) + 1;
+        const unsigned most = row16_max(best);
+        const unsigned won = most != 0 ? row16_min(best == most ? at : 0xFFFFu) : 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (column(lane, i) + 1 == won) key[i] = 0u;
+        if (lane == (j & 15)) {
+          if (j < 16) w.first = won;
+          else w.second = won;
+        }
+      }
+    }
+  }
+  return w;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* room) {
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double sum = 0.0;
+  for (unsigned i = 0; i < blockDim.x / 64; ++i) sum += room[i];
+  return sum;
+}
+// By one whole workgroup; thread e < E has expert e's count and sum of probabilities, thread 0 the rows and the squares.
+__device__ __forceinline__ void finish(const RouteArgs& a, int count, double probs, double rows, double squares, double* room) {
+  const bool mine = static_cast<int>(threadIdx.x) < a.E;
+  const double slots = block_sum(mine ? count : 0, room);
+  const double both = block_sum(mine ? count * probs : 0.0, room);
+  if (mine) a.counts[threadIdx.x] = count;
+  if (threadIdx.x == 0) {
+    a.totals[0] = static_cast<int>(rows);
+    a.totals[1] = static_cast<int>(slots);
+    *a.balance = static_cast<float>(slots > 0 ? a.E * both / (slots * rows) : both);
+    *a.zed = static_cast<float>(rows > 0 ? squares / rows : squares);
+  }
+}
+
+template <bool BF, int V, bool WHOLE>
+__global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
+  __shared__ int hist[kRouteExperts];
+  __shared__ float probs[16][kRouteExperts];
+  __shared__ float wave_squares[16];
+  __shared__ int wave_rows[16];
+  __shared__ double room[16];
+  const int lane = threadIdx.x & 15, wave = threadIdx.x >> 6;
+  const int rows_here = blockDim.x / 16;
+  const long long step = static_cast<long long>(gridDim.x) * rows_here;
+  for (int e = threadIdx.x; e < kRouteExperts; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  float sum[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+  float squares = 0.0f;
+  int rows = 0;
+  long long row = static_cast<long long>(blockIdx.x) * rows_here + (threadIdx.x >> 4);
+  // rows behind the last one are read as the last one and count for nothing
+  const auto place = [&](long long r) { return static_cast<size_t>(min(r, a.T - 1LL)) * a.ld; };
+  Raw<BF, V> next{};
+  if (a.T > 0) next = load_row<BF, V, WHOLE>(a.logits, place(row), lane, a.E);
+  // all of a wave's rows go round together: the cross-lane steps need every lane
+  for (long long first = row - (threadIdx.x >> 4 & 3); first < a.T; first += step, row += step) {
+    const Raw<BF, V> now = next;
+    if (first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step), lane, a.E);
+    const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float v = value_of<BF>(now.u, i);
+      m = open && v > lowest<BF>() ? fmaxf(m, v) : m;
+    }
+    m = row16_max(m);
+    const bool some = m > -INFINITY;
+    float e[V], s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float v = value_of<BF>(now.u, i);
+      e[i] = some && v > lowest<BF>() ? exp_down(v - m) : 0.0f;
+      s += e[i];
+    }
+    s = row16_sum(s);
+    const float each = some ? 1.0f / s : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = fmaf(e[i], each, sum[i]);
+    if (lane == 0 && some) {
+      const float lse = m + logf(s);
+      squares = fmaf(lse, lse, squares);
+      ++rows;
+    }
+    const Winners w = pick<BF, V>(now.u, open, lane, a.E, a.k);
+    const float w0 = w.first != 0 ? exp_down(value_at<BF>(a.logits, place(row) + w.first - 1) - m) : 0.0f;
+    const float w1 = w.second != 0 ? exp_down(value_at<BF>(a.logits, place(row) + w.second - 1) - m) : 0.0f;
+    const float of = a.renormalize ? row16_sum(w0 + w1) : s;
+    const float share = some ? 1.0f / of : 0.0f;
+    if (row < a.T) {
+      const size_t at = static_cast<size_t>(row) * a.k + lane;
+      if (lane < a.k) {
+        a.weights[at] = w0 * share;
+        a.experts[at] = static_cast<int>(w.first) - 1;
+        if (w.first != 0) atomicAdd(&hist[w.first - 1], 1);
+      }
+      if (lane + 16 < a.k) {
+        a.weights[at + 16] = w1 * share;
+        a.experts[at + 16] = static_cast<int>(w.second) - 1;
+        if (w.second != 0) atomicAdd(&hist[w.second - 1], 1);
+      }
+    }
+  }
+  // the wave's four tokens at a time, then the waves, in one order
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float v = sum[i];
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    if ((threadIdx.x & 63) < 16 && column(lane, i) < kRouteExperts) probs[wave][column(lane, i)] = v;
+  }
+  squares += __shfl_xor(squares, 16, 64);
+  squares += __shfl_xor(squares, 32, 64);
+  rows += __shfl_xor(rows, 16, 64);
+  rows += __shfl_xor(rows, 32, 64);
+  if ((threadIdx.x & 63) == 0) wave_squares[wave] = squares, wave_rows[wave] = rows;
+  __syncthreads();
+  const int e = threadIdx.x, waves = blockDim.x / 64;
+  float p = 0.0f;
+  if (e < a.E)
+    for (int i = 0; i < waves; ++i) p += probs[i][e];
+  float all_squares = 0.0f;
+  int all_rows = 0;
+  if (e == 0)
+    for (int i = 0; i < waves; ++i) all_squares += wave_squares[i], all_rows += wave_rows[i];
+  if (gridDim.x == 1) {
+    finish(a, e < a.E ? hist[e] : 0, p, all_rows, all_squares, room);
+    return;
+  }
+  float* sums = a.partial + static_cast<size_t>(blockIdx.x) * kRouteColumns;
+  int* counts = reinterpret_cast<int*>(a.partial + static_cast<size_t>(gridDim.x + blockIdx.x) * kRouteColumns);
+  if (e < a.E) sums[e] = p, counts[e] = hist[e];
+  if (e == 0) sums[kRouteExperts] = all_squares, counts[kRouteExperts] = all_rows;
+}
+
+// The workgroups' sums, by one: four threads to a column.
+__global__ __launch_bounds__(1024) void route_finish_kernel(RouteArgs a, int blocks) {
+  __shared__ double probs[4][kRouteExperts];
+  __shared__ int counts[4][kRouteExperts];
+  __shared__ double room[16];
+  const int e = threadIdx.x & 255, part = threadIdx.x >> 8;
+  const int* partial_counts = reinterpret_cast<const int*>(a.partial + static_cast<size_t>(blocks) * kRouteColumns);
+  double p = 0.0;
+  int c = 0;
+  if (e < a.E) {
+#pragma unroll 8
+    for (int b = part; b < blocks; b += 4) {
+      p += a.partial[static_cast<size_t>(b) * kRouteColumns + e];
+      c += partial_counts[static_cast<size_t>(b) * kRouteColumns + e];
+    }
+  }
+  probs[part][e] = p, counts[part][e] = c;
+  double squares = 0.0, rows = 0.0;
+  if (static_cast<int>(threadIdx.x) < blocks) {
+    squares = a.partial[static_cast<size_t>(threadIdx.x) * kRouteColumns + kRouteExperts];
+    rows = partial_counts[static_cast<size_t>(threadIdx.x) * kRouteColumns + kRouteExperts];
+  }
+  squares = block_sum(squares, room);
+  rows = block_sum(rows, room);
+  p = (probs[0][e] + probs[1][e]) + (probs[2][e] + probs[3][e]);
+  c = (counts[0][e] + counts[1][e]) + (counts[2][e] + counts[3][e]);
+  finish(a, c, p, rows, squares, room);
+}
+
+template <bool BF, int V, bool WHOLE>
+__global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
+  // what the winners' weights add to a token's gradient, where each lane finds its columns
+  __shared__ __align__(16) float add[16][kRouteExperts];
+  const int lane = threadIdx.x & 15;
+  float* mine = add[threadIdx.x >> 4];
+  const int n = a.totals[0], slots = a.totals[1];
+  const float toward = a.dbalance != nullptr && slots > 0 ? *a.dbalance * a.E / (static_cast<float>(slots) * n) : 0.0f;
+  const float pull = a.dzed != nullptr && n > 0 ? 2.0f * *a.dzed / n : 0.0f;
+  float g[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = column(lane, i);
+    g[i] = c < a.E ? toward * a.counts[c] : 0.0f;
+    mine[c] = 0.0f;
+  }
+  const long long step = static_cast<long long>(gridDim.x) * 16;
+  long long row = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const auto place = [&](long long r) { return static_cast<size_t>(min(r, a.T - 1LL)); };
+  Raw<BF, V> next = load_row<BF, V, WHOLE>(a.logits, place(row) * a.ld, lane, a.E);
+  for (long long first = row - (threadIdx.x >> 4 & 3); first < a.T; first += step, row += step) {
+    const Raw<BF, V> now = next;
+    if (first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step) * a.ld, lane, a.E);
+    const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
+    const size_t at = place(row) * a.k + lane;
+    const int e0 = open && lane < a.k ? a.experts[at] : -1, e1 = open && lane + 16 < a.k ? a.experts[at + 16] : -1;
+    const float d0 = e0 >= 0 && a.dweights != nullptr ? a.dweights[at] : 0.0f;
+    const float d1 = e1 >= 0 && a.dweights != nullptr ? a.dweights[at + 16] : 0.0f;
+    const float l0 = e0 >= 0 ? value_at<BF>(a.logits, place(row) * a.ld + e0) : 0.0f;
+    const float l1 = e1 >= 0 ? value_at<BF>(a.logits, place(row) * a.ld + e1) : 0.0f;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float v = value_of<BF>(now.u, i);
+      m = open && v > lowest<BF>() ? fmaxf(m, v) : m;
+    }
+    m = row16_max(m);
+    const bool some = m > -INFINITY;
+    float p[V], s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float v = value_of<BF>(now.u, i);
+      p[i] = some && v > lowest<BF>() ? exp_down(v - m) : 0.0f;
+      s += p[i];
+    }
+    s = row16_sum(s);
+    const float each = some ? 1.0f / s : 0.0f;
+    const float w0 = e0 >= 0 ? exp_down(l0 - m) : 0.0f, w1 = e1 >= 0 ? exp_down(l1 - m) : 0.0f;
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] *= each, dot = fmaf(p[i], g[i], dot);
+    float a0, a1;
+    if (a.renormalize) {
+      const float share = some ? 1.0f / row16_sum(w0 + w1) : 0.0f;
+      const float mean = row16_sum(w0 * share * d0 + w1 * share * d1);
+      a0 = w0 * share * (d0 - mean), a1 = w1 * share * (d1 - mean);
+    } else {
+      a0 = w0 * each * d0, a1 = w1 * each * d1;
+      dot += a0 + a1;
+    }
+    dot = row16_sum(dot);
+    if (e0 >= 0) mine[e0] = a0;
+    if (e1 >= 0) mine[e1] = a1;
+    wave_lds_ready();
+    const float zed = some ? pull * (m + logf(s)) - dot : 0.0f;
+    float d[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = fmaf(p[i], g[i] + zed, mine[column(lane, i)]);
+    wave_lds_ready();
+    if (e0 >= 0) mine[e0] = 0.0f;
+    if (e1 >= 0) mine[e1] = 0.0f;
+    if (row < a.T) {
+#pragma unroll
+      for (int c = 0; c < V / 4; ++c) {
+        const int col = c * 64 + lane * 4;
+        const float* v = d + 4 * c;
+        if constexpr (BF) {
+          unsigned short* to = reinterpret_cast<unsigned short*>(a.dlogits) + static_cast<size_t>(row) * a.ldd + col;
+          const u32x2 q = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+          if constexpr (WHOLE) {
+            if (col < a.E) *reinterpret_cast<u32x2*>(to) = q;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (col + i < a.E) to[i] = static_cast<unsigned short>(q[i >> 1] >> (16 * (i & 1)));
+          }
+        } else {
+          float* to = reinterpret_cast<float*>(a.dlogits) + static_cast<size_t>(row) * a.ldd + col;
+          if constexpr (WHOLE) {
+            if (col < a.E) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (col + i < a.E) to[i] = v[i];
+          }
+        }
+      }
+    }
+  }
+}
+
+// Rows that begin on four values, E a multiple of four: loads and stores of four at a time.
+bool whole_fours(const void* p, long long ld, int E, int dtype) {
+  const int size = dtype == 0 ? 4 : 2;
+  return E % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * size) == 0;
+}
+
+template <bool BF, int V, bool WHOLE>
+void enqueue(const RouteArgs& a, bool backward, hipStream_t stream) {
+  if (backward) {
+    // eight workgroups of four waves a CU
+    const long long blocks = (a.T + 15LL) / 16;
+    route_backward_kernel<BF, V, WHOLE><<<dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(256), 0, stream>>>(a);
+    return;
+  }
+  const RouteGrid g = route_grid(a.T);
+  route_kernel<BF, V, WHOLE><<<dim3(g.blocks), dim3(g.threads), 0, stream>>>(a);
+  if (g.blocks > 1) route_finish_kernel<<<dim3(1), dim3(1024), 0, stream>>>(a, g.blocks);
+}
+template <bool BF, int V>
+void enqueue(const RouteArgs& a, bool backward, bool whole, hipStream_t stream) {
+  whole ? enqueue<BF, V, true>(a, backward, stream) : enqueue<BF, V, false>(a, backward, stream);
+}
+template <bool BF>
+void enqueue(const RouteArgs& a, bool backward, bool whole, hipStream_t stream) {
+  if (a.E <= 64) enqueue<BF, 4>(a, backward, whole, stream);
+  else if (a.E <= 128) enqueue<BF, 8>(a, backward, whole, stream);
+  else enqueue<BF, 16>(a, backward, whole, stream);
+}
+hipError_t enqueue(const RouteArgs& a, bool backward, int dtype, bool whole, hipStream_t stream) {
+  dtype == 0 ? enqueue<false>(a, backward, whole, stream) : enqueue<true>(a, backward, whole, stream);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_route(const RouteArgs& a, int dtype, hipStream_t stream) {
+  return enqueue(a, false, dtype, whole_fours(a.logits, a.ld, a.E, dtype), stream);
+}
+hipError_t launch_route_backward(const RouteArgs& a, int dtype, hipStream_t stream) {
+  return enqueue(a, true, dtype, whole_fours(a.logits, a.ld, a.E, dtype) && whole_fours(a.dlogits, a.ldd, a.E, dtype), stream);
+}
+
+}  // namespace fmoe

@@ -1,0 +1,43 @@
+"""What stands around the blocks of a layer: the router's choice with its losses, and the norms before and
+after a block.
+
+The sparse layer of `flashMoeOp.FlashMoeBlockWrapper` routes inside its kernel; a model that trains, or
+that watches how its experts are used, needs the choice by itself, with the counts and losses that
+go with it: `route`. (The reference's layer has neither losses nor gradients,
+test/singleGPU/cpp/moe/reference/refFullMoe.h:9-70.)
+
+There is no fallback: everything runs on the compiled `flashMoeLauncher` extension, on the current
+stream of the tensors' device, and can be captured into a HIP graph (with its backward pass as long as no eager
+graph of the same parameters is alive: the call raises then). Wrong arguments raise RuntimeError, and so do
+inputs that carry a forward-mode tangent; gradients are differentiated once.
+"""
+from typing import NamedTuple
+
+import torch
+
+from .flashFfnOp import _STRANGERS, _stranger, flashMoeLauncher
+
+
+class Routing(NamedTuple):
+    """What `route` returns, for logits [..., E] and k winners a token."""
+
+    weights: torch.Tensor       # float32 [..., k], differentiable
+    experts: torch.Tensor       # int32 [..., k], -1 where no candidate was left
+    counts: torch.Tensor        # int32 [E]: slots that each expert won
+    balance_loss: torch.Tensor  # float32 scalar, differentiable: 1 if all experts are used and liked evenly
+    z_loss: torch.Tensor        # float32 scalar, differentiable
+
+
+def route(logits, top_k, renormalize=True, mask=None):
+    """The top_k largest of each token's logits [..., E] (float32 or bfloat16), as `Routing`.
+
+    Winners come largest first, the lowest expert of equals, as the sparse layer picks them. A logit is a candidate if
+    it is greater than its type's lowest value (NaN and -inf are none); mask [...] (bool) leaves out the tokens where
+    it is False. With p the softmax over a token's candidates, weights are p of the winners, divided by their
+    sum if renormalize; balance_loss is E sum_e (counts_e / slots won) (mean_t p_te) and z_loss the mean squared
+    logarithm of the sum of exp(logits), both over the tokens that have a candidate. Gradients reach the logits from weights and both
+    losses; the choice and the counts are constants. E up to 256, top_k up to min(E, 32)."""
+    try:
+        return Routing(*flashMoeLauncher.route(logits, top_k, bool(renormalize), mask))
+    except _STRANGERS:
+        raise _stranger("logits must be a tensor, top_k a whole number, mask a tensor or None", logits, top_k, mask) from None

@@ -335,6 +335,37 @@ int flashMoeMxfp4LinearBytes(int x_format, int rows, int n, int k, size_t* bytes
 int flashMoeMxfp4Linear(int x_format, const void* x, const void* x_scales, long long ldx, int rows, const void* codes,
                         const void* scales, int n, int k, void* y, long long ldy, void* workspace, void* stream);
 
+/* ---- What stands around a layer's blocks: the router's choice as an operator of its own, the norms before and after a
+ * block, and adapters beside a projection. No counterpart in the reference, whose layer routes inside and has no losses
+ * (test/singleGPU/cpp/moe/reference/refFullMoe.h:9-70). As of the dense block, the calls keep no state, wait for nothing,
+ * refuse what is wrong with hipErrorInvalidValue before anything is enqueued, and can be captured; calls that may run at the
+ * same time need workspaces and outputs of their own. (Symbol version LIBFLASHMOE_MI355X_0.6, same interface revision.) */
+
+typedef struct FlashMoeRouteDesc {
+  int experts;     /* E, 1..256 */
+  int top_k;       /* k, 1..min(E,32) */
+  int dtype;       /* FLASH_MOE_F32 or FLASH_MOE_BF16: the logits and their gradient */
+  int renormalize; /* nonzero: a token's weights are divided by their sum */
+} FlashMoeRouteDesc;
+
+/* The k largest of E logits a token, largest first, the lowest expert of equals, as the layer's own router picks them. A
+ * logit is a candidate if it is greater than its type's lowest value: NaN and -inf are none. p is the softmax over the candidates.
+ * logits [tokens, E] rows ld values apart (any alignment; E and ld multiples of 4 are faster); mask [tokens] bytes or NULL: a token
+ * with 0 is padding and has no candidates. weights [tokens, k]: p of the winners (renormalised on request); experts
+ * [tokens, k]; slots that no candidate is left for get expert -1 and weight 0. counts [E]: slots that each expert
+ * won. totals [2]: rows n with a candidate, and slots won. balance [1]: E sum_e counts_e / slots * sum_t p_te / n (1 if even; 0
+ * without slots). zed [1]: the mean over the n rows of the squared logarithm of the sum of exp(logits).
+ * workspace: flashMoeRouteBytes of device memory (0: may be NULL). 0 tokens: zeros. tokens * k is at most 2^30. */
+int flashMoeRouteBytes(const FlashMoeRouteDesc* desc, int tokens, size_t* bytes);
+int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
+                  float* weights, int* experts, int* counts, int* totals, float* balance, float* zed, void* workspace,
+                  void* stream);
+/* The gradient of the logits (written, not added to) from those of the weights [tokens, k], of balance [1] and of zed
+ * [1]; each may be NULL. The choice and the counts are constants. experts, counts and totals are flashMoeRoute's. */
+int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
+                          const int* experts, const int* counts, const int* totals, const float* dweights,
+                          const float* dbalance, const float* dzed, void* dlogits, long long ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
