@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libflashMoe.so")
 F32, BF16, MXFP4 = 0, 1, 2
 ACT_SILU, ACT_GELU_TANH = 0, 1
 FFN_ROW_MAJOR, FFN_MXFP4 = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_GROUP, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3, 4
 SCHED_AUTO, SCHED_STREAM, SCHED_TILED = 0, 1, 2
 FLAG_PACK_WEIGHTS = 1
 FLAG_WEIGHTS_PREPACKED = 2
@@ -54,6 +55,14 @@ class RouteDesc(ctypes.Structure):
     """Mirror of FlashMoeRouteDesc."""
 
     _fields_ = [(n, ctypes.c_int) for n in ("experts", "top_k", "dtype", "renormalize")]
+
+
+class NormDesc(ctypes.Structure):
+    """Mirror of FlashMoeNormDesc."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("hidden", "dtype", "gate", "shared")] + \
+               [(n, ctypes.c_double) for n in ("eps", "residual_scale", "branch_scale")] + \
+               [(n, ctypes.c_void_p) for n in ("post_weight", "gate_values", "next_weight")]
 
 
 # name -> (restype, argtypes); every symbol include/flash_moe.h declares
@@ -109,6 +118,11 @@ C_ABI = {
                                      ctypes.c_int] + [ctypes.c_void_p] * 8),
     "flashMoeRouteBackward": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                              ctypes.c_int] + [ctypes.c_void_p] * 7 + [ctypes.c_longlong, ctypes.c_void_p]),
+    "flashMoeBlockNorm": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [ctypes.c_void_p, ctypes.c_longlong] * 2 + [ctypes.c_int] +
+                          [ctypes.c_void_p] * 4),
+    "flashMoeBlockNormBytes": (ctypes.c_int, [ctypes.POINTER(NormDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "flashMoeBlockNormBackward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [ctypes.c_void_p, ctypes.c_longlong] * 4 +
+                                  [ctypes.c_int] + [ctypes.c_void_p] * 8),
     "flashMoeSetDenseSmallBatch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
 }
 ABI_VERSION = 3

@@ -71,6 +71,46 @@ fmoe::RouteArgs route_args(const FlashMoeRouteDesc* d, const void* logits, long 
   return a;
 }
 
+hipError_t validate(const FlashMoeNormDesc* d, int tokens, bool branch) {
+  if (d == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null description");
+  FMOE_HIP_CHECK(check_dtype(d->dtype));
+  if (d->hidden < 8 || d->hidden > fmoe::kNormWidth || d->hidden % 8 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "H=%i: a multiple of 8, at most %i", d->hidden, fmoe::kNormWidth);
+  if (tokens < 0 || tokens > 1 << 30) FMOE_FAIL(hipErrorInvalidValue, "%i tokens (at most 2^30)", tokens);
+  if (d->gate < FLASH_MOE_GATE_NONE || d->gate > FLASH_MOE_GATE_FULL)
+    FMOE_FAIL(hipErrorInvalidValue, "gate %i is none of FLASH_MOE_GATE_*", d->gate);
+  if (d->gate == FLASH_MOE_GATE_GROUP && (d->shared < 1 || tokens % d->shared != 0))
+    FMOE_FAIL(hipErrorInvalidValue, "%i tokens in groups of %i", tokens, d->shared);
+  if (!(d->eps >= 0)) FMOE_FAIL(hipErrorInvalidValue, "eps is negative or NaN");
+  if ((d->gate != FLASH_MOE_GATE_NONE) != (d->gate_values != nullptr))
+    FMOE_FAIL(hipErrorInvalidValue, "gate %i %s values", d->gate, d->gate_values != nullptr ? "with" : "without");
+  if (!branch && (d->post_weight != nullptr || d->gate != FLASH_MOE_GATE_NONE))
+    FMOE_FAIL(hipErrorInvalidValue, "a post norm or a gate without a branch");
+  if (!branch && d->next_weight == nullptr) FMOE_FAIL(hipErrorInvalidValue, "neither a branch nor a norm");
+  for (const void* p : {d->post_weight, d->next_weight, d->gate == FLASH_MOE_GATE_TOKEN ? nullptr : d->gate_values})
+    if (!on(p, 16)) FMOE_FAIL(hipErrorInvalidValue, "a weight or the gate does not begin on 16 bytes");
+  if (!on(d->gate_values, size_of(d->dtype))) FMOE_FAIL(hipErrorInvalidValue, "the gate does not begin on a value");
+  return hipSuccess;
+}
+// Rows of H values: where they begin and how far apart they lie.
+hipError_t check_rows(const char* name, const void* p, long long ld, const FlashMoeNormDesc* d) {
+  if (p == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null %s pointer", name);
+  if (!on(p, 16)) FMOE_FAIL(hipErrorInvalidValue, "%s does not begin on 16 bytes", name);
+  if (ld < d->hidden || ld > kMaxStride || ld * static_cast<long long>(size_of(d->dtype)) % 16 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "%s: %lld values from row to row (at least %i, at most %lld, whole 16 bytes)", name, ld,
+              d->hidden, kMaxStride);
+  return hipSuccess;
+}
+
+fmoe::NormArgs norm_args(const FlashMoeNormDesc* d, int tokens) {
+  fmoe::NormArgs a{};
+  a.T = tokens, a.H = d->hidden, a.gate_kind = d->gate, a.shared = d->shared;
+  a.alpha = static_cast<float>(d->residual_scale), a.beta = static_cast<float>(d->branch_scale), a.eps = static_cast<float>(d->eps);
+  a.post = d->post_weight, a.gate = d->gate_values, a.next = d->next_weight;
+  return a;
+}
+size_t partial_bytes(const fmoe::NormArgs& a) { return size_t(fmoe::norm_arrays(a)) * a.blocks * a.H * 4; }
+
 }  // namespace
 
 extern "C" {
@@ -120,6 +160,68 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
   a.experts = const_cast<int*>(experts), a.counts = const_cast<int*>(counts), a.totals = const_cast<int*>(totals);
   a.dweights = dweights, a.dbalance = dbalance, a.dzed = dzed, a.dlogits = dlogits, a.ldd = ldd;
   FMOE_HIP_CHECK(fmoe::launch_route_backward(a, desc->dtype, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+int flashMoeBlockNormBytes(const FlashMoeNormDesc* desc, int tokens, size_t* bytes) {
+  if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result");
+  // whether there is a branch is not known here, and of no consequence
+  FMOE_HIP_CHECK(validate(desc, tokens, true));
+  fmoe::NormArgs a = norm_args(desc, tokens);
+  fmoe::plan_norm_backward(a);
+  *bytes = partial_bytes(a);
+  return hipSuccess;
+}
+
+int flashMoeBlockNorm(const FlashMoeNormDesc* desc, const void* x, long long ldx, const void* branch, long long ldb, int tokens,
+                      void* y, void* h, float* kept, void* stream) {
+  FMOE_HIP_CHECK(validate(desc, tokens, branch != nullptr || tokens == 0));
+  if (tokens == 0) return hipSuccess;
+  FMOE_HIP_CHECK(check_rows("x", x, ldx, desc));
+  if (branch != nullptr) {
+    FMOE_HIP_CHECK(check_rows("branch", branch, ldb, desc));
+    FMOE_HIP_CHECK(check_rows("y", y, desc->hidden, desc));
+  } else if (y != nullptr) {
+    FMOE_FAIL(hipErrorInvalidValue, "y without a branch");
+  }
+  if (desc->next_weight != nullptr) FMOE_HIP_CHECK(check_rows("h", h, desc->hidden, desc));
+  if (!on(kept, 4)) FMOE_FAIL(hipErrorInvalidValue, "kept does not begin on 4 bytes");
+  fmoe::NormArgs a = norm_args(desc, tokens);
+  a.x = x, a.ldx = ldx, a.branch = branch, a.ldb = ldb, a.y = y, a.h = h;
+  if (kept != nullptr) a.branch_rms = kept, a.y_rms = kept + tokens;
+  FMOE_HIP_CHECK(fmoe::launch_norm(a, desc->dtype, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long long ldx, const void* branch, long long ldb,
+                              const void* dy, long long lddy, const void* dh, long long lddh, int tokens, const float* kept,
+                              void* workspace, void* dx, void* dbranch, void* dpost, void* dgate, void* dnext, void* stream) {
+  FMOE_HIP_CHECK(validate(desc, tokens, branch != nullptr || tokens == 0));
+  if (tokens > 0) {
+    FMOE_HIP_CHECK(check_rows("x", x, ldx, desc));
+    if (branch != nullptr) FMOE_HIP_CHECK(check_rows("branch", branch, ldb, desc));
+    if (dy != nullptr) FMOE_HIP_CHECK(check_rows("dy", dy, lddy, desc));
+    if (dh != nullptr) FMOE_HIP_CHECK(check_rows("dh", dh, lddh, desc));
+    FMOE_HIP_CHECK(check_word("kept", kept));
+  }
+  if ((dbranch != nullptr && branch == nullptr && tokens > 0) || (dpost != nullptr && desc->post_weight == nullptr) ||
+      (dgate != nullptr && desc->gate == FLASH_MOE_GATE_NONE) || (dnext != nullptr && desc->next_weight == nullptr))
+    FMOE_FAIL(hipErrorInvalidValue, "a gradient of an input that is not there");
+  for (const void* p : {dx, dbranch, desc->gate == FLASH_MOE_GATE_FULL ? dgate : nullptr})
+    if (!on(p, 16)) FMOE_FAIL(hipErrorInvalidValue, "a gradient does not begin on 16 bytes");
+  for (const void* p : {dpost, dgate, dnext})
+    if (!on(p, size_of(desc->dtype))) FMOE_FAIL(hipErrorInvalidValue, "a gradient does not begin on a value");
+  const bool columns = dpost != nullptr || dnext != nullptr ||
+                       (dgate != nullptr && (desc->gate == FLASH_MOE_GATE_CHANNEL || desc->gate == FLASH_MOE_GATE_GROUP));
+  if (columns) FMOE_HIP_CHECK(check_word("workspace", workspace));
+  if (!columns && tokens == 0) return hipSuccess;
+  fmoe::NormArgs a = norm_args(desc, tokens);
+  a.x = x, a.ldx = ldx, a.branch = branch, a.ldb = ldb, a.dy = dy, a.lddy = lddy, a.dh = dh, a.lddh = lddh;
+  if (tokens > 0) a.branch_rms = const_cast<float*>(kept), a.y_rms = a.branch_rms + tokens;
+  a.dx = dx, a.dbranch = dbranch, a.dpost = dpost, a.dgate = dgate, a.dnext = dnext;
+  a.partial = static_cast<float*>(workspace);
+  fmoe::plan_norm_backward(a);
+  FMOE_HIP_CHECK(fmoe::launch_norm_backward(a, desc->dtype, static_cast<hipStream_t>(stream)));
   return hipSuccess;
 }
 

@@ -41,4 +41,56 @@ inline RouteGrid route_grid(int T) {
 hipError_t launch_route(const RouteArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_route_backward(const RouteArgs& a, int dtype, hipStream_t stream);
 
+// ------------------------------------------------------------------ the norms around a block
+enum GateKind { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_GROUP = 2, GATE_TOKEN = 3, GATE_FULL = 4 };
+
+struct NormArgs {
+  const void* x;       // [T, H]
+  const void* branch;  // [T, H], or NULL: the norm in front of a block alone, y = x
+  const void* post;    // [H] or NULL
+  const void* gate;    // by kind: [H], [T / shared, H], [T] or [T, H]
+  const void* next;    // [H] or NULL
+  void* y;             // [T, H] or NULL
+  void* h;             // [T, H] if next
+  float* branch_rms;   // [T]: one over the root mean square of the branch's rows and of y's; NULL: not kept
+  float* y_rms;        // [T]
+  long long ldx, ldb;
+  int T, H, gate_kind;
+  int shared;  // rows that share a gate row (GATE_GROUP)
+  float alpha, beta, eps;
+  // backward
+  const void* dy;  // [T, H] or NULL
+  const void* dh;  // [T, H] or NULL
+  long long lddy, lddh;
+  void *dx, *dbranch, *dpost, *dgate, *dnext;  // without gaps, or NULL
+  float* partial;                              // [arrays, blocks, H]
+  // GATE_GROUP: `parts` workgroups take a group's rows each, or one takes `groups` groups
+  int blocks, parts, groups;
+};
+constexpr int kNormWidth = 8192;
+constexpr int kNormThreads = 512, kNormLane = 16;  // backward: threads of a workgroup, values a lane has of a row
+// Waves that have a row together in the backward pass.
+__host__ __device__ inline int norm_waves(int H) { return H <= 1024 ? 1 : H <= 2048 ? 2 : H <= 4096 ? 4 : 8; }
+// Workgroups of the backward pass, and which rows they take.
+inline void plan_norm_backward(NormArgs& a) {
+  const int at_once = kNormThreads / 64 / norm_waves(a.H);
+  const long long most = 512, steps = (a.T + at_once - 1LL) / at_once;
+  a.blocks = static_cast<int>(steps < 1 ? 1 : steps < most ? steps : most);
+  a.parts = 0, a.groups = 1;
+  if (a.gate_kind != GATE_GROUP || a.T == 0) return;
+  const int count = a.T / a.shared;
+  const long long rows = (a.T + a.blocks - 1LL) / a.blocks;  // a workgroup's
+  if (a.shared > rows) {
+    a.parts = static_cast<int>((a.shared + rows - 1) / rows);
+    a.blocks = count * a.parts;
+  } else {
+    a.groups = static_cast<int>((rows + a.shared - 1) / a.shared);
+    a.blocks = (count + a.groups - 1) / a.groups;
+  }
+}
+// Column sums that the workgroups leave: of the next norm's weight, of the post norm's (with a gate a channel: of both), of a group's gate.
+inline int norm_arrays(const NormArgs& a) { return a.gate_kind == GATE_GROUP ? 3 : 2; }
+hipError_t launch_norm(const NormArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_norm_backward(const NormArgs& a, int dtype, hipStream_t stream);
+
 }  // namespace fmoe

@@ -116,9 +116,161 @@ variable_list route(const at::Tensor& logits, int64_t top_k, bool renormalize, c
   return Route::apply(logits, top_k, renormalize, mask);
 }
 
+// ------------------------------------------------------------------ the norms around a block
+void check_vector(const at::Tensor& t, const char* name, const at::Tensor& x) {
+  if (!t.defined()) return;
+  check_device(t, name, x);
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must have x's dtype");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == x.size(-1), name, " must be [H] with H = ", x.size(-1));
+  check_packed(t, name);
+}
+
+// How a gate is shared among x's rows: its leading dimensions are x's up to some one, and ones from there.
+void describe_gate(FlashMoeNormDesc& d, const at::Tensor& gate, const at::Tensor& x, int64_t rows) {
+  check_device(gate, "gate", x);
+  TORCH_CHECK(gate.scalar_type() == x.scalar_type(), "gate must have x's dtype");
+  TORCH_CHECK(gate.dim() >= 1 && gate.dim() <= x.dim(), "gate must not have more dimensions than x");
+  const int64_t width = gate.size(-1), missing = x.dim() - gate.dim();
+  TORCH_CHECK(width == x.size(-1) || width == 1, "gate's last dimension must be x's or 1");
+  int64_t own = 1;
+  bool shared = false;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) {
+    const int64_t n = i < missing ? 1 : gate.size(i - missing);
+    TORCH_CHECK(n == x.size(i) ? !shared || n == 1 : n == 1,
+                "gate's leading dimensions must be x's up to some one, and 1 from there");
+    if (n != x.size(i)) shared = true;
+    own *= n;
+  }
+  TORCH_CHECK(width != 1 || own == rows, "a gate of one value a token must have x's leading dimensions");
+  d.gate = width == 1 ? FLASH_MOE_GATE_TOKEN : own == 1 ? FLASH_MOE_GATE_CHANNEL : own == rows ? FLASH_MOE_GATE_FULL : FLASH_MOE_GATE_GROUP;
+  d.shared = d.gate == FLASH_MOE_GATE_GROUP && rows > 0 ? static_cast<int>(rows / own) : 1;
+}
+
+struct NormInputs {
+  at::Tensor x, branch, post, gate, next;
+};
+at::Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
+struct NormCall {
+  FlashMoeNormDesc d;
+  Rows x, branch;
+  at::Tensor gate;
+};
+NormCall prepare(const NormInputs& in, double alpha, double beta, double eps) {
+  TORCH_CHECK(in.x.defined() && in.x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  TORCH_CHECK(in.x.dim() >= 1, "x must be [..., H]");
+  NormCall c{};
+  c.d.dtype = dtype_of(in.x, "x");
+  c.d.hidden = int_size(in.x.size(-1), "H");
+  TORCH_CHECK(c.d.hidden >= 8 && c.d.hidden % 8 == 0 && c.d.hidden <= 8192, "H must be a multiple of 8, at most 8192, not ", c.d.hidden);
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  c.d.eps = eps, c.d.residual_scale = alpha, c.d.branch_scale = beta;
+  check_vector(in.post, "post_weight", in.x);
+  check_vector(in.next, "the next norm's weight", in.x);
+  c.x = rows_of(in.x, "x");
+  if (in.branch.defined()) {
+    check_device(in.branch, "branch", in.x);
+    TORCH_CHECK(in.branch.sizes() == in.x.sizes() && in.branch.scalar_type() == in.x.scalar_type(), "branch must have x's shape and dtype");
+    c.branch = rows_of(in.branch, "branch");
+  }
+  if (in.gate.defined()) {
+    describe_gate(c.d, in.gate, in.x, c.x.count);
+    if (c.x.count == 0 && c.d.gate != FLASH_MOE_GATE_CHANNEL) c.d.gate = FLASH_MOE_GATE_NONE;  // no rows to have one
+    c.gate = in.gate.contiguous();
+    if (!begins_on_16(c.gate)) c.gate = c.gate.clone();
+    if (c.d.gate != FLASH_MOE_GATE_NONE) c.d.gate_values = c.gate.data_ptr();
+  }
+  c.d.post_weight = pointer(in.post), c.d.next_weight = pointer(in.next);
+  return c;
+}
+
+// (y, h, kept), undefined where there is none
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const NormInputs& in, double alpha, double beta, double eps, bool keep) {
+  refuse_tangent(in.x, "x");
+  refuse_tangent(in.branch, "branch");
+  refuse_tangent(in.post, "post_weight");
+  refuse_tangent(in.gate, "gate");
+  refuse_tangent(in.next, "the next norm's weight");
+  TORCH_CHECK(in.x.defined() && in.x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  const DeviceGuard guard(in.x.device());
+  const NormCall c = prepare(in, alpha, beta, eps);
+  at::Tensor y, h, kept;
+  if (in.branch.defined()) y = at::empty(in.x.sizes(), plain(in.x));
+  if (in.next.defined()) h = at::empty(in.x.sizes(), plain(in.x));
+  if (keep) kept = at::empty({2, c.x.count}, plain(in.x).dtype(at::kFloat));
+  check_hip(flashMoeBlockNorm(&c.d, pointer(c.x.t), c.x.stride, pointer(c.branch.t), c.branch.stride, c.x.count, pointer(y), pointer(h),
+                              static_cast<float*>(pointer(kept)), current_stream()),
+            "flashMoeBlockNorm");
+  return {y, h, kept};
+}
+
+struct BlockNorm : torch::autograd::Function<BlockNorm> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& branch, const OptTensor& post,
+                               const OptTensor& gate, const OptTensor& next, double alpha, double beta, double eps) {
+    const NormInputs in{x, or_none(branch), or_none(post), or_none(gate), or_none(next)};
+    const auto [y, h, kept] = norm_forward(in, alpha, beta, eps, true);
+    ctx->save_for_backward({in.x, in.branch, in.post, in.gate, in.next, kept});
+    ctx->saved_data["alpha"] = alpha;
+    ctx->saved_data["beta"] = beta;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    if (!y.defined()) return {h};
+    if (!h.defined()) return {y};
+    return {y, h};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_derivatives("block_norm and block_join");
+    const auto kept = ctx->get_saved_variables();
+    const NormInputs in{kept[0], kept[1], kept[2], kept[3], kept[4]};
+    const DeviceGuard guard(in.x.device());
+    const NormCall c = prepare(in, ctx->saved_data["alpha"].toDouble(), ctx->saved_data["beta"].toDouble(), ctx->saved_data["eps"].toDouble());
+    const at::Tensor dy = in.branch.defined() ? grads[0] : at::Tensor(), dh = in.next.defined() ? grads.back() : at::Tensor();
+    Rows dys{}, dhs{};
+    if (dy.defined()) dys = rows_of(dy, "dy");
+    if (dh.defined()) dhs = rows_of(dh, "dh");
+    variable_list out(8);
+    for (int i = 0, present = 0; i < 5; ++i)  // inputs that are not there have no place in the node
+      if (kept[i].defined() && ctx->needs_input_grad(present++)) out[i] = at::empty(kept[i].sizes(), plain(kept[i]));
+    void* dgate = pointer(out[3]);
+    if (dgate != nullptr && c.d.gate == FLASH_MOE_GATE_NONE) out[3].zero_(), dgate = nullptr;
+    size_t bytes = 0;
+    check_hip(flashMoeBlockNormBytes(&c.d, c.x.count, &bytes), "flashMoeBlockNormBytes");
+    const at::Tensor work = bytes_on(in.x, bytes);
+    check_hip(flashMoeBlockNormBackward(&c.d, pointer(c.x.t), c.x.stride, pointer(c.branch.t), c.branch.stride, pointer(dys.t), dys.stride,
+                                        pointer(dhs.t), dhs.stride, c.x.count, static_cast<float*>(pointer(kept[5])), pointer(work),
+                                        pointer(out[0]), pointer(out[1]), pointer(out[2]), dgate, pointer(out[4]), current_stream()),
+              "flashMoeBlockNormBackward");
+    return out;
+  }
+};
+
+variable_list block_norm(const at::Tensor& x, const OptTensor& branch, const OptTensor& post, const OptTensor& gate, const OptTensor& next,
+                         double alpha, double beta, double eps) {
+  const NormInputs in{x, or_none(branch), or_none(post), or_none(gate), or_none(next)};
+  TORCH_CHECK(in.x.defined(), "x tensor is undefined");
+  if (!differentiated({&in.x, &in.branch, &in.post, &in.gate, &in.next})) {
+    const auto [y, h, kept] = norm_forward(in, alpha, beta, eps, false);
+    if (!y.defined()) return {h};
+    if (!h.defined()) return {y};
+    return {y, h};
+  }
+  if (x.is_cuda()) {
+    const DeviceGuard guard(x.device());
+    if (capturing()) {
+      check_capture_behind(in.x, "x");
+      check_capture_behind(in.branch, "branch");
+      check_capture_behind(in.post, "post_weight");
+      check_capture_behind(in.gate, "gate");
+      check_capture_behind(in.next, "the next norm's weight");
+    }
+  }
+  return BlockNorm::apply(x, branch, post, gate, next, alpha, beta, eps);
+}
+
 }  // namespace
 
 void bind_layer(py::module_& m) {
   m.def("route", &route, py::arg("logits"), py::arg("top_k"), py::arg("renormalize"), py::arg("mask"),
         py::call_guard<py::gil_scoped_release>());
+  m.def("block_norm", &block_norm, py::arg("x"), py::arg("branch"), py::arg("post_weight"), py::arg("gate"), py::arg("next_weight"),
+        py::arg("residual_scale"), py::arg("branch_scale"), py::arg("eps"), py::call_guard<py::gil_scoped_release>());
 }

@@ -3,7 +3,8 @@ after a block.
 
 The sparse layer of `flashMoeOp.FlashMoeBlockWrapper` routes inside its kernel; a model that trains, or
 that watches how its experts are used, needs the choice by itself, with the counts and losses that
-go with it: `route`. (The reference's layer has neither losses nor gradients,
+go with it: `route`. Around that layer and around the dense block of `flashFfnOp` stand `block_norm`, in front of
+a block, and `block_join`, behind it. (The reference's layer has neither losses nor norms nor gradients,
 test/singleGPU/cpp/moe/reference/refFullMoe.h:9-70.)
 
 There is no fallback: everything runs on the compiled `flashMoeLauncher` extension, on the current
@@ -41,3 +42,35 @@ def route(logits, top_k, renormalize=True, mask=None):
         return Routing(*flashMoeLauncher.route(logits, top_k, bool(renormalize), mask))
     except _STRANGERS:
         raise _stranger("logits must be a tensor, top_k a whole number, mask a tensor or None", logits, top_k, mask) from None
+
+
+def block_norm(x, weight, eps=1e-6):
+    """The norm in front of a block: x / sqrt(mean x^2 + eps) * weight for x [..., H] (float32 or bfloat16) and weight [H] of
+    x's dtype. H a multiple of 8, up to 8192. Differentiable."""
+    try:
+        return flashMoeLauncher.block_norm(x, None, None, None, _present(weight), 1.0, 1.0, eps)[0]
+    except _STRANGERS:
+        raise _stranger("x and weight must be tensors, eps a number", x, weight, eps) from None
+
+
+def block_join(x, branch, post_weight=None, gate=None, next_weight=None, residual_scale=1.0, branch_scale=1.0, eps=1e-6):
+    """A block's output joins the residual stream: y = residual_scale * x + branch_scale * gate * z, where z is the
+    branch, or with post_weight [H] its norm branch / sqrt(mean branch^2 + eps) * post_weight. With next_weight [H] the result is
+    (y, h), h = y / sqrt(mean y^2 + eps) * next_weight being what the next block takes (of y before it is rounded).
+
+    x and branch [..., H] share shape and dtype (float32 or bfloat16), rows may lie apart; H a multiple of 8, up to 8192.
+    gate: [H], or x's leading dimensions up to some one, ones from there and H ([B, 1, H]: one for each sequence), or one value a
+    token ([..., 1]). All of x's dtype. Everything of a row is float32 until y and h are rounded. Differentiable in
+    all tensors."""
+    try:
+        out = flashMoeLauncher.block_norm(x, _present(branch), post_weight, gate, next_weight, residual_scale, branch_scale, eps)
+    except _STRANGERS:
+        raise _stranger("x and branch must be tensors, weights and gate tensors or None, the rest numbers", x, branch, post_weight, gate,
+                        next_weight, residual_scale, branch_scale, eps) from None
+    return out[0] if next_weight is None else tuple(out)
+
+
+def _present(t):
+    if t is None:
+        raise TypeError("None")
+    return t

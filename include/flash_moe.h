@@ -366,6 +366,43 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
                           const int* experts, const int* counts, const int* totals, const float* dweights,
                           const float* dbalance, const float* dzed, void* dlogits, long long ldd, void* stream);
 
+/* The norms around a block, fused with what joins it to the residual stream, on rows of H values:
+ *   z = post_weight * branch / rms(branch), or the branch as it is without post_weight;
+ *   y = residual_scale * x + branch_scale * gate * z;  h = next_weight * y / rms(y), with next_weight;
+ * rms(v) = sqrt(mean v^2 + eps). Without a branch y = x, and h is the norm in front of a block alone. What is computed of one
+ * row is float32, rounded once into y and once into h. */
+enum {
+  FLASH_MOE_GATE_NONE = 0,
+  FLASH_MOE_GATE_CHANNEL = 1, /* [H] */
+  FLASH_MOE_GATE_GROUP = 2,   /* [tokens / shared, H]: `shared` tokens on end have one row */
+  FLASH_MOE_GATE_TOKEN = 3,   /* [tokens] */
+  FLASH_MOE_GATE_FULL = 4     /* [tokens, H] */
+};
+typedef struct FlashMoeNormDesc {
+  int hidden;               /* H, a multiple of 8, at most 8192 */
+  int dtype;                /* FLASH_MOE_F32 or FLASH_MOE_BF16: everything but `kept` */
+  int gate;                 /* FLASH_MOE_GATE_* */
+  int shared;               /* FLASH_MOE_GATE_GROUP: divides the number of tokens */
+  double eps, residual_scale, branch_scale;
+  const void* post_weight;  /* device, [H] or NULL */
+  const void* gate_values;  /* device, by `gate`; NULL: none */
+  const void* next_weight;  /* device, [H] or NULL */
+} FlashMoeNormDesc;
+
+/* x and branch [tokens, H] rows ldx / ldb values apart (whole 16 bytes, at most 2^20), branch NULL or not; y (with a branch) and h (with
+ * next_weight) [tokens, H] without gaps. kept: NULL, or 2 * tokens floats for the backward pass. Vectors of H values begin on 16
+ * bytes. Outputs do not overlap inputs. */
+int flashMoeBlockNorm(const FlashMoeNormDesc* desc, const void* x, long long ldx, const void* branch, long long ldb, int tokens,
+                      void* y, void* h, float* kept, void* stream);
+/* Device bytes of a backward pass's workspace. */
+int flashMoeBlockNormBytes(const FlashMoeNormDesc* desc, int tokens, size_t* bytes);
+/* Gradients from dy and dh [tokens, H] rows lddy / lddh values apart (either may be NULL: zeros), written without gaps in the inputs' types
+ * and shapes, not added to; each may be NULL. Of 0 tokens the vectors' gradients are zeros (FLASH_MOE_GATE_GROUP,
+ * _TOKEN and _FULL have none then). */
+int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long long ldx, const void* branch, long long ldb,
+                              const void* dy, long long lddy, const void* dh, long long lddh, int tokens, const float* kept,
+                              void* workspace, void* dx, void* dbranch, void* dpost, void* dgate, void* dnext, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

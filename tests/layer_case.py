@@ -89,3 +89,81 @@ def route(logits, k, renormalize, mask=None, dw=None, db=None, dz=None):
     # a probability below 2^-126 is taken as zero, and what multiplies it is lost with it
     out["dlogits"] = (grad, (big + P * factor) * (rel + 60 * U) + HALF[raw.dtype] * grad.abs() + TINY * (1 + factor))
     return out
+
+
+# ------------------------------------------------------------------ the norms around a block
+def _mean(v):
+    return v.mean(-1, keepdim=True)
+
+
+def join(x, branch=None, post=None, gate=None, next_weight=None, alpha=1.0, beta=1.0, eps=1e-6, dy=None, dh=None):
+    """{name: (value, bound)} of y, h, and with dy or dh of the gradients "x", "branch", "post", "gate", "next_weight". Without a
+    branch y = x. Shapes as the operator takes them.
+
+    One over a root mean square is off by 40 steps of float32 of itself (a lane's 32 squares, 10 steps across lanes and waves, the
+    mean, eps and the root: half of those relative to it); sums over a row by 60 steps of their magnitudes, sums over tokens
+    by T / 256 + 80 (a workgroup's rows, the rows it has at once, up to 512 workgroups sixteen at a time)."""
+    half, H = HALF[x.dtype], x.shape[-1]
+    X, B, P, G, W, DY, DH = (None if t is None else t.detach().double() for t in (x, branch, post, gate, next_weight, dy, dh))
+    zero = torch.zeros_like(X)
+    if B is None:
+        y, ey = X, zero
+    else:
+        rb = 1 / (_mean(B * B) + eps).sqrt() if P is not None else torch.ones_like(_mean(B))
+        u = B * rb
+        eu = 42 * U * u.abs() if P is not None else zero
+        w = P if P is not None else torch.ones_like(zero)
+        z, ez = u * w, eu * w.abs() + U * (u * w).abs()
+        g = G if G is not None else torch.ones_like(z)
+        y = alpha * X + beta * g * z
+        ey = 2 * U * (alpha * X).abs() + abs(beta) * g.abs() * (ez + 3 * U * z.abs()) + U * y.abs()
+    out = {} if B is None else {"y": (y, ey + half * (y.abs() + ey))}
+    if W is not None:
+        ry = 1 / (_mean(y * y) + eps).sqrt()
+        er = 40 * U + _mean(ey * ey).sqrt() * ry
+        v = y * ry
+        ev = ey * ry + v.abs() * (er + U)
+        out["h"] = (v * W, ev * W.abs() + 2 * U * (v * W).abs() + half * ((v * W).abs() + ev * W.abs()))
+    if dy is None and dh is None:
+        return out
+    rows = X.numel() // H
+    tokens = (rows / 256 + 80) * U
+    columns = lambda t: t.reshape(-1, H).sum(0)  # noqa: E731
+
+    def stored(name, value, bound):
+        out[name] = (value, bound + half * (value.abs() + bound) + TINY)
+
+    t, et = (zero, zero) if DY is None else (DY, zero)
+    if W is not None:
+        if DH is None:
+            stored("next_weight", torch.zeros_like(W), torch.zeros_like(W))
+        else:
+            stored("next_weight", columns(DH * v), columns(DH.abs() * ev) + tokens * columns((DH * v).abs()))
+            q = DH * W
+            c = _mean(q * v)
+            ec = _mean(q.abs() * ev + 60 * U * (q * v).abs())
+            t = t + ry * (q - v * c)
+            et = ry * ((q.abs() + (v * c).abs()) * (er + 4 * U) + ev * c.abs() + v.abs() * ec) + 2 * U * ((0 if DY is None else DY.abs()) + t.abs())
+    stored("x", (alpha if B is not None else 1.0) * t, (abs(alpha) if B is not None else 1.0) * et + U * t.abs())
+    if B is None:
+        return out
+    d, ed = beta * t, abs(beta) * et + U * (beta * t).abs()
+    if G is not None:
+        value, bound = d * z, ed * z.abs() + d.abs() * ez + U * (d * z).abs()
+        size, steps = value.abs(), 0.0
+        shape = (1,) * (X.dim() - G.dim()) + tuple(G.shape)
+        over = [i for i in range(X.dim()) if shape[i] != X.shape[i]]
+        if over:
+            value, bound, size = (s.sum(over, keepdim=True) for s in (value, bound, size))
+            steps = 60 * U + tokens
+        stored("gate", value.reshape(G.shape), (bound + (steps + 2 * U) * size).reshape(G.shape))
+    q, eq = d * g * w, ed * (g * w).abs() + 3 * U * (d * g * w).abs()
+    if P is not None:
+        stored("post", columns(d * g * u), columns((g * u).abs() * ed + (d * g).abs() * eu + 3 * U * (d * g * u).abs()) + tokens * columns((d * g * u).abs()))
+        c = _mean(q * u)
+        ec = _mean(u.abs() * eq + q.abs() * eu + 64 * U * (q * u).abs())
+        value = rb * (q - u * c)
+        eq = rb * (eq + u.abs() * ec + c.abs() * eu + 46 * U * (q.abs() + (u * c).abs()))
+        q = value
+    stored("branch", q, eq)
+    return out

@@ -118,3 +118,114 @@ def test_route_definition(renormalize):
     # and the choice: the first of equals
     r = layer_case.route(torch.tensor([[1.0, 2.0, 2.0, 0.0], [0.0, 0.0, 0.0, 0.0]]), 3, renormalize)
     assert r["experts"].tolist() == [[1, 2, 0], [0, 1, 2]] and r["counts"].tolist() == [2, 2, 2, 0]
+
+
+# ------------------------------------------------------------------ the norms around a block
+def norm_desc(**kw):
+    d = _lib.NormDesc(64, _lib.BF16, _lib.GATE_CHANNEL, 1, 1e-6, 1.0, 1.0, 0x1000, 0x2000, 0x3000)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def norm(d=None, x=0x10000, ldx=64, branch=0x20000, ldb=64, tokens=6, y=0x30000, h=0x40000, kept=0x50000):
+    return _lib.load().flashMoeBlockNorm(ctypes.byref(d or norm_desc()), x, ldx, branch, ldb, tokens, y, h, kept, None)
+
+
+def norm_backward(d=None, x=0x10000, ldx=64, branch=0x20000, ldb=64, dy=0x30000, lddy=64, dh=0x40000, lddh=64, tokens=6, kept=0x50000,
+                  work=0x60000, dx=0x70000, dbranch=0x80000, dpost=0x90000, dgate=0xA0000, dnext=0xB0000):
+    return _lib.load().flashMoeBlockNormBackward(ctypes.byref(d or norm_desc()), x, ldx, branch, ldb, dy, lddy, dh, lddh, tokens, kept, work, dx,
+                                                 dbranch, dpost, dgate, dnext, None)
+
+
+@pytest.mark.parametrize("kw", [dict(hidden=0), dict(hidden=60), dict(hidden=8200), dict(dtype=2), dict(gate=5), dict(gate=-1), dict(gate=2, shared=4),
+                                dict(gate=2, shared=0), dict(eps=-1.0), dict(eps=float("nan")), dict(gate_values=None), dict(gate=0),
+                                dict(gate_values=0x2008), dict(gate=3, gate_values=0x2001), dict(post_weight=0x1002), dict(next_weight=0x3008)])
+def test_bad_norms(kw, capfd):
+    assert norm(d=norm_desc(**kw)) == BAD and norm_backward(d=norm_desc(**kw)) == BAD
+    assert _lib.load().flashMoeBlockNormBytes(ctypes.byref(norm_desc(**kw)), 6, ctypes.byref(ctypes.c_size_t(0))) == BAD
+    assert capfd.readouterr().out.count("[MOE ERROR:") == 3
+
+
+ALONE = dict(post_weight=None, gate=0, gate_values=None)
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(x=0x10008), dict(ldx=56), dict(ldx=68), dict(ldx=(1 << 20) + 8), dict(ldb=60), dict(branch=0x20002),
+                                dict(tokens=-1), dict(tokens=(1 << 30) + 1), dict(y=None), dict(y=0x30004), dict(h=None), dict(kept=0x50002),
+                                dict(branch=None), dict(branch=None, d=norm_desc(**ALONE)),
+                                dict(branch=None, y=None, d=norm_desc(**ALONE, next_weight=None))])
+def test_norm_refuses(kw, capfd):
+    assert norm(**kw) == BAD
+    assert "[MOE ERROR:" in capfd.readouterr().out
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(ldx=60), dict(branch=None), dict(ldb=8), dict(dy=0x30002), dict(lddy=60), dict(lddh=72 + 4),
+                                dict(kept=None), dict(work=None), dict(dx=0x70002), dict(dbranch=0x80008), dict(dpost=0x90001),
+                                dict(d=norm_desc(post_weight=None)), dict(d=norm_desc(gate=0, gate_values=None)), dict(d=norm_desc(next_weight=None)),
+                                dict(d=norm_desc(gate=4), dgate=0xA0008), dict(tokens=-1)])
+def test_norm_backward_refuses(kw, capfd):
+    assert norm_backward(**kw) == BAD
+    assert "[MOE ERROR:" in capfd.readouterr().out
+
+
+def test_no_tokens_need_no_rows():
+    assert norm(tokens=0, x=None, branch=None, y=None, h=None, kept=None) == 0
+    assert norm_backward(tokens=0, x=None, branch=None, dy=None, dh=None, kept=None, work=None, dx=None, dbranch=None, dpost=None, dgate=None,
+                         dnext=None) == 0
+
+
+def test_norm_workspace():
+    """Column sums of at most about a thousand workgroups, whatever the groups."""
+    def size(tokens, **kw):
+        n = ctypes.c_size_t(0)
+        assert _lib.load().flashMoeBlockNormBytes(ctypes.byref(norm_desc(**kw)), tokens, ctypes.byref(n)) == 0
+        return n.value
+
+    for tokens in (0, 1, 1000, 1 << 20, 1 << 30):
+        for hidden in (8, 1024, 8192):
+            assert 0 < size(tokens, hidden=hidden) <= 2 * 512 * hidden * 4
+    for count, shared in ((1, 7), (3, 5), (700, 3), (2, 100000), (513, 513), (1 << 20, 1), (1 << 10, 1 << 20)):
+        assert 0 < size(count * shared, gate=2, shared=shared) <= 3 * 1100 * 64 * 4
+
+
+@pytest.mark.parametrize("call,message", [
+    (lambda x, w: ops.block_norm(x, w), "CUDA tensor"), (lambda x, w: ops.block_norm(x, None), "must be tensors"),
+    (lambda x, w: ops.block_norm(None, w), "must be tensors"), (lambda x, w: ops.block_norm(x, w, eps="1"), "eps a number"),
+    (lambda x, w: ops.block_join(x, None), "must be tensors"), (lambda x, w: ops.block_join(x, x, gate=1.0), "gate"),
+    (lambda x, w: ops.block_join(x, x, w, None, w), "CUDA tensor"), (lambda x, w: ops.block_join(x.requires_grad_(), x), "CUDA tensor"),
+    (lambda x, w: ops.block_join(x, x, residual_scale=w), "numbers"),
+])
+def test_norms_of_other_arguments(call, message):
+    with pytest.raises(RuntimeError, match=message):
+        call(torch.zeros(3, 8), torch.ones(8))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_norms_refuse_tangents(which):
+    args = [torch.zeros(2, 8), torch.zeros(2, 8), torch.ones(8), torch.ones(8), torch.ones(8)]
+    with fwd.dual_level():
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.block_join(*args)
+
+
+@pytest.mark.parametrize("gate", [None, (8,), (2, 1, 8), (2, 3, 1), (2, 3, 8)])
+@pytest.mark.parametrize("post,nxt", [(True, True), (False, True), (True, False)])
+def test_join_definition(gate, post, nxt):
+    """The restatement's gradients against differences, and against autograd."""
+    gen = torch.Generator().manual_seed(4)
+    draw = lambda *s: torch.randn(s, generator=gen, dtype=torch.float64)  # noqa: E731
+    layer_case.HALF.setdefault(torch.float64, 0.0)
+    given = dict(x=draw(2, 3, 8), branch=draw(2, 3, 8), post=draw(8) if post else None, gate=draw(*gate) if gate else None,
+                 next_weight=draw(8) if nxt else None)
+    dy, dh = draw(2, 3, 8), draw(2, 3, 8) if nxt else None
+    more = dict(alpha=0.7, beta=1.3, eps=1e-3)
+    want = layer_case.join(**given, **more, dy=dy, dh=dh)
+    for name, t in given.items():
+        if t is not None:
+            def loss(v):
+                r = layer_case.join(**{**given, name: v}, **more)
+                return float((r["y"][0] * dy).sum() + ((r["h"][0] * dh).sum() if nxt else 0))
+            assert torch.allclose(want[name][0], differences(loss, t), rtol=0, atol=1e-7), name
+    alone = layer_case.join(given["x"], next_weight=draw(8), eps=0.0, dh=dy)
+    assert torch.allclose((alone["x"][0] * given["x"]).sum(-1), torch.zeros(2, 3, dtype=torch.float64), atol=1e-12)  # a norm has no slope along itself
