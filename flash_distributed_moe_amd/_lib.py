@@ -65,6 +65,12 @@ class NormDesc(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("post_weight", "gate_values", "next_weight")]
 
 
+class AdapterDesc(ctypes.Structure):
+    """Mirror of FlashMoeAdapterDesc."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("adapters", "rank", "n", "k")] + [(n, ctypes.c_void_p) for n in ("down", "up", "scales")]
+
+
 # name -> (restype, argtypes); every symbol include/flash_moe.h declares
 C_ABI = {
     "flashMoeVersion": (ctypes.c_char_p, []),
@@ -123,6 +129,9 @@ C_ABI = {
     "flashMoeBlockNormBytes": (ctypes.c_int, [ctypes.POINTER(NormDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "flashMoeBlockNormBackward": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [ctypes.c_void_p, ctypes.c_longlong] * 4 +
                                   [ctypes.c_int] + [ctypes.c_void_p] * 8),
+    "flashMoeAdapterBytes": (ctypes.c_int, [ctypes.POINTER(AdapterDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "flashMoeAdapterAdd": (ctypes.c_int, [ctypes.POINTER(AdapterDesc)] + [ctypes.c_void_p, ctypes.c_longlong] * 2 +
+                           [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong] + [ctypes.c_void_p] * 2),
     "flashMoeSetDenseSmallBatch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
 }
 ABI_VERSION = 3

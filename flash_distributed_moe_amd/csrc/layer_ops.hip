@@ -111,6 +111,33 @@ fmoe::NormArgs norm_args(const FlashMoeNormDesc* d, int tokens) {
 }
 size_t partial_bytes(const fmoe::NormArgs& a) { return size_t(fmoe::norm_arrays(a)) * a.blocks * a.H * 4; }
 
+hipError_t validate(const FlashMoeAdapterDesc* d, int rows) {
+  if (d == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null description");
+  if (d->adapters < 1 || d->adapters > fmoe::kAdapters || d->rank < 8 || d->rank > fmoe::kAdapterRank || d->rank % 8 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "%i adapters of rank %i: up to %i, ranks multiples of 8 up to %i", d->adapters, d->rank,
+              fmoe::kAdapters, fmoe::kAdapterRank);
+  for (const int width : {d->n, d->k})
+    if (width < 8 || width % 8 != 0 || width > kMaxStride)
+      FMOE_FAIL(hipErrorInvalidValue, "n=%i, k=%i: multiples of 8, at most %lld", d->n, d->k, kMaxStride);
+  if (rows < 0 || rows > 1 << 28) FMOE_FAIL(hipErrorInvalidValue, "%i rows (at most 2^28)", rows);
+  return hipSuccess;
+}
+hipError_t check_bf16_rows(const char* name, const void* p, long long ld, int width) {
+  if (p == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null %s pointer", name);
+  if (!on(p, 16)) FMOE_FAIL(hipErrorInvalidValue, "%s does not begin on 16 bytes", name);
+  if (ld < width || ld > kMaxStride || ld % 8 != 0)
+    FMOE_FAIL(hipErrorInvalidValue, "%s: %lld values from row to row (at least %i, at most %lld, whole 16 bytes)", name, ld, width,
+              kMaxStride);
+  return hipSuccess;
+}
+fmoe::AdapterArgs adapter_args(const FlashMoeAdapterDesc* d, int rows) {
+  fmoe::AdapterArgs a{};
+  a.T = rows, a.K = d->k, a.N = d->n, a.r = d->rank, a.adapters = d->adapters;
+  a.down = d->down, a.up = d->up, a.scales = d->scales;
+  fmoe::plan_adapters(a);
+  return a;
+}
+
 }  // namespace
 
 extern "C" {
@@ -222,6 +249,37 @@ int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long 
   a.partial = static_cast<float*>(workspace);
   fmoe::plan_norm_backward(a);
   FMOE_HIP_CHECK(fmoe::launch_norm_backward(a, desc->dtype, static_cast<hipStream_t>(stream)));
+  return hipSuccess;
+}
+
+int flashMoeAdapterBytes(const FlashMoeAdapterDesc* desc, int rows, size_t* bytes) {
+  FMOE_HIP_CHECK(validate(desc, rows));
+  if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result");
+  *bytes = rows > 0 ? fmoe::adapter_bytes(adapter_args(desc, rows)).all() : 0;
+  return hipSuccess;
+}
+
+int flashMoeAdapterAdd(const FlashMoeAdapterDesc* desc, const void* x, long long ldx, const void* y, long long ldy, const int* ids,
+                       int rows, void* out, long long ldo, void* workspace, void* stream) {
+  FMOE_HIP_CHECK(validate(desc, rows));
+  if (rows == 0) return hipSuccess;
+  FMOE_HIP_CHECK(check_bf16_rows("x", x, ldx, desc->k));
+  FMOE_HIP_CHECK(check_bf16_rows("y", y, ldy, desc->n));
+  FMOE_HIP_CHECK(check_bf16_rows("out", out, ldo, desc->n));
+  if (out == y && ldo != ldy) FMOE_FAIL(hipErrorInvalidValue, "out is y, but its rows lie otherwise");
+  FMOE_HIP_CHECK(check_word("ids", ids));
+  FMOE_HIP_CHECK(check_word("scales", desc->scales));
+  if (desc->down == nullptr || desc->up == nullptr || !on(desc->down, 16) || !on(desc->up, 16))
+    FMOE_FAIL(hipErrorInvalidValue, "adapters are missing or do not begin on 16 bytes");
+  if (workspace == nullptr || !on(workspace, 16)) FMOE_FAIL(hipErrorInvalidValue, "the workspace is missing or does not begin on 16 bytes");
+  fmoe::AdapterArgs a = adapter_args(desc, rows);
+  a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.ids = ids, a.out = out, a.ldo = ldo;
+  const fmoe::AdapterBytes b = fmoe::adapter_bytes(a);
+  char* p = static_cast<char*>(workspace);
+  a.u = reinterpret_cast<float*>(p);
+  a.order = reinterpret_cast<int*>(p + b.u);
+  a.tiles = reinterpret_cast<int*>(p + b.u + b.order);
+  FMOE_HIP_CHECK(fmoe::launch_adapters(a, static_cast<hipStream_t>(stream)));
   return hipSuccess;
 }
 

@@ -93,4 +93,48 @@ inline int norm_arrays(const NormArgs& a) { return a.gate_kind == GATE_GROUP ? 3
 hipError_t launch_norm(const NormArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_norm_backward(const NormArgs& a, int dtype, hipStream_t stream);
 
+// ------------------------------------------------------------------ adapters beside a projection
+struct AdapterArgs {
+  const void* x;        // [T, K], rows ldx values apart
+  const void* y;        // [T, N]
+  void* out;            // [T, N]; may be y
+  const int* ids;       // [T]: a row's adapter, negative: none
+  const void* down;     // [adapters, r, K]
+  const void* up;       // [adapters, N, r]
+  const float* scales;  // [adapters]
+  long long ldx, ldy, ldo;
+  int T, K, N, r, adapters;
+  float* u;    // x A^T: [splits, T, r]; of few rows scaled, of many by place in `order`
+  int* order;  // [T]: rows by adapter
+  int* tiles;  // [tiles + 1, 4]: adapter, first place, rows; the last one's first value is their number
+  int most_tiles, tile_rows, splits;
+};
+constexpr int kAdapterRank = 128, kAdapters = 1000;
+// Few rows: every row reads its adapter by itself.
+__host__ __device__ inline bool adapter_rows_alone(int T) { return T <= 128; }
+// Many: tiles of 16 or 64 rows of one adapter, whose k several workgroups share while there are few of them.
+inline void plan_adapters(AdapterArgs& a) {
+  if (adapter_rows_alone(a.T)) {
+    a.splits = 1;
+    return;
+  }
+  a.tile_rows = a.T >= 4096 ? 64 : 16;
+  const long long full = (a.T + a.tile_rows - 1LL) / a.tile_rows;
+  // a last tile each, of every adapter, of the rows without one and of those of an adapter that is not there
+  a.most_tiles = static_cast<int>(full + (a.adapters + 2 < a.T ? a.adapters + 2 : a.T));
+  const long long wanted = (512 + full - 1) / full, most = (a.K + 511) / 512;
+  a.splits = static_cast<int>(wanted < most ? wanted : most);
+}
+struct AdapterBytes {
+  size_t u, order, tiles;
+  size_t all() const { return u + order + tiles; }
+};
+inline AdapterBytes adapter_bytes(const AdapterArgs& a) {
+  const auto whole = [](size_t v) { return (v + 255) / 256 * 256; };
+  AdapterBytes b{whole(size_t(a.splits) * a.T * a.r * 4), 0, 0};
+  if (!adapter_rows_alone(a.T)) b.order = whole(size_t(a.T) * 4), b.tiles = whole((size_t(a.most_tiles) + 1) * 16);
+  return b;
+}
+hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream);
+
 }  // namespace fmoe

@@ -266,6 +266,77 @@ variable_list block_norm(const at::Tensor& x, const OptTensor& branch, const Opt
   return BlockNorm::apply(x, branch, post, gate, next, alpha, beta, eps);
 }
 
+// ------------------------------------------------------------------ adapters beside a projection
+// Whether two sets of rows share no memory: behind one another, or columns of the same rows side by side.
+bool apart(const Rows& a, const Rows& b) {
+  if (a.count == 0 || b.count == 0) return true;
+  const int64_t size = a.t.element_size(), wa = a.t.size(1) * size, wb = b.t.size(1) * size;
+  const int64_t pa = reinterpret_cast<int64_t>(a.t.data_ptr()), pb = reinterpret_cast<int64_t>(b.t.data_ptr());
+  const int64_t la = a.stride * size, lb = b.stride * size;
+  if (pa + (a.count - 1) * la + wa <= pb || pb + (b.count - 1) * lb + wb <= pa) return true;
+  if (la != lb) return false;
+  const int64_t d = ((pb - pa) % la + la) % la;
+  return d >= wa && d + wb <= la;
+}
+
+at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tensor& down, const at::Tensor& up, const at::Tensor& scales,
+                        const at::Tensor& ids, const OptTensor& out) {
+  for (const at::Tensor* t : {&y, &x, &down, &up, &scales}) refuse_tangent(*t, "an input");
+  TORCH_CHECK(!differentiated({&y, &x, &down, &up, &scales}), "adapters have no backward pass: detach the inputs or use torch.no_grad()");
+  TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  check_device(y, "y", x);
+  check_device(down, "down", x);
+  check_device(up, "up", x);
+  check_device(scales, "scales", x);
+  check_device(ids, "ids", x);
+  for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{y, "y"}, {x, "x"}, {down, "down"}, {up, "up"}})
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous(), "scales must be float32 without gaps");
+  TORCH_CHECK(ids.scalar_type() == at::kInt, "ids must be int32");
+  TORCH_CHECK(down.dim() == 3 && up.dim() == 3 && scales.dim() == 1 && down.size(0) == up.size(0) && down.size(0) == scales.size(0) &&
+                  down.size(1) == up.size(2),
+              "adapters must be down [adapters, r, K], up [adapters, N, r] and scales [adapters]");
+  check_packed(down, "down");
+  check_packed(up, "up");
+  FlashMoeAdapterDesc d{};
+  d.adapters = int_size(down.size(0), "adapters"), d.rank = int_size(down.size(1), "rank");
+  d.n = int_size(up.size(1), "N"), d.k = int_size(down.size(2), "K");
+  TORCH_CHECK(d.adapters >= 1 && d.adapters <= 1000, "1 to 1000 adapters, not ", d.adapters);
+  TORCH_CHECK(d.rank >= 8 && d.rank <= 128 && d.rank % 8 == 0, "the rank must be a multiple of 8, at most 128, not ", d.rank);
+  TORCH_CHECK(d.n >= 8 && d.n % 8 == 0 && d.k >= 8 && d.k % 8 == 0, "N and K must be multiples of 8, not ", d.n, " and ", d.k);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == d.k, "x must be [..., K] with K = ", d.k);
+  TORCH_CHECK(y.dim() == x.dim() && y.size(-1) == d.n, "y must be [..., N] with N = ", d.n);
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  TORCH_CHECK(y.sizes().slice(0, y.dim() - 1) == lead && ids.sizes() == lead, "x, y and ids must have the same leading dimensions");
+  d.down = down.data_ptr(), d.up = up.data_ptr(), d.scales = scales.data_ptr<float>();
+  const DeviceGuard guard(x.device());
+  const Rows xs = rows_of(x, "x"), ys = rows_of(y, "y");
+  at::Tensor result;
+  Rows outs;
+  if (out.has_value()) {
+    result = *out;
+    check_device(result, "out", x);
+    TORCH_CHECK(result.sizes() == y.sizes() && result.scalar_type() == y.scalar_type(), "out must have y's shape and dtype");
+    TORCH_CHECK(!result.requires_grad() || !at::GradMode::is_enabled(), "out requires a gradient");
+    outs = rows_of(result, "out");
+    TORCH_CHECK(outs.t.data_ptr() == result.data_ptr(), "out must have rows without gaps that begin on 16 bytes");
+    const bool itself = result.is_same(y) || (pointer(ys.t) == pointer(outs.t) && ys.stride == outs.stride);
+    TORCH_CHECK(itself || apart(outs, ys), "out must be y or apart from it");
+    TORCH_CHECK(apart(outs, xs), "out must be apart from x");
+  } else {
+    result = at::empty(y.sizes(), plain(y));
+    outs = rows_of(result, "out");
+  }
+  const at::Tensor which = ids.contiguous();
+  size_t bytes = 0;
+  check_hip(flashMoeAdapterBytes(&d, xs.count, &bytes), "flashMoeAdapterBytes");
+  const at::Tensor work = bytes_on(x, bytes);
+  check_hip(flashMoeAdapterAdd(&d, pointer(xs.t), xs.stride, pointer(ys.t), ys.stride, static_cast<int*>(pointer(which)), xs.count,
+                               pointer(outs.t), outs.stride, pointer(work), current_stream()),
+            "flashMoeAdapterAdd");
+  return result;
+}
+
 }  // namespace
 
 void bind_layer(py::module_& m) {
@@ -273,4 +344,6 @@ void bind_layer(py::module_& m) {
         py::call_guard<py::gil_scoped_release>());
   m.def("block_norm", &block_norm, py::arg("x"), py::arg("branch"), py::arg("post_weight"), py::arg("gate"), py::arg("next_weight"),
         py::arg("residual_scale"), py::arg("branch_scale"), py::arg("eps"), py::call_guard<py::gil_scoped_release>());
+  m.def("add_adapters", &add_adapters, py::arg("y"), py::arg("x"), py::arg("down"), py::arg("up"), py::arg("scales"), py::arg("ids"),
+        py::arg("out"), py::call_guard<py::gil_scoped_release>());
 }

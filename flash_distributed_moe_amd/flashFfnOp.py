@@ -64,9 +64,39 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
         raise _stranger("q must be Mxfp4 and dtype a torch.dtype", q, dtype) from None
 
 
-def mxfp4_linear(x, weight):
+class Adapters(NamedTuple):
+    """Low-rank adapters of one projection [N, K]: down bfloat16 [adapters, r, K], up bfloat16 [adapters, N, r], scales float32
+    [adapters]. Adapter i adds scales[i] * up[i] @ down[i] to the projection's weights. r is a multiple of 8, up to 128
+    (shorter adapters are filled up with zeros), and there are up to 1000 of them."""
+
+    down: torch.Tensor
+    up: torch.Tensor
+    scales: torch.Tensor
+
+
+def add_adapters(y, x, adapters, ids, out=None):
+    """y [..., N] + scales[i] * (x [..., K] down[i]^T) up[i]^T, i = ids[...] (int32) being each row's adapter, for y that
+    a projection of x gave: one call for the rows of many requests, in any order.
+
+    All bfloat16; float32 between the two products, rounded once. A row whose id is negative has no adapter and keeps y; a row
+    whose id names no adapter becomes NaN (ids are not read on the host). The result is new, or out, which may be y.
+    K and N multiples of 8. Not differentiable."""
+    try:
+        return flashMoeLauncher.add_adapters(y, x, adapters.down, adapters.up, adapters.scales, ids, out)
+    except _STRANGERS:
+        raise _stranger("y, x, ids and out must be tensors, adapters Adapters", y, x, adapters, ids, out) from None
+
+
+def mxfp4_linear(x, weight, adapters=None, ids=None):
     """x [..., K] (bfloat16, or Mxfp4) times the transpose of weight (Mxfp4 [N, K]): bfloat16 [..., N],
-    summed in float32. Not differentiable."""
+    summed in float32. With adapters and ids what `add_adapters` adds to that, for bfloat16 x. Not differentiable."""
+    if (adapters is None) != (ids is None):
+        raise RuntimeError("adapters and ids belong together")
+    if adapters is not None:
+        if isinstance(x, Mxfp4):
+            raise RuntimeError("adapters take bfloat16 x")
+        y = mxfp4_linear(x, weight)
+        return add_adapters(y, x, adapters, ids, out=y)
     try:
         if isinstance(x, Mxfp4):
             return flashMoeLauncher.mxfp4_linear(x.codes, x.scales, weight.codes, weight.scales)

@@ -403,6 +403,23 @@ int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long 
                               const void* dy, long long lddy, const void* dh, long long lddh, int tokens, const float* kept,
                               void* workspace, void* dx, void* dbranch, void* dpost, void* dgate, void* dnext, void* stream);
 
+/* Low-rank adapters of many requests beside a projection: out_t = y_t + scales[i] * (x_t down[i]^T) up[i]^T, i = ids[t] being the
+ * adapter of row t, in bfloat16; float32 between the two products, rounded once. y is what the projection gave. */
+typedef struct FlashMoeAdapterDesc {
+  int adapters;        /* 1..1000 */
+  int rank;            /* r, a multiple of 8, at most 128 (shorter ones are filled up with zeros) */
+  int n, k;            /* multiples of 8, at most 2^20 */
+  const void* down;    /* device, bfloat16 [adapters, r, k] */
+  const void* up;      /* device, bfloat16 [adapters, n, r] */
+  const float* scales; /* device, [adapters] */
+} FlashMoeAdapterDesc;
+int flashMoeAdapterBytes(const FlashMoeAdapterDesc* desc, int rows, size_t* bytes);
+/* x [rows, k], y and out [rows, n] rows ldx / ldy / ldo values apart (whole 16 bytes, at most 2^20); out may be y if its rows lie
+ * the same way, and overlaps nothing else. ids [rows], in any order: a row with a negative one has no adapter, one at or
+ * beyond `adapters` becomes NaN. workspace: flashMoeAdapterBytes of device memory on 16 bytes. rows is at most 2^28. */
+int flashMoeAdapterAdd(const FlashMoeAdapterDesc* desc, const void* x, long long ldx, const void* y, long long ldy, const int* ids,
+                       int rows, void* out, long long ldo, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

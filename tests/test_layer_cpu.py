@@ -6,7 +6,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from flash_distributed_moe_amd import _lib, flashLayerOp as ops
+from flash_distributed_moe_amd import _lib, flashFfnOp as fops, flashLayerOp as ops
 from tests import layer_case
 
 BAD = _lib.HIP_ERROR_INVALID_VALUE
@@ -229,3 +229,70 @@ def test_join_definition(gate, post, nxt):
             assert torch.allclose(want[name][0], differences(loss, t), rtol=0, atol=1e-7), name
     alone = layer_case.join(given["x"], next_weight=draw(8), eps=0.0, dh=dy)
     assert torch.allclose((alone["x"][0] * given["x"]).sum(-1), torch.zeros(2, 3, dtype=torch.float64), atol=1e-12)  # a norm has no slope along itself
+
+
+# ------------------------------------------------------------------ adapters beside a projection
+def adapter_desc(**kw):
+    d = _lib.AdapterDesc(4, 16, 64, 128, 0x1000, 0x2000, 0x3000)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def add(d=None, x=0x10000, ldx=128, y=0x20000, ldy=64, ids=0x30000, rows=5, out=0x40000, ldo=64, work=0x50000):
+    return _lib.load().flashMoeAdapterAdd(ctypes.byref(d or adapter_desc()), x, ldx, y, ldy, ids, rows, out, ldo, work, None)
+
+
+def adapter_size(rows, **kw):
+    n = ctypes.c_size_t(0)
+    rc = _lib.load().flashMoeAdapterBytes(ctypes.byref(adapter_desc(**kw)), rows, ctypes.byref(n))
+    return rc, n.value
+
+
+@pytest.mark.parametrize("kw", [dict(adapters=0), dict(adapters=1001), dict(rank=0), dict(rank=12), dict(rank=136), dict(n=0), dict(n=60), dict(k=4),
+                                dict(n=(1 << 20) + 8)])
+def test_bad_adapters(kw, capfd):
+    assert add(d=adapter_desc(**kw)) == BAD and adapter_size(5, **kw)[0] == BAD
+    assert capfd.readouterr().out.count("[MOE ERROR:") == 2
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(x=0x10008), dict(ldx=120), dict(ldx=132), dict(y=None), dict(ldy=56), dict(out=None), dict(out=0x40004),
+                                dict(ldo=68), dict(ldo=(1 << 20) + 8), dict(out=0x20000, ldo=72), dict(ids=None), dict(ids=0x30002), dict(rows=-1),
+                                dict(rows=(1 << 28) + 1), dict(work=None), dict(work=0x50008), dict(d=adapter_desc(down=None)),
+                                dict(d=adapter_desc(up=0x2008)), dict(d=adapter_desc(scales=None))])
+def test_adapters_refuse(kw, capfd):
+    assert add(**kw) == BAD
+    assert "[MOE ERROR:" in capfd.readouterr().out
+
+
+def test_adapter_workspace():
+    assert adapter_size(0) == (0, 0) and add(rows=0, x=None, y=None, out=None, ids=None, work=None) == 0
+    assert 5 * 16 * 4 <= adapter_size(5)[1] < 5 * 16 * 4 + 256
+    for rows in (129, 4095, 4096, 100000, 1 << 28):
+        rc, size = adapter_size(rows, adapters=1000)
+        tiles = -(-rows // (64 if rows >= 4096 else 16)) + min(rows, 1002)
+        # u at least once, the order of the rows, and 16 bytes a tile and one more
+        assert rc == 0 and size >= rows * 16 * 4 + rows * 4 + (tiles + 1) * 16
+
+
+@pytest.mark.parametrize("call,message", [
+    (lambda y, x, a, i: fops.add_adapters(y, x, a, i), "CUDA tensor"), (lambda y, x, a, i: fops.add_adapters(y, x, None, i), "must be tensors"),
+    (lambda y, x, a, i: fops.add_adapters(None, x, a, i), "must be tensors"), (lambda y, x, a, i: fops.add_adapters(y, x, a, 3), "must be tensors"),
+    (lambda y, x, a, i: fops.add_adapters(y, x, a, i, out=1), "must be tensors"),
+    (lambda y, x, a, i: fops.add_adapters(y, x.requires_grad_(), a, i), "no backward pass"),
+    (lambda y, x, a, i: fops.mxfp4_linear(x, None, a), "belong together"),
+])
+def test_adapters_of_other_arguments(call, message):
+    b = torch.bfloat16
+    a = fops.Adapters(torch.zeros(2, 8, 16, dtype=b), torch.zeros(2, 24, 8, dtype=b), torch.zeros(2))
+    with pytest.raises(RuntimeError, match=message):
+        call(torch.zeros(3, 24, dtype=b), torch.zeros(3, 16, dtype=b), a, torch.zeros(3, dtype=torch.int32))
+
+
+def test_adapters_refuse_tangents():
+    b = torch.bfloat16
+    a = fops.Adapters(torch.zeros(2, 8, 16, dtype=b), torch.zeros(2, 24, 8, dtype=b), torch.zeros(2))
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(3, 16, dtype=b), torch.ones(3, 16, dtype=b))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fops.add_adapters(torch.zeros(3, 24, dtype=b), x, a, torch.zeros(3, dtype=torch.int32))
