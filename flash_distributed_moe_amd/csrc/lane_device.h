@@ -13,7 +13,8 @@ template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v)));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140, kNextLane = 0x101;  // the lane on, 0 behind the 16th
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140, kRotate8 = 0x128;
+constexpr int kNextLane = 0x101;  // the lane on, 0 behind the 16th
 
 // Over the row of 16 lanes, in all of them, in one order: every lane gets the same bits.
 __device__ __forceinline__ float row16_sum(float v) {

@@ -110,19 +110,21 @@ struct AdapterArgs {
   int most_tiles, tile_rows, splits;
 };
 constexpr int kAdapterRank = 128, kAdapters = 1000;
-// Few rows: every row reads its adapter by itself.
-__host__ __device__ inline bool adapter_rows_alone(int T) { return T <= 128; }
+// Few rows: every row reads its adapter by itself. By rows and in tiles, us: rank 16, K=N=4096, 64 adapters, 128 rows 9.0 and 18.0, 256
+// rows 12.3 and 19.7, 512 rows 16.9 and 18.4; rank 32, K=2048, N=8192, 8 adapters 12.6 and 17.1, 21.5 and 22.6, 38.5 and 23.2;
+// rank 64, K=4096, N=12288, 200 adapters 58.9 and 62.6, 102.6 and 88.6, 186.8 and 110.0.
+__host__ __device__ inline bool adapter_rows_alone(int T) { return T <= 192; }
 // Many: tiles of 16 or 64 rows of one adapter, whose k several workgroups share while there are few of them.
 inline void plan_adapters(AdapterArgs& a) {
   if (adapter_rows_alone(a.T)) {
     a.splits = 1;
     return;
   }
-  a.tile_rows = a.T >= 4096 ? 64 : 16;
+  a.tile_rows = a.T < 4096 ? 16 : 64;
   const long long full = (a.T + a.tile_rows - 1LL) / a.tile_rows;
   // a last tile each, of every adapter, of the rows without one and of those of an adapter that is not there
   a.most_tiles = static_cast<int>(full + (a.adapters + 2 < a.T ? a.adapters + 2 : a.T));
-  const long long wanted = (512 + full - 1) / full, most = (a.K + 511) / 512;
+  const long long wanted = (256 + full - 1) / full, most = (a.K + 255) / 256;
   a.splits = static_cast<int>(wanted < most ? wanted : most);
 }
 struct AdapterBytes {

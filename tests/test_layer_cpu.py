@@ -268,7 +268,7 @@ def test_adapters_refuse(kw, capfd):
 def test_adapter_workspace():
     assert adapter_size(0) == (0, 0) and add(rows=0, x=None, y=None, out=None, ids=None, work=None) == 0
     assert 5 * 16 * 4 <= adapter_size(5)[1] < 5 * 16 * 4 + 256
-    for rows in (129, 4095, 4096, 100000, 1 << 28):
+    for rows in (193, 4095, 4096, 100000, 1 << 28):
         rc, size = adapter_size(rows, adapters=1000)
         tiles = -(-rows // (64 if rows >= 4096 else 16)) + min(rows, 1002)
         # u at least once, the order of the rows, and 16 bytes a tile and one more
