@@ -50,6 +50,33 @@ __device__ __forceinline__ float wave_sum(float v) {
   return (at(0) + at(16)) + (at(32) + at(48));
 }
 
+__device__ __forceinline__ int wave_sum(int v) {
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  v += dpp<kMirror8>(v);
+  v += dpp<kMirror16>(v);
+  const auto at = [&](int lane) { return __builtin_amdgcn_readlane(v, lane); };
+  return (at(0) + at(16)) + (at(32) + at(48));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const long long b = __builtin_bit_cast(long long, v);
+  const unsigned lo = static_cast<unsigned>(dpp<CTRL>(static_cast<int>(b))), hi = static_cast<unsigned>(dpp<CTRL>(static_cast<int>(b >> 32)));
+  return __builtin_bit_cast(double, static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  v += dpp<kMirror8>(v);
+  v += dpp<kMirror16>(v);
+  const long long b = __builtin_bit_cast(long long, v);
+  const auto at = [&](int lane) {
+    const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo));
+  };
+  return (at(0) + at(16)) + (at(32) + at(48));
+}
+
 // This wave's LDS writes have arrived before its later reads of other lanes' data.
 __device__ __forceinline__ void wave_lds_ready() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -155,7 +155,7 @@ int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long l
                   void* stream) {
   FMOE_HIP_CHECK(validate(desc, tokens));
   FMOE_HIP_CHECK(check_word("counts", counts));
-  FMOE_HIP_CHECK(check_word("totals", totals));
+  if (!on(totals, 4)) FMOE_FAIL(hipErrorInvalidValue, "totals does not begin on 4 bytes");
   FMOE_HIP_CHECK(check_word("balance", balance));
   FMOE_HIP_CHECK(check_word("zed", zed));
   if (tokens > 0) {
@@ -172,19 +172,21 @@ int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long l
 }
 
 int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
-                          const int* experts, const int* counts, const int* totals, const float* dweights,
-                          const float* dbalance, const float* dzed, void* dlogits, long long ldd, void* stream) {
+                          const float* weights, const int* experts, const int* counts, const int* totals,
+                          const float* dweights, const float* dbalance, const float* dzed, void* dlogits, long long ldd,
+                          void* stream) {
   FMOE_HIP_CHECK(validate(desc, tokens));
   if (tokens == 0) return hipSuccess;
   FMOE_HIP_CHECK(check_logits("logits", logits, ld, desc));
   FMOE_HIP_CHECK(check_logits("dlogits", dlogits, ldd, desc));
+  FMOE_HIP_CHECK(check_word("weights", weights));
   FMOE_HIP_CHECK(check_word("experts", experts));
   FMOE_HIP_CHECK(check_word("counts", counts));
   FMOE_HIP_CHECK(check_word("totals", totals));
   for (const void* p : {static_cast<const void*>(dweights), static_cast<const void*>(dbalance), static_cast<const void*>(dzed)})
     if (!on(p, 4)) FMOE_FAIL(hipErrorInvalidValue, "a gradient does not begin on 4 bytes");
   fmoe::RouteArgs a = route_args(desc, logits, ld, mask, tokens);
-  a.experts = const_cast<int*>(experts), a.counts = const_cast<int*>(counts), a.totals = const_cast<int*>(totals);
+  a.weights = const_cast<float*>(weights), a.experts = const_cast<int*>(experts), a.counts = const_cast<int*>(counts), a.totals = const_cast<int*>(totals);
   a.dweights = dweights, a.dbalance = dbalance, a.dzed = dzed, a.dlogits = dlogits, a.ldd = ldd;
   FMOE_HIP_CHECK(fmoe::launch_route_backward(a, desc->dtype, static_cast<hipStream_t>(stream)));
   return hipSuccess;

@@ -12,10 +12,10 @@ struct RouteArgs {
   const unsigned char* mask;  // [T], 0: padding; NULL: none is
   long long ld;
   int T, E, k, renormalize;
-  float* weights;   // [T, k]
+  float* weights;   // [T, k]; read by the backward pass
   int* experts;     // [T, k]
   int* counts;      // [E]
-  int* totals;      // [2]: rows with a candidate, slots filled
+  int* totals;      // [2]: rows with a candidate, slots filled; NULL: not wanted
   float* balance;   // [1]
   float* zed;       // [1]
   float* partial;   // of more than one workgroup: [blocks, kRouteColumns] sums of probabilities, then as many counts
@@ -34,7 +34,7 @@ struct RouteGrid {
   int blocks, threads;
 };
 inline RouteGrid route_grid(int T) {
-  const int threads = T <= 64 || T > 4096 ? 1024 : 256, rows = threads / 16;
+  const int threads = T <= 64 || T > 16384 ? 1024 : 256, rows = threads / 16;
   const long long blocks = (T + rows - 1LL) / rows;
   return {static_cast<int>(blocks < 1 ? 1 : blocks < 256 ? blocks : 256), threads};
 }

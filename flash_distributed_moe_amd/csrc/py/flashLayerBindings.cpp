@@ -50,7 +50,7 @@ FlashMoeRouteDesc describe(const at::Tensor& logits, int64_t top_k, bool renorma
 struct Routed {
   at::Tensor weights, experts, counts, balance, zed, totals, mask;
 };
-Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask) {
+Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask, bool keep) {
   refuse_tangent(logits, "logits");
   const FlashMoeRouteDesc d = describe(logits, top_k, renormalize, mask);
   const DeviceGuard guard(logits.device());
@@ -61,7 +61,8 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
   sizes.back() = top_k;
   const auto floats = plain(logits).dtype(at::kFloat), ints = plain(logits).dtype(at::kInt);
   r.weights = at::empty(sizes, floats), r.experts = at::empty(sizes, ints);
-  r.counts = at::empty({d.experts}, ints), r.totals = at::empty({2}, ints);
+  r.counts = at::empty({d.experts}, ints);
+  if (keep) r.totals = at::empty({2}, ints);
   r.balance = at::empty({}, floats), r.zed = at::empty({}, floats);
   size_t bytes = 0;
   check_hip(flashMoeRouteBytes(&d, rows.count, &bytes), "flashMoeRouteBytes");
@@ -69,7 +70,7 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
   if (bytes > 0) work = bytes_on(logits, bytes);
   check_hip(flashMoeRoute(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(r.mask)), rows.count,
                           static_cast<float*>(pointer(r.weights)), static_cast<int*>(pointer(r.experts)), r.counts.data_ptr<int>(),
-                          r.totals.data_ptr<int>(), r.balance.data_ptr<float>(), r.zed.data_ptr<float>(), pointer(work),
+                          static_cast<int*>(pointer(r.totals)), r.balance.data_ptr<float>(), r.zed.data_ptr<float>(), pointer(work),
                           current_stream()),
             "flashMoeRoute");
   return r;
@@ -77,8 +78,8 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
 
 struct Route : torch::autograd::Function<Route> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask) {
-    const Routed r = route_forward(logits, top_k, renormalize, mask);
-    ctx->save_for_backward({logits, r.mask, r.experts, r.counts, r.totals});
+    const Routed r = route_forward(logits, top_k, renormalize, mask, true);
+    ctx->save_for_backward({logits, r.mask, r.experts, r.counts, r.totals, r.weights});
     ctx->saved_data["top_k"] = top_k;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->mark_non_differentiable({r.experts, r.counts});
@@ -96,7 +97,7 @@ struct Route : torch::autograd::Function<Route> {
     at::Tensor out = at::empty(logits.sizes(), plain(logits));
     const auto floats = [](const at::Tensor& t) { return static_cast<const float*>(pointer(t)); };
     check_hip(flashMoeRouteBackward(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(mask)), rows.count,
-                                    static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), kept[4].data_ptr<int>(), floats(dw),
+                                    floats(kept[5]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), kept[4].data_ptr<int>(), floats(dw),
                                     floats(grads[3]), floats(grads[4]), pointer(out), d.experts, current_stream()),
               "flashMoeRouteBackward");
     return {out, at::Tensor(), at::Tensor(), at::Tensor()};
@@ -106,7 +107,7 @@ struct Route : torch::autograd::Function<Route> {
 variable_list route(const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask) {
   TORCH_CHECK(logits.defined(), "logits tensor is undefined");
   if (!differentiated({&logits})) {
-    Routed r = route_forward(logits, top_k, renormalize, mask);
+    Routed r = route_forward(logits, top_k, renormalize, mask, false);
     return {r.weights, r.experts, r.counts, r.balance, r.zed};
   }
   if (logits.is_cuda()) {

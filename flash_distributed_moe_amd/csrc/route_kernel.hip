@@ -8,9 +8,8 @@
 //   D = w_j (dw_j - sum w dw) at the winners, or with plain probabilities dw_j joins g there
 //
 // Sixteen lanes have a token, four logits of every 64 each, so that a load is whole lines of four tokens and every cross-lane step is a data
-// parallel primitive that serves four tokens. The winners are taken in k rounds. A round costs a subtraction and half a
-// three-way maximum a value, because a logit and its place are one whole number, no two of them equal: the next winner is the
-// largest of (key - last winner) in unsigned arithmetic, where what was taken already comes out small, so nothing has to be struck out.
+// parallel primitive that serves four tokens. The winners are taken in k rounds, of the lanes' greatest. For those a logit and its place are
+// one whole number, no two of them equal, so that a comparison says who goes first and a winner is found by its key.
 // A float32 logit has nine bits too many for that; where two neighbours among the first k + 1 agree in what is kept, the
 // wave takes its four tokens again by whole logits (of random ones one in some thousands).
 // Both directions are meant to be bound by reading the logits; the rounds are what competes with it.
@@ -86,14 +85,39 @@ __device__ __forceinline__ unsigned ordered(float v) {
   return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
 
-// e^x of x <= 0 to about 2^-23: what the product with log2(e) leaves out is put back to first order. (Results
-// below 2^-126 are zeros.) A fourth of the library's instructions.
+// e^x of x <= 0 with the hardware's 2^t: off by |x| 2^-24 for the product's rounding, a fifth of that for the constant's, and
+// 2^-23. Below e^-104 the result is zero, of -inf and of NaN too (a token with an infinity has a sum of zero then, and weights that
+// are NaN). The library's function takes three times as many instructions, and a token has E of these.
 __device__ __forceinline__ float exp_down(float x) {
-  x = x < -150.0f ? -150.0f : x;
-  const float t = x * 1.44269504f;
-  const float rest = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return fmaf(e, rest * 0.693147181f, e);
+  return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(x, -150.0f, 0.0f) * 1.44269504f);
+}
+
+// Value i of a lane if it is a candidate, else -inf.
+template <bool BF, int V>
+__device__ __forceinline__ void candidates(const Raw<BF, V>& r, bool open, float (&v)[V]) {
+  const float above = open ? lowest<BF>() : INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float x = value_of<BF>(r.u, i);
+    v[i] = x > above ? x : -INFINITY;
+  }
+}
+template <int V>
+__device__ __forceinline__ float lane_max(const float (&v)[V]) {
+  float m = v[V - 1];
+#pragma unroll
+  for (int i = 0; i + 1 < V; i += 2) m = fmaxf(fmaxf(m, v[i]), v[i + 1]);
+  return m;
+}
+
+// The greatest of a lane's keys below `last`, 0 if there is none. Keys have 31 bits, so of their distances from `last` (mod 2^32) those of
+// smaller keys are above 2^31 and the others below, and nothing has to be struck out: three instructions for two keys.
+template <int V>
+__device__ __forceinline__ unsigned next_below(const unsigned (&key)[V], unsigned last) {
+  unsigned best = key[V - 1] - last;
+#pragma unroll
+  for (int i = 0; i + 1 < V; i += 2) best = umax(umax(best, key[i] - last), key[i + 1] - last);
+  return best >> 31 ? best + last : 0u;
 }
 
 // Winner j of a token lies in lane j % 16, the second sixteen in `second`: 1 + its column, 0 for a slot that stays empty.
@@ -101,31 +125,33 @@ struct Winners {
   unsigned first, second;
 };
 
-template <bool BF, int V>
-__device__ __forceinline__ Winners pick(const unsigned* u, bool open, int lane, int E, int k) {
+// v: candidates(). again(): the row once more, for the tokens that are taken by whole logits; kept in registers it would cost all others.
+template <bool BF, int V, typename Again>
+__device__ __forceinline__ Winners pick(const float (&v)[V], Again again, int lane, int E, int k) {
+  // 31 bits: the logit's 16 (bfloat16) or first 23, and its place backwards, so that equals go to the lowest one; no two are equal
   unsigned key[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float v = value_of<BF>(u, i);
-    // 31 bits: the logit's 16 (bfloat16) or first 23, and its place backwards, so that equals go to the lowest one
-    const unsigned bits = BF ? ordered(v) >> 16 << 8 : ordered(v) >> 1 & 0x7FFFFF00u;
-    key[i] = open && v > lowest<BF>() ? bits | (255 - column(lane, i)) : 0u;
-  }
+  for (int i = 0; i < V; ++i) key[i] = (BF ? ordered(v[i]) >> 16 << 8 : ordered(v[i]) >> 1 & 0x7FFFFF00u) | (255 - column(lane, i));
+  // of the lowest candidate: all others' keys are those of -inf, which are below
+  const unsigned least = BF ? ordered(lowest<BF>()) >> 16 << 8 : ordered(lowest<BF>()) >> 1 & 0x7FFFFF00u;
+  // a lane's three greatest in order; a fourth, of one token in some hundreds, is looked for when it is needed
+  unsigned t0 = next_below<V>(key, 0x80000000u), t1 = next_below<V>(key, t0), t2 = next_below<V>(key, t1);
   const int rounds = BF ? k : min(k + 1, E);
-  unsigned last = 0x80000000u, first = 0, second = 0;
+  unsigned last = 0, first = 0, second = 0;
   for (int j = 0; j < rounds; ++j) {
-    unsigned best = key[0] - last;
-#pragma unroll
-    for (int i = 1; i + 1 < V; i += 2) best = umax(umax(best, key[i] - last), key[i + 1] - last);
-    best = umax(best, key[V - 1] - last);
-    const unsigned next = last != 0 ? row16_max(best) + last : 0u;
-    last = next;
+    last = row16_max(t0);
     if (j < k && lane == (j & 15)) {
       if (j < 16) first = last;
       else second = last;
     }
+    const bool mine = t0 == last;
+    t0 = mine ? t1 : t0, t1 = mine ? t2 : t1, t2 = mine ? 0u : t2;
+    if (__any(mine && t0 == 0u)) {
+      if (mine && t0 == 0u) t0 = next_below<V>(key, last);
+    }
   }
-  Winners w = {first != 0 ? 256 - (first & 255) : 0u, second != 0 ? 256 - (second & 255) : 0u};
+  const auto slot = [&](unsigned won) { return won >= least ? 256 - (won & 255) : 0u; };
+  Winners w = {slot(first), slot(second)};
   if constexpr (!BF) {
     // `last` is winner k's if there was a round for it
     const unsigned extra = rounds > k ? last : 0u;
@@ -135,14 +161,13 @@ __device__ __forceinline__ Winners pick(const unsigned* u, bool open, int lane, 
     if (lane == 15) after = second0;
     if (lane == k - 1) after = extra;
     if (lane == k - 17) after2 = extra;
-    const bool near = (lane < k && first != 0 && (first ^ after) >> 8 == 0) ||
-                      (lane + 16 < k && second != 0 && (second ^ after2) >> 8 == 0);
+    const bool near = (lane < k && first >= least && (first ^ after) >> 8 == 0) ||
+                      (lane + 16 < k && second >= least && (second ^ after2) >> 8 == 0);
     if (__any(near)) {
+      float x[V];
+      again(x);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float v = value_of<BF>(u, i);
-        key[i] = open && v > lowest<BF>() ? ordered(v) : 0u;
-      }
+      for (int i = 0; i < V; ++i) key[i] = x[i] > -INFINITY ? ordered(x[i]) : 0u;
       w = {0u, 0u};
       for (int j = 0; j < k; ++j) {
         unsigned best = 0, at = 0;
@@ -150,13 +175,13 @@ __device__ __forceinline__ Winners pick(const unsigned* u, bool open, int lane, 
         for (int i = 0; i < V; ++i)
           if (key[i] > best) best = key[i], at = column(lane, i) + 1;
         const unsigned most = row16_max(best);
-        const unsigned won = most != 0 ? row16_min(best == most ? at : 0xFFFFu) : 0u;
+        const unsigned won = row16_min(most != 0 && best == most ? at : 0xFFFFu);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           if (column(lane, i) + 1 == won) key[i] = 0u;
         if (lane == (j & 15)) {
-          if (j < 16) w.first = won;
-          else w.second = won;
+          if (j < 16) w.first = most != 0 ? won : 0u;
+          else w.second = most != 0 ? won : 0u;
         }
       }
     }
@@ -164,36 +189,31 @@ __device__ __forceinline__ Winners pick(const unsigned* u, bool open, int lane, 
   return w;
 }
 
-__device__ __forceinline__ double block_sum(double v, double* room) {
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double sum = 0.0;
-  for (unsigned i = 0; i < blockDim.x / 64; ++i) sum += room[i];
-  return sum;
-}
-// By one whole workgroup; thread e < E has expert e's count and sum of probabilities, thread 0 the rows and the squares.
-__device__ __forceinline__ void finish(const RouteArgs& a, int count, double probs, double rows, double squares, double* room) {
+struct Totals {
+  double both, squares;  // sum of counts times probabilities, of squared logsumexps
+  int slots, rows;
+};
+// By one whole workgroup; thread e < E has expert e's count and sum of probabilities, any thread some of the squares and of the rows.
+__device__ __forceinline__ void finish(const RouteArgs& a, int count, double probs, double squares, int rows, Totals* room) {
   const bool mine = static_cast<int>(threadIdx.x) < a.E;
-  const double slots = block_sum(mine ? count : 0, room);
-  const double both = block_sum(mine ? count * probs : 0.0, room);
   if (mine) a.counts[threadIdx.x] = count;
-  if (threadIdx.x == 0) {
-    a.totals[0] = static_cast<int>(rows);
-    a.totals[1] = static_cast<int>(slots);
-    *a.balance = static_cast<float>(slots > 0 ? a.E * both / (slots * rows) : both);
-    *a.zed = static_cast<float>(rows > 0 ? squares / rows : squares);
-  }
+  const Totals wave{wave_sum(mine ? count * probs : 0.0), wave_sum(squares), wave_sum(mine ? count : 0), wave_sum(rows)};
+  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = wave;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  Totals t{};
+  for (unsigned i = 0; i < blockDim.x / 64; ++i)
+    t.both += room[i].both, t.squares += room[i].squares, t.slots += room[i].slots, t.rows += room[i].rows;
+  if (a.totals != nullptr) a.totals[0] = t.rows, a.totals[1] = t.slots;
+  *a.balance = static_cast<float>(t.slots > 0 ? a.E * t.both / (static_cast<double>(t.slots) * t.rows) : t.both);
+  *a.zed = static_cast<float>(t.rows > 0 ? t.squares / t.rows : t.squares);
 }
 
 template <bool BF, int V, bool WHOLE>
 __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   __shared__ int hist[kRouteExperts];
   __shared__ float probs[16][kRouteExperts];
-  __shared__ float wave_squares[16];
-  __shared__ int wave_rows[16];
-  __shared__ double room[16];
+  __shared__ Totals room[16];
   const int lane = threadIdx.x & 15, wave = threadIdx.x >> 6;
   const int rows_here = blockDim.x / 16;
   const long long step = static_cast<long long>(gridDim.x) * rows_here;
@@ -207,28 +227,23 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   long long row = static_cast<long long>(blockIdx.x) * rows_here + (threadIdx.x >> 4);
   // rows behind the last one are read as the last one and count for nothing
   const auto place = [&](long long r) { return static_cast<size_t>(min(r, a.T - 1LL)) * a.ld; };
+  // the next row is asked for while this one is worked on, but of sixteen values a lane, where four waves hide each other's loads
+  // and the registers are needed (as it was, with 33 of them in scratch, T=131072, E=256 took 114 us instead of TODO)
+  constexpr bool kAhead = V < 16;
   Raw<BF, V> next{};
-  if (a.T > 0) next = load_row<BF, V, WHOLE>(a.logits, place(row), lane, a.E);
+  if (kAhead && a.T > 0) next = load_row<BF, V, WHOLE>(a.logits, place(row), lane, a.E);
   // all of a wave's rows go round together: the cross-lane steps need every lane
   for (long long first = row - (threadIdx.x >> 4 & 3); first < a.T; first += step, row += step) {
-    const Raw<BF, V> now = next;
-    if (first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step), lane, a.E);
+    Raw<BF, V> now = next;
+    if constexpr (!kAhead) now = load_row<BF, V, WHOLE>(a.logits, place(row), lane, a.E);
+    if (kAhead && first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step), lane, a.E);
     const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float v = value_of<BF>(now.u, i);
-      m = open && v > lowest<BF>() ? fmaxf(m, v) : m;
-    }
-    m = row16_max(m);
+    float v[V], e[V], s = 0.0f;
+    candidates(now, open, v);
+    const float m = row16_max(lane_max(v));
     const bool some = m > -INFINITY;
-    float e[V], s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float v = value_of<BF>(now.u, i);
-      e[i] = some && v > lowest<BF>() ? exp_down(v - m) : 0.0f;
-      s += e[i];
-    }
+    for (int i = 0; i < V; ++i) e[i] = exp_down(v[i] - m), s += e[i];
     s = row16_sum(s);
     const float each = some ? 1.0f / s : 0.0f;
 #pragma unroll
@@ -238,7 +253,11 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
       squares = fmaf(lse, lse, squares);
       ++rows;
     }
-    const Winners w = pick<BF, V>(now.u, open, lane, a.E, a.k);
+    const auto again = [&](float (&x)[V]) {
+      asm volatile("" ::: "memory");
+      candidates(load_row<BF, V, WHOLE>(a.logits, place(row), lane, a.E), open, x);
+    };
+    const Winners w = pick<BF, V>(v, again, lane, a.E, a.k);
     const float w0 = w.first != 0 ? exp_down(value_at<BF>(a.logits, place(row) + w.first - 1) - m) : 0.0f;
     const float w1 = w.second != 0 ? exp_down(value_at<BF>(a.logits, place(row) + w.second - 1) - m) : 0.0f;
     const float of = a.renormalize ? row16_sum(w0 + w1) : s;
@@ -265,57 +284,57 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
     v += __shfl_xor(v, 32, 64);
     if ((threadIdx.x & 63) < 16 && column(lane, i) < kRouteExperts) probs[wave][column(lane, i)] = v;
   }
-  squares += __shfl_xor(squares, 16, 64);
-  squares += __shfl_xor(squares, 32, 64);
-  rows += __shfl_xor(rows, 16, 64);
-  rows += __shfl_xor(rows, 32, 64);
-  if ((threadIdx.x & 63) == 0) wave_squares[wave] = squares, wave_rows[wave] = rows;
   __syncthreads();
   const int e = threadIdx.x, waves = blockDim.x / 64;
   float p = 0.0f;
   if (e < a.E)
     for (int i = 0; i < waves; ++i) p += probs[i][e];
-  float all_squares = 0.0f;
-  int all_rows = 0;
-  if (e == 0)
-    for (int i = 0; i < waves; ++i) all_squares += wave_squares[i], all_rows += wave_rows[i];
   if (gridDim.x == 1) {
-    finish(a, e < a.E ? hist[e] : 0, p, all_rows, all_squares, room);
+    finish(a, e < a.E ? hist[e] : 0, p, squares, rows, room);
     return;
   }
   float* sums = a.partial + static_cast<size_t>(blockIdx.x) * kRouteColumns;
   int* counts = reinterpret_cast<int*>(a.partial + static_cast<size_t>(gridDim.x + blockIdx.x) * kRouteColumns);
   if (e < a.E) sums[e] = p, counts[e] = hist[e];
-  if (e == 0) sums[kRouteExperts] = all_squares, counts[kRouteExperts] = all_rows;
+  const float wave_squares = wave_sum(squares);
+  const int wave_rows = wave_sum(rows);
+  if ((e & 63) == 0) room[wave].squares = wave_squares, room[wave].rows = wave_rows;
+  __syncthreads();
+  if (e == 0) {
+    double all_squares = 0.0;
+    int all_rows = 0;
+    for (int i = 0; i < waves; ++i) all_squares += room[i].squares, all_rows += room[i].rows;
+    sums[kRouteExperts] = static_cast<float>(all_squares), counts[kRouteExperts] = all_rows;
+  }
 }
 
 // The workgroups' sums, by one: four threads to a column.
 __global__ __launch_bounds__(1024) void route_finish_kernel(RouteArgs a, int blocks) {
   __shared__ double probs[4][kRouteExperts];
   __shared__ int counts[4][kRouteExperts];
-  __shared__ double room[16];
+  __shared__ Totals room[16];
   const int e = threadIdx.x & 255, part = threadIdx.x >> 8;
   const int* partial_counts = reinterpret_cast<const int*>(a.partial + static_cast<size_t>(blocks) * kRouteColumns);
   double p = 0.0;
   int c = 0;
   if (e < a.E) {
-#pragma unroll 8
+#pragma unroll 16
     for (int b = part; b < blocks; b += 4) {
       p += a.partial[static_cast<size_t>(b) * kRouteColumns + e];
       c += partial_counts[static_cast<size_t>(b) * kRouteColumns + e];
     }
   }
   probs[part][e] = p, counts[part][e] = c;
-  double squares = 0.0, rows = 0.0;
+  double squares = 0.0;
+  int rows = 0;
   if (static_cast<int>(threadIdx.x) < blocks) {
     squares = a.partial[static_cast<size_t>(threadIdx.x) * kRouteColumns + kRouteExperts];
     rows = partial_counts[static_cast<size_t>(threadIdx.x) * kRouteColumns + kRouteExperts];
   }
-  squares = block_sum(squares, room);
-  rows = block_sum(rows, room);
+  __syncthreads();
   p = (probs[0][e] + probs[1][e]) + (probs[2][e] + probs[3][e]);
   c = (counts[0][e] + counts[1][e]) + (counts[2][e] + counts[3][e]);
-  finish(a, c, p, rows, squares, room);
+  finish(a, c, p, squares, rows, room);
 }
 
 template <bool BF, int V, bool WHOLE>
@@ -337,47 +356,39 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
   const long long step = static_cast<long long>(gridDim.x) * 16;
   long long row = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const auto place = [&](long long r) { return static_cast<size_t>(min(r, a.T - 1LL)); };
+  struct Slot {
+    int expert;
+    float weight, d;
+  };
+  const auto slot_at = [&](size_t r, int j) {
+    const size_t at = r * a.k + j;
+    if (j >= a.k) return Slot{-1, 0.0f, 0.0f};
+    return Slot{a.experts[at], a.weights[at], a.dweights != nullptr ? a.dweights[at] : 0.0f};
+  };
   Raw<BF, V> next = load_row<BF, V, WHOLE>(a.logits, place(row) * a.ld, lane, a.E);
+  Slot coming = slot_at(place(row), lane), coming2 = slot_at(place(row), lane + 16);
   for (long long first = row - (threadIdx.x >> 4 & 3); first < a.T; first += step, row += step) {
     const Raw<BF, V> now = next;
     if (first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step) * a.ld, lane, a.E);
     const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
-    const size_t at = place(row) * a.k + lane;
-    const int e0 = open && lane < a.k ? a.experts[at] : -1, e1 = open && lane + 16 < a.k ? a.experts[at + 16] : -1;
-    const float d0 = e0 >= 0 && a.dweights != nullptr ? a.dweights[at] : 0.0f;
-    const float d1 = e1 >= 0 && a.dweights != nullptr ? a.dweights[at + 16] : 0.0f;
-    const float l0 = e0 >= 0 ? value_at<BF>(a.logits, place(row) * a.ld + e0) : 0.0f;
-    const float l1 = e1 >= 0 ? value_at<BF>(a.logits, place(row) * a.ld + e1) : 0.0f;
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float v = value_of<BF>(now.u, i);
-      m = open && v > lowest<BF>() ? fmaxf(m, v) : m;
-    }
-    m = row16_max(m);
+    const Slot one = coming, two = coming2;
+    if (first + step < a.T) coming = slot_at(place(row + step), lane), coming2 = slot_at(place(row + step), lane + 16);
+    const int e0 = open ? one.expert : -1, e1 = open ? two.expert : -1;
+    float v[V], p[V], s = 0.0f;
+    candidates(now, open, v);
+    const float m = row16_max(lane_max(v));
     const bool some = m > -INFINITY;
-    float p[V], s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float v = value_of<BF>(now.u, i);
-      p[i] = some && v > lowest<BF>() ? exp_down(v - m) : 0.0f;
-      s += p[i];
-    }
+    for (int i = 0; i < V; ++i) p[i] = exp_down(v[i] - m), s += p[i];
     s = row16_sum(s);
     const float each = some ? 1.0f / s : 0.0f;
-    const float w0 = e0 >= 0 ? exp_down(l0 - m) : 0.0f, w1 = e1 >= 0 ? exp_down(l1 - m) : 0.0f;
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) p[i] *= each, dot = fmaf(p[i], g[i], dot);
-    float a0, a1;
-    if (a.renormalize) {
-      const float share = some ? 1.0f / row16_sum(w0 + w1) : 0.0f;
-      const float mean = row16_sum(w0 * share * d0 + w1 * share * d1);
-      a0 = w0 * share * (d0 - mean), a1 = w1 * share * (d1 - mean);
-    } else {
-      a0 = w0 * each * d0, a1 = w1 * each * d1;
-      dot += a0 + a1;
-    }
+    // the weights' own slope: winners alone under renormalisation, else p's among the others
+    const float mean = a.renormalize ? row16_sum(one.weight * one.d + two.weight * two.d) : 0.0f;
+    const float a0 = one.weight * (one.d - mean), a1 = two.weight * (two.d - mean);
+    if (!a.renormalize) dot += a0 + a1;
     dot = row16_sum(dot);
     if (e0 >= 0) mine[e0] = a0;
     if (e1 >= 0) mine[e1] = a1;

@@ -59,10 +59,12 @@ def route(logits, k, renormalize, mask=None, dw=None, db=None, dz=None):
     n, slots = max(1, int(some.sum())), max(1, int(counts.sum()))
     balance = E * (counts.double() / slots * p.sum(0) / n).sum()
     zed = (lse ** 2).sum() / n
-    # a probability: the difference (|x| 2^-24 of the power), the exponential (8), the sum of up to 256 as 16 + 4 steps of terms
-    # that are off by as much (whose |x| is 6 on average at most), a division and a product
+    # a probability: of the power x 2^-24 each for the difference and for its product with log2(e), a fifth of that for the constant
+    # (log2(e) is held to 1.4 * 10^-8 of itself, 0.23 * 2^-24), the exponential (8 steps), the sum of up to 256 as 16 + 4 steps of
+    # terms that are off by as much (whose |x|, weighted with them, is the entropy less log s: 5.6 at most, 13 of its steps), a
+    # division and a product
     x = (L.detach() - m).abs()
-    rel = (x + 50) * U
+    rel = (2.25 * x + 50) * U
     P, Z = p.detach(), lse.detach()
     elsewhere = (Z.abs() + m.abs() + 60) * U  # of a logarithm of a sum
     out = {"experts": experts, "counts": counts,

@@ -37,9 +37,9 @@ def route(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, e
                                      work, None)
 
 
-def route_backward(d=None, logits=0x1000, ld=16, mask=None, tokens=100, experts=0x3000, counts=0x4000, totals=0x5000, dw=0x6000, db=0x7000,
+def route_backward(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, experts=0x3000, counts=0x4000, totals=0x5000, dw=0x6000, db=0x7000,
                    dz=0x8000, out=0x9000, ldd=16):
-    return _lib.load().flashMoeRouteBackward(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, experts, counts, totals, dw, db, dz, out,
+    return _lib.load().flashMoeRouteBackward(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, weights, experts, counts, totals, dw, db, dz, out,
                                              ldd, None)
 
 
@@ -60,7 +60,7 @@ def test_route_refuses(kw, capfd):
     assert "[MOE ERROR:" in capfd.readouterr().out
 
 
-@pytest.mark.parametrize("kw", [dict(logits=None), dict(ld=3), dict(out=None), dict(out=0x9001), dict(ldd=15), dict(experts=None), dict(counts=None),
+@pytest.mark.parametrize("kw", [dict(logits=None), dict(ld=3), dict(out=None), dict(out=0x9001), dict(ldd=15), dict(weights=None), dict(experts=None), dict(counts=None),
                                 dict(totals=None), dict(dw=0x6001), dict(dz=0x8002), dict(tokens=-1)])
 def test_route_backward_refuses(kw, capfd):
     assert route_backward(**kw) == BAD
@@ -74,8 +74,8 @@ def test_route_workspace():
         return n.value
 
     assert size(0) == size(1) == size(64) == 0
-    for tokens in (65, 100, 4096, 4097, 1 << 28):
-        rows = 16 if tokens <= 4096 else 64
+    for tokens in (65, 100, 4096, 16384, 16385, 1 << 28):
+        rows = 16 if tokens <= 16384 else 64
         assert size(tokens) == min(256, -(-tokens // rows)) * 2 * 257 * 4
     assert _lib.load().flashMoeRouteBytes(ctypes.byref(route_desc()), 1, None) == BAD
     assert route_backward(tokens=0, logits=None, out=None) == 0
