@@ -176,7 +176,7 @@ __device__ __forceinline__ bf16x8 as_bf16(u32x4 v) { return __builtin_bit_cast(b
 // TB blocks of 16 tokens, RB of 16 ranks.
 constexpr int kShrinkWaves = 4;
 template <int TB, int RB>
-__global__ __launch_bounds__(kShrinkWaves * 64) void shrink_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(kShrinkWaves * 64, TB * RB < 32 ? 2 : 1) void shrink_kernel(AdapterArgs a) {
   __shared__ __align__(16) float sums[kShrinkWaves / 2][TB * 16][RB * 16 + 4];
   if (static_cast<int>(blockIdx.x) >= a.tiles[0]) return;
   const int* tile = a.tiles + (static_cast<size_t>(blockIdx.x) + 1) * 4;
@@ -190,9 +190,12 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void shrink_kernel(AdapterArgs a
   for (int b = 0; b < TB; ++b)
 #pragma unroll
     for (int h = 0; h < 2; ++h) token[b][h] = static_cast<size_t>(a.order[first + min(b * 16 + h * 8 + (of & 7), rows - 1)]) * a.ldx + eighth;
-  size_t rank[RB];  // ranks behind the last one are read as the last one, and nobody reads their sums
+  size_t rank[RB][2];  // ranks behind the last one are read as the last one, and nobody reads their sums
 #pragma unroll
-  for (int b = 0; b < RB; ++b) rank[b] = (static_cast<size_t>(id) * a.r + min(b * 16 + of, a.r - 1)) * a.K + group * 8;
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      rank[b][h] = (static_cast<size_t>(id) * a.r + min(b * 16 + h * 8 + (of & 7), a.r - 1)) * a.K + eighth;
   f32x4 acc[TB][RB] = {};
   const auto step = [&](int k0, auto load) {
     u32x4 x[TB][2], w[RB][2];
@@ -201,10 +204,12 @@ __global__ __launch_bounds__(kShrinkWaves * 64) void shrink_kernel(AdapterArgs a
 #pragma unroll
       for (int b = 0; b < TB; ++b) x[b][h] = load(a.x, token[b][h], k0, eighth);
 #pragma unroll
-      for (int b = 0; b < RB; ++b) w[b][h] = load(a.down, rank[b] + h * 32, k0, h * 32 + group * 8);
+      for (int b = 0; b < RB; ++b) w[b][h] = load(a.down, rank[b][h], k0, eighth);
     }
 #pragma unroll
     for (int b = 0; b < TB; ++b) exchange(x[b][0], x[b][1]);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) exchange(w[b][0], w[b][1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll

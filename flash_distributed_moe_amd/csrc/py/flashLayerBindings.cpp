@@ -1,5 +1,7 @@
 // What stands around a layer's blocks, in the `flashMoeLauncher` extension: checks of the tensors, the autograd nodes, and the
 // C ABI's calls on the current stream. `flash_distributed_moe_amd/flashLayerOp.py` is the Python surface above them.
+#include <ATen/hip/EmptyTensor.h>
+
 #include "tensorChecks.h"
 
 namespace {
@@ -17,7 +19,13 @@ void refuse_second_derivatives(const char* name) {
   // Under create_graph the gradients would be taken for constants by whoever differentiates them again.
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivatives (create_graph=True)");
 }
-at::TensorOptions plain(const at::Tensor& like) { return like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous); }
+// New memory on `like`'s device, without gaps. (Past the dispatcher, which takes as long again: the smallest calls are
+// bound by the host, and make up to six of these.)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
+}
+at::Tensor fresh(const at::Tensor& like) { return fresh(like.sizes(), like.scalar_type(), like); }
+at::Tensor fresh_bytes(size_t bytes, const at::Tensor& like) { return fresh({static_cast<int64_t>(bytes)}, at::kByte, like); }
 
 // ------------------------------------------------------------------ the router's choice
 // Logits as rows, which may lie apart; copied where a row's values do.
@@ -59,15 +67,14 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
   if (mask.has_value()) r.mask = mask->contiguous();
   auto sizes = logits.sizes().vec();
   sizes.back() = top_k;
-  const auto floats = plain(logits).dtype(at::kFloat), ints = plain(logits).dtype(at::kInt);
-  r.weights = at::empty(sizes, floats), r.experts = at::empty(sizes, ints);
-  r.counts = at::empty({d.experts}, ints);
-  if (keep) r.totals = at::empty({2}, ints);
-  r.balance = at::empty({}, floats), r.zed = at::empty({}, floats);
+  r.weights = fresh(sizes, at::kFloat, logits), r.experts = fresh(sizes, at::kInt, logits);
+  r.counts = fresh({d.experts}, at::kInt, logits);
+  if (keep) r.totals = fresh({2}, at::kInt, logits);
+  r.balance = fresh({}, at::kFloat, logits), r.zed = fresh({}, at::kFloat, logits);
   size_t bytes = 0;
   check_hip(flashMoeRouteBytes(&d, rows.count, &bytes), "flashMoeRouteBytes");
   at::Tensor work;
-  if (bytes > 0) work = bytes_on(logits, bytes);
+  if (bytes > 0) work = fresh_bytes(bytes, logits);
   check_hip(flashMoeRoute(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(r.mask)), rows.count,
                           static_cast<float*>(pointer(r.weights)), static_cast<int*>(pointer(r.experts)), r.counts.data_ptr<int>(),
                           static_cast<int*>(pointer(r.totals)), r.balance.data_ptr<float>(), r.zed.data_ptr<float>(), pointer(work),
@@ -94,7 +101,7 @@ struct Route : torch::autograd::Function<Route> {
     const DeviceGuard guard(logits.device());
     const Rows rows = logit_rows(logits, "logits");
     at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
-    at::Tensor out = at::empty(logits.sizes(), plain(logits));
+    at::Tensor out = fresh(logits);
     const auto floats = [](const at::Tensor& t) { return static_cast<const float*>(pointer(t)); };
     check_hip(flashMoeRouteBackward(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(mask)), rows.count,
                                     floats(kept[5]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), kept[4].data_ptr<int>(), floats(dw),
@@ -195,9 +202,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const NormInputs& in
   const DeviceGuard guard(in.x.device());
   const NormCall c = prepare(in, alpha, beta, eps);
   at::Tensor y, h, kept;
-  if (in.branch.defined()) y = at::empty(in.x.sizes(), plain(in.x));
-  if (in.next.defined()) h = at::empty(in.x.sizes(), plain(in.x));
-  if (keep) kept = at::empty({2, c.x.count}, plain(in.x).dtype(at::kFloat));
+  if (in.branch.defined()) y = fresh(in.x);
+  if (in.next.defined()) h = fresh(in.x);
+  if (keep) kept = fresh({2, c.x.count}, at::kFloat, in.x);
   check_hip(flashMoeBlockNorm(&c.d, pointer(c.x.t), c.x.stride, pointer(c.branch.t), c.branch.stride, c.x.count, pointer(y), pointer(h),
                               static_cast<float*>(pointer(kept)), current_stream()),
             "flashMoeBlockNorm");
@@ -230,12 +237,12 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     if (dh.defined()) dhs = rows_of(dh, "dh");
     variable_list out(8);
     for (int i = 0, present = 0; i < 5; ++i)  // inputs that are not there have no place in the node
-      if (kept[i].defined() && ctx->needs_input_grad(present++)) out[i] = at::empty(kept[i].sizes(), plain(kept[i]));
+      if (kept[i].defined() && ctx->needs_input_grad(present++)) out[i] = fresh(kept[i]);
     void* dgate = pointer(out[3]);
     if (dgate != nullptr && c.d.gate == FLASH_MOE_GATE_NONE) out[3].zero_(), dgate = nullptr;
     size_t bytes = 0;
     check_hip(flashMoeBlockNormBytes(&c.d, c.x.count, &bytes), "flashMoeBlockNormBytes");
-    const at::Tensor work = bytes_on(in.x, bytes);
+    const at::Tensor work = fresh_bytes(bytes, in.x);
     check_hip(flashMoeBlockNormBackward(&c.d, pointer(c.x.t), c.x.stride, pointer(c.branch.t), c.branch.stride, pointer(dys.t), dys.stride,
                                         pointer(dhs.t), dhs.stride, c.x.count, static_cast<float*>(pointer(kept[5])), pointer(work),
                                         pointer(out[0]), pointer(out[1]), pointer(out[2]), dgate, pointer(out[4]), current_stream()),
@@ -271,7 +278,7 @@ variable_list block_norm(const at::Tensor& x, const OptTensor& branch, const Opt
 // Whether two sets of rows share no memory: behind one another, or columns of the same rows side by side.
 bool apart(const Rows& a, const Rows& b) {
   if (a.count == 0 || b.count == 0) return true;
-  const int64_t size = a.t.element_size(), wa = a.t.size(1) * size, wb = b.t.size(1) * size;
+  const int64_t size = a.t.element_size(), wa = a.t.size(-1) * size, wb = b.t.size(-1) * size;
   const int64_t pa = reinterpret_cast<int64_t>(a.t.data_ptr()), pb = reinterpret_cast<int64_t>(b.t.data_ptr());
   const int64_t la = a.stride * size, lb = b.stride * size;
   if (pa + (a.count - 1) * la + wa <= pb || pb + (b.count - 1) * lb + wb <= pa) return true;
@@ -325,13 +332,13 @@ at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tens
     TORCH_CHECK(itself || apart(outs, ys), "out must be y or apart from it");
     TORCH_CHECK(apart(outs, xs), "out must be apart from x");
   } else {
-    result = at::empty(y.sizes(), plain(y));
+    result = fresh(y);
     outs = rows_of(result, "out");
   }
   const at::Tensor which = ids.contiguous();
   size_t bytes = 0;
   check_hip(flashMoeAdapterBytes(&d, xs.count, &bytes), "flashMoeAdapterBytes");
-  const at::Tensor work = bytes_on(x, bytes);
+  const at::Tensor work = fresh_bytes(bytes, x);
   check_hip(flashMoeAdapterAdd(&d, pointer(xs.t), xs.stride, pointer(ys.t), ys.stride, static_cast<int*>(pointer(which)), xs.count,
                                pointer(outs.t), outs.stride, pointer(work), current_stream()),
             "flashMoeAdapterAdd");

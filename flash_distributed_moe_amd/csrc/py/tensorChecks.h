@@ -69,6 +69,8 @@ struct Rows {
 constexpr int64_t kMaxStride = 1 << 20;
 [[maybe_unused]] Rows rows_of(const at::Tensor& t, const char* name) {
   const int64_t width = t.size(-1), rows = width > 0 ? t.numel() / width : 0;
+  if (t.is_contiguous() && begins_on_16(t) && (rows <= 1 || (width <= kMaxStride && width * t.element_size() % 16 == 0)))
+    return {t, width, int_size(rows, name)};
   at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, width});
   int64_t stride = flat.stride(0);
   const bool apart = rows <= 1 || (stride >= width && stride <= kMaxStride && stride * flat.element_size() % 16 == 0);

@@ -106,6 +106,13 @@ def test_ways_to_hand_rows_over(ops, T):
     twice = torch.stack((ids, ids), 1)[:, 0]
     cube = ops.add_adapters(y.view(2, -1, 136), x.view(2, -1, 264), ops.Adapters(*a), twice.view(2, -1))
     assert torch.equal(cube.view(T, 136), want)
+    # columns side by side of one buffer with more dimensions, and columns that overlap
+    both = torch.zeros(2, T // 2, 264 + 136, dtype=torch.bfloat16, device="cuda")
+    both[..., :264], both[..., 264:] = x.view(2, -1, 264), y.view(2, -1, 136)
+    ops.add_adapters(both[..., 264:], both[..., :264], ops.Adapters(*a), ids.view(2, -1), out=both[..., 264:])
+    assert torch.equal(both[..., 264:].reshape(T, 136), want) and torch.equal(both[..., :264].reshape(T, 264), x)
+    with pytest.raises(RuntimeError, match="apart from x"):
+        ops.add_adapters(y.view(2, -1, 136), both[..., :264], ops.Adapters(*a), ids.view(2, -1), out=both[..., 256:392])
     one = ops.add_adapters(y[1], x[1], ops.Adapters(*a), ids[1])
     layer_case.check(one[None], *(v[1:2] for v in layer_case.adapters(y, x, *a, ids)), "one row")
 
