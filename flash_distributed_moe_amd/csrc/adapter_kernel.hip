@@ -100,7 +100,7 @@ __device__ __forceinline__ int join_bucket(int* counts, int bucket, bool real) {
 // Rows by adapter, then those without one, then those of an adapter that is not there; and the tiles they make. Which place a
 // row of an adapter has among its others may differ from call to call; no result depends on it.
 __global__ __launch_bounds__(kPlaceThreads) void place_kernel(AdapterArgs a) {
-  __shared__ int counts[kPlaceThreads], begins[kPlaceThreads];
+  __shared__ int counts[kPlaceThreads], begins[kPlaceThreads], ends[kPlaceThreads], tile_ends[kPlaceThreads];
   __shared__ int wave_rows[16], wave_tiles[16];
   const int me = threadIdx.x;
   counts[me] = 0;
@@ -128,14 +128,23 @@ __global__ __launch_bounds__(kPlaceThreads) void place_kernel(AdapterArgs a) {
   if ((me & 63) == 63) wave_rows[me >> 6] = rows_to, wave_tiles[me >> 6] = tiles_to;
   __syncthreads();
   for (int w = 0; w < me >> 6; ++w) rows_to += wave_rows[w], tiles_to += wave_tiles[w];
-  begins[me] = rows_to - rows;
+  begins[me] = rows_to - rows, ends[me] = rows_to, tile_ends[me] = tiles_to;
   counts[me] = 0;
-  for (int i = 0; i < tiles; ++i) {
-    int* tile = a.tiles + (static_cast<size_t>(tiles_to) - tiles + i + 1) * 4;
-    tile[0] = me, tile[1] = rows_to - rows + i * a.tile_rows, tile[2] = min(a.tile_rows, rows - i * a.tile_rows);
-  }
-  if (me == kPlaceThreads - 1) a.tiles[0] = tiles_to;
   __syncthreads();
+  const int total = tile_ends[kPlaceThreads - 1];
+  if (me == 0) a.tiles[0] = total;
+  for (int i = me; i < total; i += kPlaceThreads) {
+    // the first bucket that ends behind tile i has it
+    int low = 0, high = kPlaceThreads - 1;
+    while (low < high) {
+      const int mid = (low + high) / 2;
+      if (tile_ends[mid] > i) high = mid;
+      else low = mid + 1;
+    }
+    const int all = ends[low] - begins[low], mine = i - (tile_ends[low] - (all + a.tile_rows - 1) / a.tile_rows);
+    int* tile = a.tiles + (static_cast<size_t>(i) + 1) * 4;
+    tile[0] = low, tile[1] = begins[low] + mine * a.tile_rows, tile[2] = min(a.tile_rows, all - mine * a.tile_rows);
+  }
   for (long long first = 0; first < a.T; first += chunk) {
     // more rows than the threads hold: counted a second time
     if (a.T > chunk) {

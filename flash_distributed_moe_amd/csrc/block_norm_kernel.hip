@@ -94,6 +94,9 @@ __global__ void norm_kernel(NormArgs a, int waves) {
   __shared__ float room[2][16];
   const int lanes = waves * 64, first = threadIdx.x & (lanes - 1), count = a.H / P;
   const int at_once = blockDim.x / lanes, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / waves;
+  // the weights are on their way before a row's sums are waited for
+  const Pieces<V> wp = load_pieces<V>(row_at<BF>(a.post != nullptr ? a.post : a.x, 0, count, a.post != nullptr), first, lanes);
+  const Pieces<V> wn = load_pieces<V>(row_at<BF>(a.next != nullptr ? a.next : a.x, 0, count, a.next != nullptr), first, lanes);
   for (long long start = static_cast<long long>(blockIdx.x) * at_once; start < a.T; start += static_cast<long long>(gridDim.x) * at_once) {
     const bool real = start + mine < a.T;
     const long long row = real ? start + mine : a.T - 1;
@@ -101,24 +104,23 @@ __global__ void norm_kernel(NormArgs a, int waves) {
     float y[N];
     if (a.branch != nullptr) {
       const Pieces<V> b = load_pieces<V>(row_at<BF>(a.branch, row * a.ldb, count, real), first, lanes);
+      Pieces<V> g{};
       float scale = a.beta;
+      if (a.gate_kind == GATE_TOKEN) scale *= one_value<BF>(a.gate, row);
+      else if (a.gate_kind != GATE_NONE) g = load_pieces<V>(row_at<BF>(a.gate, gate_row(a, row) * a.H, count), first, lanes);
       if (a.post != nullptr) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) s = fmaf(piece_value<BF>(b.u[i / P], i % P), piece_value<BF>(b.u[i / P], i % P), s);
         const float rms = rsqrtf(row_sum(s, waves, room[0]) / a.H + a.eps);
         if (first == 0 && real && a.branch_rms != nullptr) a.branch_rms[row] = rms;
-        const Pieces<V> w = load_pieces<V>(row_at<BF>(a.post, 0, count), first, lanes);
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[i] = piece_value<BF>(b.u[i / P], i % P) * rms * piece_value<BF>(w.u[i / P], i % P);
+        for (int i = 0; i < N; ++i) y[i] = piece_value<BF>(b.u[i / P], i % P) * rms * piece_value<BF>(wp.u[i / P], i % P);
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) y[i] = piece_value<BF>(b.u[i / P], i % P);
       }
-      if (a.gate_kind == GATE_TOKEN) {
-        scale *= one_value<BF>(a.gate, row);
-      } else if (a.gate_kind != GATE_NONE) {
-        const Pieces<V> g = load_pieces<V>(row_at<BF>(a.gate, gate_row(a, row) * a.H, count), first, lanes);
+      if (a.gate_kind != GATE_NONE && a.gate_kind != GATE_TOKEN) {
 #pragma unroll
         for (int i = 0; i < N; ++i) y[i] *= piece_value<BF>(g.u[i / P], i % P);
       }
@@ -135,9 +137,8 @@ __global__ void norm_kernel(NormArgs a, int waves) {
       for (int i = 0; i < N; ++i) s = fmaf(y[i], y[i], s);
       const float rms = rsqrtf(row_sum(s, waves, room[1]) / a.H + a.eps);
       if (first == 0 && real && a.y_rms != nullptr) a.y_rms[row] = rms;
-      const Pieces<V> w = load_pieces<V>(row_at<BF>(a.next, 0, count), first, lanes);
 #pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = y[i] * rms * piece_value<BF>(w.u[i / P], i % P);
+      for (int i = 0; i < N; ++i) y[i] = y[i] * rms * piece_value<BF>(wn.u[i / P], i % P);
       store_pieces<BF, V>(row_at<BF>(a.h, row * a.H, count, real), first, lanes, y);
     }
     // a wave that is ahead writes its next sums where another may still read these

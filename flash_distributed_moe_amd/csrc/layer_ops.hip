@@ -119,7 +119,8 @@ hipError_t validate(const FlashMoeAdapterDesc* d, int rows) {
   for (const int width : {d->n, d->k})
     if (width < 8 || width % 8 != 0 || width > kMaxStride)
       FMOE_FAIL(hipErrorInvalidValue, "n=%i, k=%i: multiples of 8, at most %lld", d->n, d->k, kMaxStride);
-  if (rows < 0 || rows > 1 << 28) FMOE_FAIL(hipErrorInvalidValue, "%i rows (at most 2^28)", rows);
+  // eight workgroups for each of their tiles are still one launch
+  if (rows < 0 || rows > 1 << 26) FMOE_FAIL(hipErrorInvalidValue, "%i rows (at most 2^26)", rows);
   return hipSuccess;
 }
 hipError_t check_bf16_rows(const char* name, const void* p, long long ld, int width) {

@@ -34,7 +34,8 @@ struct RouteGrid {
   int blocks, threads;
 };
 inline RouteGrid route_grid(int T) {
-  const int threads = T <= 64 || T > 16384 ? 1024 : 256, rows = threads / 16;
+  // one workgroup has a wave for four tokens, and a thread for every expert
+  const int threads = T <= 16 ? 256 : T <= 64 ? (T + 3) / 4 * 64 : T > 16384 ? 1024 : 256, rows = threads / 16;
   const long long blocks = (T + rows - 1LL) / rows;
   return {static_cast<int>(blocks < 1 ? 1 : blocks < 256 ? blocks : 256), threads};
 }

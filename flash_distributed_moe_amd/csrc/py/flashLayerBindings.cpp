@@ -342,6 +342,7 @@ at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tens
   check_hip(flashMoeAdapterAdd(&d, pointer(xs.t), xs.stride, pointer(ys.t), ys.stride, static_cast<int*>(pointer(which)), xs.count,
                                pointer(outs.t), outs.stride, pointer(work), current_stream()),
             "flashMoeAdapterAdd");
+  if (out.has_value() && !result.is_inference()) torch::autograd::impl::bump_version(result);  // for whoever saved what was there
   return result;
 }
 

@@ -417,7 +417,7 @@ typedef struct FlashMoeAdapterDesc {
 int flashMoeAdapterBytes(const FlashMoeAdapterDesc* desc, int rows, size_t* bytes);
 /* x [rows, k], y and out [rows, n] rows ldx / ldy / ldo values apart (whole 16 bytes, at most 2^20); out may be y if its rows lie
  * the same way, and overlaps nothing else. ids [rows], in any order: a row with a negative one has no adapter, one at or
- * beyond `adapters` becomes NaN. workspace: flashMoeAdapterBytes of device memory on 16 bytes. rows is at most 2^28. */
+ * beyond `adapters` becomes NaN. workspace: flashMoeAdapterBytes of device memory on 16 bytes. rows is at most 2^26. */
 int flashMoeAdapterAdd(const FlashMoeAdapterDesc* desc, const void* x, long long ldx, const void* y, long long ldy, const int* ids,
                        int rows, void* out, long long ldo, void* workspace, void* stream);
 

@@ -187,3 +187,21 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for w, gs in zip(want, got):
         assert all(torch.equal(g, w) for g in gs)
+
+
+def test_results_in_place_are_noticed_by_autograd(ops):
+    """A product that another operator saved for its backward pass, and that out= wrote over, is not differentiated."""
+    y, x, a, ids = make(8, 64, 32, 8, 2, seed=8)
+    leaf = y.float().requires_grad_()
+    saved = torch.exp(leaf)
+    other = saved.detach().bfloat16()
+    z = torch.exp(y.detach().requires_grad_())
+    with torch.no_grad():
+        ops.add_adapters(other, x, ops.Adapters(*a), ids, out=other)
+        ops.add_adapters(z, x, ops.Adapters(*a), ids, out=z)
+    saved.sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    with torch.inference_mode():
+        w = y.clone()
+        ops.add_adapters(w, x, ops.Adapters(*a), ids, out=w)

@@ -258,7 +258,7 @@ def test_bad_adapters(kw, capfd):
 
 @pytest.mark.parametrize("kw", [dict(x=None), dict(x=0x10008), dict(ldx=120), dict(ldx=132), dict(y=None), dict(ldy=56), dict(out=None), dict(out=0x40004),
                                 dict(ldo=68), dict(ldo=(1 << 20) + 8), dict(out=0x20000, ldo=72), dict(ids=None), dict(ids=0x30002), dict(rows=-1),
-                                dict(rows=(1 << 28) + 1), dict(work=None), dict(work=0x50008), dict(d=adapter_desc(down=None)),
+                                dict(rows=(1 << 26) + 1), dict(work=None), dict(work=0x50008), dict(d=adapter_desc(down=None)),
                                 dict(d=adapter_desc(up=0x2008)), dict(d=adapter_desc(scales=None))])
 def test_adapters_refuse(kw, capfd):
     assert add(**kw) == BAD
@@ -268,7 +268,7 @@ def test_adapters_refuse(kw, capfd):
 def test_adapter_workspace():
     assert adapter_size(0) == (0, 0) and add(rows=0, x=None, y=None, out=None, ids=None, work=None) == 0
     assert 5 * 16 * 4 <= adapter_size(5)[1] < 5 * 16 * 4 + 256
-    for rows in (193, 4095, 4096, 100000, 1 << 28):
+    for rows in (193, 4095, 4096, 100000, 1 << 26):
         rc, size = adapter_size(rows, adapters=1000)
         tiles = -(-rows // (64 if rows >= 4096 else 16)) + min(rows, 1002)
         # u at least once, the order of the rows, and 16 bytes a tile and one more
