@@ -306,9 +306,16 @@ __device__ __forceinline__ void load_u(const AdapterArgs& a, Tokens<KS>& t, int 
     const int j = s * 32 + group * 8;
     f32x4 v[2] = {};
     if (j < a.r) {
-      for (int p = 0; p < a.splits; ++p) {
-        const f32x4* u = reinterpret_cast<const f32x4*>(a.u + (static_cast<size_t>(p) * a.T + place) * a.r + j);
-        v[0] += u[0], v[1] += u[1];
+      for (int p = 0; p < a.splits; p += 4) {  // four at a time in flight; behind the last one it is read again, for nothing
+        f32x4 u[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* from = a.u + (static_cast<size_t>(min(p + i, a.splits - 1)) * a.T + place) * a.r + j;
+          u[i][0] = *reinterpret_cast<const f32x4*>(from), u[i][1] = *reinterpret_cast<const f32x4*>(from + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (p + i < a.splits) v[0] += u[i][0], v[1] += u[i][1];
       }
     }
 #pragma unroll
@@ -384,8 +391,7 @@ __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a, int units) {
     }
   };
   const auto unit = [&](int n, const u32x4 (&w)[KS][4], u32x4 (&have)[2], u32x4 (&next_w)[KS][4], u32x4 (&next)[2]) {
-    load_w(n + step, next_w);
-    load_y(a, t, n + step, next);
+    if (n + step < end) load_w(n + step, next_w), load_y(a, t, n + step, next);
     add_unit(t, have, [&](int s, int f) { return s * 32 + group * 8 < a.r ? w[s][f] : u32x4{0, 0, 0, 0}; });
     store_y(a, t, n, have);
   };
@@ -450,15 +456,14 @@ __global__ __launch_bounds__(256) void expand_tall_kernel(AdapterArgs a, int uni
   u32x4 have0[2], have1[2], w0[KS], w1[KS];
   fetch(begin, w0);
   load_y(a, t, begin, have0);
-  fetch(begin + kUnit, w1);
+  if (begin + kUnit < end) fetch(begin + kUnit, w1);
   load_u(a, t, id, first, rows, wave * 16);
   keep(0, w0);
   meet();
   // a unit's B arrives two units ahead, its y one
   const auto unit = [&](int n, int turn, u32x4 (&have)[2], u32x4 (&next)[2], u32x4 (&coming)[KS], u32x4 (&free)[KS]) {
-    fetch(n + 2 * kUnit, free);
-    load_y(a, t, n + kUnit, next);
-    keep(turn ^ 1, coming);
+    if (n + 2 * kUnit < end) fetch(n + 2 * kUnit, free);
+    if (n + kUnit < end) load_y(a, t, n + kUnit, next), keep(turn ^ 1, coming);
     add_unit(t, have, [&](int s, int f) { return shared[turn][(s * 4 + f) * 64 + lane]; });
     store_y(a, t, n, have);
     meet();
@@ -482,22 +487,27 @@ void enqueue_shrink(const AdapterArgs& a, hipStream_t stream) {
 
 template <int KS>
 void enqueue_expand(const AdapterArgs& a, hipStream_t stream) {
-  // Columns of a workgroup. Every one reads its tokens' u again, but the last ones to start leave CUs idle: 8192 rows, N=12288,
-  // rank 64 with about 1000, 2000, 3300 and 5000 workgroups 99, 91, 89 and 96 us. Of 16 rows the waves have four units at a time.
-  const int across = (a.tile_rows == 64 ? 1 : 4) * kUnit, all = (a.N + across - 1) / across;
-  const long long wanted = ((a.tile_rows == 64 ? 3300 : 1024) + a.most_tiles - 1LL) / a.most_tiles;
-  if (a.tile_rows == 64) {
-    const int chunks = static_cast<int>((wanted + 7) / 8 * 8), units = (all + chunks - 1) / chunks;
+  // Columns of a workgroup. The last ones to start leave CUs idle (8192 rows, N=12288, rank 64 with about 1000, 2000, 3300 and 5000
+  // workgroups 99, 91, 89 and 96 us), but every one reads its tokens' u again, all parts of it: at least as many units as keep that
+  // to a fifth of what y takes (1024 rows, K=N=4096, rank 128 113 us without that, 45 with it). Of 16 rows the waves have four units
+  // at a time.
+  const bool tall = a.tile_rows == 64;
+  const int across = (tall ? 1 : 4) * kUnit, all = (a.N + across - 1) / across;
+  const long long wanted = ((tall ? 3300 : 1024) + a.most_tiles - 1LL) / a.most_tiles;
+  const int least = (a.r * a.splits + (tall ? 16 : 64) - 1) / (tall ? 16 : 64);
+  int units = static_cast<int>(max((all + wanted - 1) / wanted, static_cast<long long>(least)));
+  int chunks = (all + units - 1) / units;
+  if (tall) {
+    chunks = (chunks + 7) / 8 * 8, units = (all + chunks - 1) / chunks;  // columns of an XCD's own
     return expand_tall_kernel<KS><<<dim3(a.most_tiles * chunks), dim3(256), 0, stream>>>(a, units, chunks);
   }
-  const int units = static_cast<int>((all + wanted - 1) / wanted);
-  expand_kernel<KS><<<dim3(a.most_tiles, (all + units - 1) / units), dim3(256), 0, stream>>>(a, units);
+  expand_kernel<KS><<<dim3(a.most_tiles, chunks), dim3(256), 0, stream>>>(a, units);
 }
 
 }  // namespace
 
 hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream) {
-  if (adapter_rows_alone(a.T)) {
+  if (adapter_rows_alone(a)) {
     few_shrink_kernel<<<dim3((a.r + 4 * kRanks - 1) / (4 * kRanks), a.T), dim3(256), 0, stream>>>(a);
     few_expand_kernel<<<dim3((a.N + 511) / 512, a.T), dim3(256), 0, stream>>>(a);
     return hipGetLastError();

@@ -113,21 +113,25 @@ struct AdapterArgs {
   int most_tiles, tile_rows, splits;
 };
 constexpr int kAdapterRank = 128, kAdapters = 1000;
-// Few rows: every row reads its adapter by itself. By rows and in tiles, us: rank 16, K=N=4096, 64 adapters, 128 rows 9.0 and 18.0, 256
-// rows 12.3 and 19.7, 512 rows 16.9 and 18.4; rank 32, K=2048, N=8192, 8 adapters 12.6 and 17.1, 21.5 and 22.6, 38.5 and 23.2;
-// rank 64, K=4096, N=12288, 200 adapters 58.9 and 62.6, 102.6 and 88.6, 186.8 and 110.0.
-__host__ __device__ inline bool adapter_rows_alone(int T) { return T <= 192; }
+// Few rows: every row reads its adapter by itself, which costs as much for each of them; tiles cost three kernels, the more the higher
+// the rank, before the number of rows is felt. us by rows and in tiles, K=N=4096: rank 8, 768 rows 15 and 19, 1024 17 and 21; rank 16, 512 rows
+// 17 and 18, 768 22 and 20; rank 64, 256 rows 26 and 28, 384 38 and 28; rank 128, 256 rows 50 and 63, 384 72 and 55.
+__host__ __device__ inline bool adapter_rows_alone(const AdapterArgs& a) {
+  return a.T <= 4096 && static_cast<long long>(a.T) * a.r * (static_cast<long long>(a.K) + a.N) <= 56000000ll + 1400000ll * a.r;
+}
 // Many: tiles of 16 or 64 rows of one adapter, whose k several workgroups share while there are few of them.
 inline void plan_adapters(AdapterArgs& a) {
-  if (adapter_rows_alone(a.T)) {
+  if (adapter_rows_alone(a)) {
     a.splits = 1;
     return;
   }
-  a.tile_rows = a.T < 4096 ? 16 : 64;
+  // Tiles of 64 read B and A less often and fill slower: with 16 and 64 rows, K=N=4096, rank 16, 1024 rows 22 and 23 us, 2048 30 and 27; rank
+  // 64, 512 rows 24 and 30, 1024 35 and 31; of 200 adapters (N=12288) 1024 rows 125 and 137, 4096 197 and 165.
+  a.tile_rows = a.T >= 768 && static_cast<long long>(a.T) * (a.r + 8) >= 28672 && a.T >= 12 * a.adapters ? 64 : 16;
   const long long full = (a.T + a.tile_rows - 1LL) / a.tile_rows;
   // a last tile each, of every adapter, of the rows without one and of those of an adapter that is not there
   a.most_tiles = static_cast<int>(full + (a.adapters + 2 < a.T ? a.adapters + 2 : a.T));
-  const long long wanted = (256 + full - 1) / full, most = (a.K + 255) / 256;
+  const long long some = a.tile_rows == 64 ? 256 : 128, wanted = (some + full - 1) / full, most = (a.K + 511) / 512;
   a.splits = static_cast<int>(wanted < most ? wanted : most);
 }
 struct AdapterBytes {
@@ -137,7 +141,7 @@ struct AdapterBytes {
 inline AdapterBytes adapter_bytes(const AdapterArgs& a) {
   const auto whole = [](size_t v) { return (v + 255) / 256 * 256; };
   AdapterBytes b{whole(size_t(a.splits) * a.T * a.r * 4), 0, 0};
-  if (!adapter_rows_alone(a.T)) b.order = whole(size_t(a.T) * 4), b.tiles = whole((size_t(a.most_tiles) + 1) * 16);
+  if (!adapter_rows_alone(a)) b.order = whole(size_t(a.T) * 4), b.tiles = whole((size_t(a.most_tiles) + 1) * 16);
   return b;
 }
 hipError_t launch_adapters(const AdapterArgs& a, hipStream_t stream);

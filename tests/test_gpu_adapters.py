@@ -6,12 +6,15 @@ from tests import layer_case
 
 pytestmark = pytest.mark.gpu
 
-# rows, K, N, rank, adapters: one of everything, both sides of what is done row by row and in tiles of 16 and of 64 rows, every
-# number of rank blocks and steps, k that ends inside a step, columns that end inside a unit
+# rows, K, N, rank, adapters: one of everything, what is done row by row, in tiles of 16 and of 64 rows with every number of rank
+# blocks and steps, k that ends inside a step, columns that end inside a unit, one row to a tile
 SHAPES = [(1, 8, 8, 8, 1), (1, 4096, 1024, 16, 3), (3, 136, 72, 24, 2), (16, 2048, 520, 64, 5), (33, 1000, 4096, 128, 48), (64, 72, 200, 40, 1000),
-          (128, 512, 64, 8, 4), (192, 264, 72, 16, 4), (193, 8, 8, 8, 1), (193, 520, 136, 16, 7), (200, 1344, 1472, 24, 3), (333, 64, 264, 72, 60), (1000, 2048, 328, 64, 2),
-          (777, 4104, 64, 128, 1000), (4095, 128, 512, 32, 5), (4096, 264, 72, 8, 3), (5001, 200, 1032, 48, 9), (4500, 1032, 128, 128, 100),
-          (9000, 72, 2048, 56, 2)]
+          (333, 64, 264, 72, 60), (4096, 264, 72, 8, 3),
+          (700, 8192, 4104, 24, 3), (1150, 4104, 4096, 8, 70), (610, 4096, 2056, 40, 7), (400, 4104, 2120, 128, 5), (1500, 4096, 4096, 16, 1000),
+          (1000, 2048, 8200, 64, 2), (5001, 200, 1032, 48, 9), (4500, 1032, 136, 128, 100), (9000, 72, 2048, 56, 2), (4097, 8, 8, 8, 1),
+          (6000, 136, 72, 16, 500), (4200, 520, 136, 32, 3)]
+# (rows, K, N) at rank 16 of a few adapters: row by row, tiles of 16, tiles of 64
+WAYS = [(7, 264, 136), (900, 2048, 4096), (4200, 264, 136)]
 
 
 @pytest.fixture(scope="module")
@@ -51,18 +54,18 @@ def test_adapters(ops, T, K, N, r, n, order):
     assert ops.add_adapters(y, x, ops.Adapters(*a), ids, out=y) is y and torch.equal(y, got)
 
 
-@pytest.mark.parametrize("T", [1, 40, 192, 193, 300, 5000])
-def test_no_row_one_row_and_all_rows_have_an_adapter(ops, T):
-    y, x, a, ids = make(T, 264, 136, 16, 6, seed=1)
+@pytest.mark.parametrize("T,K,N", WAYS + [(1, 264, 136)])
+def test_no_row_one_row_and_all_rows_have_an_adapter(ops, T, K, N):
+    y, x, a, ids = make(T, K, N, 16, 6, seed=1)
     for which in (torch.full_like(ids, -1), torch.full_like(ids, -2 ** 31), torch.full_like(ids, 5),
                   torch.where(torch.arange(T, device="cuda") == T // 2, 3, -7).int()):
         compare(ops, y, x, a, which, ops.add_adapters(y, x, ops.Adapters(*a), which), "T=%d" % T)
 
 
-@pytest.mark.parametrize("T", [5, 192, 193, 700, 4200])
-def test_adapters_that_are_not_there(ops, T):
+@pytest.mark.parametrize("T,K,N", WAYS)
+def test_adapters_that_are_not_there(ops, T, K, N):
     """Their rows become NaN, and nobody else's."""
-    y, x, a, ids = make(T, 136, 200, 24, 4, seed=2)
+    y, x, a, ids = make(T, K, N, 16, 4, seed=2)
     bad = torch.arange(T, device="cuda") % 3 == 1
     wrong = torch.where(bad, torch.where(torch.arange(T, device="cuda") % 2 == 0, 4, 2 ** 31 - 1).int(), ids)
     got = ops.add_adapters(y, x, ops.Adapters(*a), wrong)
@@ -70,10 +73,10 @@ def test_adapters_that_are_not_there(ops, T):
     assert torch.equal(got[~bad], ops.add_adapters(y, x, ops.Adapters(*a), ids)[~bad])
 
 
-@pytest.mark.parametrize("T", [7, 250, 4100])
-def test_rows_that_are_not_finite(ops, T):
+@pytest.mark.parametrize("T,K,N", WAYS)
+def test_rows_that_are_not_finite(ops, T, K, N):
     """A row's infinities and NaN stay its own, whoever shares its tile; so do an adapter's."""
-    y, x, a, ids = make(T, 136, 200, 16, 3, "runs", seed=3)
+    y, x, a, ids = make(T, K, N, 16, 3, "runs", seed=3)
     want = ops.add_adapters(y, x, ops.Adapters(*a), ids)
     bad = x.clone()
     bad[T // 2, 5], bad[T - 1, 9] = float("nan"), float("inf")
@@ -87,32 +90,32 @@ def test_rows_that_are_not_finite(ops, T):
     assert torch.equal(got[ids != 2], want[ids != 2])
 
 
-@pytest.mark.parametrize("T", [12, 260])
-def test_ways_to_hand_rows_over(ops, T):
-    y, x, a, ids = make(T, 264, 136, 16, 6, seed=4)
+@pytest.mark.parametrize("T,K,N", [(12, 264, 136)] + WAYS[1:])
+def test_ways_to_hand_rows_over(ops, T, K, N):
+    y, x, a, ids = make(T, K, N, 16, 6, seed=4)
     want = ops.add_adapters(y, x, ops.Adapters(*a), ids)
-    wide = torch.zeros(T, 264 + 136 + 16, dtype=torch.bfloat16, device="cuda")
-    wide[:, :264], wide[:, 264:400] = x, y
-    got = ops.add_adapters(wide[:, 264:400], wide[:, :264], ops.Adapters(*a), ids)
+    wide = torch.zeros(T, K + N + 16, dtype=torch.bfloat16, device="cuda")
+    wide[:, :K], wide[:, K:K + N] = x, y
+    got = ops.add_adapters(wide[:, K:K + N], wide[:, :K], ops.Adapters(*a), ids)
     assert torch.equal(got, want)
-    out = wide[:, 264:400]
-    assert torch.equal(ops.add_adapters(y, x, ops.Adapters(*a), ids, out=out), want) and not wide[:, 400:].any() and torch.equal(wide[:, :264], x)
-    wide[:, 264:400] = y
-    ops.add_adapters(out, wide[:, :264], ops.Adapters(*a), ids, out=out)
-    assert torch.equal(wide[:, 264:400], want) and not wide[:, 400:].any() and torch.equal(wide[:, :264], x)
-    odd = torch.zeros(T, 267, dtype=torch.bfloat16, device="cuda")
+    out = wide[:, K:K + N]
+    assert torch.equal(ops.add_adapters(y, x, ops.Adapters(*a), ids, out=out), want) and not wide[:, K + N:].any() and torch.equal(wide[:, :K], x)
+    wide[:, K:K + N] = y
+    ops.add_adapters(out, wide[:, :K], ops.Adapters(*a), ids, out=out)
+    assert torch.equal(wide[:, K:K + N], want) and not wide[:, K + N:].any() and torch.equal(wide[:, :K], x)
+    odd = torch.zeros(T, K + 3, dtype=torch.bfloat16, device="cuda")
     odd[:, 3:] = x
     assert torch.equal(ops.add_adapters(y, odd[:, 3:], ops.Adapters(*a), ids), want)
     twice = torch.stack((ids, ids), 1)[:, 0]
-    cube = ops.add_adapters(y.view(2, -1, 136), x.view(2, -1, 264), ops.Adapters(*a), twice.view(2, -1))
-    assert torch.equal(cube.view(T, 136), want)
+    cube = ops.add_adapters(y.view(2, -1, N), x.view(2, -1, K), ops.Adapters(*a), twice.view(2, -1))
+    assert torch.equal(cube.view(T, N), want)
     # columns side by side of one buffer with more dimensions, and columns that overlap
-    both = torch.zeros(2, T // 2, 264 + 136, dtype=torch.bfloat16, device="cuda")
-    both[..., :264], both[..., 264:] = x.view(2, -1, 264), y.view(2, -1, 136)
-    ops.add_adapters(both[..., 264:], both[..., :264], ops.Adapters(*a), ids.view(2, -1), out=both[..., 264:])
-    assert torch.equal(both[..., 264:].reshape(T, 136), want) and torch.equal(both[..., :264].reshape(T, 264), x)
+    both = torch.zeros(2, T // 2, K + N, dtype=torch.bfloat16, device="cuda")
+    both[..., :K], both[..., K:] = x.view(2, -1, K), y.view(2, -1, N)
+    ops.add_adapters(both[..., K:], both[..., :K], ops.Adapters(*a), ids.view(2, -1), out=both[..., K:])
+    assert torch.equal(both[..., K:].reshape(T, N), want) and torch.equal(both[..., :K].reshape(T, K), x)
     with pytest.raises(RuntimeError, match="apart from x"):
-        ops.add_adapters(y.view(2, -1, 136), both[..., :264], ops.Adapters(*a), ids.view(2, -1), out=both[..., 256:392])
+        ops.add_adapters(y.view(2, -1, N), both[..., :K], ops.Adapters(*a), ids.view(2, -1), out=both[..., K - 8:K - 8 + N])
     one = ops.add_adapters(y[1], x[1], ops.Adapters(*a), ids[1])
     layer_case.check(one[None], *(v[1:2] for v in layer_case.adapters(y, x, *a, ids)), "one row")
 
@@ -156,9 +159,9 @@ def test_beside_a_projection_in_4_bits(ops, T):
             bad()
 
 
-@pytest.mark.parametrize("T", [24, 500, 4200])
-def test_captured(ops, T):
-    y, x, a, ids = make(T, 264, 520, 16, 6, seed=7)
+@pytest.mark.parametrize("T,K,N", WAYS)
+def test_captured(ops, T, K, N):
+    y, x, a, ids = make(T, K, N, 16, 6, seed=7)
     ad = ops.Adapters(*a)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -169,7 +172,7 @@ def test_captured(ops, T):
     with torch.cuda.graph(graph):
         got = ops.add_adapters(y, x, ad, ids)
     for rep in range(4):
-        fresh = make(T, 264, 520, 16, 6, order=("any", "runs")[rep % 2], seed=20 + rep)
+        fresh = make(T, K, N, 16, 6, order=("any", "runs")[rep % 2], seed=20 + rep)
         y.copy_(fresh[0]), x.copy_(fresh[1]), ids.copy_(fresh[3])
         graph.replay()
         torch.cuda.synchronize()
@@ -177,7 +180,7 @@ def test_captured(ops, T):
 
 
 def test_two_streams_at_once(ops):
-    cases = [make(600, 264, 520, 24, 6, seed=30 + i) for i in range(2)]
+    cases = [make(4300 if i else 900, 2048, 4096, 24, 6, seed=30 + i) for i in range(2)]
     want = [ops.add_adapters(y, x, ops.Adapters(*a), ids) for y, x, a, ids in cases]
     torch.cuda.synchronize()
     got = []

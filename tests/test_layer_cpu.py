@@ -268,11 +268,14 @@ def test_adapters_refuse(kw, capfd):
 def test_adapter_workspace():
     assert adapter_size(0) == (0, 0) and add(rows=0, x=None, y=None, out=None, ids=None, work=None) == 0
     assert 5 * 16 * 4 <= adapter_size(5)[1] < 5 * 16 * 4 + 256
-    for rows in (193, 4095, 4096, 100000, 1 << 26):
-        rc, size = adapter_size(rows, adapters=1000)
-        tiles = -(-rows // (64 if rows >= 4096 else 16)) + min(rows, 1002)
+    # row by row: u alone
+    assert 700 * 16 * 4 <= adapter_size(700, n=2048, k=4096)[1] < 700 * 16 * 4 + 256
+    for rows, adapters in ((900, 4), (900, 1000), (2000, 4), (4097, 1000), (100000, 1000), (1 << 26, 1000)):
+        rc, size = adapter_size(rows, adapters=adapters, n=2048, k=4096)
+        tall = rows >= 1195 and rows >= 12 * adapters
+        tiles = -(-rows // (64 if tall else 16)) + min(rows, adapters + 2)
         # u at least once, the order of the rows, and 16 bytes a tile and one more
-        assert rc == 0 and size >= rows * 16 * 4 + rows * 4 + (tiles + 1) * 16
+        assert rc == 0 and rows * 16 * 4 + rows * 4 + (tiles + 1) * 16 <= size < rows * 16 * 4 * 8 + rows * 4 + (tiles + 1) * 16 + 1024
 
 
 @pytest.mark.parametrize("call,message", [
