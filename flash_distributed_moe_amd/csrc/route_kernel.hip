@@ -86,11 +86,8 @@ __device__ __forceinline__ unsigned ordered(float v) {
 }
 
 // e^x of x <= 0 with the hardware's 2^t: off by |x| 2^-24 for the product's rounding, a fifth of that for the constant's, and
-// 2^-23. Below e^-104 the result is zero, of -inf and of NaN too (a token with an infinity has a sum of zero then, and weights that
-// are NaN). The library's function takes three times as many instructions, and a token has E of these.
-__device__ __forceinline__ float exp_down(float x) {
-  return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(x, -150.0f, 0.0f) * 1.44269504f);
-}
+// 2^-23; results below 2^-126 are zeros. The library's function takes three times as many instructions, and a token has E of these.
+__device__ __forceinline__ float exp_down(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // Value i of a lane if it is a candidate, else -inf.
 template <bool BF, int V>
@@ -243,8 +240,9 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
     const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
     float v[V], e[V], s = 0.0f;
     candidates(now, open, v);
-    const float m = row16_max(lane_max(v));
+    float m = row16_max(lane_max(v));
     const bool some = m > -INFINITY;
+    m = some ? m : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) e[i] = exp_down(v[i] - m), s += e[i];
     s = row16_sum(s);
@@ -379,8 +377,9 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
     const int e0 = open ? one.expert : -1, e1 = open ? two.expert : -1;
     float v[V], p[V], s = 0.0f;
     candidates(now, open, v);
-    const float m = row16_max(lane_max(v));
+    float m = row16_max(lane_max(v));
     const bool some = m > -INFINITY;
+    m = some ? m : 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) p[i] = exp_down(v[i] - m), s += p[i];
     s = row16_sum(s);
