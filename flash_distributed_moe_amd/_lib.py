@@ -123,7 +123,7 @@ C_ABI = {
     "flashMoeRoute": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                      ctypes.c_int] + [ctypes.c_void_p] * 8),
     "flashMoeRouteBackward": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
-                                             ctypes.c_int] + [ctypes.c_void_p] * 8 + [ctypes.c_longlong, ctypes.c_void_p]),
+                                             ctypes.c_int] + [ctypes.c_void_p] * 7 + [ctypes.c_longlong, ctypes.c_void_p]),
     "flashMoeBlockNorm": (ctypes.c_int, [ctypes.POINTER(NormDesc)] + [ctypes.c_void_p, ctypes.c_longlong] * 2 + [ctypes.c_int] +
                           [ctypes.c_void_p] * 4),
     "flashMoeBlockNormBytes": (ctypes.c_int, [ctypes.POINTER(NormDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),

@@ -152,11 +152,11 @@ int flashMoeRouteBytes(const FlashMoeRouteDesc* desc, int tokens, size_t* bytes)
 }
 
 int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
-                  float* weights, int* experts, int* counts, int* totals, float* balance, float* zed, void* workspace,
+                  float* weights, int* experts, int* counts, float* balance, float* zed, int* kept, void* workspace,
                   void* stream) {
   FMOE_HIP_CHECK(validate(desc, tokens));
   FMOE_HIP_CHECK(check_word("counts", counts));
-  if (!on(totals, 4)) FMOE_FAIL(hipErrorInvalidValue, "totals does not begin on 4 bytes");
+  if (!on(kept, 4)) FMOE_FAIL(hipErrorInvalidValue, "kept does not begin on 4 bytes");
   FMOE_HIP_CHECK(check_word("balance", balance));
   FMOE_HIP_CHECK(check_word("zed", zed));
   if (tokens > 0) {
@@ -166,15 +166,15 @@ int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long l
     if (fmoe::route_grid(tokens).blocks > 1) FMOE_HIP_CHECK(check_word("workspace", workspace));
   }
   fmoe::RouteArgs a = route_args(desc, logits, ld, mask, tokens);
-  a.weights = weights, a.experts = experts, a.counts = counts, a.totals = totals, a.balance = balance, a.zed = zed;
+  a.weights = weights, a.experts = experts, a.counts = counts, a.kept = kept, a.balance = balance, a.zed = zed;
   a.partial = static_cast<float*>(workspace);
   FMOE_HIP_CHECK(fmoe::launch_route(a, desc->dtype, static_cast<hipStream_t>(stream)));
   return hipSuccess;
 }
 
 int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
-                          const float* weights, const int* experts, const int* counts, const int* totals,
-                          const float* dweights, const float* dbalance, const float* dzed, void* dlogits, long long ldd,
+                          const float* weights, const int* experts, const int* kept, const float* dweights,
+                          const float* dbalance, const float* dzed, void* dlogits, long long ldd,
                           void* stream) {
   FMOE_HIP_CHECK(validate(desc, tokens));
   if (tokens == 0) return hipSuccess;
@@ -182,12 +182,11 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
   FMOE_HIP_CHECK(check_logits("dlogits", dlogits, ldd, desc));
   FMOE_HIP_CHECK(check_word("weights", weights));
   FMOE_HIP_CHECK(check_word("experts", experts));
-  FMOE_HIP_CHECK(check_word("counts", counts));
-  FMOE_HIP_CHECK(check_word("totals", totals));
+  FMOE_HIP_CHECK(check_word("kept", kept));
   for (const void* p : {static_cast<const void*>(dweights), static_cast<const void*>(dbalance), static_cast<const void*>(dzed)})
     if (!on(p, 4)) FMOE_FAIL(hipErrorInvalidValue, "a gradient does not begin on 4 bytes");
   fmoe::RouteArgs a = route_args(desc, logits, ld, mask, tokens);
-  a.weights = const_cast<float*>(weights), a.experts = const_cast<int*>(experts), a.counts = const_cast<int*>(counts), a.totals = const_cast<int*>(totals);
+  a.weights = const_cast<float*>(weights), a.experts = const_cast<int*>(experts), a.kept = const_cast<int*>(kept);
   a.dweights = dweights, a.dbalance = dbalance, a.dzed = dzed, a.dlogits = dlogits, a.ldd = ldd;
   FMOE_HIP_CHECK(fmoe::launch_route_backward(a, desc->dtype, static_cast<hipStream_t>(stream)));
   return hipSuccess;

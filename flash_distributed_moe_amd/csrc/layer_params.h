@@ -15,7 +15,7 @@ struct RouteArgs {
   float* weights;   // [T, k]; read by the backward pass
   int* experts;     // [T, k]
   int* counts;      // [E]
-  int* totals;      // [2]: rows with a candidate, slots filled; NULL: not wanted
+  int* kept;        // [2 + E], for the backward pass: rows with a candidate, slots filled, the counts once more; NULL: not wanted
   float* balance;   // [1]
   float* zed;       // [1]
   float* partial;   // of more than one workgroup: [blocks, kRouteColumns] sums of probabilities, then as many counts

@@ -56,7 +56,7 @@ FlashMoeRouteDesc describe(const at::Tensor& logits, int64_t top_k, bool renorma
 }
 
 struct Routed {
-  at::Tensor weights, experts, counts, balance, zed, totals, mask;
+  at::Tensor weights, experts, counts, balance, zed, kept, mask;
 };
 Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask, bool keep) {
   refuse_tangent(logits, "logits");
@@ -69,7 +69,7 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
   sizes.back() = top_k;
   r.weights = fresh(sizes, at::kFloat, logits), r.experts = fresh(sizes, at::kInt, logits);
   r.counts = fresh({d.experts}, at::kInt, logits);
-  if (keep) r.totals = fresh({2}, at::kInt, logits);
+  if (keep) r.kept = fresh({2 + d.experts}, at::kInt, logits);
   r.balance = fresh({}, at::kFloat, logits), r.zed = fresh({}, at::kFloat, logits);
   size_t bytes = 0;
   check_hip(flashMoeRouteBytes(&d, rows.count, &bytes), "flashMoeRouteBytes");
@@ -77,7 +77,7 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
   if (bytes > 0) work = fresh_bytes(bytes, logits);
   check_hip(flashMoeRoute(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(r.mask)), rows.count,
                           static_cast<float*>(pointer(r.weights)), static_cast<int*>(pointer(r.experts)), r.counts.data_ptr<int>(),
-                          static_cast<int*>(pointer(r.totals)), r.balance.data_ptr<float>(), r.zed.data_ptr<float>(), pointer(work),
+                          r.balance.data_ptr<float>(), r.zed.data_ptr<float>(), static_cast<int*>(pointer(r.kept)), pointer(work),
                           current_stream()),
             "flashMoeRoute");
   return r;
@@ -86,7 +86,8 @@ Routed route_forward(const at::Tensor& logits, int64_t top_k, bool renormalize, 
 struct Route : torch::autograd::Function<Route> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask) {
     const Routed r = route_forward(logits, top_k, renormalize, mask, true);
-    ctx->save_for_backward({logits, r.mask, r.experts, r.counts, r.totals, r.weights});
+    // the counts are kept apart: a caller may well add those of other ranks to what is returned
+    ctx->save_for_backward({logits, r.mask, r.experts, r.kept, r.weights});
     ctx->saved_data["top_k"] = top_k;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->mark_non_differentiable({r.experts, r.counts});
@@ -104,8 +105,8 @@ struct Route : torch::autograd::Function<Route> {
     at::Tensor out = fresh(logits);
     const auto floats = [](const at::Tensor& t) { return static_cast<const float*>(pointer(t)); };
     check_hip(flashMoeRouteBackward(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(mask)), rows.count,
-                                    floats(kept[5]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), kept[4].data_ptr<int>(), floats(dw),
-                                    floats(grads[3]), floats(grads[4]), pointer(out), d.experts, current_stream()),
+                                    floats(kept[4]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), floats(dw), floats(grads[3]),
+                                    floats(grads[4]), pointer(out), d.experts, current_stream()),
               "flashMoeRouteBackward");
     return {out, at::Tensor(), at::Tensor(), at::Tensor()};
   }

@@ -197,6 +197,7 @@ struct Totals {
 __device__ __forceinline__ void finish(const RouteArgs& a, int count, double probs, double squares, int rows, Totals* room) {
   const bool mine = static_cast<int>(threadIdx.x) < a.E;
   if (mine) a.counts[threadIdx.x] = count;
+  if (mine && a.kept != nullptr) a.kept[2 + threadIdx.x] = count;
   const Totals wave{wave_sum(mine ? count * probs : 0.0), wave_sum(squares), wave_sum(mine ? count : 0), wave_sum(rows)};
   if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = wave;
   __syncthreads();
@@ -204,7 +205,7 @@ __device__ __forceinline__ void finish(const RouteArgs& a, int count, double pro
   Totals t{};
   for (unsigned i = 0; i < blockDim.x / 64; ++i)
     t.both += room[i].both, t.squares += room[i].squares, t.slots += room[i].slots, t.rows += room[i].rows;
-  if (a.totals != nullptr) a.totals[0] = t.rows, a.totals[1] = t.slots;
+  if (a.kept != nullptr) a.kept[0] = t.rows, a.kept[1] = t.slots;
   *a.balance = static_cast<float>(t.slots > 0 ? a.E * t.both / (static_cast<double>(t.slots) * t.rows) : t.both);
   *a.zed = static_cast<float>(t.rows > 0 ? t.squares / t.rows : t.squares);
 }
@@ -344,14 +345,14 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
   __shared__ __align__(16) float add[16][kRouteExperts];
   const int lane = threadIdx.x & 15;
   float* mine = add[threadIdx.x >> 4];
-  const int n = a.totals[0], slots = a.totals[1];
+  const int n = a.kept[0], slots = a.kept[1];
   const float toward = a.dbalance != nullptr && slots > 0 ? *a.dbalance * a.E / (static_cast<float>(slots) * n) : 0.0f;
   const float pull = a.dzed != nullptr && n > 0 ? 2.0f * *a.dzed / n : 0.0f;
   float g[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = column(lane, i);
-    g[i] = c < a.E ? toward * a.counts[c] : 0.0f;
+    g[i] = c < a.E ? toward * a.kept[2 + c] : 0.0f;
     mine[c] = 0.0f;
   }
   const long long step = static_cast<long long>(gridDim.x) * 16;

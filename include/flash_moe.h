@@ -353,19 +353,18 @@ typedef struct FlashMoeRouteDesc {
  * logits [tokens, E] rows ld values apart (any alignment; E and ld multiples of 4 are faster); mask [tokens] bytes or NULL: a token
  * with 0 is padding and has no candidates. weights [tokens, k]: p of the winners (renormalised on request); experts
  * [tokens, k]; slots that no candidate is left for get expert -1 and weight 0. counts [E]: slots that each expert
- * won. totals [2] or NULL (the backward pass wants it): rows n with a candidate, and slots won. balance [1]: E sum_e counts_e / slots * sum_t p_te / n (1 if even; 0
+ * won. kept [2 + E] or NULL: for the backward pass, rows n with a candidate, slots won and the counts again. balance [1]: E sum_e counts_e / slots * sum_t p_te / n (1 if even; 0
  * without slots). zed [1]: the mean over the n rows of the squared logarithm of the sum of exp(logits).
  * workspace: flashMoeRouteBytes of device memory (0: may be NULL). 0 tokens: zeros. tokens * k is at most 2^30. */
 int flashMoeRouteBytes(const FlashMoeRouteDesc* desc, int tokens, size_t* bytes);
 int flashMoeRoute(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
-                  float* weights, int* experts, int* counts, int* totals, float* balance, float* zed, void* workspace,
+                  float* weights, int* experts, int* counts, float* balance, float* zed, int* kept, void* workspace,
                   void* stream);
 /* The gradient of the logits (written, not added to) from those of the weights [tokens, k], of balance [1] and of zed
- * [1]; each may be NULL. The choice and the counts are constants. weights, experts, counts and totals are flashMoeRoute's. */
+ * [1]; each may be NULL. The choice and the counts are constants. weights, experts and kept are flashMoeRoute's. */
 int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, long long ld, const unsigned char* mask, int tokens,
-                          const float* weights, const int* experts, const int* counts, const int* totals,
-                          const float* dweights, const float* dbalance, const float* dzed, void* dlogits, long long ldd,
-                          void* stream);
+                          const float* weights, const int* experts, const int* kept, const float* dweights,
+                          const float* dbalance, const float* dzed, void* dlogits, long long ldd, void* stream);
 
 /* The norms around a block, fused with what joins it to the residual stream, on rows of H values:
  *   z = post_weight * branch / rms(branch), or the branch as it is without post_weight;

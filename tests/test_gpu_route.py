@@ -182,6 +182,16 @@ def test_equal_calls_give_equal_bits(ops):
             assert torch.equal(a, b)
 
 
+def test_counts_of_other_ranks_may_be_added(ops):
+    """What is done to the returned counts does not reach the gradient."""
+    logits, gen = make(300, 40, torch.float32, seed=11)
+    leaf = logits.requires_grad_()
+    got, want = ops.route(leaf, 4), ops.route(leaf, 4)
+    got.counts.data.mul_(7)
+    a, b = (torch.autograd.grad(r.balance_loss, leaf)[0] for r in (got, want))
+    assert torch.equal(a, b)
+
+
 def test_second_derivatives_are_refused(ops):
     logits, _ = make(8, 16, torch.float32)
     leaf = logits.requires_grad_()

@@ -31,15 +31,15 @@ def route_desc(**kw):
     return d
 
 
-def route(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, experts=0x3000, counts=0x4000, totals=0x5000, balance=0x6000,
-          zed=0x7000, work=0x8000):
-    return _lib.load().flashMoeRoute(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, weights, experts, counts, totals, balance, zed,
+def route(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, experts=0x3000, counts=0x4000, balance=0x5000, zed=0x6000,
+          kept=0x7000, work=0x8000):
+    return _lib.load().flashMoeRoute(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, weights, experts, counts, balance, zed, kept,
                                      work, None)
 
 
-def route_backward(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, experts=0x3000, counts=0x4000, totals=0x5000, dw=0x6000, db=0x7000,
+def route_backward(d=None, logits=0x1000, ld=16, mask=None, tokens=100, weights=0x2000, experts=0x3000, kept=0x4000, dw=0x6000, db=0x7000,
                    dz=0x8000, out=0x9000, ldd=16):
-    return _lib.load().flashMoeRouteBackward(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, weights, experts, counts, totals, dw, db, dz, out,
+    return _lib.load().flashMoeRouteBackward(ctypes.byref(d or route_desc()), logits, ld, mask, tokens, weights, experts, kept, dw, db, dz, out,
                                              ldd, None)
 
 
@@ -53,15 +53,15 @@ def test_bad_routers(kw, capfd):
 
 
 @pytest.mark.parametrize("kw", [dict(logits=None), dict(logits=0x1002), dict(ld=15), dict(ld=(1 << 20) + 1), dict(tokens=-1), dict(tokens=(1 << 28) + 1),
-                                dict(weights=None), dict(experts=None), dict(counts=None), dict(totals=0x5002), dict(balance=None), dict(zed=None),
+                                dict(weights=None), dict(experts=None), dict(counts=None), dict(kept=0x5002), dict(balance=None), dict(zed=None),
                                 dict(work=None), dict(work=0x8001)])
 def test_route_refuses(kw, capfd):
     assert route(**kw) == BAD
     assert "[MOE ERROR:" in capfd.readouterr().out
 
 
-@pytest.mark.parametrize("kw", [dict(logits=None), dict(ld=3), dict(out=None), dict(out=0x9001), dict(ldd=15), dict(weights=None), dict(experts=None), dict(counts=None),
-                                dict(totals=None), dict(dw=0x6001), dict(dz=0x8002), dict(tokens=-1)])
+@pytest.mark.parametrize("kw", [dict(logits=None), dict(ld=3), dict(out=None), dict(out=0x9001), dict(ldd=15), dict(weights=None), dict(experts=None), dict(kept=None),
+                                dict(kept=0x4002), dict(dw=0x6001), dict(dz=0x8002), dict(tokens=-1)])
 def test_route_backward_refuses(kw, capfd):
     assert route_backward(**kw) == BAD
     assert "[MOE ERROR:" in capfd.readouterr().out
