@@ -74,8 +74,8 @@ def test_route_workspace():
         return n.value
 
     assert size(0) == size(1) == size(64) == 0
-    for tokens in (65, 100, 4096, 16384, 16385, 1 << 28):
-        rows = 16 if tokens <= 16384 else 64
+    for tokens in (65, 100, 4096, 6000, 6001, 1 << 28):
+        rows = 16 if tokens <= 6000 else 64
         assert size(tokens) == min(256, -(-tokens // rows)) * 2 * 257 * 4
     assert _lib.load().flashMoeRouteBytes(ctypes.byref(route_desc()), 1, None) == BAD
     assert route_backward(tokens=0, logits=None, out=None) == 0
