@@ -373,7 +373,9 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs a) {
     const Raw<BF, V> now = next;
     if (first + step < a.T) next = load_row<BF, V, WHOLE>(a.logits, place(row + step) * a.ld, lane, a.E);
     const bool open = row < a.T && (a.mask == nullptr || a.mask[row] != 0);
-    const Slot one = coming, two = coming2;
+    // a slot that nobody won has a constant weight, whatever its gradient is said to be
+    const auto won = [&](const Slot& s) { return static_cast<unsigned>(s.expert) < static_cast<unsigned>(a.E) ? s : Slot{-1, 0.0f, 0.0f}; };
+    const Slot one = won(coming), two = won(coming2);
     if (first + step < a.T) coming = slot_at(place(row + step), lane), coming2 = slot_at(place(row + step), lane + 16);
     const int e0 = open ? one.expert : -1, e1 = open ? two.expert : -1;
     float v[V], p[V], s = 0.0f;

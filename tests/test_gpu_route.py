@@ -166,6 +166,27 @@ def test_one_gradient_alone(ops, only):
     compare(ops, logits, 5, dw=wide[:, ::2], what="strided gradient")
 
 
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_gradients_of_slots_without_a_winner_are_not_read(ops, dtype, renormalize):
+    """Such a slot's weight is a constant, whatever arrives for it."""
+    E, k = 20, 18
+    logits, gen = make(40, E, DTYPES[dtype], seed=12)
+    logits[::2, 10:] = float("-inf")  # slots from the tenth on have no winner
+    logits[::8] = float("-inf")
+    mask = torch.arange(40, device="cuda") % 5 != 0
+    won = ops.route(logits, k, mask=mask).experts >= 0
+    dw = torch.empty(40, k, device="cuda").normal_(generator=gen)
+    grads = []
+    for fill in (0.0, float("nan"), float("inf")):
+        leaf = logits.clone().requires_grad_()
+        got = ops.route(leaf, k, renormalize=renormalize, mask=mask)
+        grads += torch.autograd.grad(got.weights, leaf, torch.where(won, dw, fill))
+    assert torch.isfinite(grads[0]).all() and grads[0].any()
+    for g in grads[1:]:
+        assert torch.equal(g, grads[0])
+
+
 def test_no_tokens(ops):
     leaf = torch.empty(0, 32, device="cuda", requires_grad=True)
     got = ops.route(leaf, 4)
