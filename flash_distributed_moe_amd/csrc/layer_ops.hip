@@ -102,10 +102,12 @@ hipError_t check_rows(const char* name, const void* p, long long ld, const Flash
   return hipSuccess;
 }
 
-fmoe::NormArgs norm_args(const FlashMoeNormDesc* d, int tokens) {
+fmoe::NormArgs norm_args(const FlashMoeNormDesc* d, int tokens, bool branch) {
   fmoe::NormArgs a{};
   a.T = tokens, a.H = d->hidden, a.gate_kind = d->gate, a.shared = d->shared;
-  a.alpha = static_cast<float>(d->residual_scale), a.beta = static_cast<float>(d->branch_scale), a.eps = static_cast<float>(d->eps);
+  // without a branch y = x, whatever the scales are
+  a.alpha = branch ? static_cast<float>(d->residual_scale) : 1.0f, a.beta = static_cast<float>(d->branch_scale);
+  a.eps = static_cast<float>(d->eps);
   a.post = d->post_weight, a.gate = d->gate_values, a.next = d->next_weight;
   return a;
 }
@@ -196,7 +198,7 @@ int flashMoeBlockNormBytes(const FlashMoeNormDesc* desc, int tokens, size_t* byt
   if (bytes == nullptr) FMOE_FAIL(hipErrorInvalidValue, "null result");
   // whether there is a branch is not known here, and of no consequence
   FMOE_HIP_CHECK(validate(desc, tokens, true));
-  fmoe::NormArgs a = norm_args(desc, tokens);
+  fmoe::NormArgs a = norm_args(desc, tokens, true);
   fmoe::plan_norm_backward(a);
   *bytes = partial_bytes(a);
   return hipSuccess;
@@ -215,7 +217,7 @@ int flashMoeBlockNorm(const FlashMoeNormDesc* desc, const void* x, long long ldx
   }
   if (desc->next_weight != nullptr) FMOE_HIP_CHECK(check_rows("h", h, desc->hidden, desc));
   if (!on(kept, 4)) FMOE_FAIL(hipErrorInvalidValue, "kept does not begin on 4 bytes");
-  fmoe::NormArgs a = norm_args(desc, tokens);
+  fmoe::NormArgs a = norm_args(desc, tokens, branch != nullptr);
   a.x = x, a.ldx = ldx, a.branch = branch, a.ldb = ldb, a.y = y, a.h = h;
   if (kept != nullptr) a.branch_rms = kept, a.y_rms = kept + tokens;
   FMOE_HIP_CHECK(fmoe::launch_norm(a, desc->dtype, static_cast<hipStream_t>(stream)));
@@ -244,7 +246,7 @@ int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long 
                        (dgate != nullptr && (desc->gate == FLASH_MOE_GATE_CHANNEL || desc->gate == FLASH_MOE_GATE_GROUP));
   if (columns) FMOE_HIP_CHECK(check_word("workspace", workspace));
   if (!columns && tokens == 0) return hipSuccess;
-  fmoe::NormArgs a = norm_args(desc, tokens);
+  fmoe::NormArgs a = norm_args(desc, tokens, branch != nullptr);
   a.x = x, a.ldx = ldx, a.branch = branch, a.ldb = ldb, a.dy = dy, a.lddy = lddy, a.dh = dh, a.lddh = lddh;
   if (tokens > 0) a.branch_rms = const_cast<float*>(kept), a.y_rms = a.branch_rms + tokens;
   a.dx = dx, a.dbranch = dbranch, a.dpost = dpost, a.dgate = dgate, a.dnext = dnext;

@@ -369,8 +369,8 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
 /* The norms around a block, fused with what joins it to the residual stream, on rows of H values:
  *   z = post_weight * branch / rms(branch), or the branch as it is without post_weight;
  *   y = residual_scale * x + branch_scale * gate * z;  h = next_weight * y / rms(y), with next_weight;
- * rms(v) = sqrt(mean v^2 + eps). Without a branch y = x, and h is the norm in front of a block alone. What is computed of one
- * row is float32, rounded once into y and once into h. */
+ * rms(v) = sqrt(mean v^2 + eps). Without a branch y = x, whatever the scales are, and h is the norm in front of a block alone. What
+ * is computed of one row is float32, rounded once into y and once into h. */
 enum {
   FLASH_MOE_GATE_NONE = 0,
   FLASH_MOE_GATE_CHANNEL = 1, /* [H] */
