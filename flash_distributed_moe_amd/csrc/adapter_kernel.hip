@@ -261,6 +261,7 @@ __global__ __launch_bounds__(kShrinkWaves * 64, TB * RB < 32 ? 2 : 1) void shrin
 // neighbouring columns of one token: row i of block f is column 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4 of a unit of 64. A wave has 16
 // tokens. KS steps of 32 ranks.
 constexpr int kUnit = 64;
+constexpr float kMostBf16 = 0x1.FEp127f;
 template <int KS>
 struct Tokens {
   const unsigned short* y[2];  // what a lane loads and stores: of tokens 0 to 7 and of 8 to 15, 16 of 128 bytes
@@ -321,7 +322,9 @@ __device__ __forceinline__ void load_u(const AdapterArgs& a, Tokens<KS>& t, int 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float f = v[i >> 2][i & 3] * scale;
-      t.big[s][i] = static_cast<__bf16>(f);
+      // a number beyond the greatest of bfloat16 would be rounded to infinity: what it is more than that is the rest's
+      const float held = fabsf(f) < INFINITY ? __builtin_amdgcn_fmed3f(f, -kMostBf16, kMostBf16) : f;
+      t.big[s][i] = static_cast<__bf16>(held);
       const float left = f - static_cast<float>(t.big[s][i]);
       t.rest[s][i] = static_cast<__bf16>(fabsf(left) < INFINITY ? left : 0.0f);  // of infinities nothing is left
     }
