@@ -32,7 +32,7 @@ at::Tensor fresh_bytes(size_t bytes, const at::Tensor& like) { return fresh({sta
 Rows logit_rows(const at::Tensor& t, const char* name) {
   const int64_t width = t.size(-1), rows = t.numel() / width;
   at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, width});
-  if (flat.numel() > 0 && (flat.stride(1) != 1 || (rows > 1 && (flat.stride(0) < width || flat.stride(0) > kMaxStride))))
+  if (flat.numel() > 0 && (flat.stride(1) != 1 || flat.is_neg() || (rows > 1 && (flat.stride(0) < width || flat.stride(0) > kMaxStride))))
     flat = flat.clone(at::MemoryFormat::Contiguous);
   return {flat, rows <= 1 ? width : flat.stride(0), int_size(rows, name)};
 }
@@ -101,12 +101,14 @@ struct Route : torch::autograd::Function<Route> {
     const FlashMoeRouteDesc d = describe(logits, ctx->saved_data["top_k"].toInt(), ctx->saved_data["renormalize"].toBool(), c10::nullopt);
     const DeviceGuard guard(logits.device());
     const Rows rows = logit_rows(logits, "logits");
-    at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
+    // as they are in memory: torch may hand a gradient over that is negated when it is read
+    const auto plain = [](const at::Tensor& t) { return !t.defined() ? t : t.is_neg() ? t.contiguous().resolve_neg() : t.contiguous(); };
+    const at::Tensor dw = plain(grads[0]), db = plain(grads[3]), dz = plain(grads[4]);
     at::Tensor out = fresh(logits);
     const auto floats = [](const at::Tensor& t) { return static_cast<const float*>(pointer(t)); };
     check_hip(flashMoeRouteBackward(&d, pointer(rows.t), rows.stride, static_cast<unsigned char*>(pointer(mask)), rows.count,
-                                    floats(kept[4]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), floats(dw), floats(grads[3]),
-                                    floats(grads[4]), pointer(out), d.experts, current_stream()),
+                                    floats(kept[4]), static_cast<int*>(pointer(kept[2])), kept[3].data_ptr<int>(), floats(dw), floats(db),
+                                    floats(dz), pointer(out), d.experts, current_stream()),
               "flashMoeRouteBackward");
     return {out, at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -185,7 +187,7 @@ NormCall prepare(const NormInputs& in, double alpha, double beta, double eps) {
     describe_gate(c.d, in.gate, in.x, c.x.count);
     if (c.x.count == 0 && c.d.gate != FLASH_MOE_GATE_CHANNEL) c.d.gate = FLASH_MOE_GATE_NONE;  // no rows to have one
     c.gate = in.gate.contiguous();
-    if (!begins_on_16(c.gate)) c.gate = c.gate.clone();
+    if (!begins_on_16(c.gate) || c.gate.is_neg()) c.gate = c.gate.clone();
     if (c.d.gate != FLASH_MOE_GATE_NONE) c.d.gate_values = c.gate.data_ptr();
   }
   c.d.post_weight = pointer(in.post), c.d.next_weight = pointer(in.next);
@@ -301,6 +303,7 @@ at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tens
   for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{y, "y"}, {x, "x"}, {down, "down"}, {up, "up"}})
     TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16");
   TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous(), "scales must be float32 without gaps");
+  TORCH_CHECK(!scales.is_neg(), "scales must not be a negated view");
   TORCH_CHECK(ids.scalar_type() == at::kInt, "ids must be int32");
   TORCH_CHECK(down.dim() == 3 && up.dim() == 3 && scales.dim() == 1 && down.size(0) == up.size(0) && down.size(0) == scales.size(0) &&
                   down.size(1) == up.size(2),

@@ -54,13 +54,14 @@ using OptTensor = c10::optional<at::Tensor>;
 [[maybe_unused]] bool begins_on_16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // A weight or code tensor as the kernels read it: without gaps. (One that is a view into something
-// larger, at an odd place, is refused rather than copied at every call.)
+// larger, at an odd place, or that is negated when it is read, is refused rather than copied at every call.)
 [[maybe_unused]] void check_packed(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(!t.is_neg(), name, " must not be a negated view");
   TORCH_CHECK(begins_on_16(t), name, " must begin on 16 bytes");
 }
 
-// t [..., width] as rows whose distance the kernels can take; copied where it cannot.
+// t [..., width] as rows whose distance the kernels can take; copied where it cannot, or where torch keeps the values negated.
 struct Rows {
   at::Tensor t;
   int64_t stride;
@@ -69,12 +70,12 @@ struct Rows {
 constexpr int64_t kMaxStride = 1 << 20;
 [[maybe_unused]] Rows rows_of(const at::Tensor& t, const char* name) {
   const int64_t width = t.size(-1), rows = width > 0 ? t.numel() / width : 0;
-  if (t.is_contiguous() && begins_on_16(t) && (rows <= 1 || (width <= kMaxStride && width * t.element_size() % 16 == 0)))
+  if (t.is_contiguous() && begins_on_16(t) && !t.is_neg() && (rows <= 1 || (width <= kMaxStride && width * t.element_size() % 16 == 0)))
     return {t, width, int_size(rows, name)};
   at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, width});
   int64_t stride = flat.stride(0);
   const bool apart = rows <= 1 || (stride >= width && stride <= kMaxStride && stride * flat.element_size() % 16 == 0);
-  if (flat.numel() > 0 && (flat.stride(1) != 1 || !apart || !begins_on_16(flat)))
+  if (flat.numel() > 0 && (flat.stride(1) != 1 || !apart || !begins_on_16(flat) || flat.is_neg()))
     flat = flat.clone(at::MemoryFormat::Contiguous);
   stride = rows <= 1 ? width : flat.stride(0);
   return {flat, stride, int_size(rows, name)};

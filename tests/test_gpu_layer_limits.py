@@ -1,8 +1,9 @@
-"""Calls of the operators around a layer's blocks at the limits of what is documented: values next to the end of their type's range."""
+"""Calls of the operators around a layer's blocks at the limits of what is documented: values next to the end of their
+type's range, views that are negated when they are read."""
 import pytest
 import torch
 
-from flash_distributed_moe_amd import flashFfnOp as fops
+from flash_distributed_moe_amd import flashFfnOp as fops, flashLayerOp as ops
 from tests import layer_case
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +35,64 @@ def test_adapters_between_the_products(T, sign):
     got = fops.add_adapters(y, x, fops.Adapters(down, up, one), ids)
     rest = torch.arange(T, device="cuda") != T // 2
     assert torch.isinf(got[T // 2]).all() and torch.isfinite(got[rest]).all()
+
+
+# ------------------------------------------------------------------ views that are negated when they are read
+def negated(values):
+    """-values as a view that carries the negation with it."""
+    t = torch.complex(torch.zeros_like(values), values).conj().imag
+    assert t.is_neg()
+    return t
+
+
+def test_negated_gradients_of_the_losses():
+    gen = torch.Generator(device="cuda").manual_seed(8000)
+    logits = torch.empty(100, 24, device="cuda").normal_(generator=gen)
+    db, dz = negated(torch.tensor(-0.3, device="cuda")), negated(torch.tensor(0.2, device="cuda"))
+    dw = negated(torch.empty(100, 4, device="cuda").normal_(generator=gen))
+    leaf = logits.clone().requires_grad_()
+    r = ops.route(leaf, 4)
+    got, = torch.autograd.grad([r.weights, r.balance_loss, r.z_loss], leaf, [dw, db, dz])
+    layer_case.check(got, *layer_case.route(logits, 4, True, None, dw.resolve_neg(), db.resolve_neg(), dz.resolve_neg())["dlogits"], "dlogits")
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_negated_inputs(packed):
+    """Rows, gates and upstream gradients; packed: without gaps, as torch keeps the negation of some of its own results."""
+    gen = torch.Generator(device="cuda").manual_seed(8001)
+    draw = lambda *s: torch.empty(s, device="cuda").normal_(generator=gen)  # noqa: E731
+    turn = (lambda t: torch._neg_view(t)) if packed else negated  # noqa: E731
+    x, branch, gate, dy, w = draw(6, 64), draw(6, 64), draw(6, 1), draw(6, 64), draw(64)
+    leaves = [t.clone().requires_grad_() for t in (x, branch, gate, w)]
+    y, h = ops.block_join(turn(leaves[0]), turn(leaves[1]), leaves[3], turn(leaves[2]), leaves[3])
+    want = layer_case.join(-x, -branch, w, -gate, w)
+    layer_case.check(y, *want["y"], "y")
+    layer_case.check(h, *want["h"], "h")
+    plain = [t.clone().requires_grad_() for t in (-x, -branch, -gate)]
+    py, ph = ops.block_join(plain[0], plain[1], w, plain[2], w)
+    got = torch.autograd.grad([y, h], leaves[:3], [turn(dy), turn(dy)])
+    want = torch.autograd.grad([py, ph], plain, [-dy, -dy])
+    for a, b in zip(got, want):
+        assert torch.equal(a, -b)
+    logits = draw(9, 1)
+    assert torch.equal(ops.route(turn(logits), 1).z_loss, ops.route(-logits, 1).z_loss)
+    one = draw(1)
+    assert torch.equal(ops.route(turn(one), 1).z_loss, ops.route(-one, 1).z_loss)
+    q = fops.quantize_mxfp4(turn(x))
+    assert torch.equal(fops.dequantize_mxfp4(q), fops.dequantize_mxfp4(fops.quantize_mxfp4(-x)))
+
+
+@pytest.mark.parametrize("which", ["post", "next", "weight", "down", "up", "scales"])
+def test_negated_weights_are_refused(which):
+    """Weights are not copied at every call."""
+    turn = lambda t, name: torch._neg_view(t) if name == which else t  # noqa: E731
+    x, w = torch.randn(3, 64, device="cuda"), torch.ones(64, device="cuda")
+    b = x.bfloat16()
+    a = dict(down=torch.zeros(1, 8, 64, device="cuda").bfloat16(), up=torch.zeros(1, 64, 8, device="cuda").bfloat16(), scales=torch.ones(1, device="cuda"))
+    with pytest.raises(RuntimeError, match="negated"):
+        if which in a:
+            fops.add_adapters(b, b, fops.Adapters(**{k: turn(t, k) for k, t in a.items()}), torch.zeros(3, dtype=torch.int32, device="cuda"))
+        elif which == "weight":
+            ops.block_norm(x, turn(w, "weight"))
+        else:
+            ops.block_join(x, x, turn(w, "post"), None, turn(w, "next"))
