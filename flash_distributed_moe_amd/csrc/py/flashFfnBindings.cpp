@@ -9,6 +9,7 @@ namespace {
 FlashMoeFfnDesc describe(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptTensor& s13,
                          const OptTensor& s2, int activation) {
   TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  check_memory(x, "x");
   TORCH_CHECK(x.dim() >= 1, "x must be [..., hidden]");
   check_device(w13, "w13", x);
   check_device(w2, "w2", x);
@@ -133,6 +134,7 @@ at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tenso
 
 std::tuple<at::Tensor, at::Tensor> mxfp4_quantize(const at::Tensor& x) {
   TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  check_memory(x, "x");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 32 == 0, "x must be [..., K], K a multiple of 32");
   const int dtype = dtype_of(x, "x"), k = int_size(x.size(-1), "K");
   const DeviceGuard guard(x.device());
@@ -152,6 +154,7 @@ std::tuple<at::Tensor, at::Tensor> mxfp4_quantize(const at::Tensor& x) {
 // codes [..., K / 2] and scales [..., K / 32]; returns K
 int check_mxfp4(const at::Tensor& codes, const at::Tensor& scales, const char* name) {
   TORCH_CHECK(codes.defined() && codes.is_cuda(), name, " codes must be a CUDA tensor (ROCm)");
+  check_memory(codes, name);
   check_device(scales, "scales", codes);
   TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, name, " codes and scales must be uint8");
   TORCH_CHECK(codes.dim() >= 1 && codes.dim() == scales.dim() && codes.size(-1) > 0 && codes.size(-1) == scales.size(-1) * 16,

@@ -19,6 +19,8 @@ void refuse_second_derivatives(const char* name) {
   // Under create_graph the gradients would be taken for constants by whoever differentiates them again.
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivatives (create_graph=True)");
 }
+// An upstream gradient; torch's zeros without memory are as good as none.
+at::Tensor upstream(const at::Tensor& t) { return t.defined() && t._is_zerotensor() ? at::Tensor() : t; }
 // New memory on `like`'s device, without gaps. (Past the dispatcher, which takes as long again: the smallest calls are
 // bound by the host, and make up to six of these.)
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
@@ -39,6 +41,7 @@ Rows logit_rows(const at::Tensor& t, const char* name) {
 
 FlashMoeRouteDesc describe(const at::Tensor& logits, int64_t top_k, bool renormalize, const OptTensor& mask) {
   TORCH_CHECK(logits.defined() && logits.is_cuda(), "logits must be a CUDA tensor (ROCm)");
+  check_memory(logits, "logits");
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "logits must be [..., E]");
   FlashMoeRouteDesc d{};
   d.dtype = dtype_of(logits, "logits");
@@ -102,7 +105,10 @@ struct Route : torch::autograd::Function<Route> {
     const DeviceGuard guard(logits.device());
     const Rows rows = logit_rows(logits, "logits");
     // as they are in memory: torch may hand a gradient over that is negated when it is read
-    const auto plain = [](const at::Tensor& t) { return !t.defined() ? t : t.is_neg() ? t.contiguous().resolve_neg() : t.contiguous(); };
+    const auto plain = [](const at::Tensor& given) {
+      const at::Tensor t = upstream(given);
+      return !t.defined() ? t : t.is_neg() ? t.contiguous().resolve_neg() : t.contiguous();
+    };
     const at::Tensor dw = plain(grads[0]), db = plain(grads[3]), dz = plain(grads[4]);
     at::Tensor out = fresh(logits);
     const auto floats = [](const at::Tensor& t) { return static_cast<const float*>(pointer(t)); };
@@ -202,6 +208,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_forward(const NormInputs& in
   refuse_tangent(in.gate, "gate");
   refuse_tangent(in.next, "the next norm's weight");
   TORCH_CHECK(in.x.defined() && in.x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  check_memory(in.x, "x");
   const DeviceGuard guard(in.x.device());
   const NormCall c = prepare(in, alpha, beta, eps);
   at::Tensor y, h, kept;
@@ -234,7 +241,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     const NormInputs in{kept[0], kept[1], kept[2], kept[3], kept[4]};
     const DeviceGuard guard(in.x.device());
     const NormCall c = prepare(in, ctx->saved_data["alpha"].toDouble(), ctx->saved_data["beta"].toDouble(), ctx->saved_data["eps"].toDouble());
-    const at::Tensor dy = in.branch.defined() ? grads[0] : at::Tensor(), dh = in.next.defined() ? grads.back() : at::Tensor();
+    const at::Tensor dy = in.branch.defined() ? upstream(grads[0]) : at::Tensor(), dh = in.next.defined() ? upstream(grads.back()) : at::Tensor();
     Rows dys{}, dhs{};
     if (dy.defined()) dys = rows_of(dy, "dy");
     if (dh.defined()) dhs = rows_of(dh, "dh");
@@ -295,6 +302,7 @@ at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tens
   for (const at::Tensor* t : {&y, &x, &down, &up, &scales}) refuse_tangent(*t, "an input");
   TORCH_CHECK(!differentiated({&y, &x, &down, &up, &scales}), "adapters have no backward pass: detach the inputs or use torch.no_grad()");
   TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
+  check_memory(x, "x");
   check_device(y, "y", x);
   check_device(down, "down", x);
   check_device(up, "up", x);

@@ -38,6 +38,7 @@ void check_tensor(const at::Tensor& t, const char* name, bool any_float = true) 
   TORCH_CHECK(t.scalar_type() == at::kFloat || (any_float && t.scalar_type() == at::kBFloat16), name,
               any_float ? " must be float32 or bfloat16" : " must be float32");
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), name, " has no memory of its own");
 }
 
 // (torch on ROCm presents its HIP devices and streams under the name "cuda")

@@ -29,9 +29,17 @@ using OptTensor = c10::optional<at::Tensor>;
   TORCH_CHECK(e == hipSuccess, what, " failed: ", hipGetErrorString(static_cast<hipError_t>(e)), " (hipError_t ", e, ")");
 }
 
+// Tensors that stand for others (of a subclass that wraps one, or inside a functional transform) have none: their addresses are null,
+// which stands for an argument that is left out, or for a view of them a number that is no address.
+[[maybe_unused]] void check_memory(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), name,
+              " has no memory of its own (a tensor subclass, or a tensor inside a functional transform)");
+}
+
 [[maybe_unused]] void check_device(const at::Tensor& t, const char* name, const at::Tensor& like) {
   TORCH_CHECK(t.defined(), name, " tensor is undefined");
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (ROCm)");
+  check_memory(t, name);
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", not on ", t.device());
 }
 
@@ -84,7 +92,11 @@ constexpr int64_t kMaxStride = 1 << 20;
 [[maybe_unused]] at::Tensor bytes_on(const at::Tensor& like, size_t bytes) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte).requires_grad(false));
 }
-[[maybe_unused]] void* pointer(const at::Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
+[[maybe_unused]] void* pointer(const at::Tensor& t) {
+  if (!t.defined() || t.numel() == 0) return nullptr;
+  check_memory(t, "a tensor");
+  return t.data_ptr();
+}
 
 // A gradient of a leaf is accumulated on the stream on which its accumulator was made, by the first graph of it
 // that is still alive. Captured into a HIP graph, a backward pass that finds an accumulator of another

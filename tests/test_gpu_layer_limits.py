@@ -1,7 +1,8 @@
 """Calls of the operators around a layer's blocks at the limits of what is documented: values next to the end of their
-type's range, views that are negated when they are read."""
+type's range, views that are negated when they are read, tensors without memory."""
 import pytest
 import torch
+from torch._subclasses import FakeTensorMode
 
 from flash_distributed_moe_amd import flashFfnOp as fops, flashLayerOp as ops
 from tests import layer_case
@@ -96,3 +97,44 @@ def test_negated_weights_are_refused(which):
             ops.block_norm(x, turn(w, "weight"))
         else:
             ops.block_join(x, x, turn(w, "post"), None, turn(w, "next"))
+
+
+# ------------------------------------------------------------------ tensors without memory
+def fake(*shape, dtype=torch.float32, view=False):
+    with FakeTensorMode():
+        t = torch.ones((2, *shape), dtype=dtype, device="cuda")
+        return t[1] if view else t[0]
+
+
+@pytest.mark.parametrize("view", [False, True])
+@pytest.mark.parametrize("which", ["mask", "post", "gate", "next", "branch", "ids", "scales"])
+def test_arguments_without_memory_are_refused(which, view):
+    """They would count as left out: rows without a mask, a norm without its weight."""
+    pick = lambda name, t: fake(*t.shape, dtype=t.dtype, view=view) if name == which else t  # noqa: E731
+    x, w = torch.randn(3, 64, device="cuda"), torch.ones(64, device="cuda")
+    b, ids = x.bfloat16(), torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="no memory of its own"):
+        if which == "mask":
+            ops.route(x, 2, mask=pick("mask", torch.ones(3, dtype=torch.bool, device="cuda")))
+        elif which in ("ids", "scales"):
+            a = fops.Adapters(torch.zeros(1, 8, 64, device="cuda").bfloat16(), torch.zeros(1, 64, 8, device="cuda").bfloat16(),
+                              pick("scales", torch.ones(1, device="cuda")))
+            fops.add_adapters(b, b, a, pick("ids", ids))
+        else:
+            ops.block_join(x, pick("branch", x), pick("post", w), pick("gate", w), pick("next", w))
+
+
+def test_gradients_of_zeros_without_memory():
+    """What torch makes for derivatives that are nothing counts as zeros."""
+    x, w = torch.randn(6, 64, device="cuda"), torch.ones(64, device="cuda")
+    leaves = [x.clone().requires_grad_(), x.clone().requires_grad_()]
+    dy = torch.randn(6, 64, device="cuda")
+    nothing = torch._efficientzerotensor((6, 64), device="cuda")
+    y, h = ops.block_join(*leaves, w, None, w)
+    got = torch.autograd.grad([y, h], leaves, [dy, nothing], retain_graph=True)
+    for a, b in zip(got, torch.autograd.grad(y, leaves, dy)):
+        assert torch.equal(a, b)
+    r = ops.route(leaves[0], 3)
+    got, = torch.autograd.grad([r.weights, r.z_loss], leaves[0], [dy[:, :3], torch._efficientzerotensor((), device="cuda")], retain_graph=True)
+    want, = torch.autograd.grad(r.weights, leaves[0], dy[:, :3])
+    assert torch.equal(got, want)

@@ -1,0 +1,30 @@
+"""Tensors that stand for others and have no memory: refused before anything is enqueued, so without a GPU. Their null addresses would
+stand for arguments that are left out, and those of views of them for memory that is not there."""
+import pytest
+import torch
+from torch._subclasses import FakeTensorMode
+
+from flash_distributed_moe_amd import flashFfnOp as fops, flashLayerOp as ops
+
+B = torch.bfloat16
+
+
+def fake(*shape, dtype=torch.float32, view=False):
+    with FakeTensorMode():
+        t = torch.ones((2, *shape), dtype=dtype, device="cuda")
+        return t[1] if view else t[0]
+
+
+@pytest.mark.parametrize("view", [False, True])
+@pytest.mark.parametrize("call", [
+    lambda f: ops.route(f(6, 16), 2), lambda f: ops.route(f(6, 16), 2, mask=f(6, dtype=torch.bool)),
+    lambda f: ops.block_norm(f(6, 64), f(64)), lambda f: ops.block_join(f(6, 64), f(6, 64), f(64), f(64), f(64)),
+    lambda f: fops.add_adapters(f(6, 64, dtype=B), f(6, 64, dtype=B), fops.Adapters(f(1, 8, 64, dtype=B), f(1, 64, 8, dtype=B), f(1)),
+                                f(6, dtype=torch.int32)),
+    lambda f: fops.quantize_mxfp4(f(6, 64)), lambda f: fops.gated_ffn(f(6, 64), f(128, 64), f(64, 64)),
+    lambda f: fops.dequantize_mxfp4(fops.Mxfp4(f(6, 32, dtype=torch.uint8), f(6, 2, dtype=torch.uint8))),
+    lambda f: fops.mxfp4_linear(f(6, 64, dtype=B), fops.Mxfp4(f(64, 32, dtype=torch.uint8), f(64, 2, dtype=torch.uint8))),
+])
+def test_tensors_without_memory_are_refused(call, view):
+    with pytest.raises(RuntimeError, match="no memory of its own"):
+        call(lambda *shape, dtype=torch.float32: fake(*shape, dtype=dtype, view=view))
