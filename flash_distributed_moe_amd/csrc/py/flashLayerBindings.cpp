@@ -297,6 +297,15 @@ bool apart(const Rows& a, const Rows& b) {
   return d >= wa && d + wb <= la;
 }
 
+// Whether rows end before t begins, or begin behind its last value; t may have gaps.
+bool behind(const Rows& a, const at::Tensor& t) {
+  if (a.count == 0 || t.numel() == 0) return true;
+  int64_t values = 1;
+  for (int64_t i = 0; i < t.dim(); ++i) values += (t.size(i) - 1) * t.stride(i);
+  const int64_t size = a.t.element_size(), pa = reinterpret_cast<int64_t>(a.t.data_ptr()), pt = reinterpret_cast<int64_t>(t.data_ptr());
+  return pa + ((a.count - 1) * a.stride + a.t.size(-1)) * size <= pt || pt + values * t.element_size() <= pa;
+}
+
 at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tensor& down, const at::Tensor& up, const at::Tensor& scales,
                         const at::Tensor& ids, const OptTensor& out) {
   for (const at::Tensor* t : {&y, &x, &down, &up, &scales}) refuse_tangent(*t, "an input");
@@ -343,6 +352,7 @@ at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tens
     const bool itself = result.is_same(y) || (pointer(ys.t) == pointer(outs.t) && ys.stride == outs.stride);
     TORCH_CHECK(itself || apart(outs, ys), "out must be y or apart from it");
     TORCH_CHECK(apart(outs, xs), "out must be apart from x");
+    for (const at::Tensor* t : {&down, &up, &scales, &ids}) TORCH_CHECK(behind(outs, *t), "out must be apart from the adapters and ids");
   } else {
     result = fresh(y);
     outs = rows_of(result, "out");

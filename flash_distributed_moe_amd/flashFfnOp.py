@@ -79,7 +79,8 @@ def add_adapters(y, x, adapters, ids, out=None):
     a projection of x gave: one call for the rows of many requests, in any order.
 
     All bfloat16; float32 between the two products, rounded once. A row whose id is negative has no adapter and keeps y; a row
-    whose id names no adapter becomes NaN (ids are not read on the host). The result is new, or out, which may be y.
+    whose id names no adapter becomes NaN (ids are not read on the host). The result is new, or out, which may be y and
+    overlaps nothing else.
     K and N multiples of 8. Not differentiable."""
     try:
         return flashMoeLauncher.add_adapters(y, x, adapters.down, adapters.up, adapters.scales, ids, out)

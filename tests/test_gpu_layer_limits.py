@@ -1,5 +1,5 @@
 """Calls of the operators around a layer's blocks at the limits of what is documented: values next to the end of their
-type's range, views that are negated when they are read, tensors without memory."""
+type's range, views that are negated when they are read, tensors without memory, results over other operands."""
 import pytest
 import torch
 from torch._subclasses import FakeTensorMode
@@ -138,3 +138,25 @@ def test_gradients_of_zeros_without_memory():
     got, = torch.autograd.grad([r.weights, r.z_loss], leaves[0], [dy[:, :3], torch._efficientzerotensor((), device="cuda")], retain_graph=True)
     want, = torch.autograd.grad(r.weights, leaves[0], dy[:, :3])
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ results over other operands
+@pytest.mark.parametrize("T", [4, 900])
+def test_results_over_the_adapters_are_refused(T):
+    """Rows that are written while others' adapters are still read."""
+    r, n = 8, 300
+    K = N = 64
+    buffer = torch.zeros(n * N * r + n * r * K, device="cuda", dtype=torch.bfloat16)
+    up, down = buffer[:n * N * r].view(n, N, r), buffer[n * N * r:].view(n, r, K)
+    x, y = torch.randn(T, K, device="cuda").bfloat16(), torch.randn(T, N, device="cuda").bfloat16()
+    places = torch.zeros(T, N // 2, device="cuda", dtype=torch.int32)  # as many bytes as y: ids are a column of it
+    ids, scales = places[:, 0], torch.ones(n, device="cuda")
+    a = fops.Adapters(down, up, scales)
+    for out in (buffer[:T * N].view(T, N), buffer[-T * N:].view(T, N), buffer[n * N * r - T * N // 2:][:T * N].view(T, N), places.view(torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="apart from the adapters and ids"):
+            fops.add_adapters(y, x, a, ids, out=out)
+    # next to them on either side
+    whole = torch.zeros(2 * T * N + N * r, device="cuda", dtype=torch.bfloat16)
+    one = fops.Adapters(torch.zeros(1, r, K, device="cuda").bfloat16(), whole[T * N:T * N + N * r].view(1, N, r), scales[:1])
+    for out in (whole[:T * N].view(T, N), whole[T * N + N * r:][:T * N].view(T, N)):
+        assert fops.add_adapters(y, x, one, ids, out=out) is out and torch.equal(out, y)

@@ -1,5 +1,6 @@
-"""Tensors that stand for others and have no memory: refused before anything is enqueued, so without a GPU. Their null addresses would
-stand for arguments that are left out, and those of views of them for memory that is not there."""
+"""What the operators around a layer's blocks refuse of torch's other kinds of tensors, before anything is enqueued, so without a GPU: those
+that stand for others and have no memory (their null addresses would stand for arguments that are left out, and those of views of
+them for memory that is not there)."""
 import pytest
 import torch
 from torch._subclasses import FakeTensorMode
