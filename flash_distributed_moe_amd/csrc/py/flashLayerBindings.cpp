@@ -309,6 +309,7 @@ bool behind(const Rows& a, const at::Tensor& t) {
 at::Tensor add_adapters(const at::Tensor& y, const at::Tensor& x, const at::Tensor& down, const at::Tensor& up, const at::Tensor& scales,
                         const at::Tensor& ids, const OptTensor& out) {
   for (const at::Tensor* t : {&y, &x, &down, &up, &scales}) refuse_tangent(*t, "an input");
+  if (out.has_value()) refuse_tangent(*out, "out");
   TORCH_CHECK(!differentiated({&y, &x, &down, &up, &scales}), "adapters have no backward pass: detach the inputs or use torch.no_grad()");
   TORCH_CHECK(x.defined() && x.is_cuda(), "x must be a CUDA tensor (ROCm)");
   check_memory(x, "x");

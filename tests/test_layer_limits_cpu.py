@@ -1,8 +1,9 @@
 """What the operators around a layer's blocks refuse of torch's other kinds of tensors, before anything is enqueued, so without a GPU: those
 that stand for others and have no memory (their null addresses would stand for arguments that are left out, and those of views of
-them for memory that is not there)."""
+them for memory that is not there), and results that carry a tangent."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 from torch._subclasses import FakeTensorMode
 
 from flash_distributed_moe_amd import flashFfnOp as fops, flashLayerOp as ops
@@ -29,3 +30,12 @@ def fake(*shape, dtype=torch.float32, view=False):
 def test_tensors_without_memory_are_refused(call, view):
     with pytest.raises(RuntimeError, match="no memory of its own"):
         call(lambda *shape, dtype=torch.float32: fake(*shape, dtype=dtype, view=view))
+
+
+def test_results_with_a_tangent_are_refused():
+    """What is written into them would leave their tangent as it was."""
+    with fwd.dual_level():
+        out = fwd.make_dual(torch.zeros(3, 24, dtype=B), torch.ones(3, 24, dtype=B))
+        a = fops.Adapters(torch.zeros(2, 8, 16, dtype=B), torch.zeros(2, 24, 8, dtype=B), torch.zeros(2))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            fops.add_adapters(torch.zeros(3, 24, dtype=B), torch.zeros(3, 16, dtype=B), a, torch.zeros(3, dtype=torch.int32), out=out)
