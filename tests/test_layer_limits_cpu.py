@@ -1,6 +1,6 @@
 """What the operators around a layer's blocks refuse of torch's other kinds of tensors, before anything is enqueued, so without a GPU: those
 that stand for others and have no memory (their null addresses would stand for arguments that are left out, and those of views of
-them for memory that is not there), and results that carry a tangent."""
+them for memory that is not there), results that carry a tangent, and scales that are learnt."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -39,3 +39,16 @@ def test_results_with_a_tangent_are_refused():
         a = fops.Adapters(torch.zeros(2, 8, 16, dtype=B), torch.zeros(2, 24, 8, dtype=B), torch.zeros(2))
         with pytest.raises(RuntimeError, match="forward-mode"):
             fops.add_adapters(torch.zeros(3, 24, dtype=B), torch.zeros(3, 16, dtype=B), a, torch.zeros(3, dtype=torch.int32), out=out)
+
+
+@pytest.mark.parametrize("name", ["residual_scale", "branch_scale", "eps"])
+def test_scales_that_are_learnt_are_refused(name):
+    """They would be read as numbers, without a gradient."""
+    x, v = torch.zeros(3, 8), torch.tensor(1.0, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.block_join(x, x, **{name: v})
+    if name == "eps":
+        with pytest.raises(RuntimeError, match="no gradient"):
+            ops.block_norm(x, torch.ones(8), eps=v)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):
+        ops.block_join(x, x, **{name: v})
