@@ -4,6 +4,28 @@
 
 #include "tensorChecks.h"
 
+#include <torch/csrc/autograd/python_variable.h>
+
+// A number of a call. A tensor of one value would be taken for the number that it holds, and whoever learns it would get no gradient.
+struct Number {
+  double value;
+};
+namespace pybind11::detail {
+template <>
+struct type_caster<Number> {
+  PYBIND11_TYPE_CASTER(Number, const_name("float"));
+  bool load(handle source, bool convert) {
+    TORCH_CHECK(PyFloat_Check(source.ptr()) || !THPVariable_Check(source.ptr()) || !at::GradMode::is_enabled() ||
+                    !THPVariable_Unpack(source.ptr()).requires_grad(),
+                "the scales and eps are numbers: there is no gradient of a tensor in their place");
+    make_caster<double> number;
+    if (!number.load(source, convert)) return false;
+    value.value = cast_op<double>(number);
+    return true;
+  }
+};
+}  // namespace pybind11::detail
+
 namespace {
 
 using torch::autograd::AutogradContext;
@@ -262,8 +284,9 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 };
 
 variable_list block_norm(const at::Tensor& x, const OptTensor& branch, const OptTensor& post, const OptTensor& gate, const OptTensor& next,
-                         double alpha, double beta, double eps) {
+                         Number residual_scale, Number branch_scale, Number epsilon) {
   const NormInputs in{x, or_none(branch), or_none(post), or_none(gate), or_none(next)};
+  const double alpha = residual_scale.value, beta = branch_scale.value, eps = epsilon.value;
   TORCH_CHECK(in.x.defined(), "x tensor is undefined");
   if (!differentiated({&in.x, &in.branch, &in.post, &in.gate, &in.next})) {
     const auto [y, h, kept] = norm_forward(in, alpha, beta, eps, false);

@@ -32,7 +32,8 @@ using OptTensor = c10::optional<at::Tensor>;
 // Tensors that stand for others (of a subclass that wraps one, or inside a functional transform) have none: their addresses are null,
 // which stands for an argument that is left out, or for a view of them a number that is no address.
 [[maybe_unused]] void check_memory(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.numel() == 0 || (t.has_storage() && t.storage().data() != nullptr), name,
+  const c10::StorageImpl* memory = t.unsafeGetTensorImpl()->unsafe_storage().unsafeGetStorageImpl();
+  TORCH_CHECK((memory != nullptr && memory->data() != nullptr) || t.numel() == 0, name,
               " has no memory of its own (a tensor subclass, or a tensor inside a functional transform)");
 }
 

@@ -47,8 +47,6 @@ def route(logits, top_k, renormalize=True, mask=None):
 def block_norm(x, weight, eps=1e-6):
     """The norm in front of a block: x / sqrt(mean x^2 + eps) * weight for x [..., H] (float32 or bfloat16) and weight [H] of
     x's dtype. H a multiple of 8, up to 8192. Differentiable in x and weight."""
-    if type(eps) is not float:
-        _constants(eps=eps)
     try:
         return flashMoeLauncher.block_norm(x, None, None, None, _present(weight), 1.0, 1.0, eps)[0]
     except _STRANGERS:
@@ -64,21 +62,12 @@ def block_join(x, branch, post_weight=None, gate=None, next_weight=None, residua
     gate: [H], or x's leading dimensions up to some one, ones from there and H ([B, 1, H]: one for each sequence), or one value a
     token ([..., 1]). All of x's dtype. Everything of a row is float32 until y and h are rounded. Differentiable in
     all tensors; the scales and eps are numbers."""
-    if not type(residual_scale) is type(branch_scale) is type(eps) is float:
-        _constants(residual_scale=residual_scale, branch_scale=branch_scale, eps=eps)
     try:
         out = flashMoeLauncher.block_norm(x, _present(branch), post_weight, gate, next_weight, residual_scale, branch_scale, eps)
     except _STRANGERS:
         raise _stranger("x and branch must be tensors, weights and gate tensors or None, the rest numbers", x, branch, post_weight, gate,
                         next_weight, residual_scale, branch_scale, eps) from None
     return out[0] if next_weight is None else tuple(out)
-
-
-def _constants(**numbers):
-    # a tensor of one value would be taken for the number that it holds, and whoever learns it would get no gradient
-    for name, v in numbers.items():
-        if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("%s is a number: there is no gradient of it" % name)
 
 
 def _present(t):
