@@ -38,6 +38,21 @@ def test_adapters_between_the_products(T, sign):
     assert torch.isinf(got[T // 2]).all() and torch.isfinite(got[rest]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_squares_beyond_float32(dtype):
+    """The row's norm is zeros, as documented, its sum with the branch is not, and no other row notices."""
+    x, w = torch.randn(5, 264, device="cuda").to(dtype), torch.ones(264, device="cuda", dtype=dtype)
+    large = x.clone()
+    large[2] = 2.0 ** 70
+    rest = torch.arange(5, device="cuda") != 2
+    h = ops.block_norm(large, w)
+    assert not h[2].any() and torch.equal(h[rest], ops.block_norm(x, w)[rest])
+    y, h = ops.block_join(x, large, w, None, w)
+    assert torch.equal(y[2], x[2])
+    y, h = ops.block_join(large, x, None, None, w)
+    assert (y[2] == 2.0 ** 70).all() and not h[2].any()
+
+
 # ------------------------------------------------------------------ views that are negated when they are read
 def negated(values):
     """-values as a view that carries the negation with it."""
