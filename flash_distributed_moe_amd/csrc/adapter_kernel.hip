@@ -493,7 +493,8 @@ void enqueue_expand(const AdapterArgs& a, hipStream_t stream) {
   // Columns of a workgroup. The last ones to start leave CUs idle (8192 rows, N=12288, rank 64 with about 1000, 2000, 3300 and 5000
   // workgroups 99, 91, 89 and 96 us), but every one reads its tokens' u again, all parts of it: at least as many units as keep that
   // to a fifth of what y takes (1024 rows, K=N=4096, rank 128 113 us without that, 45 with it), but for the eight that an XCD each
-  // has. Of 16 rows the waves have four units at a time.
+  // has. Of 16 rows the waves have four units at a time, and no such eight: there that rule leaves few workgroups where k is split most (256
+  // rows, K=N=4096, rank 128, 8 parts: one for each of 16 to 24 tiles, 45 us of the call's 60).
   const bool tall = a.tile_rows == 64;
   const int across = (tall ? 1 : 4) * kUnit, all = (a.N + across - 1) / across;
   const long long wanted = ((tall ? 3300 : 1024) + a.most_tiles - 1LL) / a.most_tiles;

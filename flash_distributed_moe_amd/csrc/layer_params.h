@@ -29,8 +29,11 @@ struct RouteArgs {
 constexpr int kRouteExperts = 256, kRouteTopK = 32;
 constexpr int kRouteColumns = kRouteExperts + 1;  // a last one for the squared logsumexps, and of the counts for the rows
 // Workgroups of a forward pass. One alone finishes by itself, which saves the second launch (64 tokens 7.3 us, in four workgroups 8.2).
-// At most one a CU, so that the one workgroup that joins their sums reads no more than half a MiB; with 256 and 1024 threads each, E=128:
-// 8192 tokens 16.2 and 13.4 us, 32768 30 and 21; E=60, 4099 tokens 4.9 and 5.7 without joining.
+// At most one a CU, so that the one workgroup that joins their sums reads no more than 514 KiB. With 256 and 1024 threads each, us with the
+// joining in a replayed graph: float32 E=128, k=8 4099 tokens 13.8 and 12.1, 8192 16.0 and 13.2, 16384 21.3 and 15.9; bfloat16 E=60, k=4 4099
+// tokens 11.2 and 8.7, 8192 11.8 and 9.6, 12000 13.1 and 14.0, 16384 14.4 and 11.9. More threads leave fewer sums to join, fewer
+// deal the tokens out more evenly. The border was set by the tokens' kernels alone (E=60, 4099 tokens 4.9 and 5.7 without joining);
+// of whole calls 1024 threads are ahead below it as well (E=128, 1000 tokens 13.5 and 11.8).
 struct RouteGrid {
   int blocks, threads;
 };
@@ -116,7 +119,8 @@ struct AdapterArgs {
 constexpr int kAdapterRank = 128, kAdapters = 1000;
 // Few rows: every row reads its adapter by itself, which costs as much for each of them; tiles cost three kernels, the more the higher
 // the rank, before the number of rows is felt. us by rows and in tiles, K=N=4096: rank 8, 768 rows 15 and 19, 1024 17 and 21; rank 16, 512 rows
-// 17 and 18, 768 22 and 20; rank 64, 256 rows 26 and 28, 384 38 and 28; rank 128, 256 rows 50 and 63, 384 72 and 55.
+// 17 and 18, 768 22 and 20; rank 64, 256 rows 26 and 28, 384 38 and 28; rank 128, 256 rows 50 and 63, 384 72 and 55. How many adapters
+// the rows have between them is not asked: it is on the device, and the number of adapters that are kept says little of it.
 __host__ __device__ inline bool adapter_rows_alone(const AdapterArgs& a) {
   return a.T <= 4096 && static_cast<long long>(a.T) * a.r * (static_cast<long long>(a.K) + a.N) <= 56000000ll + 1400000ll * a.r;
 }

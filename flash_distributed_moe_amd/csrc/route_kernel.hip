@@ -11,8 +11,12 @@
 // parallel primitive that serves four tokens. The winners are taken in k rounds, of the lanes' greatest. For those a logit and its place are
 // one whole number, no two of them equal, so that a comparison says who goes first and a winner is found by its key.
 // A float32 logit has nine bits too many for that; where two neighbours among the first k + 1 agree in what is kept, the
-// wave takes its four tokens again by whole logits (of random ones one in some thousands).
-// Both directions are meant to be bound by reading the logits; the rounds are what competes with it.
+// wave takes its four tokens again by whole logits (of normally distributed ones with an offset an expert 1 token in 300 at E=128
+// and 256, k=8, 1 wave's pass in 70; at E=256, k=32 1 token in 35, 1 pass in 9).
+// The backward pass is bound by reading and writing the logits from some 65536 tokens on (131072 x 256 in float32 51 us, 5.3 TB/s). The
+// forward pass is bound by neither memory nor the vector units: there it takes 52 us where the reading takes 25 and the instructions 31,
+// since the k + 1 rounds depend on one another and four waves a SIMD are all there is to cover them; more winners cost accordingly
+// (whole calls with k=8 and 32 58 and 169 us, in bfloat16 46 and 99).
 #include <float.h>
 
 #include "ffn_device.h"
@@ -131,7 +135,8 @@ __device__ __forceinline__ Winners pick(const float (&v)[V], Again again, int la
   for (int i = 0; i < V; ++i) key[i] = (BF ? ordered(v[i]) >> 16 << 8 : ordered(v[i]) >> 1 & 0x7FFFFF00u) | (255 - column(lane, i));
   // of the lowest candidate: all others' keys are those of -inf, which are below
   const unsigned least = BF ? ordered(lowest<BF>()) >> 16 << 8 : ordered(lowest<BF>()) >> 1 & 0x7FFFFF00u;
-  // a lane's three greatest in order; a fourth, of one token in some hundreds, is looked for when it is needed
+  // A lane's three greatest in order. When the third is taken, though nobody may want a fourth, that one is looked for: at k=8 for 1
+  // wave's pass in 3 (E=64) to 6 in 10 (E=256), at E=256, k=16 and 32 for nearly every one.
   unsigned t0 = key[V - 1];
 #pragma unroll
   for (int i = 0; i + 1 < V; i += 2) t0 = umax(umax(t0, key[i]), key[i + 1]);

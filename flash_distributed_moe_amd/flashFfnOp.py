@@ -78,10 +78,10 @@ def add_adapters(y, x, adapters, ids, out=None):
     """y [..., N] + scales[i] * (x [..., K] down[i]^T) up[i]^T, i = ids[...] (int32) being each row's adapter, for y that
     a projection of x gave: one call for the rows of many requests, in any order.
 
-    All bfloat16; float32 between the two products, rounded once. A row whose id is negative has no adapter and keeps y; a row
-    whose id names no adapter becomes NaN (ids are not read on the host). The result is new, or out, which may be y and
-    overlaps nothing else.
-    K and N multiples of 8. Not differentiable."""
+    All bfloat16, rounded once. Sums are float32, and so is what goes from the first product to the second while rows are
+    few; of many rows it is two bfloat16 parts, which leave out 2^-16 of it, so that a row's last bits may depend on how many the call has.
+    A row whose id is negative has no adapter and keeps y; a row whose id names no adapter becomes NaN (ids are not read on the
+    host). The result is new, or out, which may be y and overlaps nothing else. K and N multiples of 8. Not differentiable."""
     try:
         return flashMoeLauncher.add_adapters(y, x, adapters.down, adapters.up, adapters.scales, ids, out)
     except _STRANGERS:

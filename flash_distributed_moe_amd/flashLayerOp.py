@@ -37,7 +37,9 @@ def route(logits, top_k, renormalize=True, mask=None):
     it is False. With p the softmax over a token's candidates, weights are p of the winners, divided by their
     sum if renormalize; balance_loss is E sum_e (counts_e / slots won) (mean_t p_te) and z_loss the mean squared
     logarithm of the sum of exp(logits), both over the tokens that have a candidate. Gradients reach the logits from weights and both
-    losses; the choice and the counts are constants. E up to 256, top_k up to min(E, 32)."""
+    losses; the choice and the counts are constants. E up to 256, top_k up to min(E, 32).
+    (The sparse layer routes by itself and takes no choice from outside: beside it this call gives the counts, losses and
+    their gradient.)"""
     try:
         return Routing(*flashMoeLauncher.route(logits, top_k, bool(renormalize), mask))
     except _STRANGERS:
@@ -46,7 +48,8 @@ def route(logits, top_k, renormalize=True, mask=None):
 
 def block_norm(x, weight, eps=1e-6):
     """The norm in front of a block: x / sqrt(mean x^2 + eps) * weight for x [..., H] (float32 or bfloat16) and weight [H] of
-    x's dtype. H a multiple of 8, up to 8192. Differentiable in x and weight."""
+    x's dtype. H a multiple of 8, up to 8192. Squares are summed in float32: where they overflow (values from 10^19 / sqrt(H) on) the
+    row becomes zeros. Differentiable in x and weight."""
     try:
         return flashMoeLauncher.block_norm(x, None, None, None, _present(weight), 1.0, 1.0, eps)[0]
     except _STRANGERS:
@@ -60,8 +63,8 @@ def block_join(x, branch, post_weight=None, gate=None, next_weight=None, residua
 
     x and branch [..., H] share shape and dtype (float32 or bfloat16), rows may lie apart; H a multiple of 8, up to 8192.
     gate: [H], or x's leading dimensions up to some one, ones from there and H ([B, 1, H]: one for each sequence), or one value a
-    token ([..., 1]). All of x's dtype. Everything of a row is float32 until y and h are rounded. Differentiable in
-    all tensors; the scales and eps are numbers."""
+    token ([..., 1]). All of x's dtype. Everything of a row is float32 until y and h are rounded (squares too, as in
+    `block_norm`). Differentiable in all tensors; the scales and eps are numbers."""
     try:
         out = flashMoeLauncher.block_norm(x, _present(branch), post_weight, gate, next_weight, residual_scale, branch_scale, eps)
     except _STRANGERS:

@@ -370,7 +370,8 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
  *   z = post_weight * branch / rms(branch), or the branch as it is without post_weight;
  *   y = residual_scale * x + branch_scale * gate * z;  h = next_weight * y / rms(y), with next_weight;
  * rms(v) = sqrt(mean v^2 + eps). Without a branch y = x, whatever the scales are, and h is the norm in front of a block alone. What
- * is computed of one row is float32, rounded once into y and once into h. */
+ * is computed of one row is float32, rounded once into y and once into h; squares beyond float32 (of values from 10^19 / sqrt(H) on) make
+ * the row's norm zeros. */
 enum {
   FLASH_MOE_GATE_NONE = 0,
   FLASH_MOE_GATE_CHANNEL = 1, /* [H] */
@@ -404,7 +405,9 @@ int flashMoeBlockNormBackward(const FlashMoeNormDesc* desc, const void* x, long 
                               void* workspace, void* dx, void* dbranch, void* dpost, void* dgate, void* dnext, void* stream);
 
 /* Low-rank adapters of many requests beside a projection: out_t = y_t + scales[i] * (x_t down[i]^T) up[i]^T, i = ids[t] being the
- * adapter of row t, in bfloat16; float32 between the two products, rounded once. y is what the projection gave. */
+ * adapter of row t, in bfloat16, rounded once. x_t down[i]^T is summed in float32 and goes on as float32 while rows are few, and as two
+ * bfloat16 parts (2^-16 of it is left out) where they are many: a row's last bits may depend on how many the call has. y is what
+ * the projection gave. */
 typedef struct FlashMoeAdapterDesc {
   int adapters;        /* 1..1000 */
   int rank;            /* r, a multiple of 8, at most 128 (shorter ones are filled up with zeros) */
