@@ -48,7 +48,7 @@ def route(logits, top_k, renormalize=True, mask=None):
 
 def block_norm(x, weight, eps=1e-6):
     """The norm in front of a block: x / sqrt(mean x^2 + eps) * weight for x [..., H] (float32 or bfloat16) and weight [H] of
-    x's dtype. H a multiple of 8, up to 8192. Squares are summed in float32: where they overflow (values from 10^19 / sqrt(H) on) the
+    x's dtype. H a multiple of 8, up to 8192. Squares are summed in float32: where they overflow (values from 1.8 10^19 / sqrt(H) on) the
     row becomes zeros. Differentiable in x and weight."""
     try:
         return flashMoeLauncher.block_norm(x, None, None, None, _present(weight), 1.0, 1.0, eps)[0]

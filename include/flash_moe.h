@@ -370,7 +370,7 @@ int flashMoeRouteBackward(const FlashMoeRouteDesc* desc, const void* logits, lon
  *   z = post_weight * branch / rms(branch), or the branch as it is without post_weight;
  *   y = residual_scale * x + branch_scale * gate * z;  h = next_weight * y / rms(y), with next_weight;
  * rms(v) = sqrt(mean v^2 + eps). Without a branch y = x, whatever the scales are, and h is the norm in front of a block alone. What
- * is computed of one row is float32, rounded once into y and once into h; squares beyond float32 (of values from 10^19 / sqrt(H) on) make
+ * is computed of one row is float32, rounded once into y and once into h; squares beyond float32 (of values from 1.8 10^19 / sqrt(H) on) make
  * the row's norm zeros. */
 enum {
   FLASH_MOE_GATE_NONE = 0,
